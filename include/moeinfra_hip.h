@@ -324,6 +324,46 @@ int moe_head_argmax_bf16(const void *weight, const void *x, const void *residual
                          void *cand_ws, int64_t cand_ws_bytes, void *token_i64, void *gen_i64,
                          int64_t gen_cap, void *gen_ctr_i64, void *pos_i32, void *stream);
 
+/* ---------------------------------------------------------------- batched serving
+ * Many sequences at once.  The KV cache of a layer is a pool of pages: k_cache and v_cache are
+ * [num_pages, n_kv, page_size, head_dim] with page_stride values from page to page (at least
+ * n_kv * page_size * head_dim, a multiple of 8; page_size a power of two of 8 to 4096).  Key j of
+ * sequence s is row j % page_size of page page_table[s][j / page_size] (int32 [n_seqs,
+ * table_width]).  Entries outside [0, num_pages) are pages that the cache does not have.  Rows of
+ * qkv and q are qkv_stride / q_stride values apart.
+ *
+ * moe_rope_paged_kv_bf16: the rotary embedding (rotate-half convention; angles position * inv_freq
+ * exact, one rounding to bf16) of the q and k heads of qkv [T, (n_q + 2 n_kv) * head_dim], token t
+ * at positions[t] of sequence seq_ids[t] (int32; null: sequence t); q to q_out [T, n_q, head_dim],
+ * k and v to the sequence's page, k also to k_out [T, n_kv, head_dim] when given.  A token at a
+ * negative position is padding, none of its rows is written; one whose page the table or the cache
+ * does not have is rotated but not cached.  Tokens of a call have places of their own (of two with
+ * one place, either's values stay, value by value). */
+int moe_rope_paged_kv_bf16(const void *qkv, int64_t qkv_stride, int64_t T, int32_t n_q_heads,
+                           int32_t n_kv_heads, int32_t head_dim, const void *inv_freq_f32,
+                           const void *positions_i32, const void *seq_ids_i32,
+                           const void *page_table_i32, int64_t n_seqs, int64_t table_width,
+                           int64_t num_pages, int32_t page_size, int64_t page_stride, void *q_out,
+                           void *k_out, void *k_cache, void *v_cache, void *stream);
+
+/* moe_paged_attention_bf16: one token per sequence, q [B, n_q, head_dim] against the first
+ * lens[s] keys of sequence s (int32; clamped to [0, table_width * page_size]): fp32 scores
+ * q.k * scaling and softmax, the weights rounded to bf16 before their sum (fp32) with v; out
+ * [B, n_q * head_dim].  Keys of pages that the cache does not have weigh nothing, and what lies
+ * behind a sequence's last key in its page is not looked at; a row without any key is zeros.  head
+ * dim 64, 128 or 256.  With a workspace (moe_paged_attention_workspace_bytes, enough for any
+ * smaller batch too; 16-byte aligned, its first 65536 bytes zero before the first call, every call
+ * leaves them zero; calls that share it must be ordered) several workgroups share a sequence's
+ * keys, their results added up in a fixed order; null: one workgroup each. */
+int64_t moe_paged_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
+                                            int32_t head_dim);
+int moe_paged_attention_bf16(const void *q, int64_t q_stride, const void *k_cache,
+                             const void *v_cache, int64_t num_pages, int32_t page_size,
+                             int64_t page_stride, const void *page_table_i32, int64_t table_width,
+                             const void *lens_i32, int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
+                             int32_t head_dim, float scaling, void *out, void *workspace,
+                             int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

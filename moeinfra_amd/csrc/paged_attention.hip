@@ -1,0 +1,462 @@
+// Attention of one new token per sequence against its paged KV cache, grouped query heads: the
+// batched counterpart of few_attention (attention.hip), whose cache is one sequence's.
+//
+//   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scaling * q.k_j,  m = max_j s_j
+//
+// over the first n keys of the sequence, in fp32 with a running m; the weights are rounded to
+// bf16 as an operand of the second product (half a step, 2^-8 of a weight), their sum is not.
+#include <type_traits>
+
+#include "common.h"
+
+namespace moe {
+namespace {
+
+constexpr int kPaTile = 32;           // keys per wave and step
+constexpr int kPaWaves = 4;
+constexpr int kPaThreads = kPaWaves * kWave;
+constexpr int kPaCols = 16;           // query heads per workgroup at most
+constexpr int kPaMaxSplits = 128;     // workgroups that share a sequence's keys, per head group
+constexpr int kPaMinTiles = 2 * kPaWaves;
+constexpr int64_t kPaCounterBytes = 65536;  // arrival counters at the start of the workspace
+constexpr float kPaLog2e = 1.44269504088896341f;
+
+__device__ __forceinline__ void pa_put(float *p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float pa_get(const float *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Whether this workgroup is the last of n to arrive at *count, which it then leaves zero.  What
+// the others wrote with pa_put is there for its pa_get (their stores have completed before they
+// count themselves in).  Nothing here waits for another workgroup.
+__device__ __forceinline__ bool pa_last_of(uint32_t *count, int n) {
+  __shared__ uint32_t s_seen;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t seen = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+    if (seen == (uint32_t)n) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_seen = seen;
+  }
+  __syncthreads();
+  return s_seen == (uint32_t)n;
+}
+
+struct PaArgs {
+  const uint16_t *q;
+  int64_t q_stride;
+  const uint16_t *kc, *vc;
+  int64_t page_stride;
+  const int32_t *table;
+  int64_t width, num_pages;
+  int page_shift;
+  const int32_t *lens;
+  int B, nq, nkv, grp, qtiles;
+  float scaling;
+  uint16_t *out;
+  uint32_t *count;
+  float *part;
+  int share;  // workgroups per head group that a full batch aims at (1 << 30: no splitting)
+};
+
+__device__ __forceinline__ int pa_wave_sum(int v) {
+  for (int o = 1; o < kWave; o <<= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+__device__ __forceinline__ int pa_wave_max(int v) {
+  for (int o = 1; o < kWave; o <<= 1) v = max(v, __shfl_xor(v, o, kWave));
+  return v;
+}
+
+// Which keys a workgroup takes.  Every sequence has ceil(tiles / chunk) items of at most `chunk`
+// tiles (one without keys: an item that writes zeros), the chunk such that all items of a head
+// group are about `share`: as the lengths are known on the device only, each wave adds them up and
+// finds the item's sequence by a scan over the batch.  At most share + B items.
+struct PaItem {
+  int seq, n;         // sequence, its keys
+  int split, nact;    // this item's number and the count of them
+  int tile0, tile1;
+};
+
+__device__ __forceinline__ bool pa_item(const PaArgs &a, int item, int lane, PaItem &w) {
+  const int64_t cap64 = a.num_pages > 0 ? a.width << a.page_shift : 0;
+  const int cap = (int)(cap64 < 0x7fffffc0 ? cap64 : 0x7fffffc0);
+  auto keys = [&](int i) { return i < a.B ? min(max(a.lens[i], 0), cap) : 0; };
+  int total = 0, most = 0;
+  for (int i0 = 0; i0 < a.B; i0 += kWave) {
+    const int t = (keys(i0 + lane) + kPaTile - 1) / kPaTile;
+    total += t;
+    most = max(most, t);
+  }
+  total = __builtin_amdgcn_readfirstlane(pa_wave_sum(total));
+  most = __builtin_amdgcn_readfirstlane(pa_wave_max(most));
+  uint32_t chunk = ((uint32_t)total + a.share - 1) / (uint32_t)a.share;
+  chunk = max(chunk, (uint32_t)kPaMinTiles);
+  chunk = max(chunk, ((uint32_t)most + kPaMaxSplits - 1) / kPaMaxSplits);
+  if (a.share == (1 << 30)) chunk = 0x7fffffff;
+  int base = 0;
+  for (int i0 = 0; i0 < a.B; i0 += kWave) {
+    const int n = keys(i0 + lane);
+    const uint32_t t = ((uint32_t)n + kPaTile - 1) / kPaTile;
+    const int c = i0 + lane < a.B ? max(1, (int)((t + chunk - 1) / chunk)) : 0;
+    int incl = c;
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int v = __shfl_up(incl, o, kWave);
+      if (lane >= o) incl += v;
+    }
+    const uint64_t hit = __ballot(item < base + incl);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      const int cl = __builtin_amdgcn_readlane(c, l);
+      w.seq = i0 + l;
+      w.n = __builtin_amdgcn_readlane(n, l);
+      w.split = item - (base + __builtin_amdgcn_readlane(incl, l) - cl);
+      const int tiles = (w.n + kPaTile - 1) / kPaTile;
+      const int per = max(1, (tiles + cl - 1) / cl);
+      w.nact = max(1, (tiles + per - 1) / per);
+      w.tile0 = w.split * per;
+      w.tile1 = min(w.tile0 + per, tiles);
+      return w.split < w.nact;
+    }
+    base += __builtin_amdgcn_readlane(incl, kWave - 1);
+  }
+  return false;
+}
+
+// A workgroup takes up to 16 query heads of one KV head of one sequence against a range of its
+// keys, its four waves every fourth tile of 32.  All operands come straight from memory into the
+// matrix instructions' registers:
+//
+//   S = K Q^T   two 16x16x32 row tiles; lane l loads row l % 16 of each, dims 32 s + 8 (l / 16) .. + 7.
+//               The rows are keys 8 (r / 4) + r % 4 and the same + 4, so that lane group g = l / 16
+//               ends up with keys 8 g .. 8 g + 7 of query head l % 16: the B operand of
+//   O += V^T P  E = HD / 16 products; lane l loads keys 8 g + i, dims E (l % 16) .. + E - 1 (whole rows
+//               of the cache per instruction), and transposes 8 keys x E dims among its own
+//               registers.  Product e has dim E r + e in row r.
+//
+// No value passes through LDS or between lanes but maxima and sums.
+//
+// Bound: HBM (at 4 heads a group the products are 5 % of the matrix rate).
+template <int HD>
+__global__ void __launch_bounds__(kPaThreads)
+paged_attention_kernel(const PaArgs a) {
+  constexpr int kSteps = HD / 32;   // products of S per row tile
+  constexpr int E = HD / 16;        // dims per lane of V
+  constexpr int kPad = HD + 4;
+  __shared__ __attribute__((aligned(16))) float s_o[kPaWaves][kPaCols * kPad];
+  __shared__ float s_m[kPaWaves][kPaCols], s_l[kPaWaves][kPaCols];
+  __shared__ float s_w[kPaCols][kPaMaxSplits];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int H = a.nkv * a.qtiles;
+  const int item = (int)(blockIdx.x / (unsigned)H), unit = (int)(blockIdx.x - (unsigned)item * H);
+  const int kvh = unit / a.qtiles, col0 = (unit - kvh * a.qtiles) * kPaCols;
+  const int ncol = min(a.grp - col0, kPaCols);
+  PaItem w;
+  if (!pa_item(a, item, lane, w)) return;  // the same for the whole workgroup
+
+  const int g = lane >> 4, r = lane & 15;
+  // Q as the B operand: column r (columns past the group repeat the last one and are dropped).
+  u32x4 qf[kSteps];
+  const int head0 = kvh * a.grp + col0;
+  {
+    const uint16_t *qr = a.q + w.seq * a.q_stride + (int64_t)(head0 + min(r, ncol - 1)) * HD + 8 * g;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) qf[s] = *reinterpret_cast<const u32x4 *>(qr + 32 * s);
+  }
+  const int32_t *trow = a.table + w.seq * a.width;
+  const int64_t head_at = ((int64_t)kvh * HD) << a.page_shift;
+  const int pmask = (1 << a.page_shift) - 1;
+  // Page entry of the 8 keys from `key` (an index past the last key reads the last key's entry).
+  auto entry = [&](int key) { return trow[min(key, w.n - 1) >> a.page_shift]; };
+  auto good = [&](int p) { return (uint32_t)p < (uint64_t)a.num_pages; };
+  const int gk = (r >> 2) * 8, gv = g * 8;
+  u32x4 kf[2][kSteps];
+  uint32_t vf[8][E / 2];
+  auto load_k = [&](int k0, int page) {
+    const int64_t p = good(page) ? page : 0;
+    const uint16_t *row = a.kc + p * a.page_stride + head_at + (int64_t)(((k0 + gk) & pmask) + (r & 3)) * HD + 8 * g;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        kf[h][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + h * 4 * HD + 32 * s));
+  };
+  auto load_v = [&](int k0, int page) {
+    const int64_t p = good(page) ? page : 0;
+    const uint16_t *row = a.vc + p * a.page_stride + head_at + (int64_t)((k0 + gv) & pmask) * HD + E * r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (E == 4) {
+        typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
+        const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(row + i * HD));
+        vf[i][0] = v[0];
+        vf[i][1] = v[1];
+      } else {
+#pragma unroll
+        for (int c = 0; c < E / 8; ++c) {
+          const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + i * HD + 8 * c));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[i][4 * c + e] = v[e];
+        }
+      }
+    }
+  };
+
+  f32x4 acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;
+  int it = w.tile0 + wave;
+  int pv = 0, pk_next = 0, pv_next = 0;
+  // One tile; NEXT: another follows, whose loads are issued as soon as their registers are free.
+  auto tile = [&](auto next_c) __attribute__((always_inline)) {
+    constexpr bool kNext = decltype(next_c)::value;
+    const int k0 = it * kPaTile, k1 = k0 + kPaWaves * kPaTile;
+    f32x4 sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sc[h] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf[h][s]),
+                                                        __builtin_bit_cast(bf16x8, qf[s]), sc[h], 0, 0, 0);
+    }
+    if constexpr (kNext) load_k(k1, pk_next);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3] * a.scaling;
+    // A tile with keys past the end or pages that do not exist: such keys weigh nothing, and
+    // what lies in their place of V (anything, NaN too) is taken as zeros.
+    const bool ok = good(pv);
+    if (k0 + kPaTile > w.n || !__all(ok)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool seen = ok && k0 + gv + i < w.n;
+        x[i] = seen ? x[i] : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) vf[i][e] = seen ? vf[i][e] : 0u;
+      }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+    if (__any(mx > m)) {
+      mx = op_xor16<true>(op_xor32<true>(mx));
+      const float mn = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * kPaLog2e);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[e][v] *= alpha;
+    }
+    const float mref = m == -INFINITY ? 0.0f : m;
+    u32x4 pf;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // (The difference first: mref * log2(e) alone could overflow.)
+      const float e0 = __builtin_amdgcn_exp2f((x[2 * j] - mref) * kPaLog2e);
+      const float e1 = __builtin_amdgcn_exp2f((x[2 * j + 1] - mref) * kPaLog2e);
+      l += e0 + e1;
+      pf[j] = pack_bf16x2(e0, e1);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;  // high or low halves of two words
+      u32x4 vt;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vt[j] = __builtin_amdgcn_perm(vf[2 * j + 1][e >> 1], vf[2 * j][e >> 1], sel);
+      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vt),
+                                                       __builtin_bit_cast(bf16x8, pf), acc[e], 0, 0, 0);
+    }
+    if constexpr (kNext) {
+      load_v(k1, pv_next);
+      pv = pv_next;
+      pk_next = entry(k1 + kPaWaves * kPaTile + gk);
+      pv_next = entry(k1 + kPaWaves * kPaTile + gv);
+    }
+  };
+  if (it < w.tile1) {
+    const int k0 = it * kPaTile;
+    const int pk = entry(k0 + gk);
+    pv = entry(k0 + gv);
+    pk_next = entry(k0 + kPaWaves * kPaTile + gk);
+    pv_next = entry(k0 + kPaWaves * kPaTile + gv);
+    load_k(k0, pk);
+    load_v(k0, pv);
+    for (; it + kPaWaves < w.tile1; it += kPaWaves) tile(std::true_type{});
+    tile(std::false_type{});
+  }
+  // The waves' results meet in LDS.
+  l = op_xor16<false>(op_xor32<false>(l));
+  if (r < ncol) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<float4 *>(&s_o[wave][r * kPad + E * (4 * g + v) + e]) =
+            make_float4(acc[e][v], acc[e + 1][v], acc[e + 2][v], acc[e + 3][v]);
+    if (g == 0) {
+      s_m[wave][r] = m;
+      s_l[wave][r] = l;
+    }
+  }
+  __syncthreads();
+  const int64_t mine = (int64_t)blockIdx.x * min(a.grp, kPaCols) * (HD + 2);
+  uint16_t *const orow = a.out + ((int64_t)w.seq * a.nq + head0) * HD;
+  for (int i = threadIdx.x; i < ncol * HD; i += kPaThreads) {
+    const int c = i / HD, d = i - c * HD;
+    float mm = s_m[0][c];
+#pragma unroll
+    for (int y = 1; y < kPaWaves; ++y) mm = fmaxf(mm, s_m[y][c]);
+    const float mref = mm == -INFINITY ? 0.0f : mm;
+    float o = 0.0f, ll = 0.0f;
+#pragma unroll
+    for (int y = 0; y < kPaWaves; ++y) {
+      const float f = __builtin_amdgcn_exp2f((s_m[y][c] - mref) * kPaLog2e);
+      o = fmaf(f, s_o[y][c * kPad + d], o);
+      ll = fmaf(f, s_l[y][c], ll);
+    }
+    if (w.nact == 1) {
+      orow[i] = f32_to_bf16(ll == 0.0f ? 0.0f : o / ll);  // no key at all: zeros
+    } else {
+      float *const p = a.part + mine + c * (HD + 2);
+      pa_put(p + d, o);
+      if (d == 0) {
+        pa_put(p + HD, mm);
+        pa_put(p + HD + 1, ll);
+      }
+    }
+  }
+  if (w.nact == 1) return;
+  if (!pa_last_of(a.count + (int64_t)w.seq * H + unit, w.nact)) return;
+  // The last of the sequence's workgroups adds their results up, in the order of the keys.
+  const int64_t step = (int64_t)H * min(a.grp, kPaCols) * (HD + 2);  // from one item to the next
+  const float *const first = a.part + mine - w.split * step;
+  for (int i = threadIdx.x; i < ncol * w.nact; i += kPaThreads) {
+    const int y = i / ncol, c = i - y * ncol;
+    s_w[c][y] = pa_get(first + y * step + c * (HD + 2) + HD);
+  }
+  __syncthreads();
+  if (threadIdx.x < ncol) {
+    float mm = -INFINITY;
+    for (int y = 0; y < w.nact; ++y) mm = fmaxf(mm, s_w[threadIdx.x][y]);
+    s_m[0][threadIdx.x] = mm == -INFINITY ? 0.0f : mm;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < ncol * HD; i += kPaThreads) {
+    const int c = i / HD, d = i - c * HD;
+    const float *p = first + c * (HD + 2);
+    float o = 0.0f, ll = 0.0f;
+#pragma unroll 4
+    for (int y = 0; y < w.nact; ++y) {
+      const float f = __builtin_amdgcn_exp2f((s_w[c][y] - s_m[0][c]) * kPaLog2e);
+      o = fmaf(f, pa_get(p + y * step + d), o);
+      ll = fmaf(f, pa_get(p + y * step + HD + 1), ll);
+    }
+    orow[i] = f32_to_bf16(ll == 0.0f ? 0.0f : o / ll);
+  }
+}
+
+constexpr int kPaMaxPage = 4096;
+
+// Workgroups per head group that a launch aims at.
+int pa_share(int64_t units) {
+  const int64_t s = 3 * (int64_t)device_cu_count() / units;
+  return (int)(s < 1 ? 1 : s);
+}
+int pa_qtiles(int32_t grp) { return (grp + kPaCols - 1) / kPaCols; }
+bool pa_splits(int64_t B, int64_t units) { return B * units <= kPaCounterBytes / 4; }
+
+bool pa_sizes_ok(int64_t B, int32_t nq, int32_t nkv, int32_t hd) {
+  return B >= 0 && B <= (1 << 20) && nq > 0 && nkv > 0 && nq % nkv == 0 && nq <= (1 << 16) &&
+         (hd == 64 || hd == 128 || hd == 256);
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int64_t moe_paged_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
+                                                       int32_t head_dim) {
+  if (!moe::pa_sizes_ok(B, n_q_heads, n_kv_heads, head_dim)) return -1;
+  const int32_t grp = n_q_heads / n_kv_heads;
+  const int64_t units = (int64_t)n_kv_heads * moe::pa_qtiles(grp);
+  int64_t b = B;  // the most of any batch up to B
+  if (!moe::pa_splits(b, units)) b = moe::kPaCounterBytes / 4 / units;
+  return moe::kPaCounterBytes + (moe::pa_share(units) + b) * units * (grp < moe::kPaCols ? grp : moe::kPaCols) *
+                                    (int64_t)(head_dim + 2) * 4;
+}
+
+extern "C" int moe_paged_attention_bf16(const void *q, int64_t q_stride, const void *k_cache, const void *v_cache,
+                                        int64_t num_pages, int32_t page_size, int64_t page_stride,
+                                        const void *page_table_i32, int64_t table_width, const void *lens_i32,
+                                        int64_t B, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                        float scaling, void *out, void *workspace, int64_t workspace_bytes,
+                                        void *stream) {
+  MOE_REQUIRE(n_q_heads > 0 && n_kv_heads > 0 && n_q_heads % n_kv_heads == 0,
+              "query heads must be a multiple of the KV heads");
+  MOE_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "head dim must be 64, 128 or 256 (got %d)", head_dim);
+  MOE_REQUIRE(moe::pa_sizes_ok(B, n_q_heads, n_kv_heads, head_dim) && num_pages >= 0 &&
+                  num_pages <= 0x7fffffff && table_width >= 0,
+              "bad sizes");
+  MOE_REQUIRE(page_size >= 8 && page_size <= moe::kPaMaxPage && (page_size & (page_size - 1)) == 0,
+              "page size must be a power of two of 8 to %d (got %d)", moe::kPaMaxPage, page_size);
+  // Keys of a call are counted in 32 bits (in tiles of 32).
+  MOE_REQUIRE(table_width <= 0x7fffffff / page_size && (B == 0 || table_width * page_size <= ((int64_t)1 << 35) / B),
+              "a table of %lld pages of %d keys is too long", (long long)table_width, page_size);
+  const int64_t page_row = (int64_t)n_kv_heads * page_size * head_dim;
+  MOE_REQUIRE(page_stride % 8 == 0 && page_stride >= page_row, "page stride must be a multiple of 8 of at least %lld",
+              (long long)page_row);
+  const int64_t row = (int64_t)n_q_heads * head_dim;
+  MOE_REQUIRE(q_stride % 8 == 0 && (q_stride >= row || B <= 1), "q rows must be 16-byte aligned and apart");
+  if (B == 0) return MOE_STATUS_OK;
+  MOE_REQUIRE(q && lens_i32 && out && (page_table_i32 || table_width == 0) && ((k_cache && v_cache) || num_pages == 0),
+              "null pointer");
+  MOE_REQUIRE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (uintptr_t)out % 2 == 0,
+              "q and the caches must be 16-byte aligned");
+  const int64_t ob = 2 * B * row, cb = num_pages > 0 ? 2 * ((num_pages - 1) * page_stride + page_row) : 0;
+  MOE_REQUIRE(!moe::ranges_overlap(out, ob, q, 2 * (q_stride * (B - 1) + row)) &&
+                  !moe::ranges_overlap(out, ob, k_cache, cb) && !moe::ranges_overlap(out, ob, v_cache, cb),
+              "out must not overlap q or the caches");
+  moe::PaArgs a{};
+  a.grp = n_q_heads / n_kv_heads;
+  a.qtiles = moe::pa_qtiles(a.grp);
+  const int64_t units = (int64_t)n_kv_heads * a.qtiles;
+  const bool split = workspace != nullptr && moe::pa_splits(B, units);
+  if (workspace != nullptr) {
+    const int64_t need = moe_paged_attention_workspace_bytes(B, n_q_heads, n_kv_heads, head_dim);
+    MOE_REQUIRE(workspace_bytes >= need, "workspace too small: need %lld bytes, got %lld", (long long)need,
+                (long long)workspace_bytes);
+    MOE_REQUIRE((uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
+  }
+  a.q = (const uint16_t *)q;
+  a.q_stride = q_stride;
+  a.kc = (const uint16_t *)k_cache;
+  a.vc = (const uint16_t *)v_cache;
+  a.page_stride = page_stride;
+  a.table = (const int32_t *)page_table_i32;
+  a.width = table_width;
+  a.num_pages = num_pages;
+  a.page_shift = __builtin_ctz((unsigned)page_size);
+  a.lens = (const int32_t *)lens_i32;
+  a.B = (int)B;
+  a.nq = n_q_heads;
+  a.nkv = n_kv_heads;
+  a.scaling = scaling;
+  a.out = (uint16_t *)out;
+  a.count = (uint32_t *)workspace;
+  a.part = workspace ? (float *)((char *)workspace + moe::kPaCounterBytes) : nullptr;
+  a.share = split ? moe::pa_share(units) : 1 << 30;
+  const int64_t items = split ? a.share + B : B;
+  MOE_REQUIRE(items * units <= 0x7fffffff, "bad sizes");
+  auto kern = head_dim == 64    ? moe::paged_attention_kernel<64>
+              : head_dim == 128 ? moe::paged_attention_kernel<128>
+                                : moe::paged_attention_kernel<256>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(items * units)), dim3(moe::kPaThreads), 0, (hipStream_t)stream, a);
+  MOE_LAUNCH_CHECK();
+  return MOE_STATUS_OK;
+}

@@ -283,3 +283,135 @@ def layer_forward(table, num_experts: int, gate: torch.Tensor, x: torch.Tensor, 
                                       idx.data_ptr(), workspace.data_ptr(), workspace.numel(),
                                       _stream(dev)), "layer_forward")
     return out, logits, w, idx
+
+
+# ----------------------------------------------------------------------------- batched serving
+def _launch(fn, what: str, dev: torch.device, *args) -> None:
+    """Calls an entry point with the current stream of ``dev``, on that device (whose sizes the
+    launch is planned for, and whose default stream it may be)."""
+    if torch.cuda.current_device() == dev.index:
+        check(fn(*args, _stream(dev)), what)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, _stream(dev)), what)
+
+
+def _require_rows(t: torch.Tensor, name: str, device: torch.device, ndim: int) -> int:
+    """A bf16 tensor [rows, ...] whose rows are contiguous, but not necessarily next to each
+    other (a slice of a projection's output); returns the stride of the rows."""
+    _require_cuda(t, name)
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} must be {torch.bfloat16} (got {t.dtype})")
+    if t.device != device:
+        raise ValueError(f"{name} device {t.device} != {device}")
+    if t.ndim != ndim:
+        raise ValueError(f"{name} must have {ndim} dimensions (got {tuple(t.shape)})")
+    if t.shape[0] > 0 and not t[0].is_contiguous():
+        raise ValueError(f"{name} must have contiguous rows (got strides {t.stride()})")
+    row = t[0].numel() if t.shape[0] > 0 else 0
+    return t.stride(0) if t.shape[0] > 1 else (row + 7) // 8 * 8
+
+
+def _require_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, device: torch.device) -> int:
+    """Checks a paged cache (k and v [pages, kv heads, page size, head dim], whole pages at one
+    stride) and its table; returns the page stride."""
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _require_rows(t, name, device, 4)
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} differ in shape")
+    if k_cache.shape[0] > 1 and k_cache.stride(0) != v_cache.stride(0):
+        raise ValueError(f"k_cache and v_cache differ in page stride ({k_cache.stride(0)} != {v_cache.stride(0)})")
+    _require(page_table, "page_table", torch.int32, device)
+    if page_table.ndim != 2:
+        raise ValueError("page_table must be [sequences, pages]")
+    pages, nkv, size, hd = k_cache.shape
+    return k_cache.stride(0) if pages > 1 else nkv * size * hd
+
+
+def rope_paged_kv(qkv: torch.Tensor, positions: torch.Tensor, page_table: torch.Tensor, k_cache: torch.Tensor,
+                  v_cache: torch.Tensor, n_q_heads: int, inv_freq: torch.Tensor,
+                  seq_ids: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+                  want_k: bool = False):
+    """Rotary embedding of new tokens of many sequences, their keys and values written to the
+    sequences' pages (``k_cache`` / ``v_cache`` [pages, kv heads, page size, head dim], bf16;
+    ``page_table`` int32 [sequences, pages per sequence]).
+
+    ``qkv`` bf16 [T, (q heads + 2 kv heads) * head dim]; token t stands at ``positions[t]`` (int32)
+    of sequence ``seq_ids[t]`` (int32; None: sequence t).  ``inv_freq`` fp32 [head dim / 2].
+    Returns (rotated q bf16 [T, q heads * head dim], rotated k bf16 [T, kv heads, head dim] | None).
+    Tokens at negative positions are padding: their rows, here and in the cache, are left as they
+    were.  A token whose page the table (or the cache) does not have is rotated, not cached.  No
+    two tokens of a call may have one place."""
+    dev = qkv.device
+    stride = _require_rows(qkv, "qkv", dev, 2)
+    page_stride = _require_pages(k_cache, v_cache, page_table, dev)
+    pages, nkv, size, hd = k_cache.shape
+    nq, T = int(n_q_heads), qkv.shape[0]
+    if qkv.shape[1] != (nq + 2 * nkv) * hd:
+        raise ValueError(f"qkv rows have {qkv.shape[1]} values, {nq} query and {nkv} KV heads of {hd} need "
+                         f"{(nq + 2 * nkv) * hd}")
+    _require(positions, "positions", torch.int32, dev)
+    _require(inv_freq, "inv_freq", torch.float32, dev)
+    if positions.shape != (T,):
+        raise ValueError(f"positions must be [{T}] (got {tuple(positions.shape)})")
+    if inv_freq.numel() != hd // 2:
+        raise ValueError(f"inv_freq must have {hd // 2} values")
+    if seq_ids is not None:
+        _require(seq_ids, "seq_ids", torch.int32, dev)
+        if seq_ids.shape != (T,):
+            raise ValueError(f"seq_ids must be [{T}] (got {tuple(seq_ids.shape)})")
+    if q_out is None:
+        q_out = torch.empty((T, nq * hd), dtype=torch.bfloat16, device=dev)
+    else:
+        _require(q_out, "q_out", torch.bfloat16, dev)
+        if q_out.numel() != T * nq * hd:
+            raise ValueError("q_out has the wrong number of elements")
+    k_out = torch.empty((T, nkv, hd), dtype=torch.bfloat16, device=dev) if want_k else None
+    _launch(lib().moe_rope_paged_kv_bf16, "rope_paged_kv", dev, qkv.data_ptr(), stride, T, nq, nkv, hd,
+            inv_freq.data_ptr(), positions.data_ptr(), _ptr(seq_ids), page_table.data_ptr(), page_table.shape[0],
+            page_table.shape[1], pages, size, page_stride, q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(),
+            v_cache.data_ptr())
+    return q_out, k_out
+
+
+def paged_attention_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Workspace of ``paged_attention`` for batches of up to ``batch`` sequences: made once, then
+    shared by calls that run one after the other (one stream)."""
+    n = lib().moe_paged_attention_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim)
+    if n < 0:
+        raise ValueError(f"invalid attention sizes batch={batch} heads={n_q_heads}/{n_kv_heads} head_dim={head_dim}")
+    return torch.zeros((n,), dtype=torch.uint8, device=device)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    lens: torch.Tensor, scaling: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence, ``q`` bf16 [B, q heads, head dim], against the first
+    ``lens[b]`` (int32) keys of its pages; bf16 [B, q heads, head dim].  ``scaling`` defaults to
+    head_dim ** -0.5.  Rows without keys (padding of a batch) are zeros.  ``workspace``
+    (``paged_attention_workspace``) saves the call making one."""
+    dev = q.device
+    stride = _require_rows(q, "q", dev, 3)
+    page_stride = _require_pages(k_cache, v_cache, page_table, dev)
+    pages, nkv, size, hd = k_cache.shape
+    B, nq = q.shape[:2]
+    if q.shape[2] != hd:
+        raise ValueError(f"q has head dim {q.shape[2]}, the cache {hd}")
+    _require(lens, "lens", torch.int32, dev)
+    if lens.shape != (B,) or page_table.shape[0] != B:
+        raise ValueError(f"lens and page_table must have {B} rows (got {tuple(lens.shape)}, {tuple(page_table.shape)})")
+    if out is None:
+        out = torch.empty((B, nq, hd), dtype=torch.bfloat16, device=dev)
+    else:
+        _require(out, "out", torch.bfloat16, dev)
+        if out.numel() != B * nq * hd:
+            raise ValueError("out has the wrong number of elements")
+    if workspace is None:
+        workspace = paged_attention_workspace(B, nq, nkv, hd, dev)
+    else:
+        _require(workspace, "workspace", torch.uint8, dev)
+    _launch(lib().moe_paged_attention_bf16, "paged_attention", dev, q.data_ptr(), stride, k_cache.data_ptr(),
+            v_cache.data_ptr(), pages, size, page_stride, page_table.data_ptr(), page_table.shape[1], lens.data_ptr(),
+            B, nq, nkv, hd, hd ** -0.5 if scaling is None else float(scaling), out.data_ptr(), workspace.data_ptr(),
+            workspace.numel())
+    return out

@@ -1,0 +1,242 @@
+"""The batched serving operators on the GPU against plain 64-bit forms: rotary embedding into a
+paged cache, attention over it."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from serving_ref import Pool, assert_within, attention, rope
+
+pytestmark = pytest.mark.gpu
+
+
+def _bf(shape, seed, std=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(torch.bfloat16)
+
+
+def _inv(hd):
+    i = torch.arange(0, hd, 2, dtype=torch.int64).float()
+    return 1.0 / (1e6 ** (i / hd))
+
+
+def _same(a, b):
+    return torch.equal(a.contiguous().view(torch.int16), b.contiguous().view(torch.int16))
+
+
+# ------------------------------------------------------------------ rotary embedding, paged cache
+@pytest.mark.parametrize("nq,nkv,hd,page,interleaved,padded_rows", [
+    (32, 8, 128, 16, False, False), (8, 2, 64, 8, True, True), (3, 1, 16, 32, False, True),
+    (4, 4, 256, 64, True, False), (6, 2, 80, 128, False, False)])
+def test_rope_paged_kv(cuda_device, nq, nkv, hd, page, interleaved, padded_rows):
+    from moeinfra_amd import ops
+
+    dev = cuda_device
+    # Prompts of sequences 2 and 0, a token of sequence 1 far away, one at the first place.
+    lens = [page + 3, 0, 2 * page, 1]
+    places = [(2, p) for p in range(2 * page)] + [(0, p) for p in range(page + 3)] + [(3, 0)]
+    T = len(places)
+    pool = Pool(lens, nkv, hd, page, dev, seed=1, interleaved=interleaved, fill=7.0)
+    x = _bf((T, (nq + 2 * nkv) * hd + (16 if padded_rows else 0)), 2)[:, :(nq + 2 * nkv) * hd]
+    inv = _inv(hd)
+    kc0, vc0 = pool.k.clone(), pool.v.clone()
+    xd = torch.empty((T, x.shape[1] + (16 if padded_rows else 0)), dtype=torch.bfloat16, device=dev)[:, :x.shape[1]]
+    xd.copy_(x)
+    seq = torch.tensor([s for s, _ in places], dtype=torch.int32, device=dev)
+    pos = torch.tensor([p for _, p in places], dtype=torch.int32, device=dev)
+    q, k = ops.rope_paged_kv(xd, pos, pool.dev_table, pool.k, pool.v, nq, inv.to(dev), seq_ids=seq, want_k=True)
+    heads = x.reshape(T, nq + 2 * nkv, hd)
+    y, tol = rope(heads[:, :nq + nkv], pos.cpu(), inv)
+    assert_within(q.view(T, nq, hd), y[:, :nq], tol[:, :nq], "q")
+    assert_within(k, y[:, nq:], tol[:, nq:], "k")
+    # Exactly the new places changed, to k and v.
+    for (s, p), kk, vv in zip(places, k, heads[:, nq + nkv:].to(dev)):
+        at = int(pool.table[s, p // page])
+        kc0[at, :, p % page] = kk
+        vc0[at, :, p % page] = vv
+    assert _same(pool.k, kc0) and _same(pool.v, vc0)
+
+
+def test_rope_paged_kv_far_positions(cuda_device):
+    from moeinfra_amd import ops
+
+    nq, nkv, hd, page = 4, 2, 128, 64
+    pos = [0, 1, 4095, 131071, 1048575, 16777217, 2147483583]
+    inv = _inv(hd)
+    x = _bf((len(pos), (nq + 2 * nkv) * hd), 3).to(cuda_device)
+    pool = Pool([1] * len(pos), nkv, hd, page, cuda_device)  # a table too short for most of them
+    q, k = ops.rope_paged_kv(x, torch.tensor(pos, dtype=torch.int32, device=cuda_device), pool.dev_table, pool.k,
+                             pool.v, nq, inv.to(cuda_device), want_k=True)
+    y, tol = rope(x.cpu().view(len(pos), -1, hd)[:, :nq + nkv], pos, inv)
+    assert_within(q.view(len(pos), nq, hd), y[:, :nq], tol[:, :nq])
+    assert_within(k, y[:, nq:], tol[:, nq:])
+
+
+def test_rope_paged_kv_padding_and_missing_pages(cuda_device):
+    from moeinfra_amd import ops
+
+    dev, nq, nkv, hd, page = cuda_device, 4, 2, 64, 8
+    pool = Pool([page] * 6, nkv, hd, page, dev, fill=3.0)
+    table = pool.dev_table.clone()
+    table[3, 0] = -1
+    table[4, 0] = pool.pages
+    #        cached, padding, past the table, page -1, page past the pool, sequences that are not there
+    pos = torch.tensor([5, -1, page, 2, 2, 1, 1], dtype=torch.int32, device=dev)
+    seq = torch.tensor([0, 1, 2, 3, 4, 6, -1], dtype=torch.int32, device=dev)
+    x = _bf((7, (nq + 2 * nkv) * hd), 4).to(dev)
+    q_out = torch.full((7, nq * hd), 9.0, dtype=torch.bfloat16, device=dev)
+    kc0, vc0 = pool.k.clone(), pool.v.clone()
+    q, k = ops.rope_paged_kv(x, pos, table, pool.k, pool.v, nq, _inv(hd).to(dev), seq_ids=seq, q_out=q_out, want_k=True)
+    assert q is q_out and bool((q[1] == 9.0).all())
+    y, tol = rope(x.cpu().view(7, -1, hd)[:, :nq + nkv], pos.cpu().clamp(min=0), _inv(hd))
+    live = [0, 2, 3, 4, 5, 6]
+    assert_within(q.view(7, nq, hd)[live], y[live, :nq], tol[live, :nq])
+    at = int(pool.table[0, 0])
+    kc0[at, :, 5] = k[0]
+    vc0[at, :, 5] = x.view(7, -1, hd)[0, nq + nkv:]
+    assert _same(pool.k, kc0) and _same(pool.v, vc0)
+
+
+# ------------------------------------------------------------------ paged attention
+def _paged(dev, lens, nq, nkv, hd, page, seed=0, scaling=None, std=1.5, strided=False, workspace="own", garbage=True,
+           **kw):
+    """Runs paged_attention on random sequences and checks every row; the rows of each last page
+    behind the sequence hold NaN."""
+    from moeinfra_amd import ops
+
+    pool = Pool(lens, nkv, hd, page, dev, seed=seed, fill=math.nan if garbage else 0.0, **kw)
+    ks = [_bf((n, nkv, hd), 100 + seed + i) for i, n in enumerate(lens)]
+    vs = [_bf((n, nkv, hd), 200 + seed + i) for i, n in enumerate(lens)]
+    for i, (k, v) in enumerate(zip(ks, vs)):
+        pool.put(i, k, v)
+    q = _bf((len(lens), nq, hd), seed, std)
+    qd = q.to(dev)
+    if strided:
+        qd = torch.full((len(lens), nq + 2, hd), math.nan, dtype=torch.bfloat16, device=dev)[:, :nq]
+        qd.copy_(q)
+    ws = ops.paged_attention_workspace(len(lens), nq, nkv, hd, dev) if workspace == "own" else workspace
+    out = ops.paged_attention(qd, pool.k, pool.v, pool.dev_table, torch.tensor(lens, dtype=torch.int32, device=dev),
+                              scaling=scaling, workspace=ws)
+    _check_paged(out, q, ks, vs, nkv, hd ** -0.5 if scaling is None else scaling)
+    return out, ws
+
+
+def _check_paged(out, q, ks, vs, nkv, scaling):
+    grp = q.shape[1] // nkv
+    for i, (k, v) in enumerate(zip(ks, vs)):
+        for h in range(nkv):
+            want, tol = attention(q[i, h * grp:(h + 1) * grp], k[:, h], v[:, h], scaling)
+            assert_within(out[i, h * grp:(h + 1) * grp], want, tol, f"sequence {i} of {k.shape[0]} keys, head {h}")
+
+
+LENS = [0, 1, 7, 8, 9, 31, 32, 33, 127, 128, 129, 255, 300, 0, 513, 1000]
+
+
+@pytest.mark.parametrize("nq,nkv,hd,page", [
+    (32, 8, 128, 16), (8, 2, 64, 8), (4, 4, 128, 64), (16, 1, 128, 32), (20, 1, 64, 16), (40, 2, 128, 8),
+    (8, 4, 256, 128), (17, 1, 256, 16), (3, 3, 64, 4096), (33, 1, 128, 64)])
+def test_paged_attention(cuda_device, nq, nkv, hd, page):
+    print(f"paged attention {nq}/{nkv} heads of {hd}, pages of {page}", flush=True)
+    _paged(cuda_device, LENS, nq, nkv, hd, page, seed=nq + hd, strided=nq % 2 == 0, interleaved=page == 16)
+
+
+@pytest.mark.parametrize("lens", [[1], [33], [700], [5000], [20000, 3, 0, 900], [257] * 70, [40] * 300])
+def test_paged_attention_batches(cuda_device, lens):
+    # A lone sequence shared by many workgroups, ragged batches, more sequences than a wave has lanes.
+    print(f"paged attention of {len(lens)} sequences", flush=True)
+    _paged(cuda_device, lens, 8, 2, 128, 16, seed=len(lens))
+
+
+def test_paged_attention_without_workspace_and_reuse(cuda_device):
+    from moeinfra_amd import ops
+
+    dev = cuda_device
+    a, _ = _paged(dev, [900, 3000, 5], 8, 2, 64, 16, seed=5, workspace=None)
+    # One workspace for batches of different sizes and heads, one after the other; same bits.
+    ws = ops.paged_attention_workspace(64, 32, 8, 128, dev)
+    b, _ = _paged(dev, [900, 3000, 5], 8, 2, 64, 16, seed=5, workspace=ws)
+    _paged(dev, [3000] * 9, 32, 8, 128, 16, seed=6, workspace=ws)
+    c, _ = _paged(dev, [900, 3000, 5], 8, 2, 64, 16, seed=5, workspace=ws)
+    assert _same(a, b) and _same(a, c)
+    assert not bool(ws[:65536].any())
+
+
+def test_paged_attention_missing_pages_and_lengths(cuda_device):
+    """Pages that the cache does not have weigh nothing; lengths clamp to the table."""
+    from moeinfra_amd import ops
+
+    dev, nq, nkv, hd, page = cuda_device, 8, 2, 128, 16
+    lens = [100, 100, 64, 64, 40]
+    pool = Pool(lens, nkv, hd, page, dev, seed=8, fill=math.nan)
+    ks, vs = [_bf((n, nkv, hd), 300 + n + i) for i, n in enumerate(lens)], [_bf((n, nkv, hd), 400 + n + i) for i, n in enumerate(lens)]
+    for i, (k, v) in enumerate(zip(ks, vs)):
+        pool.put(i, k, v)
+    table = pool.dev_table.clone()
+    table[0, 2] = -7                                   # keys 32 .. 47
+    table[1, 0] = pool.pages                           # keys 0 .. 15
+    table[1, 6] = -1                                   # and the last ones
+    table[2, :] = -1                                   # all of them
+    keep = [[j for j in range(100) if not 32 <= j < 48], list(range(16, 96)), [], list(range(64)), []]
+    said = torch.tensor([100, 100, 64, 64, -3], dtype=torch.int32, device=dev)
+    q = _bf((5, nq, hd), 9, 1.5)
+    out = ops.paged_attention(q.to(dev), pool.k, pool.v, table, said)
+    _check_paged(out, q, [k[s] for k, s in zip(ks, keep)], [v[s] for v, s in zip(vs, keep)], nkv, hd ** -0.5)
+    # A length past the table: all of its pages.
+    full = ops.paged_attention(q[:1].to(dev), pool.k, pool.v, pool.dev_table[3:4, :4].contiguous(),
+                               torch.tensor([1 << 30], dtype=torch.int32, device=dev))
+    _check_paged(full, q[:1], ks[3:4], vs[3:4], nkv, hd ** -0.5)
+
+
+def test_paged_attention_extremes(cuda_device):
+    """Scores of every size: all equal, far apart, near the largest fp32 value."""
+    from moeinfra_amd import ops
+
+    dev, nq, nkv, hd, page, n = cuda_device, 4, 1, 64, 16, 200
+    pool = Pool([n], nkv, hd, page, dev, seed=10, fill=math.nan)
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    v = _bf((n, nkv, hd), 11)
+    for big in (0.0, 30.0, 1.5e18):
+        k = _bf((n, nkv, hd), 12)
+        k[:, 0, 1:] = 0
+        q = torch.zeros((1, nq, hd), dtype=torch.bfloat16)
+        q[0, :, 0] = torch.tensor([big, -big, big / 2, 1.0])
+        if big > 1e9:  # scores up to 3.2e38
+            k[:, 0, 0] = torch.linspace(-2.1e20, 2.1e20, n).to(torch.bfloat16)
+        pool.put(0, k, v)
+        out = ops.paged_attention(q.to(dev), pool.k, pool.v, pool.dev_table, lens, scaling=1.0)
+        want, tol = attention(q[0], k[:, 0], v[:, 0], 1.0)
+        if big > 1e9:
+            # Neighbouring keys are 1e36 apart in score: one key (or several with the same bf16 key)
+            # has all the weight, whatever fp32 rounds.
+            tol = 2.0 ** -8 * (want.abs() + v.double().abs().amax()) + 0 * tol
+            assert not torch.isnan(out).any()
+            rows = [0, 1, 2]
+            assert_within(out[0, rows], want[rows], tol[rows])
+        else:
+            assert_within(out[0], want, tol)
+
+
+def test_paged_attention_offsets_past_32_bits(cuda_device):
+    """A pool whose far pages lie more than 2^32 bytes (and 2^31 values) into the tensors."""
+    from moeinfra_amd import ops
+
+    dev, nq, nkv, hd, page, n = cuda_device, 32, 8, 128, 128, 300
+    pages = (1 << 31) // (nkv * page * hd) + 9
+    kc = torch.empty((pages, nkv, page, hd), dtype=torch.bfloat16, device=dev)
+    vc = torch.empty_like(kc)
+    ids = [pages - 1, 0, pages - 2]
+    k, v, q = _bf((n, nkv, hd), 20), _bf((n, nkv, hd), 21), _bf((1, nq, hd), 22, 1.5)
+    for c, at in enumerate(ids):
+        m = min(page, n - c * page)
+        kc[at, :, :m] = k[c * page:c * page + m].to(dev).transpose(0, 1)
+        vc[at, :, :m] = v[c * page:c * page + m].to(dev).transpose(0, 1)
+    table = torch.tensor([ids], dtype=torch.int32, device=dev)
+    out = ops.paged_attention(q.to(dev), kc, vc, table, torch.tensor([n], dtype=torch.int32, device=dev))
+    _check_paged(out, q, [k], [v], nkv, hd ** -0.5)
+    # ... and a token written there.
+    x = _bf((1, (nq + 2 * nkv) * hd), 23).to(dev)
+    pos = torch.tensor([n], dtype=torch.int32, device=dev)
+    _, kr = ops.rope_paged_kv(x, pos, table, kc, vc, nq, _inv(hd).to(dev), want_k=True)
+    assert _same(kc[ids[2], :, n % page], kr[0])
+    assert _same(vc[ids[2], :, n % page], x.view(1, -1, hd)[0, nq + nkv:])
