@@ -364,6 +364,19 @@ int moe_paged_attention_bf16(const void *q, int64_t q_stride, const void *k_cach
                              int32_t head_dim, float scaling, void *out, void *workspace,
                              int64_t workspace_bytes, void *stream);
 
+/* moe_packed_attention_bf16: causal attention of whole sequences packed one behind the other:
+ * sequence b is tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1], not decreasing, inside
+ * [0, T]; equal neighbours: an empty sequence), and a token sees its own sequence up to itself.  q
+ * [T, n_q, head_dim], k and v [T, n_kv, head_dim], their rows q_stride / k_stride / v_stride values
+ * apart (slices of a projection's output); out [T, n_q * head_dim].  fp32 scores q.k * scaling and
+ * softmax, the weights rounded to bf16 before their sum (fp32) with v.  Rows of no sequence are left
+ * as they were.  head dim 64, 128 or 256. */
+int moe_packed_attention_bf16(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                              const void *v, int64_t v_stride, int64_t T,
+                              const void *cu_seqlens_i32, int64_t B, int32_t n_q_heads,
+                              int32_t n_kv_heads, int32_t head_dim, float scaling, void *out,
+                              void *stream);
+
 #ifdef __cplusplus
 }
 #endif

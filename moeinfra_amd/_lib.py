@@ -89,6 +89,8 @@ SIGNATURES = {
     "moe_paged_attention_workspace_bytes": ([_i64, _i32, _i32, _i32], _i64),
     "moe_paged_attention_bf16": ([_vp, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32,
                                   ctypes.c_float, _vp, _vp, _i64, _vp], ctypes.c_int),
+    "moe_packed_attention_bf16": ([_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _i32, _i32,
+                                   ctypes.c_float, _vp, _vp], ctypes.c_int),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,390 @@
+// Causal attention of whole prompts of different lengths, packed one behind the other, grouped
+// query heads: every token sees the keys of its own sequence up to its own.  The counterpart of
+// prefill_attention (attention.hip) for many sequences, before (or without) a cache.
+//
+//   o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scaling * q.k_j
+//
+// in fp32 with a running reference m; the weights are rounded to bf16 as an operand of the second
+// product (half a step, 2^-8 of a weight), their sum is not.
+#include <type_traits>
+
+#include "common.h"
+
+namespace moe {
+namespace {
+
+constexpr int kPkRows = 32;  // rows per wave
+constexpr float kPkLog2e = 1.44269504088896341f;
+// The running reference may lag the maximum by this much (in powers of two) before the sums are
+// rescaled: weights up to 2^8, which fp32 sums and bf16 weights carry without loss.
+constexpr float kPkLag = 8.0f;
+constexpr float kPkHuge = 268435456.0f;  // 2^28: half a step of m is 2^3
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct PkArgs {
+  const uint16_t *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  const int32_t *cu;
+  int T, B, nq, nkv, grp;
+  float scaling;
+  uint16_t *out;
+};
+
+// Swizzles: 16-byte piece p of K row r lies at p ^ pk_kx(r), so that the 32 rows that a read of one
+// piece touches spread over all banks; piece p of V row r at p ^ pk_vx(r), so that four keys' 64
+// bytes (a transposing read) do.
+template <int HD>
+__device__ __forceinline__ uint32_t pk_kx(uint32_t r) {
+  return HD == 64 ? (r >> 1) & 7 : r & 15;
+}
+template <int HD>
+__device__ __forceinline__ uint32_t pk_vx(uint32_t r) {
+  return HD == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
+}
+
+// Four bf16 values of one column from four rows: lane i of 16 reads 8 bytes of row i / 4 and gets
+// column i of the four rows' 16 columns.
+__device__ __forceinline__ uint2 pk_read_tr(const uint8_t *p) {
+  const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+  return __builtin_bit_cast(uint2, v);
+}
+
+// 64 lanes' 16 bytes each from memory into LDS at dst + 16 * lane, without registers.  (In asm, as
+// the compiler would wait for all of them before the next transposing read of the other plane; the
+// caller waits for vmcnt(0) and a barrier before it reads dst.)
+__device__ __forceinline__ void pk_load_lds(const void *src, const uint8_t *dst) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)dst);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src)
+               : "memory", "m0");
+}
+
+// A workgroup's rows: tile `tile` (of `rows` rows of token x query head of the group) of the
+// sequence of tokens tok0 .. tok0 + len - 1.  Item w of a KV head is the w-th of all tiles in
+// falling order of their tile number, i.e. of their keys, so that the longest start first
+// whatever order the sequences have.  Each wave finds it alone: N(L), the tiles numbered L and
+// above, by a sum over the batch, and the level L with N(L + 1) <= w < N(L) by bisection.
+struct PkItem {
+  int tok0, len, tile;
+};
+
+__device__ __forceinline__ bool pk_item(const PkArgs &a, int rows, int w, int lane, PkItem &it) {
+  auto cut = [&](int i) { return min(max(a.cu[i], 0), a.T); };
+  auto tiles = [&](int i) {
+    const int n = i < a.B ? max(cut(i + 1) - cut(i), 0) : 0;
+    return (int)(((int64_t)n * a.grp + rows - 1) / rows);
+  };
+  const int t0 = tiles(lane);  // of the first 64 sequences
+  // (Counts are exact in fp32: a batch has fewer than 2^24 tiles.)
+  auto above = [&](int level) {
+    float n[1] = {(float)max(t0 - level, 0)};
+    lane_groups_reduce<false>(n, kWave);
+    float sum = n[0];
+    for (int i0 = kWave; i0 < a.B; i0 += kWave) {
+      float more[1] = {(float)max(tiles(i0 + lane) - level, 0)};
+      lane_groups_reduce<false>(more, kWave);
+      sum += more[0];
+    }
+    return __builtin_amdgcn_readfirstlane((int)sum);
+  };
+  if (w >= above(0)) return false;
+  int lo = 0, hi = (int)(((int64_t)a.T * a.grp + rows - 1) / rows);  // N(lo) > w, N(hi) <= w
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (above(mid) > w)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  int i = w - above(lo + 1);  // of the sequences that have a tile lo
+  for (int i0 = 0; i0 < a.B; i0 += kWave) {
+    const int t = i0 == 0 ? t0 : tiles(i0 + lane);
+    uint64_t has = __ballot(t > lo);
+    const int n = __popcll(has);
+    if (i < n) {
+      for (; i > 0; --i) has &= has - 1;
+      const int s = i0 + __builtin_ctzll(has);
+      it.tok0 = cut(s);
+      it.len = cut(s + 1) - it.tok0;
+      it.tile = lo;
+      return true;
+    }
+    i -= n;
+  }
+  return false;
+}
+
+// Rows r0 .. r1 - 1 (at most 32) of a sequence without matrix products, a row at a time, a key per
+// lane: each row reads the V rows that it sees and no others.
+template <int HD>
+__device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride, const uint16_t *k, int64_t k_stride,
+                                            const uint16_t *v, int64_t v_stride, int r0, int r1, int grp, int nq,
+                                            float scaling, uint16_t *out, int lane) {
+  for (int r = r0; r < r1; ++r) {
+    const int t = r / grp, g = r - t * grp;
+    const uint16_t *qr = q + t * q_stride + (int64_t)g * HD;
+    float m = -INFINITY, l = 0.0f, o[HD / kWave];
+    for (int e = 0; e < HD / kWave; ++e) o[e] = 0.0f;
+    for (int k0 = 0; k0 <= t; k0 += kWave) {
+      const int j = min(k0 + lane, t);
+      const uint16_t *kr = k + j * k_stride;
+      float d = 0.0f;
+      for (int i = 0; i < HD; ++i) d = fmaf(bf16_to_f32(qr[i]), bf16_to_f32(kr[i]), d);
+      const float x = k0 + lane <= t ? d * scaling : -INFINITY;
+      float mx[1] = {x};
+      lane_groups_reduce<true>(mx, kWave);
+      const float mn = fmaxf(m, mx[0]);
+      const float mref = mn == -INFINITY ? 0.0f : mn;
+      const float alpha = __builtin_amdgcn_exp2f((m - mref) * kPkLog2e);
+      const float p = __builtin_amdgcn_exp2f((x - mref) * kPkLog2e);
+      m = mn;
+      l = l * alpha + wave_sum(p);
+      for (int e = 0; e < HD / kWave; ++e) o[e] *= alpha;
+      for (int i = 0; i < min(kWave, t + 1 - k0); ++i) {
+        const float pi = bf16r(__shfl(p, i, kWave));
+        const uint16_t *vr = v + (k0 + i) * v_stride;
+        for (int e = 0; e < HD / kWave; ++e) o[e] = fmaf(pi, bf16_to_f32(vr[e * kWave + lane]), o[e]);
+      }
+    }
+    uint16_t *dst = out + ((int64_t)t * nq + g) * HD;
+    for (int e = 0; e < HD / kWave; ++e) dst[e * kWave + lane] = f32_to_bf16(l == 0.0f ? 0.0f : o[e] / l);
+  }
+}
+
+// Rows of one KV head are (token, query head of its group), r = token * group + head, so that the
+// group's heads share the K and V tiles.  A workgroup takes 32 rows per wave and walks the keys in
+// tiles, two LDS planes deep: while a tile is multiplied, the next one is on its way from
+// memory straight into the other plane.
+//
+//   S^T = K Q^T        lane (row of queries l % 32) holds 16 keys of its row per 32-key half
+//   O^T += V^T P^T     P of a lane is the B operand as it stands; V is read transposed
+//
+// A weight is 2^(s c - m) by one fused multiply-add, c = scaling * log2(e), m a rounded max s c: what
+// the rounding of m leaves cancels against the sum, as long as 2 to its power is in range.  Rows with
+// references past kPkHuge (and products that overflow) are done again without.
+template <int HD, int NW>
+__global__ void __launch_bounds__(NW *kWave, HD == 256 ? 1 : 2)
+packed_attention_kernel(const PkArgs a) {
+  constexpr int kRows = NW * kPkRows;
+  constexpr int kKeys = HD == 256 ? 32 : 64;         // keys per tile (64 of 256 dims spill registers)
+  constexpr int kST = kKeys / 32;
+  constexpr int kPlane = kKeys * HD * 2;           // bytes of a K or V tile
+  constexpr int kChunks = kPlane / 1024 / NW;        // 1 KB loads per wave and tile of K (and of V)
+  constexpr int kDT = HD / 32;                       // 32-dim output tiles
+  constexpr int kRowB = HD * 2;
+  static_assert(kChunks >= 1, "a wave loads a KB at least");
+  __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2 * kPlane];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int li = lane & 31, hh = lane >> 5;
+  // The KV head is the fast index: with a multiple of 8 heads, a head's workgroups share an XCD's L2.
+  const int w = (int)(blockIdx.x / (unsigned)a.nkv), kvh = (int)(blockIdx.x - (unsigned)w * a.nkv);
+  PkItem it;
+  if (!pk_item(a, kRows, w, lane, it)) return;  // the same for the whole workgroup
+  const int rows = it.len * a.grp;              // of the sequence (T * group < 2^31)
+  const int row0 = it.tile * kRows + wave * kPkRows;
+  const int r = min(row0 + li, rows - 1);
+  const int t = r / a.grp;                      // token of this lane's row
+  const int limit = t + 1;                      // it sees keys 0 .. limit - 1
+  const int head = kvh * a.grp + (r - t * a.grp);
+  // Keys of the wave's first and last row, and of the workgroup's last row.
+  const int first = min(row0, rows - 1) / a.grp + 1;
+  const int last = row0 < rows ? min(row0 + kPkRows - 1, rows - 1) / a.grp + 1 : 0;
+  const int nkeys = min(it.tile * kRows + kRows - 1, rows - 1) / a.grp + 1;
+  const int ntile = (nkeys + kKeys - 1) / kKeys;
+
+  // Q as the B operand: column li, dims 16 s + 8 hh .. + 7.  A negative scaling goes into its signs,
+  // one of zero into its values (masked scores, -inf, are multiplied too).
+  const uint32_t flip = a.scaling < 0.0f ? 0x80008000u : 0u, keep = a.scaling == 0.0f ? 0u : ~0u;
+  const float scaling = a.scaling == 0.0f ? 1.0f : fabsf(a.scaling);
+  const float c = scaling * kPkLog2e;
+  u32x4 qf[HD / 16];
+  {
+    const uint16_t *qr = a.q + (it.tok0 + t) * a.q_stride + (int64_t)head * HD + 8 * hh;
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) {
+      qf[s] = *reinterpret_cast<const u32x4 *>(qr + 16 * s);
+      qf[s] = (qf[s] ^ flip) & keep;
+    }
+  }
+  // Loads: 1 KB of a tile per instruction; lane l fills the 16 bytes at 16 l of it, which belong to
+  // row (1 KB chunk * 1024 + 16 l) / row bytes, and fetches the piece that the swizzle puts there.
+  // Rows past the sequence's last key repeat it (masked below).
+  const uint16_t *const kb = a.k + it.tok0 * a.k_stride + (int64_t)kvh * HD;
+  const uint16_t *const vb = a.v + it.tok0 * a.v_stride + (int64_t)kvh * HD;
+  auto load = [&](int tile, uint8_t *plane) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int at = (wave + i * NW) * 1024 + 16 * lane;
+      const uint32_t row = at / kRowB, piece = at % kRowB / 16;
+      const int64_t key = min(tile * kKeys + (int)row, nkeys - 1);
+      pk_load_lds(kb + key * a.k_stride + 8 * (piece ^ pk_kx<HD>(row)), plane + (wave + i * NW) * 1024);
+      pk_load_lds(vb + key * a.v_stride + 8 * (piece ^ pk_vx<HD>(row)), plane + kPlane + (wave + i * NW) * 1024);
+    }
+  };
+  f32x16 acc[kDT];
+#pragma unroll
+  for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[dt][v] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  bool huge = false;
+  // Operand reads: K row 32 st + li, piece 2 s + hh.  V: lane group's dims 32 dt + 16 (l / 16 % 2) ..
+  // + 15 of keys 16 s + 8 n + 4 hh .. + 3; this lane's 8 bytes are in key l % 16 / 4 of the four.
+  const uint32_t krd = li * kRowB, kx = 16 * (hh ^ pk_kx<HD>(li));
+  const uint32_t vkey = 4 * hh + ((lane & 15) >> 2);
+  const uint32_t vrd = kPlane + vkey * kRowB + 8 * (lane & 1);
+  const uint32_t vx = 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ pk_vx<HD>(vkey));
+  load(0, s_kv[0]);
+  for (int n = 0; n < ntile; ++n) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // tile n is in its plane, and the other plane is no longer read
+    if (n + 1 < ntile) load(n + 1, s_kv[(n + 1) & 1]);
+    const int k0 = n * kKeys;
+    if (k0 >= last) continue;  // none of this wave's rows sees it
+    const uint8_t *buf = s_kv[n & 1];
+    auto tile = [&](auto edge_c) __attribute__((always_inline)) {
+      constexpr bool kEdge = decltype(edge_c)::value;
+      // (Addresses are a XOR with a constant away from these: computed, not held in registers.)
+      uint32_t ka = kx, va = vx;
+      asm volatile("" : "+v"(ka), "+v"(va));
+      f32x16 sc[kST];
+#pragma unroll
+      for (int st = 0; st < kST; ++st)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sc[st][v] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < HD / 16; ++s)
+#pragma unroll
+        for (int st = 0; st < kST; ++st) {
+          const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + krd + (ka ^ (32 * s)) + 32 * st * kRowB);
+          sc[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
+                                                           __builtin_bit_cast(bf16x8, qf[s]), sc[st], 0, 0, 0);
+        }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int st = 0; st < kST; ++st)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          if constexpr (kEdge)
+            sc[st][v] = k0 + 32 * st + 8 * (v >> 2) + 4 * hh + (v & 3) < limit ? sc[st][v] : -INFINITY;
+          mx = fmaxf(mx, sc[st][v]);
+        }
+      mx = op_xor32<true>(mx) * c;
+      if (__any(mx > m + kPkLag)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+        m = mn;
+        huge |= fabsf(mn) > kPkHuge && mn != -INFINITY;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
+      }
+      const float mref = m == -INFINITY ? 0.0f : m;  // before a row's first key above -inf
+      u32x4 pf[2 * kST];
+#pragma unroll
+      for (int s = 0; s < 2 * kST; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int v = 8 * (s & 1) + 2 * j;
+          const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v], c, -mref));
+          const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v + 1], c, -mref));
+          l += e0 + e1;
+          pf[s][j] = pack_bf16x2(e0, e1);
+        }
+#pragma unroll
+      for (int s = 0; s < 2 * kST; ++s)
+#pragma unroll
+        for (int dt = 0; dt < kDT; ++dt) {
+          const uint8_t *p = buf + vrd + (va ^ (64 * dt)) + 16 * s * kRowB;
+          const uint2 x0 = pk_read_tr(p), x1 = pk_read_tr(p + 8 * kRowB);
+          const u32x4 x = {x0.x, x0.y, x1.x, x1.y};
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
+                                                            __builtin_bit_cast(bf16x8, pf[s]), acc[dt], 0, 0, 0);
+        }
+    };
+    if (k0 + kKeys <= first)
+      tile(std::false_type{});
+    else
+      tile(std::true_type{});
+  }
+  if (row0 >= rows) return;
+  l = op_xor32<false>(l);
+  // A row that stops inside a tile meets V rows that it does not see with weights of zero: an
+  // infinity or NaN there would come through.  Where a result is not finite, look at those rows,
+  // and if one of them holds such a value, take this wave's rows one by one.
+  bool bad = false;
+#pragma unroll
+  for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) bad |= !(fabsf(acc[dt][v]) <= 3.4028235e38f);
+  if (__any(bad | huge)) {
+    bool again = huge;
+    const int end = min((last + kKeys - 1) / kKeys * kKeys, nkeys);
+    for (int j = first; j < end; ++j)
+      for (int d = lane; d < HD; d += kWave) again |= (vb[j * a.v_stride + d] & 0x7f80u) == 0x7f80u;
+    if (__any(again)) {
+      pk_rows_scalar<HD>(a.q + it.tok0 * a.q_stride + (int64_t)kvh * a.grp * HD, a.q_stride, kb, a.k_stride, vb,
+                         a.v_stride, row0, min(row0 + kPkRows, rows), a.grp, a.nq, a.scaling,
+                         a.out + ((int64_t)it.tok0 * a.nq + kvh * a.grp) * HD, lane);
+      return;
+    }
+  }
+  if (row0 + li < rows) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t *orow = a.out + ((int64_t)(it.tok0 + t) * a.nq + head) * HD;
+#pragma unroll
+    for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4)
+        *reinterpret_cast<uint2 *>(orow + 32 * dt + 2 * v + 4 * hh) =
+            make_uint2(pack_bf16x2(acc[dt][v] * inv, acc[dt][v + 1] * inv),
+                       pack_bf16x2(acc[dt][v + 2] * inv, acc[dt][v + 3] * inv));
+  }
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_packed_attention_bf16(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                                         const void *v, int64_t v_stride, int64_t T, const void *cu_seqlens_i32,
+                                         int64_t B, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                         float scaling, void *out, void *stream) {
+  MOE_REQUIRE(n_q_heads > 0 && n_kv_heads > 0 && n_q_heads % n_kv_heads == 0,
+              "query heads must be a multiple of the KV heads");
+  MOE_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "head dim must be 64, 128 or 256 (got %d)", head_dim);
+  MOE_REQUIRE(scaling == scaling, "scaling is NaN");
+  const int32_t grp = n_q_heads / n_kv_heads;
+  MOE_REQUIRE(T >= 0 && B >= 0 && B <= (1 << 20) && n_q_heads <= (1 << 16) &&
+                  T * grp <= 0x7fffffff - 1024 && T <= 0x7fffffff,
+              "bad sizes");
+  const int64_t qrow = (int64_t)n_q_heads * head_dim, krow = (int64_t)n_kv_heads * head_dim;
+  MOE_REQUIRE((q_stride | k_stride | v_stride) % 8 == 0 &&
+                  (T <= 1 || (q_stride >= qrow && k_stride >= krow && v_stride >= krow)),
+              "rows of q, k and v must be 16-byte aligned and apart");
+  if (T == 0 || B == 0) return MOE_STATUS_OK;
+  MOE_REQUIRE(q && k && v && cu_seqlens_i32 && out, "null pointer");
+  MOE_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0 && (uintptr_t)out % 8 == 0,
+              "q, k and v must be 16-byte aligned, out 8-byte");
+  const int64_t ob = 2 * T * qrow;
+  MOE_REQUIRE(!moe::ranges_overlap(out, ob, q, 2 * (q_stride * (T - 1) + qrow)) &&
+                  !moe::ranges_overlap(out, ob, k, 2 * (k_stride * (T - 1) + krow)) &&
+                  !moe::ranges_overlap(out, ob, v, 2 * (v_stride * (T - 1) + krow)),
+              "out must not overlap q, k or v");
+  moe::PkArgs a{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, q_stride, k_stride, v_stride,
+                (const int32_t *)cu_seqlens_i32, (int)T, (int)B, n_q_heads, n_kv_heads, grp, scaling, (uint16_t *)out};
+  // Workgroups of 8 waves where they fill the device; else of 4, twice as many.
+  auto grid = [&](int rows) { return (T * grp / rows + (B < T ? B : T)) * n_kv_heads; };
+  const bool wide = head_dim != 256 && T * grp / (8 * moe::kPkRows) * n_kv_heads >= moe::device_cu_count();
+  const int64_t g = grid(wide ? 8 * moe::kPkRows : 4 * moe::kPkRows);
+  MOE_REQUIRE(g <= 0x7fffffff, "bad sizes");
+  auto kern = head_dim == 64    ? (wide ? moe::packed_attention_kernel<64, 8> : moe::packed_attention_kernel<64, 4>)
+              : head_dim == 128 ? (wide ? moe::packed_attention_kernel<128, 8> : moe::packed_attention_kernel<128, 4>)
+                                : moe::packed_attention_kernel<256, 4>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)g), dim3((wide ? 8 : 4) * moe::kWave), 0, (hipStream_t)stream, a);
+  MOE_LAUNCH_CHECK();
+  return MOE_STATUS_OK;
+}

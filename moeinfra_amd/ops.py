@@ -415,3 +415,30 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             B, nq, nkv, hd, hd ** -0.5 if scaling is None else float(scaling), out.data_ptr(), workspace.data_ptr(),
             workspace.numel())
     return out
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scaling: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of whole sequences packed one behind the other: sequence b is tokens
+    ``cu_seqlens[b] .. cu_seqlens[b + 1] - 1`` (int32 [B + 1], not decreasing) of ``q`` bf16
+    [T, q heads, head dim] and ``k``, ``v`` [T, kv heads, head dim], whose rows may lie apart (slices of
+    a projection's output); bf16 [T, q heads, head dim].  ``scaling`` defaults to head_dim ** -0.5.
+    Tokens of no sequence are left as they were in ``out`` (without one they hold anything)."""
+    dev = q.device
+    strides = [_require_rows(t, name, dev, 3) for t, name in ((q, "q"), (k, "k"), (v, "v"))]
+    T, nq, hd = q.shape
+    if k.shape != v.shape or k.shape[0] != T or k.shape[2] != hd:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
+    _require(cu_seqlens, "cu_seqlens", torch.int32, dev)
+    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1:
+        raise ValueError(f"cu_seqlens must be [sequences + 1] (got {tuple(cu_seqlens.shape)})")
+    if out is None:
+        out = torch.empty((T, nq, hd), dtype=torch.bfloat16, device=dev)
+    else:
+        _require(out, "out", torch.bfloat16, dev)
+        if out.numel() != T * nq * hd:
+            raise ValueError("out has the wrong number of elements")
+    _launch(lib().moe_packed_attention_bf16, "packed_attention", dev, q.data_ptr(), strides[0], k.data_ptr(),
+            strides[1], v.data_ptr(), strides[2], T, cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, nq, k.shape[1],
+            hd, hd ** -0.5 if scaling is None else float(scaling), out.data_ptr())
+    return out

@@ -240,3 +240,119 @@ def test_paged_attention_offsets_past_32_bits(cuda_device):
     _, kr = ops.rope_paged_kv(x, pos, table, kc, vc, nq, _inv(hd).to(dev), want_k=True)
     assert _same(kc[ids[2], :, n % page], kr[0])
     assert _same(vc[ids[2], :, n % page], x.view(1, -1, hd)[0, nq + nkv:])
+
+
+# ------------------------------------------------------------------ packed attention
+def _packed(dev, lens, nq, nkv, hd, seed=0, scaling=None, std=1.5, gap=0, strided=True, change=None):
+    """Runs packed_attention on sequences that start behind `gap` tokens and end `gap` before the
+    last one, and checks every row; rows outside hold NaN and are left alone."""
+    from moeinfra_amd import ops
+
+    cuts = [gap]
+    for n in lens:
+        cuts.append(cuts[-1] + n)
+    T = cuts[-1] + gap
+    q, k, v = _bf((T, nq, hd), seed, std), _bf((T, nkv, hd), seed + 1), _bf((T, nkv, hd), seed + 2)
+    if change is not None:
+        change(q, k, v, cuts)
+    outside = torch.ones(T, dtype=torch.bool)
+    outside[cuts[0]:cuts[-1]] = False
+    for t in (q, k, v):
+        t[outside] = math.nan
+    dq, dk, dv = q.to(dev), k.to(dev), v.to(dev)
+    if strided:  # slices of one projection's output
+        row = torch.cat((q.reshape(T, -1), k.reshape(T, -1), v.reshape(T, -1)), dim=1).to(dev)
+        dq = row[:, :nq * hd].view(T, nq, hd)
+        dk = row[:, nq * hd:(nq + nkv) * hd].view(T, nkv, hd)
+        dv = row[:, (nq + nkv) * hd:].view(T, nkv, hd)
+    out = torch.full((T, nq, hd), 5.0, dtype=torch.bfloat16, device=dev)
+    s = hd ** -0.5 if scaling is None else scaling
+    ops.packed_attention(dq, dk, dv, torch.tensor(cuts, dtype=torch.int32, device=dev), scaling=scaling, out=out)
+    assert bool((out[outside.to(dev)] == 5.0).all())
+    return out, q, k, v, cuts, s
+
+
+def _check_packed(out, q, k, v, cuts, scaling, rows=None):
+    nq, nkv = q.shape[1], k.shape[1]
+    for a, b in zip(cuts, cuts[1:]):
+        n = b - a
+        if n == 0:
+            continue
+        seen = torch.ones((n, n), dtype=torch.bool).tril()
+        for h in range(nq):
+            kh = h // (nq // nkv)
+            want, tol = attention(q[a:b, h], k[a:b, kh], v[a:b, kh], scaling, seen)
+            assert_within(out[a:b, h], want, tol, f"tokens {a} .. {b - 1}, head {h}")
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(32, 8, 128), (8, 2, 64), (4, 4, 128), (6, 2, 256), (16, 1, 64), (5, 1, 128),
+                                       (3, 3, 256), (40, 1, 64)])
+def test_packed_attention(cuda_device, nq, nkv, hd):
+    print(f"packed attention {nq}/{nkv} heads of {hd}", flush=True)
+    _check_packed(*_packed(cuda_device, [1, 0, 7, 64, 65, 0, 200, 1, 130], nq, nkv, hd, seed=nq, gap=3,
+                           strided=nq % 2 == 0))
+
+
+@pytest.mark.parametrize("lens", [[1], [2], [31], [257], [1500], [3] * 150, [0, 0, 5, 0], [700, 1, 900]])
+def test_packed_attention_batches(cuda_device, lens):
+    print(f"packed attention of {len(lens)} sequences", flush=True)
+    _check_packed(*_packed(cuda_device, lens, 4, 2, 128, seed=len(lens)))
+
+
+def test_packed_attention_wide_workgroups(cuda_device):
+    # Enough rows for the 8-wave workgroups: 32 heads, 64 and 128 dims.
+    for hd in (64, 128):
+        print(f"packed attention, wide, {hd}", flush=True)
+        _check_packed(*_packed(cuda_device, [700, 33, 1400], 32, 8, hd, seed=hd))
+
+
+def test_packed_attention_scalings(cuda_device):
+    for scaling in (1.0, -0.125, 0.0, 2.5):
+        print(f"scaling {scaling}", flush=True)
+        _check_packed(*_packed(cuda_device, [70, 129], 4, 2, 64, seed=3, scaling=scaling, std=0.5))
+
+
+def test_packed_attention_large_scores(cuda_device):
+    """Scores up to 3e38, where a product with log2(e) would overflow."""
+    def big(q, k, v, cuts):
+        q[:], k[:] = 0, 0
+        q[:, :, 0] = 1.5e18
+        k[:, :, 0] = torch.linspace(-2e20, 2e20, k.shape[0]).to(torch.bfloat16)[:, None]
+
+    for scaling in (1.0, 0.6):
+        out, q, k, v, cuts, s = _packed(cuda_device, [90], 2, 1, 64, seed=4, scaling=scaling, change=big)
+        # Keys are bf16 steps apart: the newest (of equal ones, all) has the weight.
+        for t in range(90):
+            same = (k[:t + 1, 0, 0] == k[t, 0, 0]).nonzero()[:, 0]
+            want = v[same, 0].double().mean(0)
+            tol = 2.0 ** -7 * v[same, 0].double().abs().mean(0) + 1e-6
+            assert_within(out[t], want.expand(2, -1), tol.expand(2, -1), f"token {t}")
+
+
+def test_packed_attention_infinities_stay_with_the_rows_that_see_them(cuda_device):
+    """An infinity or NaN in a value reaches the tokens from its own on, no earlier one and no other
+    sequence."""
+    lens = [100, 150, 40]
+
+    def spoil(q, k, v, cuts):
+        v[cuts[1] + 70, 0, 5] = math.inf
+        v[cuts[1] + 75, 1, 6] = math.nan
+        v[cuts[2], :, :] = math.nan
+
+    for hd in (64, 128, 256):
+        print(f"infinities, {hd}", flush=True)
+        out, q, k, v, cuts, s = _packed(cuda_device, lens, 4, 2, hd, seed=6, change=spoil)
+        o = out.float().cpu()
+        assert torch.isinf(o[cuts[1] + 70:cuts[2], :2, 5]).all()
+        assert torch.isnan(o[cuts[1] + 75:cuts[2], 2:, 6]).all()
+        assert torch.isnan(o[cuts[2]:cuts[3]]).all()
+        clean = lambda t: torch.where(t.isfinite(), t, 0.0).to(torch.bfloat16)
+        seen = torch.ones((150, 150), dtype=torch.bool).tril()
+        for h in range(4):
+            want, tol = attention(q[cuts[1]:cuts[2], h], k[cuts[1]:cuts[2], h // 2], clean(v[cuts[1]:cuts[2], h // 2]), s, seen)
+            keep = torch.ones((150, hd), dtype=torch.bool)
+            keep[70 if h < 2 else 75:, 5 if h < 2 else 6] = False
+            got = o[cuts[1]:cuts[2], h]
+            assert torch.isfinite(got[keep]).all()
+            assert_within(torch.where(keep, got, 0.0), torch.where(keep, want, 0.0), tol)
+        _check_packed(out, q, k, v, cuts[:2], s)

@@ -25,6 +25,13 @@ def _paged(**kw):
     return _lib.lib().moe_paged_attention_bf16(*a.values())
 
 
+def _packed(**kw):
+    a = dict(q=A, q_stride=512, k=B, k_stride=128, v=C, v_stride=128, T=10, cu=D, B=3, nq=8, nkv=2, hd=64,
+             scaling=0.125, out=E, stream=None)
+    a.update(kw)
+    return _lib.lib().moe_packed_attention_bf16(*a.values())
+
+
 REFUSED = [
     (_append, dict(hd=24), "head dim"),
     (_append, dict(hd=528), "head dim"),
@@ -69,6 +76,20 @@ REFUSED = [
     (_paged, dict(out=G + 64), "overlap"),
     (_paged, dict(ws=H, ws_bytes=4096), "workspace too small"),
     (_paged, dict(ws=H + 8, ws_bytes=1 << 30), "workspace must be"),
+    (_packed, dict(nq=9), "multiple"),
+    (_packed, dict(hd=80), "head dim"),
+    (_packed, dict(scaling=float("nan")), "NaN"),
+    (_packed, dict(T=-1), "bad sizes"),
+    (_packed, dict(T=1 << 30), "bad sizes"),
+    (_packed, dict(B=-1), "bad sizes"),
+    (_packed, dict(q_stride=504), "apart"),
+    (_packed, dict(k_stride=132), "aligned"),
+    (_packed, dict(v_stride=64), "apart"),
+    (_packed, dict(cu=None), "null"),
+    (_packed, dict(v=C + 8), "aligned"),
+    (_packed, dict(out=E + 4), "aligned"),
+    (_packed, dict(out=A + 1024), "overlap"),
+    (_packed, dict(out=C - 1024), "overlap"),
 ]
 
 
@@ -81,6 +102,8 @@ def test_refused_before_any_launch(call, change, needle):
 def test_empty_calls_do_nothing():
     assert _append(T=0, qkv=None, q=None, table=None, kc=None, vc=None) == 0
     assert _paged(B=0, q=None, out=None, lens=None) == 0
+    assert _packed(T=0, q=None, k=None, v=None, cu=None, out=None) == 0
+    assert _packed(B=0, cu=None) == 0
 
 
 def test_paged_attention_workspace_grows_with_the_batch():
@@ -97,5 +120,7 @@ def test_wrappers_take_gpu_tensors_only():
         ops.rope_paged_kv(bf(4, 768), i32(4), i32(4, 8), bf(32, 2, 16, 64), bf(32, 2, 16, 64), 8, torch.zeros(32))
     with pytest.raises(ValueError, match="GPU tensor"):
         ops.paged_attention(bf(4, 8, 64), bf(32, 2, 16, 64), bf(32, 2, 16, 64), i32(4, 8), i32(4))
+    with pytest.raises(ValueError, match="GPU tensor"):
+        ops.packed_attention(bf(4, 8, 64), bf(4, 2, 64), bf(4, 2, 64), i32(2))
     with pytest.raises(ValueError, match="invalid attention sizes"):
         ops.paged_attention_workspace(4, 8, 2, 96, "cpu")
