@@ -377,6 +377,22 @@ int moe_packed_attention_bf16(const void *q, int64_t q_stride, const void *k, in
                               int32_t n_kv_heads, int32_t head_dim, float scaling, void *out,
                               void *stream);
 
+/* moe_sample_tokens: the next token (int64) of each row of logits [B, V] (bf16, or fp32 with
+ * logits_f32 = 1; rows `stride` values apart, V up to 2^20) by a given random number u (fp32 [B], in
+ * [0, 1)).  Weights e^((x - max) / temperature); of the order by falling logit (equal ones: rising
+ * index) the first top_k are kept (0 and below, or V and above: all), of those the shortest prefix
+ * whose weights reach top_p of theirs (1 and above, NaN: all; one at least), of those the weights
+ * of min_p and above (the largest always); the token is the first index whose running sum of kept
+ * weights, by rising index, exceeds u times their sum.  Temperature 0 (and below, or NaN): the
+ * largest logit.  Logits of -inf and NaN are never drawn; a row of nothing else gives -1; next to +inf
+ * only other +inf weigh anything.  Each setting is an array with a value per row (fp32, top_k
+ * int32) or, where that is null, one value for all rows (refused outside its range).  Weights are
+ * summed as integers of 2^-43, so results do not depend on the order of any sum. */
+int moe_sample_tokens(const void *logits, int32_t logits_f32, int64_t stride, int64_t B, int64_t V,
+                      const void *u_f32, const void *temperature_f32, float temperature,
+                      const void *top_k_i32, int32_t top_k, const void *top_p_f32, float top_p,
+                      const void *min_p_f32, float min_p, void *token_i64, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

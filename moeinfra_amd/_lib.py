@@ -91,6 +91,8 @@ SIGNATURES = {
                                   ctypes.c_float, _vp, _vp, _i64, _vp], ctypes.c_int),
     "moe_packed_attention_bf16": ([_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i32, _i32, _i32,
                                    ctypes.c_float, _vp, _vp], ctypes.c_int),
+    "moe_sample_tokens": ([_vp, _i32, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _i32, _vp, ctypes.c_float,
+                           _vp, ctypes.c_float, _vp, _vp], ctypes.c_int),
 }
 
 _lock = threading.Lock()

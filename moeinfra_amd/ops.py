@@ -442,3 +442,46 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
             strides[1], v.data_ptr(), strides[2], T, cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, nq, k.shape[1],
             hd, hd ** -0.5 if scaling is None else float(scaling), out.data_ptr())
     return out
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The next token (int64 [B]) of each row of ``logits`` (bf16 or fp32 [B, V], rows may lie apart),
+    drawn by the row's random number ``u`` (fp32 [B], in [0, 1)).
+
+    Weights are e^((x - max) / temperature).  By falling logit (equal ones by rising index) the first
+    ``top_k`` tokens are kept (0: all), of those the shortest prefix that reaches ``top_p`` of their
+    weight, of those the ones of at least ``min_p`` times the largest; the token is the first, by
+    rising index, at which the kept weights add up to more than ``u`` of their sum.  Temperature 0
+    gives the largest logit.  -inf and NaN are never drawn; a row of nothing else gives -1.  Each
+    setting is a number, or a tensor with a value per row (fp32; ``top_k`` int32)."""
+    dev = logits.device
+    _require_cuda(logits, "logits")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"logits must be {torch.bfloat16} or {torch.float32} (got {logits.dtype})")
+    if logits.ndim != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"logits must be [rows, vocabulary] with contiguous rows (got {tuple(logits.shape)}, "
+                         f"strides {logits.stride()})")
+    B, V = logits.shape
+    _require(u, "u", torch.float32, dev)
+    if u.shape != (B,):
+        raise ValueError(f"u must be [{B}] (got {tuple(u.shape)})")
+    args = []
+    for value, name, dtype, cast in ((temperature, "temperature", torch.float32, float), (top_k, "top_k", torch.int32, int),
+                                     (top_p, "top_p", torch.float32, float), (min_p, "min_p", torch.float32, float)):
+        if isinstance(value, torch.Tensor):
+            _require(value, name, dtype, dev)
+            if value.shape != (B,):
+                raise ValueError(f"{name} must be a number or [{B}] (got {tuple(value.shape)})")
+            args += [value.data_ptr(), 1]
+        else:
+            args += [None, cast(value)]
+    if out is None:
+        out = torch.empty((B,), dtype=torch.int64, device=dev)
+    else:
+        _require(out, "out", torch.int64, dev)
+        if out.numel() != B:
+            raise ValueError("out has the wrong number of elements")
+    _launch(lib().moe_sample_tokens, "sample_tokens", dev, logits.data_ptr(), int(logits.dtype == torch.float32),
+            logits.stride(0) if B > 1 else V, B, V, u.data_ptr(), *args, out.data_ptr())
+    return out

@@ -54,6 +54,33 @@ def assert_within(got: torch.Tensor, want: torch.Tensor, bound: torch.Tensor, wh
                              f"{float(bound.expand_as(want).flatten()[worst])} is allowed")
 
 
+def sample(x: torch.Tensor, u: float, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> int:
+    """The token of one row of logits (see sample_tokens), in 64 bits with a sort; the settings as
+    the fp32 values that they are passed as."""
+    f32 = lambda v: float(torch.tensor(v, dtype=torch.float32))
+    x = torch.where(x.isnan(), -math.inf, x.double())
+    top = float(x.max())
+    if top == -math.inf:
+        return -1
+    order = torch.sort(x, descending=True, stable=True).indices
+    if not f32(temperature) > 0:
+        return int(order[0])
+    if top == math.inf:
+        w = (x == math.inf).double()
+    else:
+        w = torch.exp((x - top) / f32(temperature))
+    n = int((x > -math.inf).sum())
+    if top_k > 0:
+        n = min(n, top_k)
+    if f32(top_p) < 1:
+        c = torch.cumsum(w[order[:n]], 0)
+        n = min(n, 1 + int((c < f32(top_p) * c[-1]).sum()))
+    n = max(1, min(n, int((w[order[:n]] >= f32(min_p)).sum())))
+    kept = order[:n].sort().values
+    c = torch.cumsum(w[kept], 0)
+    return int(kept[min(int((c <= f32(u) * c[-1]).sum()), n - 1)])
+
+
 class Pool:
     """A paged cache on `dev` and its sequences: pages handed out in a shuffled order."""
 

@@ -1,5 +1,5 @@
 """The batched serving operators on the GPU against plain 64-bit forms: rotary embedding into a
-paged cache, attention over it."""
+paged cache, attention over it, attention of packed prompts, choice of tokens."""
 from __future__ import annotations
 
 import math
@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from serving_ref import Pool, assert_within, attention, rope
+from serving_ref import Pool, assert_within, attention, rope, sample
 
 pytestmark = pytest.mark.gpu
 
@@ -356,3 +356,128 @@ def test_packed_attention_infinities_stay_with_the_rows_that_see_them(cuda_devic
             assert torch.isfinite(got[keep]).all()
             assert_within(torch.where(keep, got, 0.0), torch.where(keep, want, 0.0), tol)
         _check_packed(out, q, k, v, cuts[:2], s)
+
+
+# ------------------------------------------------------------------ choice of tokens
+SETTINGS = [dict(), dict(temperature=0.0), dict(top_k=1), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.05),
+            dict(temperature=0.7, top_k=50, top_p=0.9), dict(temperature=1.5, top_p=0.5, min_p=0.02),
+            dict(temperature=3.0, top_k=700, top_p=0.95, min_p=0.001), dict(temperature=0.01, top_p=0.99),
+            dict(top_k=10 ** 6, top_p=1.0), dict(min_p=1.0), dict(top_p=1e-6)]
+
+
+def _sampled(dev, x, u, **settings):
+    """sample_tokens on rows x (CPU) against the sorted form, row by row."""
+    from moeinfra_amd import ops
+
+    got = ops.sample_tokens(x.to(dev), u.to(dev), **settings).cpu().tolist()
+    want = [sample(row, float(r), **settings) for row, r in zip(x, u)]
+    assert got == want, settings
+    return got
+
+
+def _logits(rows, vocab, seed, dtype, peaks=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((rows, vocab), generator=g) * 2.0
+    if peaks:
+        x = x + torch.where(torch.rand((rows, vocab), generator=g) < 0.003, 9.0 * torch.rand((rows, vocab), generator=g), 0.0)
+    return x.to(dtype), torch.rand((rows,), generator=g)
+
+
+@pytest.mark.parametrize("vocab,dtype", [(32000, torch.bfloat16), (32000, torch.float32), (50257, torch.bfloat16),
+                                         (131072, torch.bfloat16), (777, torch.float32), (8, torch.bfloat16)])
+def test_sample_tokens(cuda_device, vocab, dtype):
+    for i, settings in enumerate(SETTINGS):
+        print(f"sample {vocab} {dtype} {settings}", flush=True)
+        x, u = _logits(6, vocab, 10 * i + vocab, dtype, peaks=i % 2 == 0)
+        _sampled(cuda_device, x, u, **settings)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 7, 9, 63, 1023, 8193])
+def test_sample_tokens_odd_sizes_and_strides(cuda_device, vocab):
+    """Rows that start at any element of their 16 bytes, with NaN between them."""
+    for dtype in (torch.bfloat16, torch.float32):
+        for lead in (0, 1, 3):
+            wide = torch.full((5, vocab + 2 * lead + 1), math.nan, dtype=dtype)
+            x, u = _logits(5, vocab, vocab + lead, dtype)
+            wide[:, lead:lead + vocab] = x
+            from moeinfra_amd import ops
+
+            got = ops.sample_tokens(wide.to(cuda_device)[:, lead:lead + vocab], u.to(cuda_device), temperature=1.3,
+                                    top_p=0.8)
+            assert got.cpu().tolist() == [sample(r, float(v), temperature=1.3, top_p=0.8) for r, v in zip(x, u)]
+
+
+def test_sample_tokens_settings_per_row(cuda_device):
+    from moeinfra_amd import ops
+
+    dev = cuda_device
+    x, u = _logits(64, 5000, 31, torch.float32)
+    g = torch.Generator().manual_seed(32)
+    pick = lambda values, t: torch.tensor(values, dtype=t)[torch.randint(len(values), (64,), generator=g)]
+    par = dict(temperature=pick([0.0, 0.4, 1.0, 2.0], torch.float32), top_k=pick([-1, 0, 1, 30, 900], torch.int32),
+               top_p=pick([0.3, 0.9, 1.0, 2.0], torch.float32), min_p=pick([0.0, 0.01, 0.3], torch.float32))
+    got = ops.sample_tokens(x.to(dev), u.to(dev), **{n: v.to(dev) for n, v in par.items()})
+    want = [sample(x[i], float(u[i]), **{n: v[i].item() for n, v in par.items()}) for i in range(64)]
+    assert got.cpu().tolist() == want
+
+
+def test_sample_tokens_equal_logits(cuda_device):
+    """Ties go to the lowest index: of equal logits the first are kept."""
+    x = torch.zeros((9, 1000))
+    u = torch.tensor([0.0, 0.1, 0.25, 0.5, 0.75, 0.9, 0.99, 0.999, 0.9999999])
+    assert _sampled(cuda_device, x, u, top_k=10)[-1] == 9
+    assert _sampled(cuda_device, x, u, top_p=0.25)[-1] == 249
+    assert _sampled(cuda_device, x, u)[-1] == 999
+    assert _sampled(cuda_device, x, u, top_k=400, top_p=0.5)[-1] == 199
+    # Two levels, both zeros (equal), many of the lower one.
+    x = torch.full((9, 4099), -1.0)
+    x[:, 5::7] = 0.0
+    x[:, 12::14] = -0.0
+    for settings in (dict(top_k=3), dict(top_k=600), dict(top_p=0.2), dict(top_p=0.6), dict(min_p=0.9)):
+        _sampled(cuda_device, x, u, **settings)
+    _sampled(cuda_device, x.to(torch.bfloat16), u, top_k=587, top_p=0.999)
+
+
+def test_sample_tokens_close_and_far_logits(cuda_device):
+    """Values that differ in their last bits, in every exponent, and beyond any weight."""
+    g = torch.Generator().manual_seed(40)
+    u = torch.rand((6,), generator=g)
+    near = 1.0 + torch.randint(0, 5000, (6, 20000), generator=g).float() * 2.0 ** -23
+    far = torch.randn((6, 20000), generator=g) * 10.0 ** (torch.rand((6, 20000), generator=g) * 70 - 35)
+    lowest = torch.full((6, 20000), torch.finfo(torch.float32).min)
+    lowest[:, 100:103] = 3.0
+    for x in (near, far, lowest, -near):
+        for settings in (dict(top_k=77), dict(top_k=9000), dict(top_p=0.7), dict(temperature=1e-4, top_p=0.7),
+                         dict(temperature=1e30, top_k=5000, top_p=0.5), dict(top_k=2, min_p=0.5)):
+            _sampled(cuda_device, x, u, **settings)
+
+
+def test_sample_tokens_masked_rows(cuda_device):
+    """-inf and NaN are never drawn; rows of nothing else give -1; +inf takes all."""
+    V = 3000
+    x = torch.randn((8, V), generator=torch.Generator().manual_seed(50))
+    x[0, :] = -math.inf
+    x[1, :] = math.nan
+    x[2, :] = -math.inf
+    x[2, 1234] = -5.0
+    x[3, ::2] = math.nan
+    x[4, 1:] = -math.inf
+    x[5, [7, 900, 2999]] = math.inf
+    x[6, :2000] = torch.finfo(torch.float32).min
+    x[7, :] = torch.finfo(torch.float32).min
+    u = torch.linspace(0.05, 0.95, 8)
+    for settings in (dict(), dict(top_k=2), dict(top_p=0.5), dict(temperature=0.0), dict(temperature=0.5, top_k=20, top_p=0.8, min_p=0.1)):
+        got = _sampled(cuda_device, x, u, **settings)
+        assert got[:3] == [-1, -1, 1234] and got[4] == 0 and got[5] in (7, 900, 2999)
+        _sampled(cuda_device, x.to(torch.bfloat16), u, **settings)
+
+
+def test_sample_tokens_random_numbers_at_the_ends(cuda_device):
+    """u of 0 and next to 1, and numbers outside [0, 1), which take the first and the last kept."""
+    from moeinfra_amd import ops
+
+    x = torch.randn((1, 4000), generator=torch.Generator().manual_seed(51))
+    kept = torch.sort(x[0], descending=True).indices[:25].sort().values
+    for u, at in ((0.0, 0), (1.0 - 2.0 ** -24, 24), (1.0, 24), (7.5, 24), (-1.0, 0), (math.nan, 0)):
+        got = ops.sample_tokens(x.to(cuda_device), torch.tensor([u], device=cuda_device), top_k=25)
+        assert int(got) == int(kept[at])

@@ -32,6 +32,13 @@ def _packed(**kw):
     return _lib.lib().moe_packed_attention_bf16(*a.values())
 
 
+def _sample(**kw):
+    a = dict(logits=A, f32=0, stride=1000, B=4, V=1000, u=B, t=None, temperature=1.0, k=None, top_k=0, p=None,
+             top_p=1.0, mp=None, min_p=0.0, token=C, stream=None)
+    a.update(kw)
+    return _lib.lib().moe_sample_tokens(*a.values())
+
+
 REFUSED = [
     (_append, dict(hd=24), "head dim"),
     (_append, dict(hd=528), "head dim"),
@@ -90,6 +97,22 @@ REFUSED = [
     (_packed, dict(out=E + 4), "aligned"),
     (_packed, dict(out=A + 1024), "overlap"),
     (_packed, dict(out=C - 1024), "overlap"),
+    (_sample, dict(f32=2), "bf16"),
+    (_sample, dict(B=-1), "bad sizes"),
+    (_sample, dict(V=0), "logits"),
+    (_sample, dict(V=(1 << 20) + 1, stride=1 << 21), "logits"),
+    (_sample, dict(stride=999), "apart"),
+    (_sample, dict(temperature=-1.0), "temperature"),
+    (_sample, dict(temperature=float("nan")), "temperature"),
+    (_sample, dict(top_k=-1), "top-k"),
+    (_sample, dict(top_p=0.0), "top-p"),
+    (_sample, dict(top_p=1.5), "top-p"),
+    (_sample, dict(min_p=-0.1), "min-p"),
+    (_sample, dict(min_p=1.1), "min-p"),
+    (_sample, dict(u=None), "null"),
+    (_sample, dict(f32=1, logits=A + 2), "aligned"),
+    (_sample, dict(token=C + 4), "aligned"),
+    (_sample, dict(token=A + 800), "overlap"),
 ]
 
 
@@ -104,6 +127,7 @@ def test_empty_calls_do_nothing():
     assert _paged(B=0, q=None, out=None, lens=None) == 0
     assert _packed(T=0, q=None, k=None, v=None, cu=None, out=None) == 0
     assert _packed(B=0, cu=None) == 0
+    assert _sample(B=0, logits=None, u=None, token=None) == 0
 
 
 def test_paged_attention_workspace_grows_with_the_batch():
@@ -122,5 +146,7 @@ def test_wrappers_take_gpu_tensors_only():
         ops.paged_attention(bf(4, 8, 64), bf(32, 2, 16, 64), bf(32, 2, 16, 64), i32(4, 8), i32(4))
     with pytest.raises(ValueError, match="GPU tensor"):
         ops.packed_attention(bf(4, 8, 64), bf(4, 2, 64), bf(4, 2, 64), i32(2))
+    with pytest.raises(ValueError, match="GPU tensor"):
+        ops.sample_tokens(bf(4, 100), torch.zeros(4))
     with pytest.raises(ValueError, match="invalid attention sizes"):
         ops.paged_attention_workspace(4, 8, 2, 96, "cpu")
