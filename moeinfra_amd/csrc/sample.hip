@@ -7,12 +7,17 @@
 //   token: the first index i with  sum of the kept w_j, j <= i  >  u * (sum of all kept w)
 //
 // Kept tokens are a prefix of the order, so no sort is needed: the prefix ends at some value, found
-// through histograms of the counts and sums by value, and at some index among its equals.
+// through a histogram, and at some index among its equals.
+//
+//   sample_kernel   a workgroup per row; counts by the upper 16 bits of the logits
+//   sm_general      the same for rows with values that those counts do not hold (see there)
 //
 // A token is right or wrong, and a sum's rounding decides where u falls next to a border.  So weights
 // are evaluated in 64 bits and held as integers of 2^-43: sums of them (up to 2^20) are exact, the
 // same in any order, and nothing here depends on the order in which atomics arrive.  2^-44 of the
 // largest weight, what an integer is off by, is all that the result can differ from exact sums.
+#include <type_traits>
+
 #include "common.h"
 
 namespace moe {
@@ -47,11 +52,12 @@ __device__ __forceinline__ uint32_t sm_key(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// 2^(43 - y) in 64 bits for 0 <= y < 44: the series of 2^f, |f| <= 1/2, to f^11 (the next term is
-// 2^-47), times a power of two.
-__device__ __forceinline__ double sm_weight(double y) {
-  const double n = rint(y), t = (n - y) * 0.69314718055994530942;
-  double p = 1.0 / 39916800;
+// 2^f in 64 bits, |f| <= 1/2: the series to f^13.
+__device__ __forceinline__ double sm_exp2(double f) {
+  const double t = f * 0.69314718055994530942;
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, t, 1.0 / 479001600);
+  p = fma(p, t, 1.0 / 39916800);
   p = fma(p, t, 1.0 / 3628800);
   p = fma(p, t, 1.0 / 362880);
   p = fma(p, t, 1.0 / 40320);
@@ -62,9 +68,35 @@ __device__ __forceinline__ double sm_weight(double y) {
   p = fma(p, t, 1.0 / 6);
   p = fma(p, t, 0.5);
   p = fma(p, t, 1.0);
-  p = fma(p, t, 1.0);
-  return ldexp(p, kSmBits - (int)n);
+  return fma(p, t, 1.0);
 }
+
+constexpr int kSmTable = 32;
+
+// Weights 2^(43 - y), y = (m - x) log2(e) / T: y in 32nds is n + r, |r| <= 1/2, the power of n from
+// a table of 32 and an exponent, that of r by its series to r^5 (the next term is 2^-51).  Past
+// 2^-21 of an integer's step all is zero (-inf too).
+struct SmWeight {
+  const double *table;  // 2^(-j / 32), in LDS
+  double m, c;          // c: 32 log2(e) / T
+
+  __device__ __forceinline__ double real(float x) const {
+    constexpr double kRound = 0x1.8p52;  // the sum's low word is the nearest integer
+    constexpr double k = -0.69314718055994530942 / kSmTable;
+    const double y = fmin((m - (double)x) * c, 64.0 * kSmTable);
+    const double z = y + kRound;
+    const int n = (int)(uint32_t)__builtin_bit_cast(u64, z);
+    const double r = y - (z - kRound);
+    double p = k * k * k * k * k / 120;
+    p = fma(p, r, k * k * k * k / 24);
+    p = fma(p, r, k * k * k / 6);
+    p = fma(p, r, k * k / 2);
+    p = fma(p, r, k);
+    const double t = table[n & (kSmTable - 1)];
+    const double w = fma(t, p * r, t);
+    return __builtin_bit_cast(double, __builtin_bit_cast(u64, w) + ((u64)(uint32_t)(kSmBits - (n >> 5)) << 52));
+  }
+};
 // To the nearest integer (of values below 2^52).
 __device__ __forceinline__ u64 sm_mass(double w) {
   return __builtin_bit_cast(u64, w + 0x1p52) & ((1ull << 52) - 1);
@@ -82,14 +114,11 @@ __device__ __forceinline__ u64 sm_wave_sum(u64 v) {
   return v;
 }
 
-struct SmShared {
-  u64 mass[kSmBins];
-  uint32_t count[kSmBins];
-  u64 mass2[kSmBins];
-  uint32_t count2[kSmBins], lo2[kSmBins], hi2[kSmBins];
+// What the workgroup's waves tell each other.
+struct SmShare {
   u64 seg[kSmWaves];
   u64 part[kSmWaves], part2[kSmWaves];
-  uint32_t partk[kSmWaves];
+  uint32_t bits[kSmWaves], flags[kSmWaves];
   u64 r_a, r_b;
   int r_i;
 };
@@ -107,41 +136,82 @@ struct SmRow {
     base = row - off;
     chunks = (off + V + N - 1) / N;
   }
-  // Values of chunk c as fp32; what does not belong to the row, and NaN, is -inf.
-  __device__ __forceinline__ void load(int c, float (&x)[N]) const {
-    const int i0 = c * N - off;
-    if (i0 >= 0 && i0 + N <= V) {
-      const u32x4 v = *reinterpret_cast<const u32x4 *>(base + (int64_t)c * N);
+  // Chunks [whole0, whole1) belong to the row entirely.
+  __device__ __forceinline__ int whole0() const { return off > 0 ? 1 : 0; }
+  __device__ __forceinline__ int whole1() const { return (off + V) / N; }
+  __device__ __forceinline__ u32x4 raw(int c) const {
+    return *reinterpret_cast<const u32x4 *>(base + (int64_t)c * N);
+  }
+  // Any chunk; elements outside the row are -inf.
+  __device__ __forceinline__ u32x4 chunk(int c) const {
+    if (c >= whole0() && c < whole1()) return raw(c);
+    u32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
       if constexpr (sizeof(E) == 2) {
+        uint32_t h[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] = bf16lo_to_f32(v[e]);
-          x[2 * e + 1] = bf16hi_to_f32(v[e]);
+        for (int o = 0; o < 2; ++o) {
+          const int i = c * N + 2 * e + o;
+          h[o] = i >= off && i < off + V ? base[i] : 0xff80u;
         }
+        v[e] = h[0] | h[1] << 16;
       } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = __builtin_bit_cast(float, (uint32_t)v[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        x[e] = -INFINITY;
-        if (i0 + e >= 0 && i0 + e < V) {
-          if constexpr (sizeof(E) == 2)
-            x[e] = bf16_to_f32(base[(int64_t)c * N + e]);
-          else
-            x[e] = base[(int64_t)c * N + e];
-        }
+        const int i = c * N + e;
+        v[e] = i >= off && i < off + V ? __builtin_bit_cast(uint32_t, base[i]) : 0xff800000u;
       }
     }
-#pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
+    return v;
   }
+  // Element e of a chunk as fp32 bits.
+  static __device__ __forceinline__ uint32_t bits(const u32x4 &v, int e) {
+    if constexpr (sizeof(E) == 2) return e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16;
+    return v[e];
+  }
+  __device__ __forceinline__ int index(int c, int e) const { return c * N - off + e; }
 };
 
-// The bin (threads in order, one bin each) in which the running sum of v reaches goal (>= 1, at most
-// the whole sum): its number, and the sums of v and of v2 before it.  Uniform over the workgroup.
-__device__ __forceinline__ int sm_cross(SmShared &s, u64 v, u64 v2, u64 goal, u64 &before, u64 &before2) {
+// As fp32, NaN as -inf.
+__device__ __forceinline__ float sm_value(uint32_t bits) {
+  const float x = __builtin_bit_cast(float, bits);
+  return x == x ? x : -INFINITY;
+}
+
+// f(bits, index) of each element of chunks c0 + first, c0 + first + step, ... below c1; two more
+// chunks are on their way while one is looked at.
+template <typename E, typename F>
+__device__ __forceinline__ void sm_each(const SmRow<E> &row, int c0, int c1, int first, int step, F f) {
+  constexpr int N = SmRow<E>::N;
+  const int a = max(c0, row.whole0()) + first, b = min(c1, row.whole1());
+  if (a < b) {
+    u32x4 v0 = row.raw(a), v1 = row.raw(min(a + step, b - 1)), v2;
+    for (int c = a; c < b; c += step) {
+      v2 = row.raw(min(c + 2 * step, b - 1));
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(SmRow<E>::bits(v0, e), row.index(c, e));
+      v0 = v1;
+      v1 = v2;
+    }
+  }
+  // The row's ends, where they are shared with other rows.
+  if (first != 0) return;
+  for (int k = 0; k < 2; ++k) {
+    const int end = k == 0 ? 0 : row.chunks - 1;
+    if (end < c0 || end >= c1 || (end >= row.whole0() && end < row.whole1()) || (k == 1 && row.chunks == 1)) continue;
+    const u32x4 v = row.chunk(end);
+#pragma unroll 1
+    for (int e = 0; e < N; ++e) {
+      uint32_t x = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x = i == e ? SmRow<E>::bits(v, i) : x;
+      f(x, row.index(end, e));
+    }
+  }
+}
+
+// The thread (in order) in which the running sum of v reaches goal (>= 1, at most the whole sum), and
+// the sums of v and of v2 before it.  Uniform over the workgroup.
+__device__ __forceinline__ int sm_cross(SmShare &s, u64 v, u64 v2, u64 goal, u64 &before, u64 &before2) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   u64 a = sm_wave_incl(v, lane), b = sm_wave_incl(v2, lane);
   if (lane == kWave - 1) {
@@ -167,7 +237,7 @@ __device__ __forceinline__ int sm_cross(SmShared &s, u64 v, u64 v2, u64 goal, u6
   return i;
 }
 
-__device__ __forceinline__ u64 sm_block_sum(SmShared &s, u64 v) {
+__device__ __forceinline__ u64 sm_block_sum(SmShare &s, u64 v) {
   v = sm_wave_sum(v);
   if ((threadIdx.x & (kWave - 1)) == 0) s.part[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -177,22 +247,17 @@ __device__ __forceinline__ u64 sm_block_sum(SmShared &s, u64 v) {
   return sum;
 }
 
-// The first index at which the running sum of f(value, index) over the row exceeds its target,
+// The first index at which the running sum of f(bits, index) over the row exceeds its target,
 // pick(whole sum); -1 if the whole sum is zero.
 template <typename E, typename F, typename P>
-__device__ __forceinline__ int sm_locate(SmShared &s, const SmRow<E> &row, F f, P pick) {
+__device__ __forceinline__ int sm_locate(SmShare &s, const SmRow<E> &row, F f, P pick) {
   constexpr int N = SmRow<E>::N;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   // A stretch of whole chunks per wave.
   const int per = (row.chunks + kSmWaves - 1) / kSmWaves;
-  const int c0 = wave * per, c1 = min(c0 + per, row.chunks);
   u64 sum = 0;
-  for (int c = c0 + lane; c < c1; c += kWave) {
-    float x[N];
-    row.load(c, x);
-#pragma unroll
-    for (int e = 0; e < N; ++e) sum += f(x[e], c * N - row.off + e);
-  }
+  sm_each(row, min(wave * per, row.chunks), min(wave * per + per, row.chunks), lane, kWave,
+          [&](uint32_t bits, int i) { sum += f(bits, i); });
   sum = sm_wave_sum(sum);
   if (lane == 0) s.seg[wave] = sum;
   __syncthreads();
@@ -206,12 +271,12 @@ __device__ __forceinline__ int sm_locate(SmShared &s, const SmRow<E> &row, F f, 
   const int e0 = w * per, e1 = min(e0 + per, row.chunks);
   for (int cb = e0; cb < e1; cb += kSmThreads) {
     const int c = cb + threadIdx.x;
-    float x[N];
+    u32x4 v = {0, 0, 0, 0};
     u64 own = 0;
     if (c < e1) {
-      row.load(c, x);
+      v = row.chunk(c);
 #pragma unroll
-      for (int e = 0; e < N; ++e) own += f(x[e], c * N - row.off + e);
+      for (int e = 0; e < N; ++e) own += f(SmRow<E>::bits(v, e), row.index(c, e));
     }
     const u64 block = sm_block_sum(s, own);
     if (target >= block) {
@@ -225,8 +290,8 @@ __device__ __forceinline__ int sm_locate(SmShared &s, const SmRow<E> &row, F f, 
       int at = -1;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        run += f(x[e], c * N - row.off + e);
-        if (at < 0 && run > target) at = c * N - row.off + e;
+        run += f(SmRow<E>::bits(v, e), row.index(c, e));
+        if (at < 0 && run > target) at = row.index(c, e);
       }
       s.r_i = at;
     }
@@ -238,100 +303,74 @@ __device__ __forceinline__ int sm_locate(SmShared &s, const SmRow<E> &row, F f, 
   return -1;
 }
 
-template <typename E>
-__global__ void __launch_bounds__(kSmThreads)
-sample_kernel(const SmArgs a) {
-  constexpr int N = SmRow<E>::N;
-  __shared__ SmShared s;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  const int64_t r = blockIdx.x;
-  const SmRow<E> row((const E *)a.logits + r * a.stride, a.V);
-  const float T = a.temperature ? a.temperature[r] : a.temperature0;
-  const int k = a.top_k ? a.top_k[r] : a.top_k0;
-  const float p = a.top_p ? a.top_p[r] : a.top_p0;
-  const float mp = a.min_p ? a.min_p[r] : a.min_p0;
-  const float u = a.u[r];
+struct SmGeneral {
+  u64 mass[kSmBins];
+  uint32_t count[kSmBins];
+  u64 mass2[kSmBins];
+  uint32_t count2[kSmBins], lo2[kSmBins], hi2[kSmBins];
+};
 
-  // The largest value.
-  float mx = -INFINITY;
-  for (int c = threadIdx.x; c < row.chunks; c += kSmThreads) {
-    float x[N];
-    row.load(c, x);
-#pragma unroll
-    for (int e = 0; e < N; ++e) mx = fmaxf(mx, x[e]);
-  }
-  {
-    float v[1] = {mx};
-    lane_groups_reduce<true>(v, kWave);
-    if (lane == 0) s.partk[wave] = __builtin_bit_cast(uint32_t, v[0]);
-    __syncthreads();
-    mx = -INFINITY;
-    for (int w = 0; w < kSmWaves; ++w) mx = fmaxf(mx, __builtin_bit_cast(float, s.partk[w]));
-    __syncthreads();
-  }
-  if (mx == -INFINITY) {  // nothing to choose from
-    if (threadIdx.x == 0) a.token[r] = -1;
-    return;
-  }
-  const uint32_t key_max = sm_key(mx);
-  // Greedy: the first of the order (temperatures of zero and below, and NaN).
-  if (!(T > 0.0f) || k == 1) {
-    const int at = sm_locate(s, row, [&](float x, int) { return (u64)(x == mx); }, [](u64) { return (u64)0; });
-    if (threadIdx.x == 0) a.token[r] = at;
-    return;
-  }
+// What a row is asked for.
+struct SmAsk {
+  float T, p, min_p, u;
+  int k;
+};
+
+__device__ __forceinline__ u64 sm_target(float u, u64 total) {
+  const double y = (double)u * (double)total;
+  const u64 t = y > 0.0 ? (y < 0x1p63 ? (u64)y : total) : 0;
+  return t < total ? t : total - 1;
+}
+
+// Any row with the maximum mx above -inf: two levels of 1024 linear bins by value below the maximum,
+// then, should a bin of a bin hold several values, a bisection.
+template <typename E>
+__device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> row, const SmAsk a, float mx,
+                                       const double *table) {
   // With an infinite maximum only its equals weigh anything: as zeros over -inf.
   const bool infinite = mx == INFINITY;
   const double m = infinite ? 0.0 : (double)mx;
   auto value = [&](float x) { return infinite ? (x == INFINITY ? 0.0f : -INFINITY) : x; };
-  const double c2 = kSmLog2e / (double)T;
+  const double c2 = kSmLog2e / (double)a.T;
+  const SmWeight weight{table, m, c2 * kSmTable};
   const float fm = (float)m;
   const double bs = c2 * (kSmBins / kSmSpan);
   const float bin_scale = bs < 1e30 ? (float)bs : 1e30f;
   // Linear bins below the maximum, 44 powers of two of weight deep; the last takes the rest.
   auto place = [&](float x) { return (fm - x) * bin_scale; };
-  auto weight = [&](float x) {  // unrounded
-    const double y = (m - (double)x) * c2;
-    return y < kSmSpan ? sm_weight(y) : 0.0;
-  };
-  const bool by_k = k > 0 && k < a.V, by_p = p < 1.0f;
+  const bool by_k = a.k > 0 && a.k < row.V, by_p = a.p < 1.0f;
   uint32_t key = 0;   // kept: what is above this key, and its equals up to index `cut`
   int cut = 0x7fffffff;
   if (by_k || by_p) {
     // Counts and sums by value.
     for (int i = threadIdx.x; i < kSmBins; i += kSmThreads) {
-      s.mass[i] = 0;
-      s.count[i] = 0;
+      g.mass[i] = 0;
+      g.count[i] = 0;
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < row.chunks; c += kSmThreads) {
-      float x[N];
-      row.load(c, x);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float v = value(x[e]);
-        if (v == -INFINITY) continue;
-        const int b = (int)fminf(place(v), (float)(kSmBins - 1));
-        atomicAdd(&s.count[b], 1u);
-        if (by_p) {
-          const u64 w = sm_mass(weight(v));
-          if (w != 0) atomicAdd(&s.mass[b], w);
-        }
+    sm_each(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, [&](uint32_t bits, int) {
+      const float v = value(sm_value(bits));
+      if (v == -INFINITY) return;
+      const int b = (int)fminf(place(v), (float)(kSmBins - 1));
+      atomicAdd(&g.count[b], 1u);
+      if (by_p) {
+        const u64 w = sm_mass(weight.real(v));
+        if (w != 0) atomicAdd(&g.mass[b], w);
       }
-    }
+    });
     __syncthreads();
     // The value at which the running count (or sum) of the order reaches goal: its key, how many of
     // its equals are needed and there, and the sum above it.
     auto select = [&](bool count, u64 goal, uint32_t &key_out, u64 &need, u64 &ties, u64 &above, u64 &each) {
       u64 before, before2;
-      const u64 own = count ? (u64)s.count[threadIdx.x] : s.mass[threadIdx.x];
-      const int b = sm_cross(s, own, s.mass[threadIdx.x], goal, before, before2);
+      const u64 own = count ? (u64)g.count[threadIdx.x] : g.mass[threadIdx.x];
+      const int b = sm_cross(s, own, g.mass[threadIdx.x], goal, before, before2);
       const float fb = (float)b;
       for (int i = threadIdx.x; i < kSmBins; i += kSmThreads) {
-        s.mass2[i] = 0;
-        s.count2[i] = 0;
-        s.lo2[i] = ~0u;
-        s.hi2[i] = 0;
+        g.mass2[i] = 0;
+        g.count2[i] = 0;
+        g.lo2[i] = ~0u;
+        g.hi2[i] = 0;
       }
       __syncthreads();
       auto inside = [&](float v, int &sub) {
@@ -341,47 +380,37 @@ sample_kernel(const SmArgs a) {
         sub = (int)fminf((t - fb) * (float)kSmBins, (float)(kSmBins - 1));
         return true;
       };
-      for (int c = threadIdx.x; c < row.chunks; c += kSmThreads) {
-        float x[N];
-        row.load(c, x);
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          int sub;
-          const float v = value(x[e]);
-          if (!inside(v, sub)) continue;
-          const uint32_t kk = sm_key(v);
-          atomicAdd(&s.count2[sub], 1u);
-          const u64 w = sm_mass(weight(v));
-          if (w != 0) atomicAdd(&s.mass2[sub], w);
-          atomicMin(&s.lo2[sub], kk);
-          atomicMax(&s.hi2[sub], kk);
-        }
-      }
+      sm_each(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, [&](uint32_t bits, int) {
+        int sub;
+        const float v = value(sm_value(bits));
+        if (!inside(v, sub)) return;
+        const uint32_t kk = sm_key(v);
+        atomicAdd(&g.count2[sub], 1u);
+        const u64 w = sm_mass(weight.real(v));
+        if (w != 0) atomicAdd(&g.mass2[sub], w);
+        atomicMin(&g.lo2[sub], kk);
+        atomicMax(&g.hi2[sub], kk);
+      });
       __syncthreads();
       u64 in1, in2;
-      const u64 own2 = count ? (u64)s.count2[threadIdx.x] : s.mass2[threadIdx.x];
-      const int sb = sm_cross(s, own2, s.mass2[threadIdx.x], goal - before, in1, in2);
+      const u64 own2 = count ? (u64)g.count2[threadIdx.x] : g.mass2[threadIdx.x];
+      const int sb = sm_cross(s, own2, g.mass2[threadIdx.x], goal - before, in1, in2);
       before += in1;
       before2 += in2;
-      uint32_t lo = s.lo2[sb], hi = s.hi2[sb];
-      ties = s.count2[sb];
-      each = ties > 0 ? s.mass2[sb] / ties : 0;
+      uint32_t lo = g.lo2[sb], hi = g.hi2[sb];
+      ties = g.count2[sb];
+      each = ties > 0 ? g.mass2[sb] / ties : 0;
       // Several values in one bin of a bin: the largest key at which the goal is reached, by bisection.
       if (lo != hi) {
         auto sums = [&](uint32_t from, u64 &n, u64 &sum) {  // of the bin's values from that key on
           u64 nn = 0, ss = 0;
-          for (int c = threadIdx.x; c < row.chunks; c += kSmThreads) {
-            float x[N];
-            row.load(c, x);
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-              int sub;
-              const float v = value(x[e]);
-              if (!inside(v, sub) || sub != sb || sm_key(v) < from) continue;
-              ++nn;
-              ss += sm_mass(weight(v));
-            }
-          }
+          sm_each(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, [&](uint32_t bits, int) {
+            int sub;
+            const float v = value(sm_value(bits));
+            if (!inside(v, sub) || sub != sb || sm_key(v) < from) return;
+            ++nn;
+            ss += sm_mass(weight.real(v));
+          });
           n = sm_block_sum(s, nn);
           sum = sm_block_sum(s, ss);
         };
@@ -410,18 +439,18 @@ sample_kernel(const SmArgs a) {
     };
     u64 total = 0, all = 0;
     {
-      all = sm_block_sum(s, (u64)s.count[threadIdx.x]);
-      if (by_p) total = sm_block_sum(s, s.mass[threadIdx.x]);
+      all = sm_block_sum(s, (u64)g.count[threadIdx.x]);
+      if (by_p) total = sm_block_sum(s, g.mass[threadIdx.x]);
     }
     u64 need = 0, ties = 0, above, each;
     bool limited = false;
-    if (by_k && (u64)k < all) {
-      select(true, (u64)k, key, need, ties, above, each);
+    if (by_k && (u64)a.k < all) {
+      select(true, (u64)a.k, key, need, ties, above, each);
       total = above + need * each;
       limited = true;
     }
     if (by_p) {
-      const double want = ceil((double)p * (double)total);
+      const double want = ceil((double)a.p * (double)total);
       u64 goal = want >= 1.0 ? (u64)want : 1;  // (p of zero and below, or NaN: the first of the order)
       goal = goal < total ? goal : total;
       select(false, goal, key, need, ties, above, each);
@@ -430,30 +459,381 @@ sample_kernel(const SmArgs a) {
     if (limited && need < ties) {
       const uint32_t kk = key;
       const u64 n = need;
-      cut = sm_locate(s, row, [&](float x, int) {
-        const float v = value(x);
+      cut = sm_locate(s, row, [&](uint32_t bits, int) {
+        const float v = value(sm_value(bits));
         return (u64)(v != -INFINITY && sm_key(v) == kk);
       }, [&](u64) { return n - 1; });
     }
   }
-  (void)key_max;
-  const double floor_w = ldexp((double)mp, kSmBits);
+  const double floor_w = (double)a.min_p * 0x1p43;
   const int at = sm_locate(
       s, row,
-      [&](float x, int i) -> u64 {
-        const float v = value(x);
+      [&](uint32_t bits, int i) -> u64 {
+        const float v = value(sm_value(bits));
         const uint32_t kk = sm_key(v);
         if (v == -INFINITY || kk < key || (kk == key && i > cut)) return 0;
-        const double w = weight(v);
+        const double w = weight.real(v);
         // (The largest is kept whatever min_p asks for.)
         return w >= floor_w || v == fm ? sm_mass(w) : 0;
       },
-      [&](u64 total) {
-        const double y = (double)u * (double)total;
-        u64 t = y > 0.0 ? (y < 0x1p63 ? (u64)y : total) : 0;
-        return t < total ? t : total - 1;
-      });
-  if (threadIdx.x == 0) a.token[r] = at;
+      [&](u64 total) { return sm_target(a.u, total); });
+  return at;
+}
+
+// Bins of the first histogram: the upper 16 bits of a logit (all of a bf16 one) with a magnitude in
+// [2^-32, 2^8), larger values first, zero in the middle.
+constexpr uint32_t kSmLow = 95 << 7;               // upper 16 bits of 2^-32
+constexpr uint32_t kSmSide = (135 << 7) - kSmLow;  // bins of a sign
+constexpr int kSmEntries = 2 * kSmSide + 1;
+constexpr int kSmPer = (kSmEntries + kSmThreads - 1) / kSmThreads;  // 11: odd, so that threads meet no bank twice
+constexpr int kSmNone = kSmThreads * kSmPer;                          // no bin: never drawn
+constexpr int kSmList = kSmThreads;                                   // logits of one bin that are ranked directly
+
+// Upper 16 bits of a bin's values (of the smallest magnitude).
+__device__ __forceinline__ float sm_bin_value(int bin, uint32_t low_bits) {
+  uint32_t h = 0;
+  if (bin < (int)kSmSide) h = kSmLow + kSmSide - 1 - bin;
+  if (bin > (int)kSmSide) h = 0x8000u | (kSmLow + bin - kSmSide - 1);
+  return __builtin_bit_cast(float, h << 16 | (bin == (int)kSmSide ? 0u : low_bits));
+}
+
+// The bin of a logit.  kSmNone for -inf and NaN; for finite values below -2^8 too, noted in `far`;
+// others without a bin (magnitudes below 2^-32, from 2^8 on) are noted in `odd`.
+__device__ __forceinline__ int sm_bin(uint32_t bits, bool &far, bool &odd) {
+  const uint32_t h = bits >> 16 & 0x7fffu, d = h - kSmLow;
+  const bool neg = (int32_t)bits < 0;
+  const int bin = neg ? (int)(kSmSide + 1 + d) : (int)(kSmSide - 1 - d);
+  if (d < kSmSide) return bin;
+  if ((bits & 0x7fffffffu) == 0) return kSmSide;
+  if ((bits & 0x7fffffffu) > 0x7f800000u || bits == 0xff800000u) return kSmNone;
+  if (neg && h >= kSmLow + kSmSide)
+    far = true;
+  else
+    odd = true;
+  return kSmNone;
+}
+
+// LDS of a row in bf16: a bin holds one value.  (127 KB)
+struct SmExact {
+  uint32_t count[kSmNone];
+  u64 weight[kSmEntries];  // of a bin's value, 0 where it is not kept
+};
+// LDS of a row in fp32: one bin's logits are ranked. (61 KB)
+struct SmRanked {
+  uint32_t count[kSmNone];
+  u64 mass[kSmList];
+  uint32_t key[kSmList];
+  int index[kSmList];
+  int n;
+};
+
+// A workgroup per row.
+//   1  the largest logit, and the counts of the bins
+//   2  the bin where top-k and top-p end, from sums over the bins: in bf16 they are exact, a bin's
+//      count times its value's weight; in fp32 a guess, which a pass over the logits checks and
+//      corrects while it adds the weights up, and the logits of the bin found are ranked
+//   3  the token, from sums over stretches of the row
+//
+// Bound: passes over the row (each of the LDS atomics of 1, of some 10 instructions per logit of 3,
+// and in fp32 of the 64-bit weights of 2) on one CU.
+template <typename E>
+__global__ void __launch_bounds__(kSmThreads)
+sample_kernel(const SmArgs a) {
+  constexpr bool kExact = sizeof(E) == 2;
+  using Bins = std::conditional_t<kExact, SmExact, SmRanked>;
+  __shared__ union {
+    Bins bins;
+    SmGeneral general;
+  } lds;
+  Bins &b = lds.bins;
+  __shared__ SmShare s;
+  __shared__ double table[kSmTable];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
+  const int64_t r = blockIdx.x;
+  const SmRow<E> row((const E *)a.logits + r * a.stride, a.V);
+  const SmAsk ask{a.temperature ? a.temperature[r] : a.temperature0, a.top_p ? a.top_p[r] : a.top_p0,
+                  a.min_p ? a.min_p[r] : a.min_p0, a.u[r], a.top_k ? a.top_k[r] : a.top_k0};
+  // Greedy: the first of the order (temperatures of zero and below, and NaN).
+  const bool greedy = !(ask.T > 0.0f) || ask.k == 1;
+  const bool by_k = ask.k > 0 && ask.k < a.V, by_p = ask.p < 1.0f;
+
+  float mx = -INFINITY;
+  bool far = false, odd = false;
+  if (greedy || (!kExact && !by_k && !by_p)) {  // no counts needed
+    sm_each(row, 0, row.chunks, tid, kSmThreads,
+            [&](uint32_t bits, int) { mx = fmaxf(mx, __builtin_bit_cast(float, bits)); });
+  } else {
+    for (int i = tid; i < kSmNone; i += kSmThreads) b.count[i] = 0;
+    __syncthreads();
+    sm_each(row, 0, row.chunks, tid, kSmThreads, [&](uint32_t bits, int) {
+      mx = fmaxf(mx, __builtin_bit_cast(float, bits));  // (NaN gives way)
+      const int bin = sm_bin(bits, far, odd);
+      if (bin != kSmNone) atomicAdd(&b.count[bin], 1u);
+    });
+  }
+  {
+    float v[1] = {mx};
+    lane_groups_reduce<true>(v, kWave);
+    const uint32_t flags = (__any(far) ? 1u : 0u) | (__any(odd) ? 2u : 0u);
+    if (lane == 0) {
+      s.bits[wave] = __builtin_bit_cast(uint32_t, v[0]);
+      s.flags[wave] = flags;
+    }
+    if (tid < kSmTable)
+      table[tid] = tid <= kSmTable / 2 ? sm_exp2(-tid / 32.0) : 0.5 * sm_exp2(1.0 - tid / 32.0);
+    __syncthreads();
+    mx = -INFINITY;
+    uint32_t all = 0;
+    for (int w = 0; w < kSmWaves; ++w) {
+      mx = fmaxf(mx, __builtin_bit_cast(float, s.bits[w]));
+      all |= s.flags[w];
+    }
+    far = all & 1u;
+    odd = all & 2u;
+  }
+  if (mx == -INFINITY) {  // nothing to choose from
+    if (tid == 0) a.token[r] = -1;
+    return;
+  }
+  if (greedy) {
+    const int at = sm_locate(
+        s, row, [&](uint32_t bits, int) { return (u64)(__builtin_bit_cast(float, bits) == mx); },
+        [](u64) { return (u64)0; });
+    if (tid == 0) a.token[r] = at;
+    return;
+  }
+  const double c2 = kSmLog2e / (double)ask.T;
+  // What is below -2^8 has no bin: without weight next to the maximum, or the general form's.
+  if (odd || mx == INFINITY || (far && ((double)mx + 256.0) * c2 < kSmSpan + 1.0)) {
+    const int at = sm_general(lds.general, s, row, ask, mx, table);
+    if (tid == 0) a.token[r] = at;
+    return;
+  }
+  const SmWeight weight{table, (double)mx, c2 * kSmTable};
+  const double floor_w = (double)ask.min_p * 0x1p43;
+  auto target = [&](u64 total) { return sm_target(ask.u, total); };
+
+  // This thread's bins: their counts, and their weight (fp32: as if all lay in the bin's middle).
+  u64 n_own = 0, m_own = 0;
+  // (The largest logit's bin: as if all were it, so that there is some weight.)
+  bool unused = false;
+  const int top = sm_bin(__builtin_bit_cast(uint32_t, mx), unused, unused);
+  auto bin_weight = [&](int bin) {
+    return sm_mass(weight.real(bin == top ? mx : sm_bin_value(bin, kExact ? 0u : 0x8000u)));
+  };
+  if (kExact || by_k || by_p) {
+#pragma unroll 1
+    for (int i = 0; i < kSmPer; ++i) {
+      const int bin = tid * kSmPer + i;
+      const uint32_t n = b.count[bin];
+      if (n == 0) continue;
+      const u64 w = bin_weight(bin);
+      if constexpr (kExact) b.weight[bin] = w;
+      n_own += n;
+      m_own += n * w;
+    }
+  }
+  // The bin in which the running count (or weight) reaches goal, and both before it.
+  auto edge_of = [&](bool count, u64 goal, u64 &n_before, u64 &m_before) {
+    u64 before, before2;
+    const int t = sm_cross(s, count ? n_own : m_own, count ? m_own : n_own, goal, before, before2);
+    if (tid == t) {
+      u64 n = count ? before : before2, m = count ? before2 : before;
+      int bin = tid * kSmPer;
+      for (int i = 0; i < kSmPer; ++i) {
+        const uint32_t nb = b.count[tid * kSmPer + i];
+        if (nb == 0) continue;
+        bin = tid * kSmPer + i;
+        const u64 w = bin_weight(bin);
+        if ((count ? n + nb : m + nb * w) >= goal) break;
+        n += nb;
+        m += nb * w;
+      }
+      s.r_i = bin;
+      s.r_a = n;
+      s.r_b = m;
+    }
+    __syncthreads();
+    const int bin = s.r_i;
+    n_before = s.r_a;
+    m_before = s.r_b;
+    __syncthreads();
+    return bin;
+  };
+  auto goal_of = [&](u64 total) {  // (p of zero and below: the first of the order)
+    const double want = ceil((double)ask.p * (double)total);
+    const u64 goal = want >= 1.0 ? (u64)want : 1;
+    return goal < total ? goal : total;
+  };
+
+  if constexpr (kExact) {
+    int edge = kSmEntries - 1;  // kept: the bins before it, and of its values those of index <= cut
+    int cut = 0x7fffffff;
+    u64 need = ~0ull;
+    __syncthreads();
+    if (by_k || by_p) {
+      const u64 all = sm_block_sum(s, n_own);
+      u64 total = sm_block_sum(s, m_own), n0, m0;
+      if (by_k && (u64)ask.k < all) {
+        edge = edge_of(true, (u64)ask.k, n0, m0);
+        need = (u64)ask.k - n0;
+        total = m0 + need * b.weight[edge];
+      }
+      if (by_p) {
+        const u64 goal = goal_of(total);
+        edge = edge_of(false, goal, n0, m0);
+        const u64 w = b.weight[edge];
+        need = w > 0 ? (goal - m0 + w - 1) / w : 1;
+      }
+      if (need < b.count[edge])
+        cut = sm_locate(
+            s, row,
+            [&](uint32_t bits, int) {
+              bool x = false, y = false;
+              return (u64)(sm_bin(bits, x, y) == edge);
+            },
+            [&](u64) { return need - 1; });
+    }
+    if (ask.min_p > 0.0f) {
+      __syncthreads();
+      for (int i = 0; i < kSmPer; ++i) {
+        const int bin = tid * kSmPer + i;
+        if (b.count[bin] != 0 && !((double)b.weight[bin] >= floor_w) && sm_bin_value(bin, 0) != mx) b.weight[bin] = 0;
+      }
+      __syncthreads();
+    }
+    const int at = sm_locate(
+        s, row,
+        [&](uint32_t bits, int i) -> u64 {
+          bool x = false, y = false;
+          const int bin = sm_bin(bits, x, y);
+          if (bin > edge || (bin == edge && i > cut)) return 0;
+          return b.weight[bin];
+        },
+        target);
+    if (tid == 0) a.token[r] = at;
+  } else {
+    uint32_t key = 0;  // kept: larger keys, and this one up to index `cut`
+    int cut = 0x7fffffff;
+    auto kept = [&](uint32_t k, int i) { return k > key || (k == key && i <= cut); };
+    int last = kSmEntries - 1;  // the last bin with kept logits
+    u64 n0 = 0, m0 = 0;
+    bool failed = false;     // a bin too full to rank
+    __syncthreads();
+    // The logits of `bin` that are kept into the list.
+    auto put = [&](uint32_t k, int i, u64 m) {
+      const int at = atomicAdd(&b.n, 1);
+      if (at < kSmList) {
+        b.key[at] = k;
+        b.index[at] = i;
+        b.mass[at] = m;
+      }
+    };
+    auto better = [&](int i, int j) {  // of the list, in the order
+      return b.key[i] > b.key[j] || (b.key[i] == b.key[j] && b.index[i] < b.index[j]);
+    };
+    auto decide = [&](bool mine) {  // the list's last kept logit, found by one thread
+      if (mine) {
+        s.r_a = b.key[tid];
+        s.r_i = b.index[tid];
+      }
+      __syncthreads();
+      key = (uint32_t)s.r_a;
+      cut = s.r_i;
+      __syncthreads();
+    };
+    u64 estimate = 0;
+    if (by_k || by_p) {
+      const u64 all = sm_block_sum(s, n_own);
+      estimate = sm_block_sum(s, m_own);
+      if (by_k && (u64)ask.k < all) {
+        last = edge_of(true, (u64)ask.k, n0, m0);
+        failed = b.count[last] > kSmList;
+        if (!failed) {
+          if (tid == 0) b.n = 0;
+          __syncthreads();
+          sm_each(row, 0, row.chunks, tid, kSmThreads, [&](uint32_t bits, int i) {
+            bool x = false, y = false;
+            if (sm_bin(bits, x, y) == last) put(sm_key(__builtin_bit_cast(float, bits)), i, 0);
+          });
+          __syncthreads();
+          const int n = b.n;
+          u64 rank = 0;
+          if (tid < n)
+            for (int i = 0; i < n; ++i) rank += better(i, tid);
+          decide(tid < n && rank == (u64)ask.k - n0 - 1);
+          estimate = m0 + ((u64)ask.k - n0) * bin_weight(last);
+        }
+      }
+    }
+    if (by_p && !failed) {
+      int lo = 0, hi = last;
+      u64 want = goal_of(estimate > 0 ? estimate : 1), goal = 0;
+      bool known = false;
+      for (int tries = 0;; ++tries) {
+        int g = tries < 6 ? edge_of(false, want, n0, m0) : lo + (hi - lo) / 2;
+        g = min(max(g, lo), hi);
+        failed = b.count[g] > kSmList;
+        if (failed) break;  // uniform
+        if (tid == 0) b.n = 0;
+        __syncthreads();
+        u64 above = 0, inside = 0, rest = 0;
+        sm_each(row, 0, row.chunks, tid, kSmThreads, [&](uint32_t bits, int i) {
+          bool x = false, y = false;
+          const int bin = sm_bin(bits, x, y);
+          if (bin > last || (known && bin > g)) return;
+          const float v = __builtin_bit_cast(float, bits);
+          const uint32_t k = sm_key(v);
+          if (!kept(k, i)) return;
+          const u64 m = sm_mass(weight.real(v));
+          above += bin < g ? m : 0;
+          rest += bin > g ? m : 0;
+          if (bin == g) {
+            inside += m;
+            put(k, i, m);
+          }
+        });
+        above = sm_block_sum(s, above);
+        inside = sm_block_sum(s, inside);
+        if (!known) {
+          rest = sm_block_sum(s, rest);
+          goal = goal_of(above + inside + rest);
+          known = true;
+        }
+        if (above >= goal) {
+          hi = g - 1;
+          want = m0 > above - goal ? m0 - (above - goal) : 1;
+        } else if (above + inside < goal) {
+          lo = g + 1;
+          want = m0 + b.count[g] * bin_weight(g) + (goal - above - inside);
+          want = want < estimate ? want : estimate;
+        } else {
+          const int n = b.n;
+          u64 sum = above;
+          if (tid < n)
+            for (int i = 0; i < n; ++i) sum += better(i, tid) ? b.mass[i] : 0;
+          decide(tid < n && sum < goal && sum + b.mass[tid] >= goal);
+          break;
+        }
+      }
+    }
+    int at;
+    if (failed) {
+      __syncthreads();
+      at = sm_general(lds.general, s, row, ask, mx, table);
+    } else {
+      at = sm_locate(
+          s, row,
+          [&](uint32_t bits, int i) -> u64 {
+            const float v = sm_value(bits);
+            if (!kept(sm_key(v), i) || v == -INFINITY) return 0;
+            const double w = weight.real(v);
+            return w >= floor_w || v == mx ? sm_mass(w) : 0;
+          },
+          target);
+    }
+    if (tid == 0) a.token[r] = at;
+  }
 }
 
 }  // namespace

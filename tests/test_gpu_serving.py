@@ -452,6 +452,25 @@ def test_sample_tokens_close_and_far_logits(cuda_device):
             _sampled(cuda_device, x, u, **settings)
 
 
+def test_sample_tokens_values_without_a_bin(cuda_device):
+    """Logits of tiny and large magnitude, and more fp32 logits in one bin (equal ones, and different
+    ones that share their upper 16 bits) than are ranked at once."""
+    g = torch.Generator().manual_seed(45)
+    u = torch.rand((6,), generator=g)
+    base = torch.randn((6, 9000), generator=g) * 2.0
+    tiny, large, low, shared, equal = (base.clone() for _ in range(5))
+    tiny[:, ::7] = 1e-12 * torch.randn((6, 1286), generator=g)
+    large[:, ::9] += 300.0
+    low[:, ::3] = -400.0 + torch.randn((6, 3000), generator=g)
+    shared[:, :4000] = 5.0 + torch.rand((6, 4000), generator=g) * 2.0 ** -7
+    equal[:, 3000:] = 1.25
+    for x in (tiny, large, low, shared, equal):
+        for settings in (dict(top_k=40), dict(top_k=3500), dict(top_p=0.7), dict(temperature=20.0, top_k=8000, top_p=0.97),
+                         dict(temperature=0.05, top_p=0.9), dict(min_p=0.2)):
+            _sampled(cuda_device, x, u, **settings)
+            _sampled(cuda_device, x.to(torch.bfloat16), u, **settings)
+
+
 def test_sample_tokens_masked_rows(cuda_device):
     """-inf and NaN are never drawn; rows of nothing else give -1; +inf takes all."""
     V = 3000
