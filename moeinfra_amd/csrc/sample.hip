@@ -102,21 +102,36 @@ __device__ __forceinline__ u64 sm_mass(double w) {
   return __builtin_bit_cast(u64, w + 0x1p52) & ((1ull << 52) - 1);
 }
 
-__device__ __forceinline__ u64 sm_wave_incl(u64 v, int lane) {
-  for (int o = 1; o < kWave; o <<= 1) {
-    const u64 x = __shfl_up(v, o, kWave);
-    if (lane >= o) v += x;
-  }
+// A DPP move of 64 bits; lanes without a source (and rows not in the mask) get zero.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 sm_dpp(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+  return lo | (u64)hi << 32;
+}
+__device__ __forceinline__ u64 sm_readlane(u64 v, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane) |
+         (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32;
+}
+// Inclusive sums over a row of 16 lanes (row_shr 1, 2, 4, 8), and over the wave (then lane 15 of
+// each odd row's neighbour, and lane 31, broadcast to what follows).
+__device__ __forceinline__ u64 sm_row_incl(u64 v) {
+  v += sm_dpp<0x111, 0xf>(v);
+  v += sm_dpp<0x112, 0xf>(v);
+  v += sm_dpp<0x114, 0xf>(v);
+  v += sm_dpp<0x118, 0xf>(v);
   return v;
 }
-__device__ __forceinline__ u64 sm_wave_sum(u64 v) {
-  for (int o = 1; o < kWave; o <<= 1) v += __shfl_xor(v, o, kWave);
+__device__ __forceinline__ u64 sm_wave_incl(u64 v) {
+  v = sm_row_incl(v);
+  v += sm_dpp<0x142, 0xa>(v);
+  v += sm_dpp<0x143, 0xc>(v);
   return v;
 }
+__device__ __forceinline__ u64 sm_wave_sum(u64 v) { return sm_readlane(sm_wave_incl(v), kWave - 1); }
 
 // What the workgroup's waves tell each other.
 struct SmShare {
-  u64 seg[kSmWaves];
   u64 part[kSmWaves], part2[kSmWaves];
   uint32_t bits[kSmWaves], flags[kSmWaves];
   u64 r_a, r_b;
@@ -177,53 +192,73 @@ __device__ __forceinline__ float sm_value(uint32_t bits) {
   return x == x ? x : -INFINITY;
 }
 
-// f(bits, index) of each element of chunks c0 + first, c0 + first + step, ... below c1; two more
-// chunks are on their way while one is looked at.
+// f(chunk, number) of chunks c0 + first, c0 + first + step, ... below c1 (those at the row's ends by
+// first = 0); two more are on their way while one is looked at.
 template <typename E, typename F>
-__device__ __forceinline__ void sm_each(const SmRow<E> &row, int c0, int c1, int first, int step, F f) {
-  constexpr int N = SmRow<E>::N;
+__device__ __forceinline__ void sm_chunks(const SmRow<E> &row, int c0, int c1, int first, int step, F f) {
   const int a = max(c0, row.whole0()) + first, b = min(c1, row.whole1());
   if (a < b) {
     u32x4 v0 = row.raw(a), v1 = row.raw(min(a + step, b - 1)), v2;
     for (int c = a; c < b; c += step) {
       v2 = row.raw(min(c + 2 * step, b - 1));
-#pragma unroll
-      for (int e = 0; e < N; ++e) f(SmRow<E>::bits(v0, e), row.index(c, e));
+      f(v0, c);
       v0 = v1;
       v1 = v2;
     }
   }
-  // The row's ends, where they are shared with other rows.
   if (first != 0) return;
   for (int k = 0; k < 2; ++k) {
     const int end = k == 0 ? 0 : row.chunks - 1;
     if (end < c0 || end >= c1 || (end >= row.whole0() && end < row.whole1()) || (k == 1 && row.chunks == 1)) continue;
-    const u32x4 v = row.chunk(end);
-#pragma unroll 1
-    for (int e = 0; e < N; ++e) {
-      uint32_t x = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) x = i == e ? SmRow<E>::bits(v, i) : x;
-      f(x, row.index(end, e));
-    }
+    f(row.chunk(end), end);
   }
 }
 
-// The thread (in order) in which the running sum of v reaches goal (>= 1, at most the whole sum), and
-// the sums of v and of v2 before it.  Uniform over the workgroup.
-__device__ __forceinline__ int sm_cross(SmShare &s, u64 v, u64 v2, u64 goal, u64 &before, u64 &before2) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  u64 a = sm_wave_incl(v, lane), b = sm_wave_incl(v2, lane);
+// f(bits, index) of every element of the row, shared by the workgroup's threads.
+template <typename E, typename F>
+__device__ __forceinline__ void sm_each(const SmRow<E> &row, F f) {
+  sm_chunks(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, [&](const u32x4 &v, int c) {
+#pragma unroll
+    for (int e = 0; e < SmRow<E>::N; ++e) f(SmRow<E>::bits(v, e), row.index(c, e));
+  });
+}
+
+// The largest element of a chunk (NaN gives way).
+template <typename E>
+__device__ __forceinline__ float sm_largest(const u32x4 &v) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < SmRow<E>::N; ++e) m = fmaxf(m, __builtin_bit_cast(float, SmRow<E>::bits(v, e)));
+  return m;
+}
+
+// Two sums over the threads in order: up to and with this thread's in a and b, all threads' in
+// all_a and all_b.
+struct SmScan {
+  u64 a, b, all_a, all_b;
+};
+__device__ __forceinline__ SmScan sm_scan(SmShare &s, u64 v, u64 v2) {
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  SmScan x{sm_wave_incl(v), sm_wave_incl(v2), 0, 0};
   if (lane == kWave - 1) {
-    s.part[wave] = a;
-    s.part2[wave] = b;
+    s.part[wave] = x.a;
+    s.part2[wave] = x.b;
   }
-  if (threadIdx.x == 0) s.r_i = kSmThreads - 1;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) {
-    a += s.part[w];
-    b += s.part2[w];
+  const u64 p = sm_row_incl(s.part[lane & (kSmWaves - 1)]), p2 = sm_row_incl(s.part2[lane & (kSmWaves - 1)]);
+  if (wave > 0) {
+    x.a += sm_readlane(p, wave - 1);
+    x.b += sm_readlane(p2, wave - 1);
   }
+  x.all_a = sm_readlane(p, kSmWaves - 1);
+  x.all_b = sm_readlane(p2, kSmWaves - 1);
+  __syncthreads();
+  return x;
+}
+
+// The thread in which the running sum x.a (its own part v) reaches goal (>= 1, at most all), and the
+// sums before it.  Uniform over the workgroup.
+__device__ __forceinline__ int sm_cross(SmShare &s, u64 a, u64 v, u64 b, u64 v2, u64 goal, u64 &before, u64 &before2) {
   if (a >= goal && a - v < goal) {
     s.r_i = threadIdx.x;
     s.r_a = a - v;
@@ -239,58 +274,90 @@ __device__ __forceinline__ int sm_cross(SmShare &s, u64 v, u64 v2, u64 goal, u64
 
 __device__ __forceinline__ u64 sm_block_sum(SmShare &s, u64 v) {
   v = sm_wave_sum(v);
-  if ((threadIdx.x & (kWave - 1)) == 0) s.part[threadIdx.x >> 6] = v;
+  const int lane = threadIdx.x & (kWave - 1);
+  if (lane == 0) s.part[threadIdx.x >> 6] = v;
   __syncthreads();
-  u64 sum = 0;
-  for (int w = 0; w < kSmWaves; ++w) sum += s.part[w];
+  v = sm_readlane(sm_row_incl(s.part[lane & (kSmWaves - 1)]), kSmWaves - 1);
   __syncthreads();
-  return sum;
+  return v;
 }
 
-// The first index at which the running sum of f(bits, index) over the row exceeds its target,
-// pick(whole sum); -1 if the whole sum is zero.
+// The first index at which the running weight of the row exceeds its target, pick(all of it); -1 if
+// there is none.  Elements weigh f(bits, index, equal); those for which it sets `equal` weigh `each`
+// as long as there have been no more than `need` of them.  A chunk whose largest element is below
+// `least` weighs nothing.
 template <typename E, typename F, typename P>
-__device__ __forceinline__ int sm_locate(SmShare &s, const SmRow<E> &row, F f, P pick) {
+__device__ __forceinline__ int sm_locate(SmShare &s, const SmRow<E> &row, float least, u64 need, u64 each, F f, P pick) {
   constexpr int N = SmRow<E>::N;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  auto add = [&](const u32x4 &v, int c, u64 &sum, u64 &n) {
+    if (!(sm_largest<E>(v) >= least)) return;
+    u64 m[N];
+    uint32_t k = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      bool equal = false;
+      m[e] = f(SmRow<E>::bits(v, e), row.index(c, e), equal);
+      k += equal;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum += m[e];
+    n += k;
+  };
   // A stretch of whole chunks per wave.
   const int per = (row.chunks + kSmWaves - 1) / kSmWaves;
-  u64 sum = 0;
-  sm_each(row, min(wave * per, row.chunks), min(wave * per + per, row.chunks), lane, kWave,
-          [&](uint32_t bits, int i) { sum += f(bits, i); });
+  u64 sum = 0, n = 0;
+  sm_chunks(row, min(wave * per, row.chunks), min(wave * per + per, row.chunks), lane, kWave,
+            [&](const u32x4 &v, int c) { add(v, c, sum, n); });
   sum = sm_wave_sum(sum);
-  if (lane == 0) s.seg[wave] = sum;
+  n = sm_wave_sum(n);
+  if (lane == 0) {
+    s.part[wave] = sum;
+    s.part2[wave] = n;
+  }
   __syncthreads();
-  u64 total = 0;
-  for (int w = 0; w < kSmWaves; ++w) total += s.seg[w];
-  u64 target = total > 0 ? pick(total) : 0;
-  int w = 0;
-  while (w < kSmWaves - 1 && target >= s.seg[w]) target -= s.seg[w++];
+  // Every wave: the stretches' running sums in its rows of 16 lanes, and the one with the target.
+  const u64 mine = s.part[lane & (kSmWaves - 1)], equals = s.part2[lane & (kSmWaves - 1)];
+  const u64 run_m = sm_row_incl(mine), run_n = sm_row_incl(equals);
+  const u64 upto = run_m + min(run_n, need) * each;
+  const u64 total = sm_readlane(upto, kSmWaves - 1);
   __syncthreads();
   if (total == 0) return -1;
+  u64 target = pick(total);
+  const int w = __builtin_ctzll(__ballot(upto > target));
+  if (w > 0) {
+    target -= sm_readlane(upto, w - 1);
+    need -= min(sm_readlane(run_n, w - 1), need);
+  }
   const int e0 = w * per, e1 = min(e0 + per, row.chunks);
   for (int cb = e0; cb < e1; cb += kSmThreads) {
     const int c = cb + threadIdx.x;
     u32x4 v = {0, 0, 0, 0};
-    u64 own = 0;
+    u64 own = 0, k = 0;
     if (c < e1) {
       v = row.chunk(c);
-#pragma unroll
-      for (int e = 0; e < N; ++e) own += f(SmRow<E>::bits(v, e), row.index(c, e));
+      add(v, c, own, k);
     }
-    const u64 block = sm_block_sum(s, own);
-    if (target >= block) {
-      target -= block;
+    const SmScan x = sm_scan(s, own, k);
+    const u64 here = x.all_a + min(x.all_b, need) * each;
+    if (target >= here) {
+      target -= here;
+      need -= min(x.all_b, need);
       continue;
     }
-    u64 before, dummy;
-    const int t = sm_cross(s, own, 0, target + 1, before, dummy);
-    if ((int)threadIdx.x == t) {
-      u64 run = before;
+    const u64 end = x.a + min(x.b, need) * each;
+    u64 run = x.a - own + min(x.b - k, need) * each;
+    if (run <= target && target < end) {
+      u64 left = need - min(x.b - k, need);
       int at = -1;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        run += f(SmRow<E>::bits(v, e), row.index(c, e));
+        bool equal = false;
+        run += f(SmRow<E>::bits(v, e), row.index(c, e), equal);
+        if (equal && left > 0) {
+          run += each;
+          --left;
+        }
         if (at < 0 && run > target) at = row.index(c, e);
       }
       s.r_i = at;
@@ -348,7 +415,7 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
       g.count[i] = 0;
     }
     __syncthreads();
-    sm_each(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, [&](uint32_t bits, int) {
+    sm_each(row, [&](uint32_t bits, int) {
       const float v = value(sm_value(bits));
       if (v == -INFINITY) return;
       const int b = (int)fminf(place(v), (float)(kSmBins - 1));
@@ -364,7 +431,8 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
     auto select = [&](bool count, u64 goal, uint32_t &key_out, u64 &need, u64 &ties, u64 &above, u64 &each) {
       u64 before, before2;
       const u64 own = count ? (u64)g.count[threadIdx.x] : g.mass[threadIdx.x];
-      const int b = sm_cross(s, own, g.mass[threadIdx.x], goal, before, before2);
+      const SmScan x = sm_scan(s, own, g.mass[threadIdx.x]);
+      const int b = sm_cross(s, x.a, own, x.b, g.mass[threadIdx.x], goal, before, before2);
       const float fb = (float)b;
       for (int i = threadIdx.x; i < kSmBins; i += kSmThreads) {
         g.mass2[i] = 0;
@@ -380,7 +448,7 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
         sub = (int)fminf((t - fb) * (float)kSmBins, (float)(kSmBins - 1));
         return true;
       };
-      sm_each(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, [&](uint32_t bits, int) {
+      sm_each(row, [&](uint32_t bits, int) {
         int sub;
         const float v = value(sm_value(bits));
         if (!inside(v, sub)) return;
@@ -394,7 +462,8 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
       __syncthreads();
       u64 in1, in2;
       const u64 own2 = count ? (u64)g.count2[threadIdx.x] : g.mass2[threadIdx.x];
-      const int sb = sm_cross(s, own2, g.mass2[threadIdx.x], goal - before, in1, in2);
+      const SmScan x2 = sm_scan(s, own2, g.mass2[threadIdx.x]);
+      const int sb = sm_cross(s, x2.a, own2, x2.b, g.mass2[threadIdx.x], goal - before, in1, in2);
       before += in1;
       before2 += in2;
       uint32_t lo = g.lo2[sb], hi = g.hi2[sb];
@@ -404,7 +473,7 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
       if (lo != hi) {
         auto sums = [&](uint32_t from, u64 &n, u64 &sum) {  // of the bin's values from that key on
           u64 nn = 0, ss = 0;
-          sm_each(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, [&](uint32_t bits, int) {
+          sm_each(row, [&](uint32_t bits, int) {
             int sub;
             const float v = value(sm_value(bits));
             if (!inside(v, sub) || sub != sb || sm_key(v) < from) return;
@@ -459,16 +528,19 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
     if (limited && need < ties) {
       const uint32_t kk = key;
       const u64 n = need;
-      cut = sm_locate(s, row, [&](uint32_t bits, int) {
-        const float v = value(sm_value(bits));
-        return (u64)(v != -INFINITY && sm_key(v) == kk);
-      }, [&](u64) { return n - 1; });
+      cut = sm_locate(
+          s, row, -INFINITY, 0, 0,
+          [&](uint32_t bits, int, bool &) {
+            const float v = value(sm_value(bits));
+            return (u64)(v != -INFINITY && sm_key(v) == kk);
+          },
+          [&](u64) { return n - 1; });
     }
   }
   const double floor_w = (double)a.min_p * 0x1p43;
-  const int at = sm_locate(
-      s, row,
-      [&](uint32_t bits, int i) -> u64 {
+  return sm_locate(
+      s, row, -INFINITY, 0, 0,
+      [&](uint32_t bits, int i, bool &) -> u64 {
         const float v = value(sm_value(bits));
         const uint32_t kk = sm_key(v);
         if (v == -INFINITY || kk < key || (kk == key && i > cut)) return 0;
@@ -477,40 +549,47 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
         return w >= floor_w || v == fm ? sm_mass(w) : 0;
       },
       [&](u64 total) { return sm_target(a.u, total); });
-  return at;
 }
 
 // Bins of the first histogram: the upper 16 bits of a logit (all of a bf16 one) with a magnitude in
-// [2^-32, 2^8), larger values first, zero in the middle.
+// [2^-32, 2^8), larger values first, zero in the middle; the first and the last are for what has none.
 constexpr uint32_t kSmLow = 95 << 7;               // upper 16 bits of 2^-32
 constexpr uint32_t kSmSide = (135 << 7) - kSmLow;  // bins of a sign
-constexpr int kSmEntries = 2 * kSmSide + 1;
+constexpr int kSmZero = 1 + kSmSide;
+constexpr int kSmEntries = 2 * kSmSide + 3;
 constexpr int kSmPer = (kSmEntries + kSmThreads - 1) / kSmThreads;  // 11: odd, so that threads meet no bank twice
-constexpr int kSmNone = kSmThreads * kSmPer;                          // no bin: never drawn
-constexpr int kSmList = kSmThreads;                                   // logits of one bin that are ranked directly
+constexpr int kSmNone = kSmThreads * kSmPer;
+constexpr int kSmList = kSmThreads;  // logits of one bin that are ranked directly
 
-// Upper 16 bits of a bin's values (of the smallest magnitude).
-__device__ __forceinline__ float sm_bin_value(int bin, uint32_t low_bits) {
-  uint32_t h = 0;
-  if (bin < (int)kSmSide) h = kSmLow + kSmSide - 1 - bin;
-  if (bin > (int)kSmSide) h = 0x8000u | (kSmLow + bin - kSmSide - 1);
-  return __builtin_bit_cast(float, h << 16 | (bin == (int)kSmSide ? 0u : low_bits));
+__device__ __forceinline__ uint32_t sm_upper(uint32_t bits) { return bits >> 16 & 0x7fffu; }
+
+// The bin of a logit: kSmZero -+ (upper bits - kSmLow + 1), upper bits below kSmLow taken for zero's
+// and those above the last bin's for the one after it.
+__device__ __forceinline__ int sm_bin(uint32_t bits) {
+  const uint32_t h = min(max(sm_upper(bits), kSmLow - 1), kSmLow + kSmSide);
+  const int sign = (int)bits >> 31;  // -1 below zero
+  return (int)~(h ^ (uint32_t)sign) + (sign & -(int)(2 * kSmLow - 1)) + (int)(kSmZero + kSmLow);
 }
 
-// The bin of a logit.  kSmNone for -inf and NaN; for finite values below -2^8 too, noted in `far`;
-// others without a bin (magnitudes below 2^-32, from 2^8 on) are noted in `odd`.
-__device__ __forceinline__ int sm_bin(uint32_t bits, bool &far, bool &odd) {
-  const uint32_t h = bits >> 16 & 0x7fffu, d = h - kSmLow;
-  const bool neg = (int32_t)bits < 0;
-  const int bin = neg ? (int)(kSmSide + 1 + d) : (int)(kSmSide - 1 - d);
-  if (d < kSmSide) return bin;
-  if ((bits & 0x7fffffffu) == 0) return kSmSide;
-  if ((bits & 0x7fffffffu) > 0x7f800000u || bits == 0xff800000u) return kSmNone;
-  if (neg && h >= kSmLow + kSmSide)
+// A bin's value: of the magnitude's upper bits and these lower ones.
+__device__ __forceinline__ float sm_bin_value(int bin, uint32_t low_bits) {
+  uint32_t h = 0;
+  if (bin < kSmZero) h = kSmLow - 1 + kSmZero - bin;
+  if (bin > kSmZero) h = 0x8000u | (kSmLow - 1 + bin - kSmZero);
+  return __builtin_bit_cast(float, h << 16 | (bin == kSmZero ? 0u : low_bits));
+}
+
+// Logits that sm_bin takes for others: -inf and NaN do not matter; finite ones below -2^8 are noted
+// in `far`, tiny ones and those from 2^8 on in `odd`.  Whether the logit counts in its bin.
+__device__ __forceinline__ bool sm_counts(uint32_t bits, bool &far, bool &odd) {
+  const uint32_t h = sm_upper(bits), rest = bits & 0x7fffffffu;
+  if (h - kSmLow < kSmSide || rest == 0) return true;
+  if (rest > 0x7f800000u || bits == 0xff800000u) return false;
+  if ((int)bits < 0 && h >= kSmLow + kSmSide)
     far = true;
   else
     odd = true;
-  return kSmNone;
+  return false;
 }
 
 // LDS of a row in bf16: a bin holds one value.  (127 KB)
@@ -560,15 +639,32 @@ sample_kernel(const SmArgs a) {
   float mx = -INFINITY;
   bool far = false, odd = false;
   if (greedy || (!kExact && !by_k && !by_p)) {  // no counts needed
-    sm_each(row, 0, row.chunks, tid, kSmThreads,
-            [&](uint32_t bits, int) { mx = fmaxf(mx, __builtin_bit_cast(float, bits)); });
+    sm_each(row, [&](uint32_t bits, int) { mx = fmaxf(mx, __builtin_bit_cast(float, bits)); });
   } else {
     for (int i = tid; i < kSmNone; i += kSmThreads) b.count[i] = 0;
     __syncthreads();
-    sm_each(row, 0, row.chunks, tid, kSmThreads, [&](uint32_t bits, int) {
-      mx = fmaxf(mx, __builtin_bit_cast(float, bits));  // (NaN gives way)
-      const int bin = sm_bin(bits, far, odd);
-      if (bin != kSmNone) atomicAdd(&b.count[bin], 1u);
+    sm_chunks(row, 0, row.chunks, tid, kSmThreads, [&](const u32x4 &v, int) {
+      constexpr int N = SmRow<E>::N;
+      mx = fmaxf(mx, sm_largest<E>(v));
+      // Whether all have bins: magnitudes at most the last one's, and either zero (which one less
+      // takes past all others) or the first one's at least.
+      uint32_t most = 0, least = ~0u;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const uint32_t x = SmRow<E>::bits(v, e);
+        most = max(most, sm_upper(x));
+        least = min(least, kExact ? sm_upper(x) - 1 : (x & 0x7fffffffu) - 1);
+      }
+      if (most < kSmLow + kSmSide && least >= (kExact ? kSmLow - 1 : (kSmLow << 16) - 1)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) atomicAdd(&b.count[sm_bin(SmRow<E>::bits(v, e))], 1u);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const uint32_t x = SmRow<E>::bits(v, e);
+          if (sm_counts(x, far, odd)) atomicAdd(&b.count[sm_bin(x)], 1u);
+        }
+      }
     });
   }
   {
@@ -597,7 +693,7 @@ sample_kernel(const SmArgs a) {
   }
   if (greedy) {
     const int at = sm_locate(
-        s, row, [&](uint32_t bits, int) { return (u64)(__builtin_bit_cast(float, bits) == mx); },
+        s, row, mx, 0, 0, [&](uint32_t bits, int, bool &) { return (u64)(__builtin_bit_cast(float, bits) == mx); },
         [](u64) { return (u64)0; });
     if (tid == 0) a.token[r] = at;
     return;
@@ -616,8 +712,7 @@ sample_kernel(const SmArgs a) {
   // This thread's bins: their counts, and their weight (fp32: as if all lay in the bin's middle).
   u64 n_own = 0, m_own = 0;
   // (The largest logit's bin: as if all were it, so that there is some weight.)
-  bool unused = false;
-  const int top = sm_bin(__builtin_bit_cast(uint32_t, mx), unused, unused);
+  const int top = sm_bin(__builtin_bit_cast(uint32_t, mx));
   auto bin_weight = [&](int bin) {
     return sm_mass(weight.real(bin == top ? mx : sm_bin_value(bin, kExact ? 0u : 0x8000u)));
   };
@@ -633,32 +728,38 @@ sample_kernel(const SmArgs a) {
       m_own += n * w;
     }
   }
+  const SmScan run = kExact || by_k || by_p ? sm_scan(s, n_own, m_own) : SmScan{};
   // The bin in which the running count (or weight) reaches goal, and both before it.
   auto edge_of = [&](bool count, u64 goal, u64 &n_before, u64 &m_before) {
-    u64 before, before2;
-    const int t = sm_cross(s, count ? n_own : m_own, count ? m_own : n_own, goal, before, before2);
+    u64 x, y;
+    const int t = count ? sm_cross(s, run.a, n_own, run.b, m_own, goal, x, y)
+                        : sm_cross(s, run.b, m_own, run.a, n_own, goal, y, x);
     if (tid == t) {
-      u64 n = count ? before : before2, m = count ? before2 : before;
-      int bin = tid * kSmPer;
+      int edge = tid * kSmPer;
+#pragma unroll 1
       for (int i = 0; i < kSmPer; ++i) {
-        const uint32_t nb = b.count[tid * kSmPer + i];
-        if (nb == 0) continue;
-        bin = tid * kSmPer + i;
-        const u64 w = bin_weight(bin);
-        if ((count ? n + nb : m + nb * w) >= goal) break;
-        n += nb;
-        m += nb * w;
+        const uint32_t n = b.count[tid * kSmPer + i];
+        if (n == 0) continue;
+        edge = tid * kSmPer + i;
+        u64 w;
+        if constexpr (kExact)
+          w = b.weight[edge];
+        else
+          w = bin_weight(edge);
+        if ((count ? x + n : y + n * w) >= goal) break;
+        x += n;
+        y += n * w;
       }
-      s.r_i = bin;
-      s.r_a = n;
-      s.r_b = m;
+      s.r_i = edge;
+      s.r_a = x;
+      s.r_b = y;
     }
     __syncthreads();
-    const int bin = s.r_i;
+    const int edge = s.r_i;
     n_before = s.r_a;
     m_before = s.r_b;
     __syncthreads();
-    return bin;
+    return edge;
   };
   auto goal_of = [&](u64 total) {  // (p of zero and below: the first of the order)
     const double want = ceil((double)ask.p * (double)total);
@@ -667,14 +768,12 @@ sample_kernel(const SmArgs a) {
   };
 
   if constexpr (kExact) {
-    int edge = kSmEntries - 1;  // kept: the bins before it, and of its values those of index <= cut
-    int cut = 0x7fffffff;
-    u64 need = ~0ull;
-    __syncthreads();
+    int edge = kSmEntries;  // kept: the bins before it, and the first `need` of its logits
+    u64 need = ~0ull, each = 0;
+    float least = -INFINITY;
     if (by_k || by_p) {
-      const u64 all = sm_block_sum(s, n_own);
-      u64 total = sm_block_sum(s, m_own), n0, m0;
-      if (by_k && (u64)ask.k < all) {
+      u64 total = run.all_b, n0, m0;
+      if (by_k && (u64)ask.k < run.all_a) {
         edge = edge_of(true, (u64)ask.k, n0, m0);
         need = (u64)ask.k - n0;
         total = m0 + need * b.weight[edge];
@@ -685,29 +784,26 @@ sample_kernel(const SmArgs a) {
         const u64 w = b.weight[edge];
         need = w > 0 ? (goal - m0 + w - 1) / w : 1;
       }
-      if (need < b.count[edge])
-        cut = sm_locate(
-            s, row,
-            [&](uint32_t bits, int) {
-              bool x = false, y = false;
-              return (u64)(sm_bin(bits, x, y) == edge);
-            },
-            [&](u64) { return need - 1; });
-    }
-    if (ask.min_p > 0.0f) {
-      __syncthreads();
-      for (int i = 0; i < kSmPer; ++i) {
-        const int bin = tid * kSmPer + i;
-        if (b.count[bin] != 0 && !((double)b.weight[bin] >= floor_w) && sm_bin_value(bin, 0) != mx) b.weight[bin] = 0;
+      if (b.count[edge] != 0) {
+        each = b.weight[edge];
+        least = sm_bin_value(edge, 0);
+        if (!((double)each >= floor_w) && least != mx) each = 0;
       }
-      __syncthreads();
     }
+    // Weights of what is not kept are taken as zero; the edge's are counted apart.
+    __syncthreads();
+    for (int i = 0; i < kSmPer; ++i) {
+      const int bin = tid * kSmPer + i;
+      if (b.count[bin] == 0) continue;
+      if (bin >= edge || (!((double)b.weight[bin] >= floor_w) && sm_bin_value(bin, 0) != mx)) b.weight[bin] = 0;
+    }
+    if (tid == 0) b.weight[0] = b.weight[kSmEntries - 1] = 0;  // what has no bin
+    __syncthreads();
     const int at = sm_locate(
-        s, row,
-        [&](uint32_t bits, int i) -> u64 {
-          bool x = false, y = false;
-          const int bin = sm_bin(bits, x, y);
-          if (bin > edge || (bin == edge && i > cut)) return 0;
+        s, row, least, need, each,
+        [&](uint32_t bits, int, bool &equal) -> u64 {
+          const int bin = sm_bin(bits);
+          equal = bin == edge;
           return b.weight[bin];
         },
         target);
@@ -744,17 +840,15 @@ sample_kernel(const SmArgs a) {
     };
     u64 estimate = 0;
     if (by_k || by_p) {
-      const u64 all = sm_block_sum(s, n_own);
-      estimate = sm_block_sum(s, m_own);
-      if (by_k && (u64)ask.k < all) {
+      estimate = run.all_b;
+      if (by_k && (u64)ask.k < run.all_a) {
         last = edge_of(true, (u64)ask.k, n0, m0);
         failed = b.count[last] > kSmList;
         if (!failed) {
           if (tid == 0) b.n = 0;
           __syncthreads();
-          sm_each(row, 0, row.chunks, tid, kSmThreads, [&](uint32_t bits, int i) {
-            bool x = false, y = false;
-            if (sm_bin(bits, x, y) == last) put(sm_key(__builtin_bit_cast(float, bits)), i, 0);
+          sm_each(row, [&](uint32_t bits, int i) {
+            if (sm_bin(bits) == last && sm_counts(bits, far, odd)) put(sm_key(__builtin_bit_cast(float, bits)), i, 0);
           });
           __syncthreads();
           const int n = b.n;
@@ -778,10 +872,9 @@ sample_kernel(const SmArgs a) {
         if (tid == 0) b.n = 0;
         __syncthreads();
         u64 above = 0, inside = 0, rest = 0;
-        sm_each(row, 0, row.chunks, tid, kSmThreads, [&](uint32_t bits, int i) {
-          bool x = false, y = false;
-          const int bin = sm_bin(bits, x, y);
-          if (bin > last || (known && bin > g)) return;
+        sm_each(row, [&](uint32_t bits, int i) {
+          const int bin = sm_bin(bits);
+          if (bin > last || (known && bin > g) || !sm_counts(bits, far, odd)) return;
           const float v = __builtin_bit_cast(float, bits);
           const uint32_t k = sm_key(v);
           if (!kept(k, i)) return;
@@ -822,9 +915,12 @@ sample_kernel(const SmArgs a) {
       __syncthreads();
       at = sm_general(lds.general, s, row, ask, mx, table);
     } else {
+      // The value of the last key kept (0: everything).
+      const float least =
+          key == 0 ? -INFINITY : __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
       at = sm_locate(
-          s, row,
-          [&](uint32_t bits, int i) -> u64 {
+          s, row, least, 0, 0,
+          [&](uint32_t bits, int i, bool &) -> u64 {
             const float v = sm_value(bits);
             if (!kept(sm_key(v), i) || v == -INFINITY) return 0;
             const double w = weight.real(v);
