@@ -71,30 +71,30 @@ __device__ __forceinline__ double sm_exp2(double f) {
   return fma(p, t, 1.0);
 }
 
-constexpr int kSmTable = 32;
+constexpr int kSmTable = 256;
 
-// Weights 2^(43 - y), y = (m - x) log2(e) / T: y in 32nds is n + r, |r| <= 1/2, the power of n from
-// a table of 32 and an exponent, that of r by its series to r^5 (the next term is 2^-51).  Past
-// 2^-21 of an integer's step all is zero (-inf too).
+// Weights 2^(43 - y), y = (m - x) log2(e) / T below 64 (what is further away weighs nothing, -inf too).
+// One multiply-add leaves y as a fixed-point number in the low bits: whole powers and 256ths in the
+// upper word, the rest r of a 256th in the lower.  The power of the 256ths comes from a table, that of
+// r as 1 + t + t^2 / 2 + t^3 / 6, t = -r ln(2) / 256, in fp32: off by 2^-31 of the weight.  (In 64 bits
+// throughout, from a table of 32 and to t^5, an instruction more costs 8 cycles of a wave: 250 for a
+// weight instead of 110.)
 struct SmWeight {
-  const double *table;  // 2^(-j / 32), in LDS
-  double m, c;          // c: 32 log2(e) / T
+  const double *table;  // 2^(-j / 256), in LDS
+  double m, c, most;    // c: log2(e) / T; the difference with y = 63
 
+  // (An infinite temperature still keeps -inf from weighing anything.)
+  __device__ __forceinline__ SmWeight(const double *table_, double m_, double c_)
+      : table(table_), m(m_), c(fmax(c_, 1e-290)), most(63.0 / c) {}
   __device__ __forceinline__ double real(float x) const {
-    constexpr double kRound = 0x1.8p52;  // the sum's low word is the nearest integer
-    constexpr double k = -0.69314718055994530942 / kSmTable;
-    const double y = fmin((m - (double)x) * c, 64.0 * kSmTable);
-    const double z = y + kRound;
-    const int n = (int)(uint32_t)__builtin_bit_cast(u64, z);
-    const double r = y - (z - kRound);
-    double p = k * k * k * k * k / 120;
-    p = fma(p, r, k * k * k * k / 24);
-    p = fma(p, r, k * k * k / 6);
-    p = fma(p, r, k * k / 2);
-    p = fma(p, r, k);
-    const double t = table[n & (kSmTable - 1)];
-    const double w = fma(t, p * r, t);
-    return __builtin_bit_cast(double, __builtin_bit_cast(u64, w) + ((u64)(uint32_t)(kSmBits - (n >> 5)) << 52));
+    const double d = fmin(m - (double)x, most);
+    const u64 z = __builtin_bit_cast(u64, fma(d, c, 0x1.8p12));
+    const uint32_t n = (uint32_t)(z >> 32);
+    const float t = (float)(uint32_t)z * (float)(-0.69314718055994530942 / kSmTable * 0x1p-32);
+    const float q = t * fmaf(t, fmaf(t, 1.0f / 6, 0.5f), 1.0f);
+    const double p = table[n & (kSmTable - 1)];
+    const u64 w = __builtin_bit_cast(u64, fma(p, (double)q, p));
+    return __builtin_bit_cast(double, w + ((u64)(kSmBits - (n >> 8 & 63)) << 52));
   }
 };
 // To the nearest integer (of values below 2^52).
@@ -399,7 +399,7 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
   const double m = infinite ? 0.0 : (double)mx;
   auto value = [&](float x) { return infinite ? (x == INFINITY ? 0.0f : -INFINITY) : x; };
   const double c2 = kSmLog2e / (double)a.T;
-  const SmWeight weight{table, m, c2 * kSmTable};
+  const SmWeight weight(table, m, c2);
   const float fm = (float)m;
   const double bs = c2 * (kSmBins / kSmSpan);
   const float bin_scale = bs < 1e30 ? (float)bs : 1e30f;
@@ -600,9 +600,8 @@ struct SmExact {
 // LDS of a row in fp32: one bin's logits are ranked. (61 KB)
 struct SmRanked {
   uint32_t count[kSmNone];
+  u64 rank[kSmList];  // key and index: better logits have larger ones
   u64 mass[kSmList];
-  uint32_t key[kSmList];
-  int index[kSmList];
   int n;
 };
 
@@ -676,16 +675,14 @@ sample_kernel(const SmArgs a) {
       s.flags[wave] = flags;
     }
     if (tid < kSmTable)
-      table[tid] = tid <= kSmTable / 2 ? sm_exp2(-tid / 32.0) : 0.5 * sm_exp2(1.0 - tid / 32.0);
+      table[tid] = tid <= kSmTable / 2 ? sm_exp2(-tid / (double)kSmTable) : 0.5 * sm_exp2(1.0 - tid / (double)kSmTable);
     __syncthreads();
-    mx = -INFINITY;
-    uint32_t all = 0;
-    for (int w = 0; w < kSmWaves; ++w) {
-      mx = fmaxf(mx, __builtin_bit_cast(float, s.bits[w]));
-      all |= s.flags[w];
-    }
-    far = all & 1u;
-    odd = all & 2u;
+    v[0] = __builtin_bit_cast(float, s.bits[lane & (kSmWaves - 1)]);
+    const uint32_t f = s.flags[lane & (kSmWaves - 1)];
+    lane_groups_reduce<true>(v, kSmWaves);
+    mx = v[0];
+    far = __any(f & 1u);
+    odd = __any(f & 2u);
   }
   if (mx == -INFINITY) {  // nothing to choose from
     if (tid == 0) a.token[r] = -1;
@@ -705,11 +702,13 @@ sample_kernel(const SmArgs a) {
     if (tid == 0) a.token[r] = at;
     return;
   }
-  const SmWeight weight{table, (double)mx, c2 * kSmTable};
+  const SmWeight weight(table, (double)mx, c2);
   const double floor_w = (double)ask.min_p * 0x1p43;
   auto target = [&](u64 total) { return sm_target(ask.u, total); };
 
   // This thread's bins: their counts, and their weight (fp32: as if all lay in the bin's middle).
+  uint32_t n_bin[kSmPer];
+  u64 w_bin[kSmPer];
   u64 n_own = 0, m_own = 0;
   // (The largest logit's bin: as if all were it, so that there is some weight.)
   const int top = sm_bin(__builtin_bit_cast(uint32_t, mx));
@@ -717,15 +716,16 @@ sample_kernel(const SmArgs a) {
     return sm_mass(weight.real(bin == top ? mx : sm_bin_value(bin, kExact ? 0u : 0x8000u)));
   };
   if (kExact || by_k || by_p) {
-#pragma unroll 1
+#pragma unroll
+    for (int i = 0; i < kSmPer; ++i) n_bin[i] = b.count[tid * kSmPer + i];
+#pragma unroll
     for (int i = 0; i < kSmPer; ++i) {
-      const int bin = tid * kSmPer + i;
-      const uint32_t n = b.count[bin];
-      if (n == 0) continue;
-      const u64 w = bin_weight(bin);
-      if constexpr (kExact) b.weight[bin] = w;
-      n_own += n;
-      m_own += n * w;
+      w_bin[i] = 0;
+      if (n_bin[i] == 0) continue;
+      w_bin[i] = bin_weight(tid * kSmPer + i);
+      if constexpr (kExact) b.weight[tid * kSmPer + i] = w_bin[i];
+      n_own += n_bin[i];
+      m_own += n_bin[i] * w_bin[i];
     }
   }
   const SmScan run = kExact || by_k || by_p ? sm_scan(s, n_own, m_own) : SmScan{};
@@ -736,19 +736,15 @@ sample_kernel(const SmArgs a) {
                         : sm_cross(s, run.b, m_own, run.a, n_own, goal, y, x);
     if (tid == t) {
       int edge = tid * kSmPer;
-#pragma unroll 1
+      bool found = false;
+#pragma unroll
       for (int i = 0; i < kSmPer; ++i) {
-        const uint32_t n = b.count[tid * kSmPer + i];
-        if (n == 0) continue;
+        if (found || n_bin[i] == 0) continue;
         edge = tid * kSmPer + i;
-        u64 w;
-        if constexpr (kExact)
-          w = b.weight[edge];
-        else
-          w = bin_weight(edge);
-        if ((count ? x + n : y + n * w) >= goal) break;
-        x += n;
-        y += n * w;
+        const u64 m = n_bin[i] * w_bin[i];
+        found = (count ? x + n_bin[i] : y + m) >= goal;
+        x += found ? 0 : n_bin[i];
+        y += found ? 0 : m;
       }
       s.r_i = edge;
       s.r_a = x;
@@ -792,10 +788,11 @@ sample_kernel(const SmArgs a) {
     }
     // Weights of what is not kept are taken as zero; the edge's are counted apart.
     __syncthreads();
+#pragma unroll
     for (int i = 0; i < kSmPer; ++i) {
       const int bin = tid * kSmPer + i;
-      if (b.count[bin] == 0) continue;
-      if (bin >= edge || (!((double)b.weight[bin] >= floor_w) && sm_bin_value(bin, 0) != mx)) b.weight[bin] = 0;
+      if (n_bin[i] != 0 && (bin >= edge || (!((double)w_bin[i] >= floor_w) && sm_bin_value(bin, 0) != mx)))
+        b.weight[bin] = 0;
     }
     if (tid == 0) b.weight[0] = b.weight[kSmEntries - 1] = 0;  // what has no bin
     __syncthreads();
@@ -809,33 +806,29 @@ sample_kernel(const SmArgs a) {
         target);
     if (tid == 0) a.token[r] = at;
   } else {
-    uint32_t key = 0;  // kept: larger keys, and this one up to index `cut`
+    float least = -INFINITY;  // kept: larger logits, and this one up to index `cut`
     int cut = 0x7fffffff;
-    auto kept = [&](uint32_t k, int i) { return k > key || (k == key && i <= cut); };
-    int last = kSmEntries - 1;  // the last bin with kept logits
+    auto kept = [&](float x, int i) { return (x > least) | ((x == least) & (i <= cut)); };
+    int last = kSmEntries - 2;  // the last bin with kept logits
     u64 n0 = 0, m0 = 0;
     bool failed = false;     // a bin too full to rank
     __syncthreads();
-    // The logits of `bin` that are kept into the list.
+    // The smallest logit of a bin.
+    auto bin_floor = [&](int bin) { return sm_bin_value(bin, bin > kSmZero ? 0xffffu : 0u); };
+    // A logit of the bin that is ranked into the list.
     auto put = [&](uint32_t k, int i, u64 m) {
       const int at = atomicAdd(&b.n, 1);
       if (at < kSmList) {
-        b.key[at] = k;
-        b.index[at] = i;
+        b.rank[at] = (u64)k << 32 | (uint32_t)~i;
         b.mass[at] = m;
       }
     };
-    auto better = [&](int i, int j) {  // of the list, in the order
-      return b.key[i] > b.key[j] || (b.key[i] == b.key[j] && b.index[i] < b.index[j]);
-    };
     auto decide = [&](bool mine) {  // the list's last kept logit, found by one thread
-      if (mine) {
-        s.r_a = b.key[tid];
-        s.r_i = b.index[tid];
-      }
+      if (mine) s.r_a = b.rank[tid];
       __syncthreads();
-      key = (uint32_t)s.r_a;
-      cut = s.r_i;
+      const uint32_t key = (uint32_t)(s.r_a >> 32);
+      cut = (int)~(uint32_t)s.r_a;
+      least = __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
       __syncthreads();
     };
     u64 estimate = 0;
@@ -853,8 +846,11 @@ sample_kernel(const SmArgs a) {
           __syncthreads();
           const int n = b.n;
           u64 rank = 0;
-          if (tid < n)
-            for (int i = 0; i < n; ++i) rank += better(i, tid);
+          if (tid < n) {
+            const u64 mine = b.rank[tid];
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) rank += b.rank[i] > mine;
+          }
           decide(tid < n && rank == (u64)ask.k - n0 - 1);
           estimate = m0 + ((u64)ask.k - n0) * bin_weight(last);
         }
@@ -871,26 +867,41 @@ sample_kernel(const SmArgs a) {
         if (failed) break;  // uniform
         if (tid == 0) b.n = 0;
         __syncthreads();
-        u64 above = 0, inside = 0, rest = 0;
-        sm_each(row, [&](uint32_t bits, int i) {
-          const int bin = sm_bin(bits);
-          if (bin > last || (known && bin > g) || !sm_counts(bits, far, odd)) return;
-          const float v = __builtin_bit_cast(float, bits);
-          const uint32_t k = sm_key(v);
-          if (!kept(k, i)) return;
-          const u64 m = sm_mass(weight.real(v));
-          above += bin < g ? m : 0;
-          rest += bin > g ? m : 0;
-          if (bin == g) {
-            inside += m;
-            put(k, i, m);
+        u64 above = 0, inside = 0, all = 0;
+        const float in_bin = bin_floor(g), over = bin_floor(g - 1);
+        sm_chunks(row, 0, row.chunks, tid, kSmThreads, [&](const u32x4 &v, int c) {
+          constexpr int N = SmRow<E>::N;
+          const float top = sm_largest<E>(v);
+          if (!(top >= least)) return;
+          float x[N];
+          u64 m[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) {  // (no branches: the elements' chains of 64-bit steps overlap)
+            x[e] = __builtin_bit_cast(float, SmRow<E>::bits(v, e));
+            m[e] = sm_mass(weight.real(x[e]));
+          }
+          if (least != -INFINITY) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) m[e] = kept(x[e], row.index(c, e)) ? m[e] : 0;
+          }
+#pragma unroll
+          for (int e = 0; e < N; ++e) all += m[e];
+          if (top >= in_bin) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              above += x[e] >= over ? m[e] : 0;
+              if (x[e] >= in_bin && !(x[e] >= over) && kept(x[e], row.index(c, e))) {
+                inside += m[e];
+                put(sm_key(x[e]), row.index(c, e), m[e]);
+              }
+            }
           }
         });
-        above = sm_block_sum(s, above);
-        inside = sm_block_sum(s, inside);
+        const SmScan both = sm_scan(s, above, inside);
+        above = both.all_a;
+        inside = both.all_b;
         if (!known) {
-          rest = sm_block_sum(s, rest);
-          goal = goal_of(above + inside + rest);
+          goal = goal_of(sm_block_sum(s, all));
           known = true;
         }
         if (above >= goal) {
@@ -903,8 +914,11 @@ sample_kernel(const SmArgs a) {
         } else {
           const int n = b.n;
           u64 sum = above;
-          if (tid < n)
-            for (int i = 0; i < n; ++i) sum += better(i, tid) ? b.mass[i] : 0;
+          if (tid < n) {
+            const u64 mine = b.rank[tid];
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) sum += b.rank[i] > mine ? b.mass[i] : 0;
+          }
           decide(tid < n && sum < goal && sum + b.mass[tid] >= goal);
           break;
         }
@@ -915,16 +929,14 @@ sample_kernel(const SmArgs a) {
       __syncthreads();
       at = sm_general(lds.general, s, row, ask, mx, table);
     } else {
-      // The value of the last key kept (0: everything).
-      const float least =
-          key == 0 ? -INFINITY : __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
       at = sm_locate(
           s, row, least, 0, 0,
           [&](uint32_t bits, int i, bool &) -> u64 {
-            const float v = sm_value(bits);
-            if (!kept(sm_key(v), i) || v == -INFINITY) return 0;
-            const double w = weight.real(v);
-            return w >= floor_w || v == mx ? sm_mass(w) : 0;
+            const float x = __builtin_bit_cast(float, bits);
+            const double w = weight.real(x);
+            bool in = kept(x, i);
+            if (floor_w > 0.0) in &= (w >= floor_w) | (x == mx);
+            return in ? sm_mass(w) : 0;
           },
           target);
     }
