@@ -16,16 +16,21 @@ constexpr int kPaTile = 32;           // keys per wave and step
 constexpr int kPaWaves = 4;
 constexpr int kPaThreads = kPaWaves * kWave;
 constexpr int kPaCols = 16;           // query heads per workgroup at most
-constexpr int kPaMaxSplits = 128;     // workgroups that share a sequence's keys, per head group
+constexpr int kPaMaxSplits = 64;      // workgroups that share a sequence's keys, per head group
+constexpr int kPaJoin = 16;
 constexpr int kPaMinTiles = 2 * kPaWaves;
 constexpr int64_t kPaCounterBytes = 65536;  // arrival counters at the start of the workspace
 constexpr float kPaLog2e = 1.44269504088896341f;
 
-__device__ __forceinline__ void pa_put(float *p, float v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Partial results pass between workgroups (of other XCDs) through device-scope accesses, two
+// floats at a time.
+__device__ __forceinline__ void pa_put(float *p, float x, float y) {
+  __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint32_t, x) | (uint64_t)__builtin_bit_cast(uint32_t, y) << 32,
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float pa_get(const float *p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ float2 pa_get(const float *p) {
+  const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32)));
 }
 
 // Whether this workgroup is the last of n to arrive at *count, which it then leaves zero.  What
@@ -61,13 +66,27 @@ struct PaArgs {
   int share;  // workgroups per head group that a full batch aims at (1 << 30: no splitting)
 };
 
-__device__ __forceinline__ int pa_wave_sum(int v) {
-  for (int o = 1; o < kWave; o <<= 1) v += __shfl_xor(v, o, kWave);
-  return v;
+// Inclusive sum and maximum (of values of 0 and above) over the wave: row_shr 1, 2, 4, 8 within 16
+// lanes, then lane 15 and lane 31 broadcast to what follows.  The last lane's are the wave's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int pa_dpp(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ int pa_wave_max(int v) {
-  for (int o = 1; o < kWave; o <<= 1) v = max(v, __shfl_xor(v, o, kWave));
-  return v;
+__device__ __forceinline__ int pa_incl(int v) {
+  v += pa_dpp<0x111, 0xf>(v);
+  v += pa_dpp<0x112, 0xf>(v);
+  v += pa_dpp<0x114, 0xf>(v);
+  v += pa_dpp<0x118, 0xf>(v);
+  v += pa_dpp<0x142, 0xa>(v);
+  return v + pa_dpp<0x143, 0xc>(v);
+}
+__device__ __forceinline__ int pa_max(int v) {
+  v = max(v, pa_dpp<0x111, 0xf>(v));
+  v = max(v, pa_dpp<0x112, 0xf>(v));
+  v = max(v, pa_dpp<0x114, 0xf>(v));
+  v = max(v, pa_dpp<0x118, 0xf>(v));
+  v = max(v, pa_dpp<0x142, 0xa>(v));
+  return max(v, pa_dpp<0x143, 0xc>(v));
 }
 
 // Which keys a workgroup takes.  Every sequence has ceil(tiles / chunk) items of at most `chunk`
@@ -90,8 +109,8 @@ __device__ __forceinline__ bool pa_item(const PaArgs &a, int item, int lane, PaI
     total += t;
     most = max(most, t);
   }
-  total = __builtin_amdgcn_readfirstlane(pa_wave_sum(total));
-  most = __builtin_amdgcn_readfirstlane(pa_wave_max(most));
+  total = __builtin_amdgcn_readlane(pa_incl(total), kWave - 1);
+  most = __builtin_amdgcn_readlane(pa_max(most), kWave - 1);
   uint32_t chunk = ((uint32_t)total + a.share - 1) / (uint32_t)a.share;
   chunk = max(chunk, (uint32_t)kPaMinTiles);
   chunk = max(chunk, ((uint32_t)most + kPaMaxSplits - 1) / kPaMaxSplits);
@@ -101,11 +120,7 @@ __device__ __forceinline__ bool pa_item(const PaArgs &a, int item, int lane, PaI
     const int n = keys(i0 + lane);
     const uint32_t t = ((uint32_t)n + kPaTile - 1) / kPaTile;
     const int c = i0 + lane < a.B ? max(1, (int)((t + chunk - 1) / chunk)) : 0;
-    int incl = c;
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int v = __shfl_up(incl, o, kWave);
-      if (lane >= o) incl += v;
-    }
+    const int incl = pa_incl(c);
     const uint64_t hit = __ballot(item < base + incl);
     if (hit != 0) {
       const int l = __builtin_ctzll(hit);
@@ -140,7 +155,7 @@ __device__ __forceinline__ bool pa_item(const PaArgs &a, int item, int lane, PaI
 //
 // Bound: HBM (at 4 heads a group the products are 5 % of the matrix rate).
 template <int HD>
-__global__ void __launch_bounds__(kPaThreads)
+__global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 3)
 paged_attention_kernel(const PaArgs a) {
   constexpr int kSteps = HD / 32;   // products of S per row tile
   constexpr int E = HD / 16;        // dims per lane of V
@@ -148,6 +163,7 @@ paged_attention_kernel(const PaArgs a) {
   __shared__ __attribute__((aligned(16))) float s_o[kPaWaves][kPaCols * kPad];
   __shared__ float s_m[kPaWaves][kPaCols], s_l[kPaWaves][kPaCols];
   __shared__ float s_w[kPaCols][kPaMaxSplits];
+  static_assert(kPaMaxSplits == kWave, "a lane per partial result");
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int H = a.nkv * a.qtiles;
@@ -308,57 +324,64 @@ paged_attention_kernel(const PaArgs a) {
   __syncthreads();
   const int64_t mine = (int64_t)blockIdx.x * min(a.grp, kPaCols) * (HD + 2);
   uint16_t *const orow = a.out + ((int64_t)w.seq * a.nq + head0) * HD;
-  for (int i = threadIdx.x; i < ncol * HD; i += kPaThreads) {
-    const int c = i / HD, d = i - c * HD;
+  for (int i = threadIdx.x; i < ncol * (HD / 2); i += kPaThreads) {
+    const int c = i / (HD / 2), d = 2 * (i - c * (HD / 2));
     float mm = s_m[0][c];
 #pragma unroll
     for (int y = 1; y < kPaWaves; ++y) mm = fmaxf(mm, s_m[y][c]);
     const float mref = mm == -INFINITY ? 0.0f : mm;
-    float o = 0.0f, ll = 0.0f;
+    float o0 = 0.0f, o1 = 0.0f, ll = 0.0f;
 #pragma unroll
     for (int y = 0; y < kPaWaves; ++y) {
       const float f = __builtin_amdgcn_exp2f((s_m[y][c] - mref) * kPaLog2e);
-      o = fmaf(f, s_o[y][c * kPad + d], o);
+      const float2 o = *reinterpret_cast<const float2 *>(&s_o[y][c * kPad + d]);
+      o0 = fmaf(f, o.x, o0);
+      o1 = fmaf(f, o.y, o1);
       ll = fmaf(f, s_l[y][c], ll);
     }
-    if (w.nact == 1) {
-      orow[i] = f32_to_bf16(ll == 0.0f ? 0.0f : o / ll);  // no key at all: zeros
+    if (w.nact == 1) {  // (no key at all: zeros)
+      const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+      *reinterpret_cast<uint32_t *>(orow + c * HD + d) = pack_bf16x2(o0 * inv, o1 * inv);
     } else {
       float *const p = a.part + mine + c * (HD + 2);
-      pa_put(p + d, o);
-      if (d == 0) {
-        pa_put(p + HD, mm);
-        pa_put(p + HD + 1, ll);
-      }
+      pa_put(p + d, o0, o1);
+      if (d == 0) pa_put(p + HD, mm, ll);
     }
   }
   if (w.nact == 1) return;
   if (!pa_last_of(a.count + (int64_t)w.seq * H + unit, w.nact)) return;
-  // The last of the sequence's workgroups adds their results up, in the order of the keys.
+  // The last of the sequence's workgroups adds their results up, in the order of the keys: the
+  // weights of the partial results first, then a thread takes two neighbouring values, kPaJoin
+  // partial results under way at a time.
   const int64_t step = (int64_t)H * min(a.grp, kPaCols) * (HD + 2);  // from one item to the next
   const float *const first = a.part + mine - w.split * step;
-  for (int i = threadIdx.x; i < ncol * w.nact; i += kPaThreads) {
-    const int y = i / ncol, c = i - y * ncol;
-    s_w[c][y] = pa_get(first + y * step + c * (HD + 2) + HD);
+  for (int c = wave; c < ncol; c += kPaWaves) {
+    const bool has = lane < w.nact;
+    const float2 ml = has ? pa_get(first + lane * step + c * (HD + 2) + HD) : make_float2(-INFINITY, 0.0f);
+    float mx[1] = {ml.x};
+    lane_groups_reduce<true>(mx, kWave);
+    const float f = __builtin_amdgcn_exp2f((ml.x - (mx[0] == -INFINITY ? 0.0f : mx[0])) * kPaLog2e);
+    float ll[1] = {has ? f * ml.y : 0.0f};
+    lane_groups_reduce<false>(ll, kWave);
+    s_w[c][lane] = ll[0] == 0.0f ? 0.0f : f / ll[0];
   }
   __syncthreads();
-  if (threadIdx.x < ncol) {
-    float mm = -INFINITY;
-    for (int y = 0; y < w.nact; ++y) mm = fmaxf(mm, s_w[threadIdx.x][y]);
-    s_m[0][threadIdx.x] = mm == -INFINITY ? 0.0f : mm;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < ncol * HD; i += kPaThreads) {
-    const int c = i / HD, d = i - c * HD;
-    const float *p = first + c * (HD + 2);
-    float o = 0.0f, ll = 0.0f;
-#pragma unroll 4
-    for (int y = 0; y < w.nact; ++y) {
-      const float f = __builtin_amdgcn_exp2f((s_w[c][y] - s_m[0][c]) * kPaLog2e);
-      o = fmaf(f, pa_get(p + y * step + d), o);
-      ll = fmaf(f, pa_get(p + y * step + HD + 1), ll);
+  for (int i = threadIdx.x; i < ncol * (HD / 2); i += kPaThreads) {
+    const int c = i / (HD / 2), d = 2 * (i - c * (HD / 2));
+    const float *p = first + c * (HD + 2) + d;
+    float o0 = 0.0f, o1 = 0.0f;
+    for (int y0 = 0; y0 < w.nact; y0 += kPaJoin) {
+      float2 po[kPaJoin];
+#pragma unroll
+      for (int y = 0; y < kPaJoin; ++y) po[y] = y0 + y < w.nact ? pa_get(p + (y0 + y) * step) : make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int y = 0; y < kPaJoin; ++y) {
+        const float f = s_w[c][min(y0 + y, kPaMaxSplits - 1)];
+        o0 = y0 + y < w.nact ? fmaf(f, po[y].x, o0) : o0;
+        o1 = y0 + y < w.nact ? fmaf(f, po[y].y, o1) : o1;
+      }
     }
-    orow[i] = f32_to_bf16(ll == 0.0f ? 0.0f : o / ll);
+    *reinterpret_cast<uint32_t *>(orow + c * HD + d) = pack_bf16x2(o0, o1);
   }
 }
 
@@ -416,8 +439,8 @@ extern "C" int moe_paged_attention_bf16(const void *q, int64_t q_stride, const v
   if (B == 0) return MOE_STATUS_OK;
   MOE_REQUIRE(q && lens_i32 && out && (page_table_i32 || table_width == 0) && ((k_cache && v_cache) || num_pages == 0),
               "null pointer");
-  MOE_REQUIRE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (uintptr_t)out % 2 == 0,
-              "q and the caches must be 16-byte aligned");
+  MOE_REQUIRE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (uintptr_t)out % 4 == 0,
+              "q and the caches must be 16-byte aligned, out 4-byte");
   const int64_t ob = 2 * B * row, cb = num_pages > 0 ? 2 * ((num_pages - 1) * page_stride + page_row) : 0;
   MOE_REQUIRE(!moe::ranges_overlap(out, ob, q, 2 * (q_stride * (B - 1) + row)) &&
                   !moe::ranges_overlap(out, ob, k_cache, cb) && !moe::ranges_overlap(out, ob, v_cache, cb),
