@@ -15,10 +15,14 @@ namespace {
 constexpr int kPaTile = 32;           // keys per wave and step
 constexpr int kPaWaves = 4;
 constexpr int kPaThreads = kPaWaves * kWave;
+// Workgroups that a CU's registers hold (of 256 dims two would spill: 16 sequences of 4000 keys 81 us
+// instead of 71).
+constexpr int pa_resident(int hd) { return hd == 64 ? 4 : hd == 128 ? 3 : 1; }
 constexpr int kPaCols = 16;           // query heads per workgroup at most
 constexpr int kPaMaxSplits = 64;      // workgroups that share a sequence's keys, per head group
-constexpr int kPaJoin = 16;
+constexpr int kPaJoin = 8;            // partial results that a thread has under way at a time
 constexpr int kPaMinTiles = 2 * kPaWaves;
+constexpr int kPaStart = 4;           // tiles' time that beginning a sequence takes
 constexpr int64_t kPaCounterBytes = 65536;  // arrival counters at the start of the workspace
 constexpr float kPaLog2e = 1.44269504088896341f;
 
@@ -63,7 +67,7 @@ struct PaArgs {
   uint16_t *out;
   uint32_t *count;
   float *part;
-  int share;  // workgroups per head group that a full batch aims at (1 << 30: no splitting)
+  int share;  // workgroups per head group that a batch is shared by (0: a sequence each)
 };
 
 // Inclusive sum and maximum (of values of 0 and above) over the wave: row_shr 1, 2, 4, 8 within 16
@@ -89,59 +93,58 @@ __device__ __forceinline__ int pa_max(int v) {
   return max(v, pa_dpp<0x143, 0xc>(v));
 }
 
-// Which keys a workgroup takes.  Every sequence has ceil(tiles / chunk) items of at most `chunk`
-// tiles (one without keys: an item that writes zeros), the chunk such that all items of a head
-// group are about `share`: as the lengths are known on the device only, each wave adds them up and
-// finds the item's sequence by a scan over the batch.  At most share + B items.
+// What the workgroups of a head group share, by the lengths, which are known on the device only (each
+// wave adds them up for itself):
+//   - a sequence each (per = 0), while the longest is at most half as long again as a fair share, or
+//     short (300 keys: 7 us, two parts 9);
+//   - parts of `per` tiles of a sequence each, if there are workgroups for all of them;
+//   - else all tiles, one sequence behind the other, each behind kPaStart of nothing (what it costs to
+//     begin one), `per` of it all for each workgroup, so that all are busy to the end.
+// 64 sequences of 500 keys: 25 us as the first, 35 as the second; 40 of 1 to 9000: 102 us as the
+// third, 112 as the second; 16 of 500: 12 us as the second, 15 as the third.
 struct PaItem {
-  int seq, n;         // sequence, its keys
-  int split, nact;    // this item's number and the count of them
-  int tile0, tile1;
+  int seq, n;          // sequence, its keys
+  int tile0, tile1;    // this workgroup's tiles of it
+  int head, split, nact;  // workgroups head .. head + nact - 1 share it, this one is head + split
+  bool inside;         // it starts inside workgroup head's tiles, not with them
 };
 
-__device__ __forceinline__ bool pa_item(const PaArgs &a, int item, int lane, PaItem &w) {
-  const int64_t cap64 = a.num_pages > 0 ? a.width << a.page_shift : 0;
-  const int cap = (int)(cap64 < 0x7fffffc0 ? cap64 : 0x7fffffc0);
-  auto keys = [&](int i) { return i < a.B ? min(max(a.lens[i], 0), cap) : 0; };
+struct PaPlan {
+  int per, total;
+  bool aligned;  // the second form
+};
+
+__device__ __forceinline__ int pa_keys(const PaArgs &a, int i) {
+  const int64_t all = a.num_pages > 0 ? a.width << a.page_shift : 0;
+  return i < a.B ? min(max(a.lens[i], 0), (int)(all < 0x7fffffc0 ? all : 0x7fffffc0)) : 0;
+}
+__device__ __forceinline__ int pa_tiles(int keys) { return (int)(((uint32_t)keys + kPaTile - 1) / kPaTile); }
+
+__device__ __forceinline__ PaPlan pa_plan(const PaArgs &a, int lane) {
+  if (a.share == 0) return {0, 0, false};
   int total = 0, most = 0;
   for (int i0 = 0; i0 < a.B; i0 += kWave) {
-    const int t = (keys(i0 + lane) + kPaTile - 1) / kPaTile;
+    const int t = pa_tiles(pa_keys(a, i0 + lane));
     total += t;
     most = max(most, t);
   }
   total = __builtin_amdgcn_readlane(pa_incl(total), kWave - 1);
   most = __builtin_amdgcn_readlane(pa_max(most), kWave - 1);
-  uint32_t chunk = ((uint32_t)total + a.share - 1) / (uint32_t)a.share;
-  chunk = max(chunk, (uint32_t)kPaMinTiles);
-  chunk = max(chunk, ((uint32_t)most + kPaMaxSplits - 1) / kPaMaxSplits);
-  if (a.share == (1 << 30)) chunk = 0x7fffffff;
-  int base = 0;
-  for (int i0 = 0; i0 < a.B; i0 += kWave) {
-    const int n = keys(i0 + lane);
-    const uint32_t t = ((uint32_t)n + kPaTile - 1) / kPaTile;
-    const int c = i0 + lane < a.B ? max(1, (int)((t + chunk - 1) / chunk)) : 0;
-    const int incl = pa_incl(c);
-    const uint64_t hit = __ballot(item < base + incl);
-    if (hit != 0) {
-      const int l = __builtin_ctzll(hit);
-      const int cl = __builtin_amdgcn_readlane(c, l);
-      w.seq = i0 + l;
-      w.n = __builtin_amdgcn_readlane(n, l);
-      w.split = item - (base + __builtin_amdgcn_readlane(incl, l) - cl);
-      const int tiles = (w.n + kPaTile - 1) / kPaTile;
-      const int per = max(1, (tiles + cl - 1) / cl);
-      w.nact = max(1, (tiles + per - 1) / per);
-      w.tile0 = w.split * per;
-      w.tile1 = min(w.tile0 + per, tiles);
-      return w.split < w.nact;
-    }
-    base += __builtin_amdgcn_readlane(incl, kWave - 1);
-  }
-  return false;
+  const int fair = (int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share);
+  if (most <= kPaMinTiles + kPaMinTiles / 2 || most <= fair + fair / 2) return {0, 0, false};
+  // (A sequence meets at most kPaMaxSplits workgroups, also where it starts inside the tiles of one.)
+  const uint32_t per = max(max(fair, kPaMinTiles), (most + kPaMaxSplits - 3) / (kPaMaxSplits - 2));
+  int parts = 0;
+  for (int i0 = 0; i0 < a.B; i0 += kWave)
+    parts += i0 + lane < a.B ? max(1, (int)((pa_tiles(pa_keys(a, i0 + lane)) + per - 1) / per)) : 0;
+  parts = __builtin_amdgcn_readlane(pa_incl(parts), kWave - 1);
+  if (parts <= a.share) return {(int)per, parts * (int)per, true};
+  total += kPaStart * a.B;
+  return {(int)max(per, ((uint32_t)total + a.share - 1) / (uint32_t)a.share), total, false};
 }
 
-// A workgroup takes up to 16 query heads of one KV head of one sequence against a range of its
-// keys, its four waves every fourth tile of 32.  All operands come straight from memory into the
+// A workgroup takes up to 16 query heads of one KV head against its tiles, its four waves every
+// fourth tile (32 keys) of a sequence.  All operands come straight from memory into the
 // matrix instructions' registers:
 //
 //   S = K Q^T   two 16x16x32 row tiles; lane l loads row l % 16 of each, dims 32 s + 8 (l / 16) .. + 7.
@@ -155,7 +158,7 @@ __device__ __forceinline__ bool pa_item(const PaArgs &a, int item, int lane, PaI
 //
 // Bound: HBM (at 4 heads a group the products are 5 % of the matrix rate).
 template <int HD>
-__global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 3)
+__global__ void __launch_bounds__(kPaThreads, pa_resident(HD))
 paged_attention_kernel(const PaArgs a) {
   constexpr int kSteps = HD / 32;   // products of S per row tile
   constexpr int E = HD / 16;        // dims per lane of V
@@ -167,28 +170,30 @@ paged_attention_kernel(const PaArgs a) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int H = a.nkv * a.qtiles;
-  const int item = (int)(blockIdx.x / (unsigned)H), unit = (int)(blockIdx.x - (unsigned)item * H);
+  const int wg = (int)(blockIdx.x / (unsigned)H), unit = (int)(blockIdx.x - (unsigned)wg * H);
   const int kvh = unit / a.qtiles, col0 = (unit - kvh * a.qtiles) * kPaCols;
   const int ncol = min(a.grp - col0, kPaCols);
-  PaItem w;
-  if (!pa_item(a, item, lane, w)) return;  // the same for the whole workgroup
-
+  const PaPlan plan = pa_plan(a, lane);
+  // This workgroup's part of it all.  (A sequence without keys is where its start is.)
+  const int begin = min(wg, a.share) * plan.per, end = begin + plan.per;
+  if (plan.per > 0 ? wg >= a.share || begin >= plan.total : wg >= a.B) return;
   const int g = lane >> 4, r = lane & 15;
+  const int64_t head_at = ((int64_t)kvh * HD) << a.page_shift;
+  const int pmask = (1 << a.page_shift) - 1;
+  const int head0 = kvh * a.grp + col0;
+  auto good = [&](int p) { return (uint32_t)p < (uint64_t)a.num_pages; };
+  const int gk = (r >> 2) * 8, gv = g * 8;
+  auto sequence = [&](const PaItem &w, bool later) __attribute__((always_inline)) {
   // Q as the B operand: column r (columns past the group repeat the last one and are dropped).
   u32x4 qf[kSteps];
-  const int head0 = kvh * a.grp + col0;
   {
     const uint16_t *qr = a.q + w.seq * a.q_stride + (int64_t)(head0 + min(r, ncol - 1)) * HD + 8 * g;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) qf[s] = *reinterpret_cast<const u32x4 *>(qr + 32 * s);
   }
   const int32_t *trow = a.table + w.seq * a.width;
-  const int64_t head_at = ((int64_t)kvh * HD) << a.page_shift;
-  const int pmask = (1 << a.page_shift) - 1;
   // Page entry of the 8 keys from `key` (an index past the last key reads the last key's entry).
   auto entry = [&](int key) { return trow[min(key, w.n - 1) >> a.page_shift]; };
-  auto good = [&](int p) { return (uint32_t)p < (uint64_t)a.num_pages; };
-  const int gk = (r >> 2) * 8, gv = g * 8;
   u32x4 kf[2][kSteps];
   uint32_t vf[8][E / 2];
   auto load_k = [&](int k0, int page) {
@@ -322,7 +327,9 @@ paged_attention_kernel(const PaArgs a) {
     }
   }
   __syncthreads();
-  const int64_t mine = (int64_t)blockIdx.x * min(a.grp, kPaCols) * (HD + 2);
+  // A workgroup has at most two sequences in part, its first and its last: a place for each.
+  const int64_t place = (int64_t)min(a.grp, kPaCols) * (HD + 2), step = 2 * H * place;
+  float *const own = a.part + (2 * (int64_t)wg + (later ? 1 : 0)) * H * place + unit * place;
   uint16_t *const orow = a.out + ((int64_t)w.seq * a.nq + head0) * HD;
   for (int i = threadIdx.x; i < ncol * (HD / 2); i += kPaThreads) {
     const int c = i / (HD / 2), d = 2 * (i - c * (HD / 2));
@@ -343,21 +350,27 @@ paged_attention_kernel(const PaArgs a) {
       const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
       *reinterpret_cast<uint32_t *>(orow + c * HD + d) = pack_bf16x2(o0 * inv, o1 * inv);
     } else {
-      float *const p = a.part + mine + c * (HD + 2);
+      float *const p = own + c * (HD + 2);
       pa_put(p + d, o0, o1);
       if (d == 0) pa_put(p + HD, mm, ll);
     }
   }
-  if (w.nact == 1) return;
-  if (!pa_last_of(a.count + (int64_t)w.seq * H + unit, w.nact)) return;
+  if (w.nact == 1 || !pa_last_of(a.count + (int64_t)w.seq * H + unit, w.nact)) {
+    __syncthreads();  // (before the arrays are used again)
+    return;
+  }
   // The last of the sequence's workgroups adds their results up, in the order of the keys: the
   // weights of the partial results first, then a thread takes two neighbouring values, kPaJoin
   // partial results under way at a time.
-  const int64_t step = (int64_t)H * min(a.grp, kPaCols) * (HD + 2);  // from one item to the next
-  const float *const first = a.part + mine - w.split * step;
+  // Result y is workgroup head + y's: in its first place, but in its last if the sequence starts
+  // inside its tiles (y = 0).
+  const float *const all = a.part + 2 * (int64_t)w.head * H * place + unit * place;
+  // (Offsets in 32 bits: the workspace has no more.)
+  const uint32_t step32 = (uint32_t)step, inside = w.inside ? (uint32_t)(H * place) : 0;
+  auto result = [&](int y, uint32_t at) { return pa_get(all + ((uint32_t)y * step32 + (y == 0 ? inside : 0) + at)); };
   for (int c = wave; c < ncol; c += kPaWaves) {
     const bool has = lane < w.nact;
-    const float2 ml = has ? pa_get(first + lane * step + c * (HD + 2) + HD) : make_float2(-INFINITY, 0.0f);
+    const float2 ml = has ? result(lane, c * (HD + 2) + HD) : make_float2(-INFINITY, 0.0f);
     float mx[1] = {ml.x};
     lane_groups_reduce<true>(mx, kWave);
     const float f = __builtin_amdgcn_exp2f((ml.x - (mx[0] == -INFINITY ? 0.0f : mx[0])) * kPaLog2e);
@@ -368,12 +381,11 @@ paged_attention_kernel(const PaArgs a) {
   __syncthreads();
   for (int i = threadIdx.x; i < ncol * (HD / 2); i += kPaThreads) {
     const int c = i / (HD / 2), d = 2 * (i - c * (HD / 2));
-    const float *p = first + c * (HD + 2) + d;
     float o0 = 0.0f, o1 = 0.0f;
     for (int y0 = 0; y0 < w.nact; y0 += kPaJoin) {
       float2 po[kPaJoin];
 #pragma unroll
-      for (int y = 0; y < kPaJoin; ++y) po[y] = y0 + y < w.nact ? pa_get(p + (y0 + y) * step) : make_float2(0.0f, 0.0f);
+      for (int y = 0; y < kPaJoin; ++y) po[y] = y0 + y < w.nact ? result(y0 + y, c * (HD + 2) + d) : make_float2(0.0f, 0.0f);
 #pragma unroll
       for (int y = 0; y < kPaJoin; ++y) {
         const float f = s_w[c][min(y0 + y, kPaMaxSplits - 1)];
@@ -382,15 +394,51 @@ paged_attention_kernel(const PaArgs a) {
       }
     }
     *reinterpret_cast<uint32_t *>(orow + c * HD + d) = pack_bf16x2(o0, o1);
+  }  __syncthreads();  // (as above)
+  };
+
+  int base = 0;  // tiles of the sequences before these 64
+  for (int i0 = plan.per > 0 ? 0 : wg & ~(kWave - 1); i0 < a.B; i0 += kWave) {
+    const int keys = pa_keys(a, i0 + lane), tiles = pa_tiles(keys);
+    int cost = kPaStart + tiles;
+    if (plan.aligned) cost = max(1, (int)(((uint32_t)tiles + plan.per - 1) / (uint32_t)plan.per)) * plan.per;
+    cost = i0 + lane < a.B ? cost : 0;
+    const int incl = pa_incl(cost), start = base + incl - (plan.aligned ? cost : tiles);  // of the tiles
+    base += __builtin_amdgcn_readlane(incl, kWave - 1);
+    const int at = tiles > 0 || plan.aligned ? start : start - kPaStart;
+    uint64_t mine = plan.per > 0 ? __ballot(cost > 0 && at < end && (at >= begin || start + tiles > begin))
+                                 : 1ull << (wg & (kWave - 1));
+    for (; mine != 0; mine &= mine - 1) {
+      const int from = __builtin_ctzll(mine);
+      PaItem w;
+      w.seq = i0 + from;
+      w.n = __builtin_amdgcn_readlane(keys, from);
+      const int s0 = __builtin_amdgcn_readlane(start, from), nt = pa_tiles(w.n);
+      w.tile0 = 0;
+      w.tile1 = nt;
+      w.nact = 1;
+      w.split = 0;
+      w.head = 0;
+      if (plan.per > 0 && nt > 0) {
+        w.tile0 = max(begin - s0, 0);
+        w.tile1 = min(end - s0, nt);
+        w.head = s0 / plan.per;
+        w.nact = (s0 + nt - 1) / plan.per - w.head + 1;
+        w.split = wg - w.head;
+      }
+      w.inside = plan.per > 0 && s0 - w.head * plan.per > 0;
+      sequence(w, s0 > begin);
+    }
+    if (plan.per == 0 || base >= end) break;
   }
 }
 
 constexpr int kPaMaxPage = 4096;
 
-// Workgroups per head group that a launch aims at.
-int pa_share(int64_t units) {
-  const int64_t s = 3 * (int64_t)device_cu_count() / units;
-  return (int)(s < 1 ? 1 : s);
+// Workgroups of a head group that run at once.
+int64_t pa_share(int64_t units, int hd) {
+  const int64_t s = pa_resident(hd) * (int64_t)device_cu_count() / units;
+  return s < 1 ? 1 : s;
 }
 int pa_qtiles(int32_t grp) { return (grp + kPaCols - 1) / kPaCols; }
 bool pa_splits(int64_t B, int64_t units) { return B * units <= kPaCounterBytes / 4; }
@@ -408,9 +456,7 @@ extern "C" int64_t moe_paged_attention_workspace_bytes(int64_t B, int32_t n_q_he
   if (!moe::pa_sizes_ok(B, n_q_heads, n_kv_heads, head_dim)) return -1;
   const int32_t grp = n_q_heads / n_kv_heads;
   const int64_t units = (int64_t)n_kv_heads * moe::pa_qtiles(grp);
-  int64_t b = B;  // the most of any batch up to B
-  if (!moe::pa_splits(b, units)) b = moe::kPaCounterBytes / 4 / units;
-  return moe::kPaCounterBytes + (moe::pa_share(units) + b) * units * (grp < moe::kPaCols ? grp : moe::kPaCols) *
+  return moe::kPaCounterBytes + 2 * moe::pa_share(units, head_dim) * units * (grp < moe::kPaCols ? grp : moe::kPaCols) *
                                     (int64_t)(head_dim + 2) * 4;
 }
 
@@ -473,8 +519,8 @@ extern "C" int moe_paged_attention_bf16(const void *q, int64_t q_stride, const v
   a.out = (uint16_t *)out;
   a.count = (uint32_t *)workspace;
   a.part = workspace ? (float *)((char *)workspace + moe::kPaCounterBytes) : nullptr;
-  a.share = split ? moe::pa_share(units) : 1 << 30;
-  const int64_t items = split ? a.share + B : B;
+  a.share = split ? (int)moe::pa_share(units, head_dim) : 0;
+  const int64_t items = a.share > B ? a.share : B;
   MOE_REQUIRE(items * units <= 0x7fffffff, "bad sizes");
   auto kern = head_dim == 64    ? moe::paged_attention_kernel<64>
               : head_dim == 128 ? moe::paged_attention_kernel<128>
