@@ -89,7 +89,10 @@ __device__ __forceinline__ bool pk_item(const PkArgs &a, int rows, int w, int la
     return __builtin_amdgcn_readfirstlane((int)sum);
   };
   if (w >= above(0)) return false;
-  int lo = 0, hi = (int)(((int64_t)a.T * a.grp + rows - 1) / rows);  // N(lo) > w, N(hi) <= w
+  float most[1] = {(float)t0};
+  for (int i0 = kWave; i0 < a.B; i0 += kWave) most[0] = fmaxf(most[0], (float)tiles(i0 + lane));
+  lane_groups_reduce<true>(most, kWave);
+  int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)most[0]);  // N(lo) > w, N(hi) <= w
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (above(mid) > w)
@@ -183,31 +186,10 @@ packed_attention_kernel(const PkArgs a) {
   PkItem it;
   if (!pk_item(a, kRows, w, lane, it)) return;  // the same for the whole workgroup
   const int rows = it.len * a.grp;              // of the sequence (T * group < 2^31)
-  const int row0 = it.tile * kRows + wave * kPkRows;
-  const int r = min(row0 + li, rows - 1);
-  const int t = r / a.grp;                      // token of this lane's row
-  const int limit = t + 1;                      // it sees keys 0 .. limit - 1
-  const int head = kvh * a.grp + (r - t * a.grp);
-  // Keys of the wave's first and last row, and of the workgroup's last row.
-  const int first = min(row0, rows - 1) / a.grp + 1;
-  const int last = row0 < rows ? min(row0 + kPkRows - 1, rows - 1) / a.grp + 1 : 0;
+  // Keys of the workgroup's last row.
   const int nkeys = min(it.tile * kRows + kRows - 1, rows - 1) / a.grp + 1;
   const int ntile = (nkeys + kKeys - 1) / kKeys;
 
-  // Q as the B operand: column li, dims 16 s + 8 hh .. + 7.  A negative scaling goes into its signs,
-  // one of zero into its values (masked scores, -inf, are multiplied too).
-  const uint32_t flip = a.scaling < 0.0f ? 0x80008000u : 0u, keep = a.scaling == 0.0f ? 0u : ~0u;
-  const float scaling = a.scaling == 0.0f ? 1.0f : fabsf(a.scaling);
-  const float c = scaling * kPkLog2e;
-  u32x4 qf[HD / 16];
-  {
-    const uint16_t *qr = a.q + (it.tok0 + t) * a.q_stride + (int64_t)head * HD + 8 * hh;
-#pragma unroll
-    for (int s = 0; s < HD / 16; ++s) {
-      qf[s] = *reinterpret_cast<const u32x4 *>(qr + 16 * s);
-      qf[s] = (qf[s] ^ flip) & keep;
-    }
-  }
   // Loads: 1 KB of a tile per instruction; lane l fills the 16 bytes at 16 l of it, which belong to
   // row (1 KB chunk * 1024 + 16 l) / row bytes, and fetches the piece that the swizzle puts there.
   // Rows past the sequence's last key repeat it (masked below).
@@ -223,6 +205,31 @@ packed_attention_kernel(const PkArgs a) {
       pk_load_lds(vb + key * a.v_stride + 8 * (piece ^ pk_vx<HD>(row)), plane + kPlane + (wave + i * NW) * 1024);
     }
   };
+  load(0, s_kv[0]);
+
+  const int row0 = it.tile * kRows + wave * kPkRows;
+  const int r = min(row0 + li, rows - 1);
+  const int t = r / a.grp;                      // token of this lane's row
+  const int limit = t + 1;                      // it sees keys 0 .. limit - 1
+  const int head = kvh * a.grp + (r - t * a.grp);
+  // Keys of the wave's first and last row.
+  const int first = min(row0, rows - 1) / a.grp + 1;
+  const int last = row0 < rows ? min(row0 + kPkRows - 1, rows - 1) / a.grp + 1 : 0;
+
+  // Q as the B operand: column li, dims 16 s + 8 hh .. + 7.  A negative scaling goes into its signs,
+  // one of zero into its values (masked scores, -inf, are multiplied too).
+  const uint32_t flip = a.scaling < 0.0f ? 0x80008000u : 0u, keep = a.scaling == 0.0f ? 0u : ~0u;
+  const float scaling = a.scaling == 0.0f ? 1.0f : fabsf(a.scaling);
+  const float c = scaling * kPkLog2e;
+  u32x4 qf[HD / 16];
+  {
+    const uint16_t *qr = a.q + (it.tok0 + t) * a.q_stride + (int64_t)head * HD + 8 * hh;
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) {
+      qf[s] = *reinterpret_cast<const u32x4 *>(qr + 16 * s);
+      qf[s] = (qf[s] ^ flip) & keep;
+    }
+  }
   f32x16 acc[kDT];
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt)
@@ -236,7 +243,6 @@ packed_attention_kernel(const PkArgs a) {
   const uint32_t vkey = 4 * hh + ((lane & 15) >> 2);
   const uint32_t vrd = kPlane + vkey * kRowB + 8 * (lane & 1);
   const uint32_t vx = 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ pk_vx<HD>(vkey));
-  load(0, s_kv[0]);
   for (int n = 0; n < ntile; ++n) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // tile n is in its plane, and the other plane is no longer read
@@ -311,6 +317,7 @@ packed_attention_kernel(const PkArgs a) {
     else
       tile(std::true_type{});
   }
+  __syncthreads();  // (the planes are free)
   if (row0 >= rows) return;
   l = op_xor32<false>(l);
   // A row that stops inside a tile meets V rows that it does not see with weights of zero: an
@@ -333,16 +340,28 @@ packed_attention_kernel(const PkArgs a) {
       return;
     }
   }
-  if (row0 + li < rows) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t *orow = a.out + ((int64_t)(it.tok0 + t) * a.nq + head) * HD;
+  // The wave's rows through LDS (32 rows of the plane that nobody reads any more; pieces of 16 bytes
+  // swizzled by row), so that whole rows are written: a store of 16 bytes per lane, not 8 of each of 32
+  // rows.
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t place = ((int64_t)(it.tok0 + t) * a.nq + head) * HD;
+  uint8_t *const mine = s_kv[0] + wave * kPkRows * kRowB;
+  constexpr uint32_t kSwz = HD == 64 ? 7 : 15;
 #pragma unroll
-    for (int dt = 0; dt < kDT; ++dt)
+  for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
-      for (int v = 0; v < 16; v += 4)
-        *reinterpret_cast<uint2 *>(orow + 32 * dt + 2 * v + 4 * hh) =
-            make_uint2(pack_bf16x2(acc[dt][v] * inv, acc[dt][v + 1] * inv),
-                       pack_bf16x2(acc[dt][v + 2] * inv, acc[dt][v + 3] * inv));
+    for (int v = 0; v < 16; v += 4)
+      *reinterpret_cast<uint2 *>(mine + li * kRowB + 16 * ((4 * dt + v / 4) ^ (li & kSwz)) + 8 * hh) =
+          make_uint2(pack_bf16x2(acc[dt][v] * inv, acc[dt][v + 1] * inv),
+                     pack_bf16x2(acc[dt][v + 2] * inv, acc[dt][v + 3] * inv));
+  constexpr int kPieces = kRowB / 16, kStep = kWave / kPieces;  // lanes per row, rows per store
+#pragma unroll
+  for (int i = 0; i < kPkRows / kStep; ++i) {
+    const int row = i * kStep + lane / kPieces, piece = lane % kPieces;
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + row * kRowB + 16 * (piece ^ (row & kSwz)));
+    const uint32_t lo = __shfl((uint32_t)place, row, kWave), hi = __shfl((uint32_t)(place >> 32), row, kWave);
+    if (row0 + row < rows)
+      *reinterpret_cast<u32x4 *>(a.out + (int64_t)(lo | (uint64_t)hi << 32) + 8 * piece) = v;
   }
 }
 
@@ -367,8 +386,8 @@ extern "C" int moe_packed_attention_bf16(const void *q, int64_t q_stride, const 
               "rows of q, k and v must be 16-byte aligned and apart");
   if (T == 0 || B == 0) return MOE_STATUS_OK;
   MOE_REQUIRE(q && k && v && cu_seqlens_i32 && out, "null pointer");
-  MOE_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0 && (uintptr_t)out % 8 == 0,
-              "q, k and v must be 16-byte aligned, out 8-byte");
+  MOE_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) % 16 == 0,
+              "q, k, v and out must be 16-byte aligned");
   const int64_t ob = 2 * T * qrow;
   MOE_REQUIRE(!moe::ranges_overlap(out, ob, q, 2 * (q_stride * (T - 1) + qrow)) &&
                   !moe::ranges_overlap(out, ob, k, 2 * (k_stride * (T - 1) + krow)) &&
