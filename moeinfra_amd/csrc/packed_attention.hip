@@ -166,20 +166,25 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
 // A weight is 2^(s c - m) by one fused multiply-add, c = scaling * log2(e), m a rounded max s c: what
 // the rounding of m leaves cancels against the sum, as long as 2 to its power is in range.  Rows with
 // references past kPkHuge (and products that overflow) are done again without.
-template <int HD, int NW>
-__global__ void __launch_bounds__(NW *kWave, HD == 256 ? 1 : 2)
+//
+// KG key groups of RW waves: with two, the second takes every other tile of the same rows, which halves
+// the chain of a row tile's keys; the groups' sums meet in LDS.
+template <int HD, int RW, int KG>
+__global__ void __launch_bounds__(RW *KG *kWave, HD == 256 ? 1 : 2)
 packed_attention_kernel(const PkArgs a) {
-  constexpr int kRows = NW * kPkRows;
+  constexpr int NW = RW * KG, kRows = RW * kPkRows;
   constexpr int kKeys = HD == 256 ? 32 : 64;         // keys per tile (64 of 256 dims spill registers)
   constexpr int kST = kKeys / 32;
   constexpr int kPlane = kKeys * HD * 2;           // bytes of a K or V tile
   constexpr int kChunks = kPlane / 1024 / NW;        // 1 KB loads per wave and tile of K (and of V)
+  constexpr int kStage = KG * 2 * kPlane;            // bytes of the tiles of a step
   constexpr int kDT = HD / 32;                       // 32-dim output tiles
   constexpr int kRowB = HD * 2;
   static_assert(kChunks >= 1, "a wave loads a KB at least");
-  __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2 * kPlane];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][kStage];
   const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int loader = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int wave = loader % RW, kgrp = loader / RW;  // row and key group
   const int li = lane & 31, hh = lane >> 5;
   // The KV head is the fast index: with a multiple of 8 heads, a head's workgroups share an XCD's L2.
   const int w = (int)(blockIdx.x / (unsigned)a.nkv), kvh = (int)(blockIdx.x - (unsigned)w * a.nkv);
@@ -195,15 +200,18 @@ packed_attention_kernel(const PkArgs a) {
   // Rows past the sequence's last key repeat it (masked below).
   const uint16_t *const kb = a.k + it.tok0 * a.k_stride + (int64_t)kvh * HD;
   const uint16_t *const vb = a.v + it.tok0 * a.v_stride + (int64_t)kvh * HD;
-  auto load = [&](int tile, uint8_t *plane) __attribute__((always_inline)) {
+  auto load = [&](int at_step, uint8_t *stage) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int at = (wave + i * NW) * 1024 + 16 * lane;
-      const uint32_t row = at / kRowB, piece = at % kRowB / 16;
-      const int64_t key = min(tile * kKeys + (int)row, nkeys - 1);
-      pk_load_lds(kb + key * a.k_stride + 8 * (piece ^ pk_kx<HD>(row)), plane + (wave + i * NW) * 1024);
-      pk_load_lds(vb + key * a.v_stride + 8 * (piece ^ pk_vx<HD>(row)), plane + kPlane + (wave + i * NW) * 1024);
-    }
+    for (int n = 0; n < KG; ++n)
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int chunk = (loader + i * NW) * 1024, at = chunk + 16 * lane;
+        const uint32_t row = at / kRowB, piece = at % kRowB / 16;
+        const int64_t key = min((at_step * KG + n) * kKeys + (int)row, nkeys - 1);
+        uint8_t *const plane = stage + n * 2 * kPlane + chunk;
+        pk_load_lds(kb + key * a.k_stride + 8 * (piece ^ pk_kx<HD>(row)), plane);
+        pk_load_lds(vb + key * a.v_stride + 8 * (piece ^ pk_vx<HD>(row)), plane + kPlane);
+      }
   };
   load(0, s_kv[0]);
 
@@ -243,81 +251,114 @@ packed_attention_kernel(const PkArgs a) {
   const uint32_t vkey = 4 * hh + ((lane & 15) >> 2);
   const uint32_t vrd = kPlane + vkey * kRowB + 8 * (lane & 1);
   const uint32_t vx = 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ pk_vx<HD>(vkey));
-  for (int n = 0; n < ntile; ++n) {
+  const int steps = (ntile + KG - 1) / KG;
+  // One step; EDGE: some row of the workgroup stops inside it.
+  auto step = [&](int n, auto edge_c) __attribute__((always_inline)) {
+    constexpr bool kEdge = decltype(edge_c)::value;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // tile n is in its plane, and the other plane is no longer read
-    if (n + 1 < ntile) load(n + 1, s_kv[(n + 1) & 1]);
-    const int k0 = n * kKeys;
-    if (k0 >= last) continue;  // none of this wave's rows sees it
-    const uint8_t *buf = s_kv[n & 1];
-    auto tile = [&](auto edge_c) __attribute__((always_inline)) {
-      constexpr bool kEdge = decltype(edge_c)::value;
-      // (Addresses are a XOR with a constant away from these: computed, not held in registers.)
-      uint32_t ka = kx, va = vx;
-      asm volatile("" : "+v"(ka), "+v"(va));
-      f32x16 sc[kST];
+    __syncthreads();  // step n is in its plane, and the other plane is no longer read
+    if (n + 1 < steps) load(n + 1, s_kv[(n + 1) & 1]);
+    const int k0 = (n * KG + kgrp) * kKeys;
+    if (kEdge && k0 >= last) return;  // none of this wave's rows sees it
+    const uint8_t *buf = s_kv[n & 1] + kgrp * 2 * kPlane;
+    // (Addresses are a XOR with a constant away from these: computed, not held in registers.)
+    uint32_t ka = kx, va = vx;
+    asm volatile("" : "+v"(ka), "+v"(va));
+    f32x16 sc[kST];
 #pragma unroll
-      for (int st = 0; st < kST; ++st)
+    for (int st = 0; st < kST; ++st)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) sc[st][v] = 0.0f;
+      for (int v = 0; v < 16; ++v) sc[st][v] = 0.0f;
 #pragma unroll
-      for (int s = 0; s < HD / 16; ++s)
+    for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
-        for (int st = 0; st < kST; ++st) {
-          const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + krd + (ka ^ (32 * s)) + 32 * st * kRowB);
-          sc[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
-                                                           __builtin_bit_cast(bf16x8, qf[s]), sc[st], 0, 0, 0);
-        }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int st = 0; st < kST; ++st)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          if constexpr (kEdge)
-            sc[st][v] = k0 + 32 * st + 8 * (v >> 2) + 4 * hh + (v & 3) < limit ? sc[st][v] : -INFINITY;
-          mx = fmaxf(mx, sc[st][v]);
-        }
-      mx = op_xor32<true>(mx) * c;
-      if (__any(mx > m + kPkLag)) {
-        const float mn = fmaxf(m, mx);
-        const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
-        m = mn;
-        huge |= fabsf(mn) > kPkHuge && mn != -INFINITY;
-        l *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < kDT; ++dt)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
+      for (int st = 0; st < kST; ++st) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + krd + (ka ^ (32 * s)) + 32 * st * kRowB);
+        sc[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
+                                                         __builtin_bit_cast(bf16x8, qf[s]), sc[st], 0, 0, 0);
       }
-      const float mref = m == -INFINITY ? 0.0f : m;  // before a row's first key above -inf
-      u32x4 pf[2 * kST];
+    float mx = -INFINITY;
 #pragma unroll
-      for (int s = 0; s < 2 * kST; ++s)
+    for (int st = 0; st < kST; ++st)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int v = 8 * (s & 1) + 2 * j;
-          const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v], c, -mref));
-          const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v + 1], c, -mref));
-          l += e0 + e1;
-          pf[s][j] = pack_bf16x2(e0, e1);
-        }
+      for (int v = 0; v < 16; ++v) {
+        if constexpr (kEdge)
+          sc[st][v] = k0 + 32 * st + 8 * (v >> 2) + 4 * hh + (v & 3) < limit ? sc[st][v] : -INFINITY;
+        mx = fmaxf(mx, sc[st][v]);
+      }
+    mx = op_xor32<true>(mx) * c;
+    if (__any(mx > m + kPkLag)) {
+      const float mn = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+      m = mn;
+      huge |= fabsf(mn) > kPkHuge && mn != -INFINITY;
+      l *= alpha;
 #pragma unroll
-      for (int s = 0; s < 2 * kST; ++s)
+      for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < kDT; ++dt) {
-          const uint8_t *p = buf + vrd + (va ^ (64 * dt)) + 16 * s * kRowB;
-          const uint2 x0 = pk_read_tr(p), x1 = pk_read_tr(p + 8 * kRowB);
-          const u32x4 x = {x0.x, x0.y, x1.x, x1.y};
-          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
-                                                            __builtin_bit_cast(bf16x8, pf[s]), acc[dt], 0, 0, 0);
-        }
-    };
-    if (k0 + kKeys <= first)
-      tile(std::false_type{});
-    else
-      tile(std::true_type{});
-  }
+        for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
+    }
+    const float mref = m == -INFINITY ? 0.0f : m;  // before a row's first key above -inf
+    u32x4 pf[2 * kST];
+#pragma unroll
+    for (int s = 0; s < 2 * kST; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int v = 8 * (s & 1) + 2 * j;
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v], c, -mref));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v + 1], c, -mref));
+        l += e0 + e1;
+        pf[s][j] = pack_bf16x2(e0, e1);
+      }
+#pragma unroll
+    for (int s = 0; s < 2 * kST; ++s)
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) {
+        const uint8_t *p = buf + vrd + (va ^ (64 * dt)) + 16 * s * kRowB;
+        const uint2 x0 = pk_read_tr(p), x1 = pk_read_tr(p + 8 * kRowB);
+        const u32x4 x = {x0.x, x0.y, x1.x, x1.y};
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
+                                                          __builtin_bit_cast(bf16x8, pf[s]), acc[dt], 0, 0, 0);
+      }
+  };
+  // Steps that every row sees whole, then those where rows stop: apart, so that the long loop has no
+  // masks and keeps its sums where they are.
+  const int full = (it.tile * kRows / a.grp + 1) / (KG * kKeys);
+  for (int n = 0; n < full; ++n) step(n, std::false_type{});
+  for (int n = full; n < steps; ++n) step(n, std::true_type{});
   __syncthreads();  // (the planes are free)
+  // A row wave's part of them: the second key group's sums, then the rows on their way out.
+  constexpr int kJoin = KG == 1 ? kPkRows * kRowB : (16 * kDT + 4) * kWave * 4;
+  static_assert(RW * kJoin <= 2 * kStage && kPkRows * kRowB <= kJoin, "the parts fit the planes");
+  uint8_t *const mine = &s_kv[0][0] + wave * kJoin;
+  if constexpr (KG == 2) {
+    float4 *const o = reinterpret_cast<float4 *>(mine) + lane;
+    if (kgrp == 1) {
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+        for (int v = 0; v < 16; v += 4)
+          o[(4 * dt + v / 4) * kWave] = make_float4(acc[dt][v], acc[dt][v + 1], acc[dt][v + 2], acc[dt][v + 3]);
+      o[4 * kDT * kWave] = make_float4(m, l, huge ? 1.0f : 0.0f, 0.0f);
+    }
+    __syncthreads();
+    if (kgrp == 1) return;
+    const float4 ml = o[4 * kDT * kWave];
+    const float mn = fmaxf(m, ml.x), mref = mn == -INFINITY ? 0.0f : mn;
+    const float a0 = __builtin_amdgcn_exp2f(m - mref), a1 = __builtin_amdgcn_exp2f(ml.x - mref);
+    l = l * a0 + ml.y * a1;
+    huge |= ml.z != 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4) {
+        const float4 x = o[(4 * dt + v / 4) * kWave];
+        acc[dt][v] = acc[dt][v] * a0 + x.x * a1;
+        acc[dt][v + 1] = acc[dt][v + 1] * a0 + x.y * a1;
+        acc[dt][v + 2] = acc[dt][v + 2] * a0 + x.z * a1;
+        acc[dt][v + 3] = acc[dt][v + 3] * a0 + x.w * a1;
+      }
+  }
   if (row0 >= rows) return;
   l = op_xor32<false>(l);
   // A row that stops inside a tile meets V rows that it does not see with weights of zero: an
@@ -345,7 +386,6 @@ packed_attention_kernel(const PkArgs a) {
   // rows.
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t place = ((int64_t)(it.tok0 + t) * a.nq + head) * HD;
-  uint8_t *const mine = s_kv[0] + wave * kPkRows * kRowB;
   constexpr uint32_t kSwz = HD == 64 ? 7 : 15;
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt)
@@ -395,15 +435,24 @@ extern "C" int moe_packed_attention_bf16(const void *q, int64_t q_stride, const 
               "out must not overlap q, k or v");
   moe::PkArgs a{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, q_stride, k_stride, v_stride,
                 (const int32_t *)cu_seqlens_i32, (int)T, (int)B, n_q_heads, n_kv_heads, grp, scaling, (uint16_t *)out};
-  // Workgroups of 8 waves where they fill the device; else of 4, twice as many.
-  auto grid = [&](int rows) { return (T * grp / rows + (B < T ? B : T)) * n_kv_heads; };
-  const bool wide = head_dim != 256 && T * grp / (8 * moe::kPkRows) * n_kv_heads >= moe::device_cu_count();
-  const int64_t g = grid(wide ? 8 * moe::kPkRows : 4 * moe::kPkRows);
+  auto tiles = [&](int rows) { return (T * grp / rows + (B < T ? B : T)) * n_kv_heads; };
+  const int64_t cus = moe::device_cu_count();
+  // 128 rows a workgroup, two of them on a CU.  Few, of sequences of some length: in two key groups
+  // (1500 tokens 36 us instead of 42; 9 sequences of 3333 56 instead of 39).  Many, of more KV heads
+  // than an XCD's L2 takes one of: 256 rows, which read K and V half as often (8192 tokens of 16 / 16
+  // heads 281 us instead of 304; of 32 / 8 heads the same).
+  const bool paired = head_dim != 256 && tiles(128) <= 2 * cus && T >= 256 * B;
+  const bool wide = head_dim != 256 && n_kv_heads > 8 && tiles(256) >= 2 * cus;
+  const int64_t g = tiles(wide ? 256 : 128);
   MOE_REQUIRE(g <= 0x7fffffff, "bad sizes");
-  auto kern = head_dim == 64    ? (wide ? moe::packed_attention_kernel<64, 8> : moe::packed_attention_kernel<64, 4>)
-              : head_dim == 128 ? (wide ? moe::packed_attention_kernel<128, 8> : moe::packed_attention_kernel<128, 4>)
-                                : moe::packed_attention_kernel<256, 4>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)g), dim3((wide ? 8 : 4) * moe::kWave), 0, (hipStream_t)stream, a);
+  auto kern = head_dim == 64    ? (paired ? moe::packed_attention_kernel<64, 4, 2>
+                                   : wide ? moe::packed_attention_kernel<64, 8, 1>
+                                          : moe::packed_attention_kernel<64, 4, 1>)
+              : head_dim == 128 ? (paired ? moe::packed_attention_kernel<128, 4, 2>
+                                   : wide ? moe::packed_attention_kernel<128, 8, 1>
+                                          : moe::packed_attention_kernel<128, 4, 1>)
+                                : moe::packed_attention_kernel<256, 4, 1>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)g), dim3((paired || wide ? 8 : 4) * moe::kWave), 0, (hipStream_t)stream, a);
   MOE_LAUNCH_CHECK();
   return MOE_STATUS_OK;
 }
