@@ -156,12 +156,18 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
 }
 
 // Rows of one KV head are (token, query head of its group), r = token * group + head, so that the
-// group's heads share the K and V tiles.  A workgroup takes 32 rows per wave and walks the keys in
-// tiles, two LDS planes deep: while a tile is multiplied, the next one is on its way from
-// memory straight into the other plane.
+// group's heads share the K and V tiles.  A workgroup takes 32 rows per row wave and walks the keys in
+// tiles, two LDS planes deep: while a tile is multiplied, the next one is on its way from memory
+// straight into the other plane.
 //
 //   S^T = K Q^T        lane (row of queries l % 32) holds 16 keys of its row per 32-key half
 //   O^T += V^T P^T     P of a lane is the B operand as it stands; V is read transposed
+//
+// Bound: a tile of 64 keys costs a wave 1024 cycles of products and about as many of vector
+// instructions (512 of them the exponentials), and LDS as many of operand reads for the 8 waves of a
+// CU; they overlap between its waves.  16384 tokens in 3 sequences, 32 / 8 heads of 128: 1640-1840 us,
+// 900-1010 TFLOP/s; many short sequences are bound by their queries and outputs (64 of 256: 335 MB in
+// 120 us).
 //
 // A weight is 2^(s c - m) by one fused multiply-add, c = scaling * log2(e), m a rounded max s c: what
 // the rounding of m leaves cancels against the sum, as long as 2 to its power is in range.  Rows with
@@ -439,14 +445,13 @@ extern "C" int moe_packed_attention_bf16(const void *q, int64_t q_stride, const 
   const int64_t cus = moe::device_cu_count();
   // 128 rows a workgroup, two of them on a CU.  Few, of sequences of some length: in two key groups
   // (1500 tokens 36 us instead of 42; 9 sequences of 3333 56 instead of 39).  Many, of more KV heads
-  // than an XCD's L2 takes one of: 256 rows, which read K and V half as often (8192 tokens of 16 / 16
-  // heads 281 us instead of 304; of 32 / 8 heads the same).
+  // than there are XCDs, whose L2s then hold parts of several: 256 rows, which read K and V half as
+  // often (8192 tokens of 16 / 16 heads of 128 281 us instead of 304; of 32 / 8 heads the same).
   const bool paired = head_dim != 256 && tiles(128) <= 2 * cus && T >= 256 * B;
-  const bool wide = head_dim != 256 && n_kv_heads > 8 && tiles(256) >= 2 * cus;
+  const bool wide = head_dim == 128 && n_kv_heads > 8 && tiles(256) >= 2 * cus && !paired;
   const int64_t g = tiles(wide ? 256 : 128);
   MOE_REQUIRE(g <= 0x7fffffff, "bad sizes");
   auto kern = head_dim == 64    ? (paired ? moe::packed_attention_kernel<64, 4, 2>
-                                   : wide ? moe::packed_attention_kernel<64, 8, 1>
                                           : moe::packed_attention_kernel<64, 4, 1>)
               : head_dim == 128 ? (paired ? moe::packed_attention_kernel<128, 4, 2>
                                    : wide ? moe::packed_attention_kernel<128, 8, 1>

@@ -306,6 +306,14 @@ def test_packed_attention_wide_workgroups(cuda_device):
         _check_packed(*_packed(cuda_device, [700, 33, 1400], 32, 8, hd, seed=hd))
 
 
+@pytest.mark.parametrize("lens,nq,nkv,hd", [([1900, 2300], 16, 16, 128), ([300, 280], 4, 1, 64), ([900], 6, 2, 256),
+                                            ([600, 599, 3], 8, 1, 128)])
+def test_packed_attention_kernels(cuda_device, lens, nq, nkv, hd):
+    # 256 rows a workgroup (many rows of 16 KV heads), two key groups (few), the large head dim.
+    print(f"packed attention {lens} {nq}/{nkv} heads of {hd}", flush=True)
+    _check_packed(*_packed(cuda_device, lens, nq, nkv, hd, seed=hd))
+
+
 def test_packed_attention_scalings(cuda_device):
     for scaling in (1.0, -0.125, 0.0, 2.5):
         print(f"scaling {scaling}", flush=True)
@@ -500,3 +508,204 @@ def test_sample_tokens_random_numbers_at_the_ends(cuda_device):
     for u, at in ((0.0, 0), (1.0 - 2.0 ** -24, 24), (1.0, 24), (7.5, 24), (-1.0, 0), (math.nan, 0)):
         got = ops.sample_tokens(x.to(cuda_device), torch.tensor([u], device=cuda_device), top_k=25)
         assert int(got) == int(kept[at])
+
+
+# ------------------------------------------------------------------ together
+class _Server:
+    """A layer's attention of a batch of sequences: prompts in one packed pass, then steps, and a
+    choice of tokens; the state that a server keeps."""
+
+    def __init__(self, dev, lens, steps, nq=8, nkv=2, hd=64, page=16, vocab=500):
+        from moeinfra_amd import ops
+
+        self.dev, self.nq, self.nkv, self.hd, self.lens = dev, nq, nkv, hd, list(lens)
+        self.pool = Pool([n + steps for n in lens], nkv, hd, page, dev, seed=60, fill=math.nan)
+        self.inv = _inv(hd).to(dev)
+        self.ws = ops.paged_attention_workspace(len(lens), nq, nkv, hd, dev)
+        self.pos = torch.tensor(lens, dtype=torch.int32, device=dev)       # of the next token; -1: padding
+        self.seen = self.pos + 1
+        g = torch.Generator().manual_seed(61)
+        self.embed = (torch.randn((vocab, (nq + 2 * nkv) * hd), generator=g)).to(torch.bfloat16).to(dev)
+        self.head = (torch.randn((nq * hd, vocab), generator=g) * 0.1).to(torch.bfloat16).to(dev)
+        self.tok = torch.zeros((len(lens),), dtype=torch.int64, device=dev)
+        self.u = torch.zeros((len(lens),), device=dev)
+        self.x = torch.empty((len(lens), self.embed.shape[1]), dtype=torch.bfloat16, device=dev)
+        self.attn = torch.empty((len(lens), nq, hd), dtype=torch.bfloat16, device=dev)
+
+    def prompts(self, qkv):
+        from moeinfra_amd import ops
+
+        lens = self.lens
+        seq = torch.tensor([i for i, n in enumerate(lens) for _ in range(n)], dtype=torch.int32, device=self.dev)
+        pos = torch.tensor([p for n in lens for p in range(n)], dtype=torch.int32, device=self.dev)
+        cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=self.dev)
+        q, k = ops.rope_paged_kv(qkv, pos, self.pool.dev_table, self.pool.k, self.pool.v, self.nq, self.inv,
+                                 seq_ids=seq, want_k=True)
+        v = qkv[:, (self.nq + self.nkv) * self.hd:].view(-1, self.nkv, self.hd)
+        return ops.packed_attention(q.view(-1, self.nq, self.hd), k, v, cu)
+
+    def step(self):
+        """One token of each sequence: embedding, rotation into the cache, attention, logits, the
+        next token; positions advance (padding rows stay at -1)."""
+        from moeinfra_amd import ops
+
+        torch.index_select(self.embed, 0, self.tok, out=self.x)
+        q, _ = ops.rope_paged_kv(self.x, self.pos, self.pool.dev_table, self.pool.k, self.pool.v, self.nq, self.inv)
+        ops.paged_attention(q.view(-1, self.nq, self.hd), self.pool.k, self.pool.v, self.pool.dev_table, self.seen,
+                            out=self.attn, workspace=self.ws)
+        logits = self.attn.view(len(self.lens), -1) @ self.head
+        ops.sample_tokens(logits, self.u, temperature=0.9, top_k=100, top_p=0.95, out=self.tok)
+        live = (self.pos >= 0).to(torch.int32)
+        self.pos += live
+        self.seen += live
+        return logits
+
+
+def test_prompts_and_steps_together(cuda_device):
+    """Packed prompts into the cache, then steps over it, against the 64-bit forms fed with the
+    bf16 tensors that pass between the operators."""
+    dev, lens, steps = cuda_device, [37, 1, 130], 4
+    sv = _Server(dev, lens, steps)
+    nq, nkv, hd = sv.nq, sv.nkv, sv.hd
+    qkv = _bf((sum(lens), (nq + 2 * nkv) * hd), 62).to(dev)
+    out = sv.prompts(qkv)
+    heads = qkv.cpu().view(-1, nq + 2 * nkv, hd)
+    pos = [p for n in lens for p in range(n)]
+    rot, _ = rope(heads[:, :nq + nkv], pos, _inv(hd))
+    rot = rot.to(torch.bfloat16)
+    # (A rotated value next to a tie may be rounded to the other side than here: a step of 2^-7 of one
+    # product of about 9 at most, times the scaling of 1/8, moves a score by 2^-7 and a weight by
+    # twice that.  Such values are 2^-13 of all, more than one in a score hardly ever.)
+    slack = 2.0 ** -6
+    ks, vs, at = [], [], 0
+    for i, n in enumerate(lens):
+        ks.append(rot[at:at + n, nq:])
+        vs.append(heads[at:at + n, nq + nkv:])
+        for h in range(nq):
+            seen = torch.ones((n, n), dtype=torch.bool).tril()
+            want, tol = attention(rot[at:at + n, h], ks[i][:, h // (nq // nkv)], vs[i][:, h // (nq // nkv)], hd ** -0.5, seen)
+            assert_within(out[at:at + n, h], want, tol + slack * vs[i].double().abs().amax(), f"prompt {i}")
+        at += n
+    g = torch.Generator().manual_seed(63)
+    for s in range(steps):
+        tok = sv.tok.cpu()
+        sv.u.copy_(torch.rand((3,), generator=g))
+        u = sv.u.cpu()
+        logits = sv.step()
+        x = sv.embed[tok.to(dev)].cpu().view(3, nq + 2 * nkv, hd)
+        r, _ = rope(x[:, :nq + nkv], [n + s for n in lens], _inv(hd))
+        r = r.to(torch.bfloat16)
+        for i in range(3):
+            ks[i] = torch.cat((ks[i], r[i:i + 1, nq:]))
+            vs[i] = torch.cat((vs[i], x[i:i + 1, nq + nkv:]))
+            for h in range(nq):
+                want, tol = attention(r[i, h:h + 1], ks[i][:, h // (nq // nkv)], vs[i][:, h // (nq // nkv)], hd ** -0.5)
+                assert_within(sv.attn[i, h:h + 1], want, tol + slack * vs[i].double().abs().amax(), f"step {s}")
+        assert sv.tok.cpu().tolist() == [sample(logits[i].float().cpu(), float(u[i]), temperature=0.9, top_k=100, top_p=0.95)
+                                         for i in range(3)]
+
+
+def test_steps_replayed_from_a_graph(cuda_device):
+    """The step captured once (a batch with padding rows) and replayed, against eager steps, with
+    eager work on the same workspace between the replays."""
+    dev, lens, steps = cuda_device, [37, 700, 5, 1], 6
+    runs = []
+    for captured in (False, True):
+        sv = _Server(dev, lens, steps + 2)
+        sv.prompts(_bf((sum(lens), (sv.nq + 2 * sv.nkv) * sv.hd), 64).to(dev))
+        sv.pos[2] = -1       # padding from here on
+        sv.seen[2] = 0
+        g = torch.Generator().manual_seed(65)
+        got = []
+        graph = None
+        if captured:
+            state = [t.clone() for t in (sv.pos, sv.seen, sv.tok, sv.pool.k, sv.pool.v)]
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                sv.step()
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                sv.step()
+            for t, saved in zip((sv.pos, sv.seen, sv.tok, sv.pool.k, sv.pool.v), state):
+                t.copy_(saved)
+        for s in range(steps):
+            sv.u.copy_(torch.rand((4,), generator=g))
+            if captured:
+                graph.replay()
+            else:
+                sv.step()
+            got.append((sv.tok.cpu().tolist(), sv.attn.clone()))
+            _paged(dev, [300 + s, 2, 90], sv.nq, sv.nkv, sv.hd, 16, seed=s, workspace=sv.ws)
+        assert not bool(sv.ws[:65536].any())
+        assert bool((sv.attn[2] == 0).all())
+        runs.append(got)
+    for (a, x), (b, y) in zip(*runs):
+        assert a == b and _same(x, y)
+
+
+def test_operators_on_another_stream(cuda_device):
+    """Each operator on a side stream, its inputs made there."""
+    from moeinfra_amd import ops
+
+    dev = cuda_device
+    main = _paged(dev, [50, 600], 8, 2, 64, 16, seed=70)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _paged(dev, [50, 600], 8, 2, 64, 16, seed=70)[0]
+        assert _same(main, got)
+        _check_packed(*_packed(dev, [70, 3], 4, 2, 64, seed=71))
+        x, u = _logits(3, 900, 72, torch.float32)
+        _sampled(dev, x, u, top_p=0.9)
+    side.synchronize()
+
+
+def test_wrappers_refuse_what_does_not_fit(cuda_device):
+    from moeinfra_amd import ops
+
+    dev = cuda_device
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device=dev)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)
+    f32 = lambda *s: torch.zeros(s, device=dev)
+    kc, table = bf(4, 2, 16, 64), i32(3, 2)
+    vc = bf(4, 2, 16, 64)
+    bad = [
+        (lambda: ops.rope_paged_kv(bf(3, 768), i32(4), table, kc, vc, 8, f32(32)), "positions"),
+        (lambda: ops.rope_paged_kv(bf(3, 760), i32(3), table, kc, vc, 8, f32(32)), "qkv rows"),
+        (lambda: ops.rope_paged_kv(bf(3, 768), i32(3), table, kc, vc, 8, f32(31)), "inv_freq"),
+        (lambda: ops.rope_paged_kv(bf(3, 768), i32(3), table, kc, bf(5, 2, 16, 64), 8, f32(32)), "differ"),
+        (lambda: ops.rope_paged_kv(bf(3, 768).float(), i32(3), table, kc, vc, 8, f32(32)), "bfloat16"),
+        (lambda: ops.rope_paged_kv(bf(3, 768), i32(3).long(), table, kc, vc, 8, f32(32)), "int32"),
+        (lambda: ops.rope_paged_kv(bf(3, 768), i32(3), table, kc, kc, 8, f32(32)), "caches of their own"),
+        (lambda: ops.rope_paged_kv(bf(3, 768), i32(3), table, kc, vc, 8, f32(32), seq_ids=i32(2)), "seq_ids"),
+        (lambda: ops.paged_attention(bf(3, 8, 64), kc, vc, table, i32(2)), "3 rows"),
+        (lambda: ops.paged_attention(bf(3, 8, 128), kc, vc, table, i32(3)), "head dim"),
+        (lambda: ops.paged_attention(bf(3, 7, 64), kc, vc, table, i32(3)), "invalid attention sizes"),
+        (lambda: ops.paged_attention(bf(3, 64, 8).transpose(1, 2), kc, vc, table, i32(3)), "contiguous rows"),
+        (lambda: ops.paged_attention(bf(3, 8, 64), kc, vc, table, i32(3), workspace=f32(4).to(torch.uint8)), "too small"),
+        (lambda: ops.paged_attention(bf(3, 8, 64), kc.transpose(1, 2), vc.transpose(1, 2), table, i32(3)), "contiguous rows"),
+        (lambda: ops.packed_attention(bf(5, 8, 64), bf(5, 2, 64), bf(4, 2, 64), i32(2)), "do not fit"),
+        (lambda: ops.packed_attention(bf(5, 8, 64), bf(5, 3, 64), bf(5, 3, 64), i32(2)), "multiple"),
+        (lambda: ops.packed_attention(bf(5, 8, 96), bf(5, 2, 96), bf(5, 2, 96), i32(2)), "head dim"),
+        (lambda: ops.packed_attention(bf(5, 8, 64), bf(5, 2, 64), bf(5, 2, 64), i32(2, 2)), "cu_seqlens"),
+        (lambda: ops.sample_tokens(bf(3, 10).half(), f32(3)), "bfloat16"),
+        (lambda: ops.sample_tokens(bf(10, 3).t(), f32(3)), "contiguous rows"),
+        (lambda: ops.sample_tokens(bf(3, 10), f32(2)), "u must be"),
+        (lambda: ops.sample_tokens(bf(3, 10), f32(3), top_k=f32(3)), "top_k"),
+        (lambda: ops.sample_tokens(bf(3, 10), f32(3), top_p=f32(2)), "top_p"),
+        (lambda: ops.sample_tokens(bf(3, 10), f32(3), top_p=0.0), "top-p"),
+        (lambda: ops.sample_tokens(bf(3, 10), f32(3), out=i32(3)), "out"),
+    ]
+    for call, needle in bad:
+        with pytest.raises(ValueError, match=needle):
+            call()
+    # Nothing to do.
+    assert ops.packed_attention(bf(0, 8, 64), bf(0, 2, 64), bf(0, 2, 64), i32(1)).shape == (0, 8, 64)
+    assert ops.paged_attention(bf(0, 8, 64), kc, vc, i32(0, 2), i32(0)).shape == (0, 8, 64)
+    assert ops.sample_tokens(bf(0, 10), f32(0)).shape == (0,)
+    assert ops.rope_paged_kv(bf(0, 768), i32(0), table, kc, vc, 8, f32(32))[0].shape == (0, 512)
+    # A pool without pages: no keys.
+    none = ops.paged_attention(bf(3, 8, 64), kc[:0], vc[:0], table, i32(3) + 20)
+    assert bool((none == 0).all())
