@@ -287,26 +287,49 @@ def layer_forward(table, num_experts: int, gate: torch.Tensor, x: torch.Tensor, 
 
 # ----------------------------------------------------------------------------- batched serving
 # These calls are short (a decode step makes dozens, most of a few us on the device), so their
-# checks are written for the host's time: plain attributes, no views.  The stream is the raw handle
-# of torch.cuda.current_stream, without the Python object around it (0.1 instead of 1.9 us).
+# checks are written for the host's time: what is right takes one expression per tensor, and only
+# what is not goes through the functions that say why.  The stream is the raw handle of
+# torch.cuda.current_stream, without the Python object around it (0.1 instead of 1.9 us).  Of the
+# 8 to 10 us of a call, the launch takes 4.
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+
+
 def _launch(fn, what: str, dev: torch.device, *args) -> None:
     """Calls an entry point with the current stream of ``dev``, on that device (whose sizes the
     launch is planned for, and whose default stream it may be)."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), what)
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), what)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
 
 
-def _require_rows(t: torch.Tensor, name: str, device: torch.device, ndim: int) -> int:
-    """A bf16 tensor [rows, ...] whose rows are contiguous, but not necessarily next to each
-    other (a slice of a projection's output); returns the stride of the rows."""
+def _plain(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device, shape=None) -> int:
+    """The address of a contiguous tensor of this type, device and (unless None) shape."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == dev and t.is_contiguous()):
+        _require(t, name, dtype, dev)
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)} (got {tuple(t.shape)})")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, name: str, dev: torch.device, ndim: int) -> int:
+    """The stride of the rows of a bf16 tensor [rows, ...] whose rows are contiguous, but not
+    necessarily next to each other (a slice of a projection's output)."""
+    if isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.device == dev and t.ndim == ndim and t.is_contiguous():
+        n = t.shape[0]
+        if n > 1:
+            return t.stride(0)
+        if n == 1:
+            return (t.numel() + 7) // 8 * 8  # (there is no other row)
     _require_cuda(t, name)
-    if t.dtype is not torch.bfloat16:
-        raise ValueError(f"{name} must be {torch.bfloat16} (got {t.dtype})")
-    if t.device != device:
-        raise ValueError(f"{name} device {t.device} != {device}")
+    if t.dtype is not _BF16:
+        raise ValueError(f"{name} must be {_BF16} (got {t.dtype})")
+    if t.device != dev:
+        raise ValueError(f"{name} device {t.device} != {dev}")
     shape, strides = t.shape, t.stride()
     if len(shape) != ndim:
         raise ValueError(f"{name} must have {ndim} dimensions (got {tuple(shape)})")
@@ -318,17 +341,27 @@ def _require_rows(t: torch.Tensor, name: str, device: torch.device, ndim: int) -
     return strides[0] if shape[0] > 1 else (row + 7) // 8 * 8
 
 
-def _require_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, device: torch.device) -> int:
-    """Checks a paged cache (k and v [pages, kv heads, page size, head dim], whole pages at one
-    stride) and its table; returns the page stride."""
-    stride = _require_rows(k_cache, "k_cache", device, 4)
-    if _require_rows(v_cache, "v_cache", device, 4) != stride or k_cache.shape != v_cache.shape:
+def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: torch.device) -> int:
+    """The page stride of a paged cache (k and v [pages, kv heads, page size, head dim], whole pages
+    at one stride)."""
+    stride = _rows(k_cache, "k_cache", dev, 4)
+    if _rows(v_cache, "v_cache", dev, 4) != stride or k_cache.shape != v_cache.shape:
         raise ValueError(f"k_cache {tuple(k_cache.shape)} of page stride {stride} and v_cache {tuple(v_cache.shape)} of "
                          f"page stride {v_cache.stride(0)} differ")
-    _require(page_table, "page_table", torch.int32, device)
-    if page_table.ndim != 2:
-        raise ValueError("page_table must be [sequences, pages]")
     return stride
+
+
+def _out(out: Optional[torch.Tensor], name: str, dtype: torch.dtype, dev: torch.device, shape) -> torch.Tensor:
+    """A caller's output, checked for its number of elements, or a new one."""
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    _plain(out, name, dtype, dev)
+    n = 1
+    for s in shape:
+        n *= s
+    if out.numel() != n:
+        raise ValueError(f"{name} has the wrong number of elements")
+    return out
 
 
 def rope_paged_kv(qkv: torch.Tensor, positions: torch.Tensor, page_table: torch.Tensor, k_cache: torch.Tensor,
@@ -345,34 +378,26 @@ def rope_paged_kv(qkv: torch.Tensor, positions: torch.Tensor, page_table: torch.
     Tokens at negative positions are padding: their rows, here and in the cache, are left as they
     were.  A token whose page the table (or the cache) does not have is rotated, not cached.  No
     two tokens of a call may have one place."""
+    _require_cuda(qkv, "qkv")
     dev = qkv.device
-    stride = _require_rows(qkv, "qkv", dev, 2)
-    page_stride = _require_pages(k_cache, v_cache, page_table, dev)
+    stride = _rows(qkv, "qkv", dev, 2)
+    page_stride = _pages(k_cache, v_cache, dev)
     pages, nkv, size, hd = k_cache.shape
-    nq, T = int(n_q_heads), qkv.shape[0]
-    if qkv.shape[1] != (nq + 2 * nkv) * hd:
-        raise ValueError(f"qkv rows have {qkv.shape[1]} values, {nq} query and {nkv} KV heads of {hd} need "
-                         f"{(nq + 2 * nkv) * hd}")
-    _require(positions, "positions", torch.int32, dev)
-    _require(inv_freq, "inv_freq", torch.float32, dev)
-    if positions.shape != (T,):
-        raise ValueError(f"positions must be [{T}] (got {tuple(positions.shape)})")
-    if inv_freq.numel() != hd // 2:
-        raise ValueError(f"inv_freq must have {hd // 2} values")
-    if seq_ids is not None:
-        _require(seq_ids, "seq_ids", torch.int32, dev)
-        if seq_ids.shape != (T,):
-            raise ValueError(f"seq_ids must be [{T}] (got {tuple(seq_ids.shape)})")
-    if q_out is None:
-        q_out = torch.empty((T, nq * hd), dtype=torch.bfloat16, device=dev)
-    else:
-        _require(q_out, "q_out", torch.bfloat16, dev)
-        if q_out.numel() != T * nq * hd:
-            raise ValueError("q_out has the wrong number of elements")
-    k_out = torch.empty((T, nkv, hd), dtype=torch.bfloat16, device=dev) if want_k else None
-    _launch(lib().moe_rope_paged_kv_bf16, "rope_paged_kv", dev, qkv.data_ptr(), stride, T, nq, nkv, hd,
-            inv_freq.data_ptr(), positions.data_ptr(), _ptr(seq_ids), page_table.data_ptr(), page_table.shape[0],
-            page_table.shape[1], pages, size, page_stride, q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(),
+    T, row = qkv.shape
+    nq = int(n_q_heads)
+    if row != (nq + 2 * nkv) * hd:
+        raise ValueError(f"qkv rows have {row} values, {nq} query and {nkv} KV heads of {hd} need {(nq + 2 * nkv) * hd}")
+    table = _plain(page_table, "page_table", _I32, dev)
+    if page_table.ndim != 2:
+        raise ValueError("page_table must be [sequences, pages]")
+    n_seqs, width = page_table.shape
+    pos = _plain(positions, "positions", _I32, dev, (T,))
+    freq = _plain(inv_freq, "inv_freq", _F32, dev, (hd // 2,))
+    seqs = None if seq_ids is None else _plain(seq_ids, "seq_ids", _I32, dev, (T,))
+    q_out = _out(q_out, "q_out", _BF16, dev, (T, nq * hd))
+    k_out = torch.empty((T, nkv, hd), dtype=_BF16, device=dev) if want_k else None
+    _launch(lib().moe_rope_paged_kv_bf16, "rope_paged_kv", dev, qkv.data_ptr(), stride, T, nq, nkv, hd, freq, pos, seqs,
+            table, n_seqs, width, pages, size, page_stride, q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(),
             v_cache.data_ptr())
     return q_out, k_out
 
@@ -393,30 +418,25 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``lens[b]`` (int32) keys of its pages; bf16 [B, q heads, head dim].  ``scaling`` defaults to
     head_dim ** -0.5.  Rows without keys (padding of a batch) are zeros.  ``workspace``
     (``paged_attention_workspace``) saves the call making one."""
+    _require_cuda(q, "q")
     dev = q.device
-    stride = _require_rows(q, "q", dev, 3)
-    page_stride = _require_pages(k_cache, v_cache, page_table, dev)
+    stride = _rows(q, "q", dev, 3)
+    page_stride = _pages(k_cache, v_cache, dev)
     pages, nkv, size, hd = k_cache.shape
-    B, nq = q.shape[:2]
-    if q.shape[2] != hd:
-        raise ValueError(f"q has head dim {q.shape[2]}, the cache {hd}")
-    _require(lens, "lens", torch.int32, dev)
-    if lens.shape != (B,) or page_table.shape[0] != B:
-        raise ValueError(f"lens and page_table must have {B} rows (got {tuple(lens.shape)}, {tuple(page_table.shape)})")
-    if out is None:
-        out = torch.empty((B, nq, hd), dtype=torch.bfloat16, device=dev)
-    else:
-        _require(out, "out", torch.bfloat16, dev)
-        if out.numel() != B * nq * hd:
-            raise ValueError("out has the wrong number of elements")
+    B, nq, q_dim = q.shape
+    if q_dim != hd:
+        raise ValueError(f"q has head dim {q_dim}, the cache {hd}")
+    table = _plain(page_table, "page_table", _I32, dev)
+    if page_table.ndim != 2 or page_table.shape[0] != B:
+        raise ValueError(f"page_table must have {B} rows of pages (got {tuple(page_table.shape)})")
+    n = _plain(lens, "lens", _I32, dev, (B,))
+    out = _out(out, "out", _BF16, dev, (B, nq, hd))
     if workspace is None:
         workspace = paged_attention_workspace(B, nq, nkv, hd, dev)
-    else:
-        _require(workspace, "workspace", torch.uint8, dev)
     _launch(lib().moe_paged_attention_bf16, "paged_attention", dev, q.data_ptr(), stride, k_cache.data_ptr(),
-            v_cache.data_ptr(), pages, size, page_stride, page_table.data_ptr(), page_table.shape[1], lens.data_ptr(),
-            B, nq, nkv, hd, hd ** -0.5 if scaling is None else float(scaling), out.data_ptr(), workspace.data_ptr(),
-            workspace.numel())
+            v_cache.data_ptr(), pages, size, page_stride, table, page_table.shape[1], n, B, nq, nkv, hd,
+            hd ** -0.5 if scaling is None else scaling, out.data_ptr(),
+            _plain(workspace, "workspace", torch.uint8, dev), workspace.numel())
     return out
 
 
@@ -427,23 +447,19 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     [T, q heads, head dim] and ``k``, ``v`` [T, kv heads, head dim], whose rows may lie apart (slices of
     a projection's output); bf16 [T, q heads, head dim].  ``scaling`` defaults to head_dim ** -0.5.
     Tokens of no sequence are left as they were in ``out`` (without one they hold anything)."""
+    _require_cuda(q, "q")
     dev = q.device
-    strides = [_require_rows(t, name, dev, 3) for t, name in ((q, "q"), (k, "k"), (v, "v"))]
+    q_stride, k_stride, v_stride = _rows(q, "q", dev, 3), _rows(k, "k", dev, 3), _rows(v, "v", dev, 3)
     T, nq, hd = q.shape
     if k.shape != v.shape or k.shape[0] != T or k.shape[2] != hd:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
-    _require(cu_seqlens, "cu_seqlens", torch.int32, dev)
+    cu = _plain(cu_seqlens, "cu_seqlens", _I32, dev)
     if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1:
         raise ValueError(f"cu_seqlens must be [sequences + 1] (got {tuple(cu_seqlens.shape)})")
-    if out is None:
-        out = torch.empty((T, nq, hd), dtype=torch.bfloat16, device=dev)
-    else:
-        _require(out, "out", torch.bfloat16, dev)
-        if out.numel() != T * nq * hd:
-            raise ValueError("out has the wrong number of elements")
-    _launch(lib().moe_packed_attention_bf16, "packed_attention", dev, q.data_ptr(), strides[0], k.data_ptr(),
-            strides[1], v.data_ptr(), strides[2], T, cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, nq, k.shape[1],
-            hd, hd ** -0.5 if scaling is None else float(scaling), out.data_ptr())
+    out = _out(out, "out", _BF16, dev, (T, nq, hd))
+    _launch(lib().moe_packed_attention_bf16, "packed_attention", dev, q.data_ptr(), q_stride, k.data_ptr(), k_stride,
+            v.data_ptr(), v_stride, T, cu, cu_seqlens.numel() - 1, nq, k.shape[1], hd,
+            hd ** -0.5 if scaling is None else scaling, out.data_ptr())
     return out
 
 
@@ -458,33 +474,27 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     rising index, at which the kept weights add up to more than ``u`` of their sum.  Temperature 0
     gives the largest logit.  -inf and NaN are never drawn; a row of nothing else gives -1.  Each
     setting is a number, or a tensor with a value per row (fp32; ``top_k`` int32)."""
-    dev = logits.device
     _require_cuda(logits, "logits")
-    if logits.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"logits must be {torch.bfloat16} or {torch.float32} (got {logits.dtype})")
-    if logits.ndim != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    dev, f32 = logits.device, logits.dtype is _F32
+    if not f32 and logits.dtype is not _BF16:
+        raise ValueError(f"logits must be {_BF16} or {_F32} (got {logits.dtype})")
+    if logits.ndim != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError(f"logits must be [rows, vocabulary] with contiguous rows (got {tuple(logits.shape)}, "
                          f"strides {logits.stride()})")
     B, V = logits.shape
-    _require(u, "u", torch.float32, dev)
-    if u.shape != (B,):
-        raise ValueError(f"u must be [{B}] (got {tuple(u.shape)})")
-    args = []
-    for value, name, dtype, cast in ((temperature, "temperature", torch.float32, float), (top_k, "top_k", torch.int32, int),
-                                     (top_p, "top_p", torch.float32, float), (min_p, "min_p", torch.float32, float)):
-        if isinstance(value, torch.Tensor):
-            _require(value, name, dtype, dev)
-            if value.shape != (B,):
-                raise ValueError(f"{name} must be a number or [{B}] (got {tuple(value.shape)})")
-            args += [value.data_ptr(), 1]
-        else:
-            args += [None, cast(value)]
-    if out is None:
-        out = torch.empty((B,), dtype=torch.int64, device=dev)
-    else:
-        _require(out, "out", torch.int64, dev)
-        if out.numel() != B:
-            raise ValueError("out has the wrong number of elements")
-    _launch(lib().moe_sample_tokens, "sample_tokens", dev, logits.data_ptr(), int(logits.dtype == torch.float32),
-            logits.stride(0) if B > 1 else V, B, V, u.data_ptr(), *args, out.data_ptr())
+    shape = (B,)
+    numbers = _plain(u, "u", _F32, dev, shape)
+    out = _out(out, "out", torch.int64, dev, shape)
+    tensor = torch.Tensor
+    t = k = p = m = None
+    if isinstance(temperature, tensor):
+        t, temperature = _plain(temperature, "temperature", _F32, dev, shape), 1.0
+    if isinstance(top_k, tensor):
+        k, top_k = _plain(top_k, "top_k", _I32, dev, shape), 0
+    if isinstance(top_p, tensor):
+        p, top_p = _plain(top_p, "top_p", _F32, dev, shape), 1.0
+    if isinstance(min_p, tensor):
+        m, min_p = _plain(min_p, "min_p", _F32, dev, shape), 0.0
+    _launch(lib().moe_sample_tokens, "sample_tokens", dev, logits.data_ptr(), int(f32), logits.stride(0) if B > 1 else V,
+            B, V, numbers, t, temperature, k, top_k, p, top_p, m, min_p, out.data_ptr())
     return out

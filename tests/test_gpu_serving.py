@@ -680,7 +680,7 @@ def test_wrappers_refuse_what_does_not_fit(cuda_device):
         (lambda: ops.rope_paged_kv(bf(3, 768), i32(3).long(), table, kc, vc, 8, f32(32)), "int32"),
         (lambda: ops.rope_paged_kv(bf(3, 768), i32(3), table, kc, kc, 8, f32(32)), "caches of their own"),
         (lambda: ops.rope_paged_kv(bf(3, 768), i32(3), table, kc, vc, 8, f32(32), seq_ids=i32(2)), "seq_ids"),
-        (lambda: ops.paged_attention(bf(3, 8, 64), kc, vc, table, i32(2)), "3 rows"),
+        (lambda: ops.paged_attention(bf(3, 8, 64), kc, vc, table, i32(2)), "lens must be"),
         (lambda: ops.paged_attention(bf(3, 8, 128), kc, vc, table, i32(3)), "head dim"),
         (lambda: ops.paged_attention(bf(3, 7, 64), kc, vc, table, i32(3)), "invalid attention sizes"),
         (lambda: ops.paged_attention(bf(3, 64, 8).transpose(1, 2), kc, vc, table, i32(3)), "contiguous rows"),
