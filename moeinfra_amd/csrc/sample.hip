@@ -193,17 +193,22 @@ __device__ __forceinline__ float sm_value(uint32_t bits) {
 }
 
 // f(chunk, number) of chunks c0 + first, c0 + first + step, ... below c1 (those at the row's ends by
-// first = 0); two more are on their way while one is looked at.
+// first = 0), beginning with a sixteenth times `turn` of them; two more are on their way while one is
+// looked at.
 template <typename E, typename F>
-__device__ __forceinline__ void sm_chunks(const SmRow<E> &row, int c0, int c1, int first, int step, F f) {
-  const int a = max(c0, row.whole0()) + first, b = min(c1, row.whole1());
-  if (a < b) {
-    u32x4 v0 = row.raw(a), v1 = row.raw(min(a + step, b - 1)), v2;
-    for (int c = a; c < b; c += step) {
-      v2 = row.raw(min(c + 2 * step, b - 1));
-      f(v0, c);
+__device__ __forceinline__ void sm_chunks(const SmRow<E> &row, int c0, int c1, int first, int step, int turn, F f) {
+  const int a = max(c0, row.whole0()), b = min(c1, row.whole1());
+  const int n = max(b - a + step - 1, 0) / step;  // steps (the last one's chunks not all there)
+  if (n > 0) {
+    int i = n * turn / 16;
+    auto at = [&](int k) { return a + first + (i + k < n ? i + k : i + k < 2 * n ? i + k - n : 0) * step; };
+    u32x4 v0 = row.raw(min(at(0), b - 1)), v1 = row.raw(min(at(1), b - 1)), v2;
+    for (int k = 0; k < n; ++k) {
+      v2 = row.raw(min(at(2), b - 1));
+      if (at(0) < b) f(v0, at(0));
       v0 = v1;
       v1 = v2;
+      i = i + 1 < n ? i + 1 : 0;
     }
   }
   if (first != 0) return;
@@ -214,10 +219,70 @@ __device__ __forceinline__ void sm_chunks(const SmRow<E> &row, int c0, int c1, i
   }
 }
 
+// The part of a row that a thread looks at in each pass: every 64th chunk of its wave's stretch (a
+// sixteenth of the row).  NC > 0: at most NC chunks, read once and kept in registers (16 of them are
+// half of a thread's: a row of 131072 bf16 logits is then read once, 256 KB a CU, instead of in each
+// pass: 256 rows top-p 44 -> 35 us); 0: read again in each pass.
+//
+// Wave w begins with its w-th: stretches often lie powers of two apart, and in step all waves would ask
+// the same few memory channels (greedy, 256 rows of 131072: 29 us instead of 23).
+template <typename E, int NC>
+struct SmMine {
+  const SmRow<E> &row;
+  int c0, c1, turn;
+  u32x4 v[NC > 0 ? NC : 1];
+
+  // The chunk in v[i].
+  __device__ __forceinline__ int at(int i) const {
+    return c0 + ((i + turn) & (NC - 1)) * kWave + (int)(threadIdx.x & (kWave - 1));
+  }
+
+  __device__ __forceinline__ SmMine(const SmRow<E> &row_) : row(row_) {
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int per = (row.chunks + kSmWaves - 1) / kSmWaves;
+    c0 = min(wave * per, row.chunks);
+    c1 = min(c0 + per, row.chunks);
+    turn = wave;
+    if constexpr (NC > 0) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)  // (the row has whole chunks)
+        v[i] = row.raw(min(max(at(i), row.whole0()), row.whole1() - 1));
+      // The row's ends, where they are shared with other rows.
+      for (int k = 0; k < 2; ++k) {
+        const int end = k == 0 ? 0 : row.chunks - 1;
+        if (end < c0 || end >= c1 || (end >= row.whole0() && end < row.whole1())) continue;
+        if (lane == (end - c0) % kWave) {
+          const u32x4 x = row.chunk(end);
+#pragma unroll
+          for (int i = 0; i < NC; ++i) v[i] = at(i) == end ? x : v[i];
+        }
+      }
+    }
+  }
+  // f(chunk, number) of each.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    if constexpr (NC > 0) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        // (One chunk after the other, and nothing of one pass kept for the next but the chunk itself:
+        // otherwise the compiler runs out of registers.)
+        u32x4 x = v[i];
+        int c = at(i);
+        asm volatile("" : "+v"(x), "+v"(c));
+        if (c < c1) f(x, c);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      sm_chunks(row, c0, c1, (int)(threadIdx.x & (kWave - 1)), kWave, turn, f);
+    }
+  }
+};
+
 // f(bits, index) of every element of the row, shared by the workgroup's threads.
 template <typename E, typename F>
 __device__ __forceinline__ void sm_each(const SmRow<E> &row, F f) {
-  sm_chunks(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, [&](const u32x4 &v, int c) {
+  sm_chunks(row, 0, row.chunks, (int)threadIdx.x, kSmThreads, 0, [&](const u32x4 &v, int c) {
 #pragma unroll
     for (int e = 0; e < SmRow<E>::N; ++e) f(SmRow<E>::bits(v, e), row.index(c, e));
   });
@@ -286,9 +351,11 @@ __device__ __forceinline__ u64 sm_block_sum(SmShare &s, u64 v) {
 // there is none.  Elements weigh f(bits, index, equal); those for which it sets `equal` weigh `each`
 // as long as there have been no more than `need` of them.  A chunk whose largest element is below
 // `least` weighs nothing.
-template <typename E, typename F, typename P>
-__device__ __forceinline__ int sm_locate(SmShare &s, const SmRow<E> &row, float least, u64 need, u64 each, F f, P pick) {
+template <typename E, int NC, typename F, typename P>
+__device__ __forceinline__ int sm_locate(SmShare &s, const SmMine<E, NC> &mine, float least, u64 need, u64 each, F f,
+                                         P pick) {
   constexpr int N = SmRow<E>::N;
+  const SmRow<E> &row = mine.row;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   auto add = [&](const u32x4 &v, int c, u64 &sum, u64 &n) {
     if (!(sm_largest<E>(v) >= least)) return;
@@ -304,11 +371,9 @@ __device__ __forceinline__ int sm_locate(SmShare &s, const SmRow<E> &row, float 
     for (int e = 0; e < N; ++e) sum += m[e];
     n += k;
   };
-  // A stretch of whole chunks per wave.
-  const int per = (row.chunks + kSmWaves - 1) / kSmWaves;
+  const int per = (row.chunks + kSmWaves - 1) / kSmWaves;  // of a wave's stretch
   u64 sum = 0, n = 0;
-  sm_chunks(row, min(wave * per, row.chunks), min(wave * per + per, row.chunks), lane, kWave,
-            [&](const u32x4 &v, int c) { add(v, c, sum, n); });
+  mine.each([&](const u32x4 &v, int c) { add(v, c, sum, n); });
   sum = sm_wave_sum(sum);
   n = sm_wave_sum(n);
   if (lane == 0) {
@@ -317,8 +382,8 @@ __device__ __forceinline__ int sm_locate(SmShare &s, const SmRow<E> &row, float 
   }
   __syncthreads();
   // Every wave: the stretches' running sums in its rows of 16 lanes, and the one with the target.
-  const u64 mine = s.part[lane & (kSmWaves - 1)], equals = s.part2[lane & (kSmWaves - 1)];
-  const u64 run_m = sm_row_incl(mine), run_n = sm_row_incl(equals);
+  const u64 part = s.part[lane & (kSmWaves - 1)], equals = s.part2[lane & (kSmWaves - 1)];
+  const u64 run_m = sm_row_incl(part), run_n = sm_row_incl(equals);
   const u64 upto = run_m + min(run_n, need) * each;
   const u64 total = sm_readlane(upto, kSmWaves - 1);
   __syncthreads();
@@ -394,6 +459,7 @@ __device__ __forceinline__ u64 sm_target(float u, u64 total) {
 template <typename E>
 __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> row, const SmAsk a, float mx,
                                        const double *table) {
+  const SmMine<E, 0> mine(row);
   // With an infinite maximum only its equals weigh anything: as zeros over -inf.
   const bool infinite = mx == INFINITY;
   const double m = infinite ? 0.0 : (double)mx;
@@ -529,7 +595,7 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
       const uint32_t kk = key;
       const u64 n = need;
       cut = sm_locate(
-          s, row, -INFINITY, 0, 0,
+          s, mine, -INFINITY, 0, 0,
           [&](uint32_t bits, int, bool &) {
             const float v = value(sm_value(bits));
             return (u64)(v != -INFINITY && sm_key(v) == kk);
@@ -539,7 +605,7 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
   }
   const double floor_w = (double)a.min_p * 0x1p43;
   return sm_locate(
-      s, row, -INFINITY, 0, 0,
+      s, mine, -INFINITY, 0, 0,
       [&](uint32_t bits, int i, bool &) -> u64 {
         const float v = value(sm_value(bits));
         const uint32_t kk = sm_key(v);
@@ -592,15 +658,11 @@ __device__ __forceinline__ bool sm_counts(uint32_t bits, bool &far, bool &odd) {
   return false;
 }
 
-// LDS of a row in bf16: a bin holds one value.  (127 KB)
-struct SmExact {
+struct SmBins {
   uint32_t count[kSmNone];
-  u64 weight[kSmEntries];  // of a bin's value, 0 where it is not kept
-};
-// LDS of a row in fp32: one bin's logits are ranked. (61 KB)
-struct SmRanked {
-  uint32_t count[kSmNone];
-  u64 rank[kSmList];  // key and index: better logits have larger ones
+  u64 weight[kSmEntries];  // of a bin's value (fp32: of its middle), where there are logits
+  // fp32: one bin's logits, to be ranked.
+  u64 rank[kSmList];       // key and index: better logits have larger ones
   u64 mass[kSmList];
   int n;
 };
@@ -614,57 +676,81 @@ struct SmRanked {
 //
 // Bound: passes over the row (each of the LDS atomics of 1, of some 10 instructions per logit of 3,
 // and in fp32 of the 64-bit weights of 2) on one CU.
-template <typename E>
+template <typename E, int NC>
 __global__ void __launch_bounds__(kSmThreads)
 sample_kernel(const SmArgs a) {
   constexpr bool kExact = sizeof(E) == 2;
-  using Bins = std::conditional_t<kExact, SmExact, SmRanked>;
+  constexpr int N = SmRow<E>::N;
   __shared__ union {
-    Bins bins;
+    SmBins bins;
     SmGeneral general;
   } lds;
-  Bins &b = lds.bins;
+  SmBins &b = lds.bins;
   __shared__ SmShare s;
   __shared__ double table[kSmTable];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
   const int64_t r = blockIdx.x;
   const SmRow<E> row((const E *)a.logits + r * a.stride, a.V);
+  const SmMine<E, NC> mine(row);
   const SmAsk ask{a.temperature ? a.temperature[r] : a.temperature0, a.top_p ? a.top_p[r] : a.top_p0,
                   a.min_p ? a.min_p[r] : a.min_p0, a.u[r], a.top_k ? a.top_k[r] : a.top_k0};
   // Greedy: the first of the order (temperatures of zero and below, and NaN).
   const bool greedy = !(ask.T > 0.0f) || ask.k == 1;
   const bool by_k = ask.k > 0 && ask.k < a.V, by_p = ask.p < 1.0f;
 
+  if (tid < kSmTable)
+    table[tid] = tid <= kSmTable / 2 ? sm_exp2(-tid / (double)kSmTable) : 0.5 * sm_exp2(1.0 - tid / (double)kSmTable);
   float mx = -INFINITY;
   bool far = false, odd = false;
   if (greedy || (!kExact && !by_k && !by_p)) {  // no counts needed
-    sm_each(row, [&](uint32_t bits, int) { mx = fmaxf(mx, __builtin_bit_cast(float, bits)); });
+    mine.each([&](const u32x4 &v, int) { mx = fmaxf(mx, sm_largest<E>(v)); });
   } else {
     for (int i = tid; i < kSmNone; i += kSmThreads) b.count[i] = 0;
     __syncthreads();
-    sm_chunks(row, 0, row.chunks, tid, kSmThreads, [&](const u32x4 &v, int) {
-      constexpr int N = SmRow<E>::N;
-      mx = fmaxf(mx, sm_largest<E>(v));
-      // Whether all have bins: magnitudes at most the last one's, and either zero (which one less
-      // takes past all others) or the first one's at least.
-      uint32_t most = 0, least = ~0u;
+    uint32_t later = 0;  // chunks with logits that have no bin, a bit each
+    auto slow = [&](const u32x4 &v) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const uint32_t x = SmRow<E>::bits(v, e);
-        most = max(most, sm_upper(x));
-        least = min(least, kExact ? sm_upper(x) - 1 : (x & 0x7fffffffu) - 1);
+        if (sm_counts(x, far, odd)) atomicAdd(&b.count[sm_bin(x)], 1u);
       }
-      if (most < kSmLow + kSmSide && least >= (kExact ? kSmLow - 1 : (kSmLow << 16) - 1)) {
+    };
+    mine.each([&](const u32x4 &v, int c) {
+      mx = fmaxf(mx, sm_largest<E>(v));
+      // Whether all have bins: magnitudes at most the last one's, and either zero (which one less
+      // takes past all others) or the first one's at least.  -inf (a mask's) is left out.
+      auto low = [&](uint32_t x) { return kExact ? sm_upper(x) - 1 : (x & 0x7fffffffu) - 1; };
+      constexpr uint32_t kLeast = kExact ? kSmLow - 1 : (kSmLow << 16) - 1;
+      uint32_t most = 0, least = ~0u;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        most = max(most, sm_upper(SmRow<E>::bits(v, e)));
+        least = min(least, low(SmRow<E>::bits(v, e)));
+      }
+      if (most < kSmLow + kSmSide && least >= kLeast) {
 #pragma unroll
         for (int e = 0; e < N; ++e) atomicAdd(&b.count[sm_bin(SmRow<E>::bits(v, e))], 1u);
-      } else {
+        return;
+      }
+      bool fine = true;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const uint32_t x = SmRow<E>::bits(v, e);
+        fine &= (x == 0xff800000u) | ((sm_upper(x) < kSmLow + kSmSide) & (low(x) >= kLeast));
+      }
+      if (fine) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const uint32_t x = SmRow<E>::bits(v, e);
-          if (sm_counts(x, far, odd)) atomicAdd(&b.count[sm_bin(x)], 1u);
+          if (x != 0xff800000u) atomicAdd(&b.count[sm_bin(x)], 1u);
         }
+      } else if (NC > 0) {
+        later |= 1u << ((c - mine.c0) / kWave);
+      } else {
+        slow(v);
       }
     });
+    for (; later != 0; later &= later - 1) slow(row.chunk(mine.c0 + __builtin_ctz(later) * kWave + lane));
   }
   {
     float v[1] = {mx};
@@ -674,8 +760,6 @@ sample_kernel(const SmArgs a) {
       s.bits[wave] = __builtin_bit_cast(uint32_t, v[0]);
       s.flags[wave] = flags;
     }
-    if (tid < kSmTable)
-      table[tid] = tid <= kSmTable / 2 ? sm_exp2(-tid / (double)kSmTable) : 0.5 * sm_exp2(1.0 - tid / (double)kSmTable);
     __syncthreads();
     v[0] = __builtin_bit_cast(float, s.bits[lane & (kSmWaves - 1)]);
     const uint32_t f = s.flags[lane & (kSmWaves - 1)];
@@ -690,7 +774,7 @@ sample_kernel(const SmArgs a) {
   }
   if (greedy) {
     const int at = sm_locate(
-        s, row, mx, 0, 0, [&](uint32_t bits, int, bool &) { return (u64)(__builtin_bit_cast(float, bits) == mx); },
+        s, mine, mx, 0, 0, [&](uint32_t bits, int, bool &) { return (u64)(__builtin_bit_cast(float, bits) == mx); },
         [](u64) { return (u64)0; });
     if (tid == 0) a.token[r] = at;
     return;
@@ -706,45 +790,41 @@ sample_kernel(const SmArgs a) {
   const double floor_w = (double)ask.min_p * 0x1p43;
   auto target = [&](u64 total) { return sm_target(ask.u, total); };
 
-  // This thread's bins: their counts, and their weight (fp32: as if all lay in the bin's middle).
-  uint32_t n_bin[kSmPer];
-  u64 w_bin[kSmPer];
-  u64 n_own = 0, m_own = 0;
-  // (The largest logit's bin: as if all were it, so that there is some weight.)
+  // The bins' weights (fp32: as if all of a bin lay in its middle; those of the largest logit's bin as
+  // if all were it, so that there is some weight).
   const int top = sm_bin(__builtin_bit_cast(uint32_t, mx));
-  auto bin_weight = [&](int bin) {
-    return sm_mass(weight.real(bin == top ? mx : sm_bin_value(bin, kExact ? 0u : 0x8000u)));
-  };
+  u64 n_own = 0, m_own = 0;  // counts and weights of this thread's bins, kSmPer in order
   if (kExact || by_k || by_p) {
+    for (int bin = tid; bin < kSmEntries; bin += kSmThreads)  // (bins with logits are next to each other: all take part)
+      if (b.count[bin] != 0)
+        b.weight[bin] = sm_mass(weight.real(bin == top ? mx : sm_bin_value(bin, kExact ? 0u : 0x8000u)));
+    if (tid == 0) b.weight[0] = b.weight[kSmEntries - 1] = 0;  // what has no bin
+    __syncthreads();
+    uint32_t n[kSmPer];
 #pragma unroll
-    for (int i = 0; i < kSmPer; ++i) n_bin[i] = b.count[tid * kSmPer + i];
+    for (int i = 0; i < kSmPer; ++i) n[i] = b.count[tid * kSmPer + i];
 #pragma unroll
     for (int i = 0; i < kSmPer; ++i) {
-      w_bin[i] = 0;
-      if (n_bin[i] == 0) continue;
-      w_bin[i] = bin_weight(tid * kSmPer + i);
-      if constexpr (kExact) b.weight[tid * kSmPer + i] = w_bin[i];
-      n_own += n_bin[i];
-      m_own += n_bin[i] * w_bin[i];
+      if (n[i] == 0) continue;
+      n_own += n[i];
+      m_own += n[i] * b.weight[tid * kSmPer + i];
     }
   }
   const SmScan run = kExact || by_k || by_p ? sm_scan(s, n_own, m_own) : SmScan{};
-  // The bin in which the running count (or weight) reaches goal, and both before it.
+  // The bin in which the running count (or weight) reaches goal (1 at least, at most all), and both
+  // before it.  Uniform over the workgroup.
   auto edge_of = [&](bool count, u64 goal, u64 &n_before, u64 &m_before) {
-    u64 x, y;
-    const int t = count ? sm_cross(s, run.a, n_own, run.b, m_own, goal, x, y)
-                        : sm_cross(s, run.b, m_own, run.a, n_own, goal, y, x);
-    if (tid == t) {
-      int edge = tid * kSmPer;
-      bool found = false;
-#pragma unroll
-      for (int i = 0; i < kSmPer; ++i) {
-        if (found || n_bin[i] == 0) continue;
-        edge = tid * kSmPer + i;
-        const u64 m = n_bin[i] * w_bin[i];
-        found = (count ? x + n_bin[i] : y + m) >= goal;
-        x += found ? 0 : n_bin[i];
-        y += found ? 0 : m;
+    u64 x = run.a - n_own, y = run.b - m_own;
+    if (count ? run.a >= goal && x < goal : run.b >= goal && y < goal) {
+      int edge = 0;
+      for (int bin = tid * kSmPer; bin < tid * kSmPer + kSmPer; ++bin) {
+        const uint32_t n = b.count[bin];
+        if (n == 0) continue;
+        edge = bin;
+        const u64 m = n * b.weight[bin];
+        if ((count ? x + n : y + m) >= goal) break;
+        x += n;
+        y += m;
       }
       s.r_i = edge;
       s.r_a = x;
@@ -786,22 +866,18 @@ sample_kernel(const SmArgs a) {
         if (!((double)each >= floor_w) && least != mx) each = 0;
       }
     }
-    // Weights of what is not kept are taken as zero; the edge's are counted apart.
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kSmPer; ++i) {
-      const int bin = tid * kSmPer + i;
-      if (n_bin[i] != 0 && (bin >= edge || (!((double)w_bin[i] >= floor_w) && sm_bin_value(bin, 0) != mx)))
-        b.weight[bin] = 0;
+    if (ask.min_p > 0.0f) {
+      __syncthreads();
+      for (int bin = tid; bin < kSmEntries; bin += kSmThreads)
+        if (b.count[bin] != 0 && !((double)b.weight[bin] >= floor_w) && bin != top) b.weight[bin] = 0;
+      __syncthreads();
     }
-    if (tid == 0) b.weight[0] = b.weight[kSmEntries - 1] = 0;  // what has no bin
-    __syncthreads();
     const int at = sm_locate(
-        s, row, least, need, each,
+        s, mine, least, need, each,
         [&](uint32_t bits, int, bool &equal) -> u64 {
           const int bin = sm_bin(bits);
           equal = bin == edge;
-          return b.weight[bin];
+          return b.weight[bin < edge ? bin : 0];  // (the edge's are counted apart)
         },
         target);
     if (tid == 0) a.token[r] = at;
@@ -812,7 +888,6 @@ sample_kernel(const SmArgs a) {
     int last = kSmEntries - 2;  // the last bin with kept logits
     u64 n0 = 0, m0 = 0;
     bool failed = false;     // a bin too full to rank
-    __syncthreads();
     // The smallest logit of a bin.
     auto bin_floor = [&](int bin) { return sm_bin_value(bin, bin > kSmZero ? 0xffffu : 0u); };
     // A logit of the bin that is ranked into the list.
@@ -840,8 +915,14 @@ sample_kernel(const SmArgs a) {
         if (!failed) {
           if (tid == 0) b.n = 0;
           __syncthreads();
-          sm_each(row, [&](uint32_t bits, int i) {
-            if (sm_bin(bits) == last && sm_counts(bits, far, odd)) put(sm_key(__builtin_bit_cast(float, bits)), i, 0);
+          const float from = bin_floor(last), over = bin_floor(last - 1);
+          mine.each([&](const u32x4 &v, int c) {
+            if (!(sm_largest<E>(v) >= from)) return;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              const float x = __builtin_bit_cast(float, SmRow<E>::bits(v, e));
+              if (x >= from && !(x >= over)) put(sm_key(x), row.index(c, e), 0);
+            }
           });
           __syncthreads();
           const int n = b.n;
@@ -852,7 +933,7 @@ sample_kernel(const SmArgs a) {
             for (int i = 0; i < n; ++i) rank += b.rank[i] > mine;
           }
           decide(tid < n && rank == (u64)ask.k - n0 - 1);
-          estimate = m0 + ((u64)ask.k - n0) * bin_weight(last);
+          estimate = m0 + ((u64)ask.k - n0) * b.weight[last];
         }
       }
     }
@@ -869,10 +950,9 @@ sample_kernel(const SmArgs a) {
         __syncthreads();
         u64 above = 0, inside = 0, all = 0;
         const float in_bin = bin_floor(g), over = bin_floor(g - 1);
-        sm_chunks(row, 0, row.chunks, tid, kSmThreads, [&](const u32x4 &v, int c) {
-          constexpr int N = SmRow<E>::N;
-          const float top = sm_largest<E>(v);
-          if (!(top >= least)) return;
+        mine.each([&](const u32x4 &v, int c) {
+          const float largest = sm_largest<E>(v);
+          if (!(largest >= least)) return;
           float x[N];
           u64 m[N];
 #pragma unroll
@@ -886,7 +966,7 @@ sample_kernel(const SmArgs a) {
           }
 #pragma unroll
           for (int e = 0; e < N; ++e) all += m[e];
-          if (top >= in_bin) {
+          if (largest >= in_bin) {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
               above += x[e] >= over ? m[e] : 0;
@@ -909,7 +989,7 @@ sample_kernel(const SmArgs a) {
           want = m0 > above - goal ? m0 - (above - goal) : 1;
         } else if (above + inside < goal) {
           lo = g + 1;
-          want = m0 + b.count[g] * bin_weight(g) + (goal - above - inside);
+          want = m0 + (b.count[g] != 0 ? b.count[g] * b.weight[g] : 0) + (goal - above - inside);
           want = want < estimate ? want : estimate;
         } else {
           const int n = b.n;
@@ -930,7 +1010,7 @@ sample_kernel(const SmArgs a) {
       at = sm_general(lds.general, s, row, ask, mx, table);
     } else {
       at = sm_locate(
-          s, row, least, 0, 0,
+          s, mine, least, 0, 0,
           [&](uint32_t bits, int i, bool &) -> u64 {
             const float x = __builtin_bit_cast(float, bits);
             const double w = weight.real(x);
@@ -969,7 +1049,17 @@ extern "C" int moe_sample_tokens(const void *logits, int32_t logits_f32, int64_t
   moe::SmArgs a{logits, stride, (int)V, (const float *)u_f32, (const float *)temperature_f32,
                 (const int32_t *)top_k_i32, (const float *)top_p_f32, (const float *)min_p_f32, temperature, top_p,
                 min_p, top_k, (int64_t *)token_i64};
-  auto kern = logits_f32 ? moe::sample_kernel<float> : moe::sample_kernel<uint16_t>;
+  // Chunks of 16 bytes per thread: (V + a chunk's end at most) / chunk / threads, in sixteenths of a row
+  // rounded up.  Rows without whole chunks, and those of more, are read again in each pass.
+  const int64_t n = logits_f32 ? 4 : 8;
+  const int64_t per = ((V + 2 * n - 2) / n + moe::kSmWaves - 1) / moe::kSmWaves;  // of a wave's stretch
+  const int64_t chunks = V < 2 * n ? moe::kSmNone : (per + moe::kWave - 1) / moe::kWave;
+  auto kern = logits_f32 ? (chunks <= 8    ? moe::sample_kernel<float, 8>
+                            : chunks <= 16 ? moe::sample_kernel<float, 16>
+                                           : moe::sample_kernel<float, 0>)
+                         : (chunks <= 4    ? moe::sample_kernel<uint16_t, 4>
+                            : chunks <= 16 ? moe::sample_kernel<uint16_t, 16>
+                                           : moe::sample_kernel<uint16_t, 0>);
   hipLaunchKernelGGL(kern, dim3((unsigned)B), dim3(moe::kSmThreads), 0, (hipStream_t)stream, a);
   MOE_LAUNCH_CHECK();
   return MOE_STATUS_OK;
