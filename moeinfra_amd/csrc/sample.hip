@@ -52,6 +52,10 @@ __device__ __forceinline__ uint32_t sm_key(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+__device__ __forceinline__ float sm_from_key(uint32_t key) {
+  return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
 // 2^f in 64 bits, |f| <= 1/2: the series to f^13.
 __device__ __forceinline__ double sm_exp2(double f) {
   const double t = f * 0.69314718055994530942;
@@ -350,10 +354,10 @@ __device__ __forceinline__ u64 sm_block_sum(SmShare &s, u64 v) {
 // The first index at which the running weight of the row exceeds its target, pick(all of it); -1 if
 // there is none.  Elements weigh f(bits, index, equal); those for which it sets `equal` weigh `each`
 // as long as there have been no more than `need` of them.  A chunk whose largest element is below
-// `least` weighs nothing.
+// `least` weighs nothing.  known: this thread's part of the weight, where a pass has it already.
 template <typename E, int NC, typename F, typename P>
 __device__ __forceinline__ int sm_locate(SmShare &s, const SmMine<E, NC> &mine, float least, u64 need, u64 each, F f,
-                                         P pick) {
+                                         P pick, const u64 *known = nullptr) {
   constexpr int N = SmRow<E>::N;
   const SmRow<E> &row = mine.row;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -373,7 +377,10 @@ __device__ __forceinline__ int sm_locate(SmShare &s, const SmMine<E, NC> &mine, 
   };
   const int per = (row.chunks + kSmWaves - 1) / kSmWaves;  // of a wave's stretch
   u64 sum = 0, n = 0;
-  mine.each([&](const u32x4 &v, int c) { add(v, c, sum, n); });
+  if (known != nullptr)
+    sum = *known;
+  else
+    mine.each([&](const u32x4 &v, int c) { add(v, c, sum, n); });
   sum = sm_wave_sum(sum);
   n = sm_wave_sum(n);
   if (lane == 0) {
@@ -732,13 +739,13 @@ sample_kernel(const SmArgs a) {
         for (int e = 0; e < N; ++e) atomicAdd(&b.count[sm_bin(SmRow<E>::bits(v, e))], 1u);
         return;
       }
-      bool fine = true;
+      int fine = 1;  // (not short-circuited: no branches)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const uint32_t x = SmRow<E>::bits(v, e);
-        fine &= (x == 0xff800000u) | ((sm_upper(x) < kSmLow + kSmSide) & (low(x) >= kLeast));
+        fine &= (int)(x == 0xff800000u) | ((int)(sm_upper(x) < kSmLow + kSmSide) & (int)(low(x) >= kLeast));
       }
-      if (fine) {
+      if (fine != 0) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const uint32_t x = SmRow<E>::bits(v, e);
@@ -787,7 +794,9 @@ sample_kernel(const SmArgs a) {
     return;
   }
   const SmWeight weight(table, (double)mx, c2);
-  const double floor_w = (double)ask.min_p * 0x1p43;
+  // What min_p asks of a weight (the largest is kept whatever it asks).
+  const double floor_d = ceil((double)ask.min_p * 0x1p43);
+  const u64 floor_w = floor_d > 0.0 ? (floor_d < 0x1p44 ? (u64)floor_d : 1ull << 44) : ask.min_p <= 0.0f ? 0 : 1ull << 44;
   auto target = [&](u64 total) { return sm_target(ask.u, total); };
 
   // The bins' weights (fp32: as if all of a bin lay in its middle; those of the largest logit's bin as
@@ -863,13 +872,13 @@ sample_kernel(const SmArgs a) {
       if (b.count[edge] != 0) {
         each = b.weight[edge];
         least = sm_bin_value(edge, 0);
-        if (!((double)each >= floor_w) && least != mx) each = 0;
+        if (each < floor_w && edge != top) each = 0;
       }
     }
-    if (ask.min_p > 0.0f) {
+    if (floor_w > 0) {
       __syncthreads();
       for (int bin = tid; bin < kSmEntries; bin += kSmThreads)
-        if (b.count[bin] != 0 && !((double)b.weight[bin] >= floor_w) && bin != top) b.weight[bin] = 0;
+        if (b.count[bin] != 0 && b.weight[bin] < floor_w && bin != top) b.weight[bin] = 0;
       __syncthreads();
     }
     const int at = sm_locate(
@@ -884,7 +893,9 @@ sample_kernel(const SmArgs a) {
   } else {
     float least = -INFINITY;  // kept: larger logits, and this one up to index `cut`
     int cut = 0x7fffffff;
-    auto kept = [&](float x, int i) { return (x > least) | ((x == least) & (i <= cut)); };
+    auto kept = [&](float x, int i) {  // (not short-circuited: no branches)
+      return ((int)(x > least) | ((int)(x == least) & (int)(i <= cut))) != 0;
+    };
     int last = kSmEntries - 2;  // the last bin with kept logits
     u64 n0 = 0, m0 = 0;
     bool failed = false;     // a bin too full to rank
@@ -901,12 +912,11 @@ sample_kernel(const SmArgs a) {
     auto decide = [&](bool mine) {  // the list's last kept logit, found by one thread
       if (mine) s.r_a = b.rank[tid];
       __syncthreads();
-      const uint32_t key = (uint32_t)(s.r_a >> 32);
       cut = (int)~(uint32_t)s.r_a;
-      least = __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
+      least = sm_from_key((uint32_t)(s.r_a >> 32));
       __syncthreads();
     };
-    u64 estimate = 0;
+    u64 estimate = 0, sure = 0;
     if (by_k || by_p) {
       estimate = run.all_b;
       if (by_k && (u64)ask.k < run.all_a) {
@@ -949,6 +959,7 @@ sample_kernel(const SmArgs a) {
         if (tid == 0) b.n = 0;
         __syncthreads();
         u64 above = 0, inside = 0, all = 0;
+        sure = 0;
         const float in_bin = bin_floor(g), over = bin_floor(g - 1);
         mine.each([&](const u32x4 &v, int c) {
           const float largest = sm_largest<E>(v);
@@ -969,7 +980,9 @@ sample_kernel(const SmArgs a) {
           if (largest >= in_bin) {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-              above += x[e] >= over ? m[e] : 0;
+              const u64 over_it = x[e] >= over ? m[e] : 0;
+              above += over_it;
+              sure += ((int)(m[e] >= floor_w) | (int)(x[e] == mx)) != 0 ? over_it : 0;
               if (x[e] >= in_bin && !(x[e] >= over) && kept(x[e], row.index(c, e))) {
                 inside += m[e];
                 put(sm_key(x[e]), row.index(c, e), m[e]);
@@ -1000,6 +1013,20 @@ sample_kernel(const SmArgs a) {
             for (int i = 0; i < n; ++i) sum += b.rank[i] > mine ? b.mass[i] : 0;
           }
           decide(tid < n && sum < goal && sum + b.mass[tid] >= goal);
+          // What is sure to be kept, by this thread's chunks, and the bin's kept logits, by their
+          // stretch (given to its wave's first thread), are the row's weight.
+          if (tid < kSmWaves) s.part[tid] = 0;
+          __syncthreads();
+          if (tid < n) {
+            const u64 mine_r = b.rank[tid], m = b.mass[tid];
+            const float x = sm_from_key((uint32_t)(mine_r >> 32));
+            const int index = (int)~(uint32_t)mine_r;
+            if (kept(x, index) && (m >= floor_w || x == mx))
+              atomicAdd(&s.part[((index + row.off) / N) / ((row.chunks + kSmWaves - 1) / kSmWaves)], m);
+          }
+          __syncthreads();
+          if (lane == 0) sure += s.part[wave];
+          __syncthreads();
           break;
         }
       }
@@ -1013,12 +1040,10 @@ sample_kernel(const SmArgs a) {
           s, mine, least, 0, 0,
           [&](uint32_t bits, int i, bool &) -> u64 {
             const float x = __builtin_bit_cast(float, bits);
-            const double w = weight.real(x);
-            bool in = kept(x, i);
-            if (floor_w > 0.0) in &= (w >= floor_w) | (x == mx);
-            return in ? sm_mass(w) : 0;
+            const u64 m = sm_mass(weight.real(x));
+            return ((int)kept(x, i) & ((int)(m >= floor_w) | (int)(x == mx))) != 0 ? m : 0;
           },
-          target);
+          target, by_p ? &sure : nullptr);
     }
     if (tid == 0) a.token[r] = at;
   }
