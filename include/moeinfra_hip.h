@@ -387,7 +387,8 @@ int moe_packed_attention_bf16(const void *q, int64_t q_stride, const void *k, in
  * largest logit.  Logits of -inf and NaN are never drawn; a row of nothing else gives -1; next to +inf
  * only other +inf weigh anything.  Each setting is an array with a value per row (fp32, top_k
  * int32) or, where that is null, one value for all rows (refused outside its range).  Weights are
- * summed as integers of 2^-43, so results do not depend on the order of any sum. */
+ * summed as integers (of 2^-51 of the largest, fewer bits where V needs them: 2^-49 at 32000), so
+ * results do not depend on the order of any sum. */
 int moe_sample_tokens(const void *logits, int32_t logits_f32, int64_t stride, int64_t B, int64_t V,
                       const void *u_f32, const void *temperature_f32, float temperature,
                       const void *top_k_i32, int32_t top_k, const void *top_p_f32, float top_p,

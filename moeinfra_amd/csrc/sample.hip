@@ -13,9 +13,10 @@
 //   sm_general      the same for rows with values that those counts do not hold (see there)
 //
 // A token is right or wrong, and a sum's rounding decides where u falls next to a border.  So weights
-// are evaluated in 64 bits and held as integers of 2^-43: sums of them (up to 2^20) are exact, the
-// same in any order, and nothing here depends on the order in which atomics arrive.  2^-44 of the
-// largest weight, what an integer is off by, is all that the result can differ from exact sums.
+// are evaluated in 64 bits and held as integers: of 2^-51 of the largest, or as many fewer bits as a
+// sum over the vocabulary needs to stay below 2^64 (32000: 2^-49).  Their sums are exact, the same in
+// any order, and nothing here depends on the order in which atomics arrive.  What the result can
+// differ from exact sums by is half an integer a weight, and 2^-31 of it.
 #include <type_traits>
 
 #include "common.h"
@@ -27,8 +28,7 @@ constexpr int kSmThreads = 1024;
 constexpr int kSmWaves = kSmThreads / kWave;
 constexpr int kSmBins = kSmThreads;
 constexpr int64_t kSmMaxVocab = 1 << 20;
-constexpr int kSmBits = 43;            // a weight of 1 is 2^43
-constexpr double kSmSpan = 44.0;       // in powers of two: what is further below the maximum weighs 0
+constexpr double kSmSpan = 53.0;       // in powers of two: what is further below the maximum weighs 0
 constexpr double kSmLog2e = 1.44269504088896340736;
 
 typedef unsigned long long u64;
@@ -77,7 +77,7 @@ __device__ __forceinline__ double sm_exp2(double f) {
 
 constexpr int kSmTable = 256;
 
-// Weights 2^(43 - y), y = (m - x) log2(e) / T below 64 (what is further away weighs nothing, -inf too).
+// Weights 2^(bits - y), y = (m - x) log2(e) / T below 64 (what is further away weighs nothing, -inf too).
 // One multiply-add leaves y as a fixed-point number in the low bits: whole powers and 256ths in the
 // upper word, the rest r of a 256th in the lower.  The power of the 256ths comes from a table, that of
 // r as 1 + t + t^2 / 2 + t^3 / 6, t = -r ln(2) / 256, in fp32: off by 2^-31 of the weight.  (In 64 bits
@@ -86,10 +86,11 @@ constexpr int kSmTable = 256;
 struct SmWeight {
   const double *table;  // 2^(-j / 256), in LDS
   double m, c, most;    // c: log2(e) / T; the difference with y = 63
+  uint32_t bits;
 
   // (An infinite temperature still keeps -inf from weighing anything.)
-  __device__ __forceinline__ SmWeight(const double *table_, double m_, double c_)
-      : table(table_), m(m_), c(fmax(c_, 1e-290)), most(63.0 / c) {}
+  __device__ __forceinline__ SmWeight(const double *table_, double m_, double c_, int V)
+      : table(table_), m(m_), c(fmax(c_, 1e-290)), most(63.0 / c), bits(min(51, 32 + __clz(V))) {}
   __device__ __forceinline__ double real(float x) const {
     const double d = fmin(m - (double)x, most);
     const u64 z = __builtin_bit_cast(u64, fma(d, c, 0x1.8p12));
@@ -98,7 +99,7 @@ struct SmWeight {
     const float q = t * fmaf(t, fmaf(t, 1.0f / 6, 0.5f), 1.0f);
     const double p = table[n & (kSmTable - 1)];
     const u64 w = __builtin_bit_cast(u64, fma(p, (double)q, p));
-    return __builtin_bit_cast(double, w + ((u64)(kSmBits - (n >> 8 & 63)) << 52));
+    return __builtin_bit_cast(double, w + ((u64)(bits - (n >> 8 & 63)) << 52));
   }
 };
 // To the nearest integer (of values below 2^52).
@@ -457,7 +458,7 @@ struct SmAsk {
 
 __device__ __forceinline__ u64 sm_target(float u, u64 total) {
   const double y = (double)u * (double)total;
-  const u64 t = y > 0.0 ? (y < 0x1p63 ? (u64)y : total) : 0;
+  const u64 t = y > 0.0 ? (y < 0x1p63 * 2 ? (u64)y : total) : 0;
   return t < total ? t : total - 1;
 }
 
@@ -472,7 +473,7 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
   const double m = infinite ? 0.0 : (double)mx;
   auto value = [&](float x) { return infinite ? (x == INFINITY ? 0.0f : -INFINITY) : x; };
   const double c2 = kSmLog2e / (double)a.T;
-  const SmWeight weight(table, m, c2);
+  const SmWeight weight(table, m, c2, row.V);
   const float fm = (float)m;
   const double bs = c2 * (kSmBins / kSmSpan);
   const float bin_scale = bs < 1e30 ? (float)bs : 1e30f;
@@ -610,7 +611,7 @@ __device__ __noinline__ int sm_general(SmGeneral &g, SmShare &s, const SmRow<E> 
           [&](u64) { return n - 1; });
     }
   }
-  const double floor_w = (double)a.min_p * 0x1p43;
+  const double floor_w = ldexp((double)a.min_p, weight.bits);
   return sm_locate(
       s, mine, -INFINITY, 0, 0,
       [&](uint32_t bits, int i, bool &) -> u64 {
@@ -633,6 +634,7 @@ constexpr int kSmEntries = 2 * kSmSide + 3;
 constexpr int kSmPer = (kSmEntries + kSmThreads - 1) / kSmThreads;  // 11: odd, so that threads meet no bank twice
 constexpr int kSmNone = kSmThreads * kSmPer;
 constexpr int kSmList = kSmThreads;  // logits of one bin that are ranked directly
+constexpr int kSmNear = 6;           // neighbours of a guessed bin that are tried
 
 __device__ __forceinline__ uint32_t sm_upper(uint32_t bits) { return bits >> 16 & 0x7fffu; }
 
@@ -677,8 +679,9 @@ struct SmBins {
 // A workgroup per row.
 //   1  the largest logit, and the counts of the bins
 //   2  the bin where top-k and top-p end, from sums over the bins: in bf16 they are exact, a bin's
-//      count times its value's weight; in fp32 a guess, which a pass over the logits checks and
-//      corrects while it adds the weights up, and the logits of the bin found are ranked
+//      count times its value's weight; in fp32 a guess, which a pass over the logits checks while it
+//      adds the weights up (one row in ten needs a neighbour instead), and the logits of the bin
+//      found are ranked
 //   3  the token, from sums over stretches of the row
 //
 // Bound: passes over the row (each of the LDS atomics of 1, of some 10 instructions per logit of 3,
@@ -793,10 +796,10 @@ sample_kernel(const SmArgs a) {
     if (tid == 0) a.token[r] = at;
     return;
   }
-  const SmWeight weight(table, (double)mx, c2);
+  const SmWeight weight(table, (double)mx, c2, a.V);
   // What min_p asks of a weight (the largest is kept whatever it asks).
-  const double floor_d = ceil((double)ask.min_p * 0x1p43);
-  const u64 floor_w = floor_d > 0.0 ? (floor_d < 0x1p44 ? (u64)floor_d : 1ull << 44) : ask.min_p <= 0.0f ? 0 : 1ull << 44;
+  const double floor_d = ceil(ldexp((double)ask.min_p, weight.bits));
+  const u64 floor_w = floor_d <= 0.0 ? 0 : floor_d < 0x1p52 ? (u64)floor_d : 1ull << 52;  // (NaN: all the largest)
   auto target = [&](u64 total) { return sm_target(ask.u, total); };
 
   // The bins' weights (fp32: as if all of a bin lay in its middle; those of the largest logit's bin as
@@ -948,21 +951,51 @@ sample_kernel(const SmArgs a) {
       }
     }
     if (by_p && !failed) {
-      int lo = 0, hi = last;
-      u64 want = goal_of(estimate > 0 ? estimate : 1), goal = 0;
-      bool known = false;
+      int lo = 1, hi = last, g = 0;
+      u64 goal = 0, above = 0, inside = 0, bin_sure = 0;  // weights before bin g, in it, and (this thread's) sure in it
       for (int tries = 0;; ++tries) {
-        int g = tries < 6 ? edge_of(false, want, n0, m0) : lo + (hi - lo) / 2;
+        // The bin is guessed, then its neighbours are tried, which takes only their own weights; after
+        // kSmNear of them, by bisection.
+        int step = 0;
+        if (tries == 0) {
+          g = edge_of(false, goal_of(estimate), n0, m0);
+        } else if (tries <= kSmNear) {
+          step = lo > g ? 1 : -1;
+          if (step > 0) {
+            above += inside;
+            sure += bin_sure;
+          }
+          g += step;
+          while ((step > 0 ? g < hi : g > lo) && b.count[g] == 0) g += step;
+        } else {
+          g = lo + (hi - lo) / 2;
+        }
         g = min(max(g, lo), hi);
         failed = b.count[g] > kSmList;
         if (failed) break;  // uniform
         if (tid == 0) b.n = 0;
         __syncthreads();
-        u64 above = 0, inside = 0, all = 0;
-        sure = 0;
         const float in_bin = bin_floor(g), over = bin_floor(g - 1);
+        u64 before = 0, here = 0, all = 0;
+        if (step == 0) sure = 0;
+        bin_sure = 0;
+        auto take = [&](float x, int i, u64 m) {  // of the bin
+          here += m;
+          bin_sure += m >= floor_w || x == mx ? m : 0;
+          put(sm_key(x), i, m);
+        };
         mine.each([&](const u32x4 &v, int c) {
           const float largest = sm_largest<E>(v);
+          if (step != 0) {
+            if (!(largest >= in_bin)) return;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              const float x = __builtin_bit_cast(float, SmRow<E>::bits(v, e));
+              const int i = row.index(c, e);
+              if (x >= in_bin && !(x >= over) && kept(x, i)) take(x, i, sm_mass(weight.real(x)));
+            }
+            return;
+          }
           if (!(largest >= least)) return;
           float x[N];
           u64 m[N];
@@ -981,29 +1014,24 @@ sample_kernel(const SmArgs a) {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
               const u64 over_it = x[e] >= over ? m[e] : 0;
-              above += over_it;
+              before += over_it;
               sure += ((int)(m[e] >= floor_w) | (int)(x[e] == mx)) != 0 ? over_it : 0;
-              if (x[e] >= in_bin && !(x[e] >= over) && kept(x[e], row.index(c, e))) {
-                inside += m[e];
-                put(sm_key(x[e]), row.index(c, e), m[e]);
-              }
+              if (x[e] >= in_bin && !(x[e] >= over) && kept(x[e], row.index(c, e))) take(x[e], row.index(c, e), m[e]);
             }
           }
         });
-        const SmScan both = sm_scan(s, above, inside);
-        above = both.all_a;
+        const SmScan both = sm_scan(s, before, here);
         inside = both.all_b;
-        if (!known) {
-          goal = goal_of(sm_block_sum(s, all));
-          known = true;
+        if (step == 0) above = both.all_a;
+        if (step < 0) {
+          above -= inside;
+          sure -= bin_sure;
         }
+        if (tries == 0) goal = goal_of(sm_block_sum(s, all));
         if (above >= goal) {
           hi = g - 1;
-          want = m0 > above - goal ? m0 - (above - goal) : 1;
         } else if (above + inside < goal) {
           lo = g + 1;
-          want = m0 + (b.count[g] != 0 ? b.count[g] * b.weight[g] : 0) + (goal - above - inside);
-          want = want < estimate ? want : estimate;
         } else {
           const int n = b.n;
           u64 sum = above;

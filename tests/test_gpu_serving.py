@@ -479,6 +479,20 @@ def test_sample_tokens_values_without_a_bin(cuda_device):
             _sampled(cuda_device, x.to(torch.bfloat16), u, **settings)
 
 
+def test_sample_tokens_many_fp32_rows(cuda_device):
+    """Enough rows that the bin where top-p ends is guessed wrong, by one and by more: lopsided bins
+    (values at one end of their 16-bit prefix), and a few heavy ones."""
+    V = 4000
+    x, u = _logits(96, V, 90, torch.float32)
+    low = (x.view(torch.int32) & ~0xffff).view(torch.float32)            # all at their bin's small end
+    x[:32] = low[:32]
+    x[32:64] = (low.view(torch.int32) | 0xfff0).view(torch.float32)[32:64]
+    x[64:70, 17::400] = 9.0 + torch.arange(10) * 2.0 ** -9              # ten that share two bins
+    for settings in (dict(top_p=0.9), dict(top_p=0.35), dict(temperature=0.2, top_p=0.8), dict(top_k=900, top_p=0.97),
+                     dict(top_p=0.6, min_p=0.002), dict(temperature=0.03, top_p=0.5)):
+        _sampled(cuda_device, x, u, **settings)
+
+
 def test_sample_tokens_masked_rows(cuda_device):
     """-inf and NaN are never drawn; rows of nothing else give -1; +inf takes all."""
     V = 3000
