@@ -114,9 +114,10 @@ struct PaPlan {
   bool aligned;  // the second form
 };
 
+// (Short of 2^31 by more than the tiles that are looked ahead.)
 __device__ __forceinline__ int pa_keys(const PaArgs &a, int i) {
   const int64_t all = a.num_pages > 0 ? a.width << a.page_shift : 0;
-  return i < a.B ? min(max(a.lens[i], 0), (int)(all < 0x7fffffc0 ? all : 0x7fffffc0)) : 0;
+  return i < a.B ? min(max(a.lens[i], 0), (int)(all < 0x7ffffc00 ? all : 0x7ffffc00)) : 0;
 }
 __device__ __forceinline__ int pa_tiles(int keys) { return (int)(((uint32_t)keys + kPaTile - 1) / kPaTile); }
 

@@ -225,12 +225,11 @@ __device__ __forceinline__ void sm_chunks(const SmRow<E> &row, int c0, int c1, i
 }
 
 // The part of a row that a thread looks at in each pass: every 64th chunk of its wave's stretch (a
-// sixteenth of the row).  NC > 0: at most NC chunks, read once and kept in registers (16 of them are
-// half of a thread's: a row of 131072 bf16 logits is then read once, 256 KB a CU, instead of in each
-// pass: 256 rows top-p 44 -> 35 us); 0: read again in each pass.
+// sixteenth of the row).  NC > 0: at most NC chunks, read once and kept in registers; 0: read again in
+// each pass.
 //
 // Wave w begins with its w-th: stretches often lie powers of two apart, and in step all waves would ask
-// the same few memory channels (greedy, 256 rows of 131072: 29 us instead of 23).
+// the same few memory channels (two light passes over 256 rows of 131072: 29 us instead of 23).
 template <typename E, int NC>
 struct SmMine {
   const SmRow<E> &row;
@@ -712,7 +711,30 @@ sample_kernel(const SmArgs a) {
     table[tid] = tid <= kSmTable / 2 ? sm_exp2(-tid / (double)kSmTable) : 0.5 * sm_exp2(1.0 - tid / (double)kSmTable);
   float mx = -INFINITY;
   bool far = false, odd = false;
-  if (greedy || (!kExact && !by_k && !by_p)) {  // no counts needed
+  if (greedy) {
+    // The largest key, and of its equals the lowest index, as one integer.
+    float top = -INFINITY;
+    int first = 0x7fffffff;
+    mine.each([&](const u32x4 &v, int c) {
+      const float m = sm_largest<E>(v);
+      if (!(m >= top)) return;
+      int at = 0;
+#pragma unroll
+      for (int e = N - 1; e >= 0; --e)
+        at = __builtin_bit_cast(float, SmRow<E>::bits(v, e)) == m ? row.index(c, e) : at;
+      first = m > top ? at : min(first, at);
+      top = m;
+    });
+    u64 best = (u64)sm_key(top) << 32 | (uint32_t)~first;
+    for (int o = 1; o < kWave; o <<= 1) best = max(best, (u64)__shfl_xor(best, o, kWave));
+    if (lane == 0) s.part[wave] = best;
+    __syncthreads();
+    best = s.part[lane & (kSmWaves - 1)];
+    for (int o = 1; o < kSmWaves; o <<= 1) best = max(best, (u64)__shfl_xor(best, o, kWave));
+    if (tid == 0) a.token[r] = sm_from_key((uint32_t)(best >> 32)) == -INFINITY ? -1 : (int64_t)(int)~(uint32_t)best;
+    return;
+  }
+  if (!kExact && !by_k && !by_p) {  // no counts needed
     mine.each([&](const u32x4 &v, int) { mx = fmaxf(mx, sm_largest<E>(v)); });
   } else {
     for (int i = tid; i < kSmNone; i += kSmThreads) b.count[i] = 0;
@@ -780,13 +802,6 @@ sample_kernel(const SmArgs a) {
   }
   if (mx == -INFINITY) {  // nothing to choose from
     if (tid == 0) a.token[r] = -1;
-    return;
-  }
-  if (greedy) {
-    const int at = sm_locate(
-        s, mine, mx, 0, 0, [&](uint32_t bits, int, bool &) { return (u64)(__builtin_bit_cast(float, bits) == mx); },
-        [](u64) { return (u64)0; });
-    if (tid == 0) a.token[r] = at;
     return;
   }
   const double c2 = kSmLog2e / (double)ask.T;
@@ -1102,17 +1117,17 @@ extern "C" int moe_sample_tokens(const void *logits, int32_t logits_f32, int64_t
   moe::SmArgs a{logits, stride, (int)V, (const float *)u_f32, (const float *)temperature_f32,
                 (const int32_t *)top_k_i32, (const float *)top_p_f32, (const float *)min_p_f32, temperature, top_p,
                 min_p, top_k, (int64_t *)token_i64};
-  // Chunks of 16 bytes per thread: (V + a chunk's end at most) / chunk / threads, in sixteenths of a row
-  // rounded up.  Rows without whole chunks, and those of more, are read again in each pass.
+  // Chunks of 16 bytes per thread: a row's (one more where rows do not start on one), in sixteenths
+  // rounded up, by 64.  Kept in registers up to 4 of bf16 and 8 of fp32 (32768 logits; 64 fp32 rows of
+  // 32000 without top-k and top-p 13 us, 16 read again in each pass); more make the passes too long
+  // for the instruction cache (16: 256 bf16 rows of 131072 46 us, 42 read again).
   const int64_t n = logits_f32 ? 4 : 8;
-  const int64_t per = ((V + 2 * n - 2) / n + moe::kSmWaves - 1) / moe::kSmWaves;  // of a wave's stretch
-  const int64_t chunks = V < 2 * n ? moe::kSmNone : (per + moe::kWave - 1) / moe::kWave;
-  auto kern = logits_f32 ? (chunks <= 8    ? moe::sample_kernel<float, 8>
-                            : chunks <= 16 ? moe::sample_kernel<float, 16>
-                                           : moe::sample_kernel<float, 0>)
-                         : (chunks <= 4    ? moe::sample_kernel<uint16_t, 4>
-                            : chunks <= 16 ? moe::sample_kernel<uint16_t, 16>
-                                           : moe::sample_kernel<uint16_t, 0>);
+  const bool even = (uintptr_t)logits % 16 == 0 && (stride % n == 0 || B == 1);
+  const int64_t per = ((V + (even ? n - 1 : 2 * n - 2)) / n + moe::kSmWaves - 1) / moe::kSmWaves;
+  const int64_t chunks = (per + moe::kWave - 1) / moe::kWave;
+  const bool whole = V >= 2 * n;  // (a row without whole chunks has none to keep)
+  auto kern = logits_f32 ? (whole && chunks <= 8 ? moe::sample_kernel<float, 8> : moe::sample_kernel<float, 0>)
+                         : (whole && chunks <= 4 ? moe::sample_kernel<uint16_t, 4> : moe::sample_kernel<uint16_t, 0>);
   hipLaunchKernelGGL(kern, dim3((unsigned)B), dim3(moe::kSmThreads), 0, (hipStream_t)stream, a);
   MOE_LAUNCH_CHECK();
   return MOE_STATUS_OK;
