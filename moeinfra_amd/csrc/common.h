@@ -12,6 +12,8 @@ namespace moe {
 void set_error(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
 // Number of compute units of the current device (cached per device).
 int device_cu_count();
+// Whether a launch may have so many workgroups (the runtime takes fewer than 2^32 threads).
+inline bool launch_fits(int64_t groups, int threads) { return groups < ((int64_t)1 << 32) / threads; }
 
 constexpr int kWave = 64;
 

@@ -450,14 +450,15 @@ extern "C" int moe_packed_attention_bf16(const void *q, int64_t q_stride, const 
   const bool paired = head_dim != 256 && tiles(128) <= 2 * cus && T >= 256 * B;
   const bool wide = head_dim == 128 && n_kv_heads > 8 && tiles(256) >= 2 * cus && !paired;
   const int64_t g = tiles(wide ? 256 : 128);
-  MOE_REQUIRE(g <= 0x7fffffff, "bad sizes");
+  const int threads = (paired || wide ? 8 : 4) * moe::kWave;
+  MOE_REQUIRE(moe::launch_fits(g, threads), "bad sizes");
   auto kern = head_dim == 64    ? (paired ? moe::packed_attention_kernel<64, 4, 2>
                                           : moe::packed_attention_kernel<64, 4, 1>)
               : head_dim == 128 ? (paired ? moe::packed_attention_kernel<128, 4, 2>
                                    : wide ? moe::packed_attention_kernel<128, 8, 1>
                                           : moe::packed_attention_kernel<128, 4, 1>)
                                 : moe::packed_attention_kernel<256, 4, 1>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)g), dim3((paired || wide ? 8 : 4) * moe::kWave), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)g), dim3(threads), 0, (hipStream_t)stream, a);
   MOE_LAUNCH_CHECK();
   return MOE_STATUS_OK;
 }

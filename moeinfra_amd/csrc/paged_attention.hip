@@ -522,7 +522,7 @@ extern "C" int moe_paged_attention_bf16(const void *q, int64_t q_stride, const v
   a.part = workspace ? (float *)((char *)workspace + moe::kPaCounterBytes) : nullptr;
   a.share = split ? (int)moe::pa_share(units, head_dim) : 0;
   const int64_t items = a.share > B ? a.share : B;
-  MOE_REQUIRE(items * units <= 0x7fffffff, "bad sizes");
+  MOE_REQUIRE(moe::launch_fits(items * units, moe::kPaThreads), "bad sizes");
   auto kern = head_dim == 64    ? moe::paged_attention_kernel<64>
               : head_dim == 128 ? moe::paged_attention_kernel<128>
                                 : moe::paged_attention_kernel<256>;

@@ -104,8 +104,8 @@ extern "C" int moe_rope_paged_kv_bf16(const void *qkv, int64_t qkv_stride, int64
                                       int64_t num_pages, int32_t page_size, int64_t page_stride,
                                       void *q_out, void *k_out, void *k_cache, void *v_cache,
                                       void *stream) {
-  MOE_REQUIRE(T >= 0 && T <= 0x7fffffff && n_q_heads > 0 && n_kv_heads > 0 && n_seqs >= 0 && table_width >= 0 &&
-                  num_pages >= 0 && num_pages <= 0x7fffffff,
+  MOE_REQUIRE(T >= 0 && moe::launch_fits(T, moe::kPkvThreads) && n_q_heads > 0 && n_kv_heads > 0 &&
+                  n_seqs >= 0 && table_width >= 0 && num_pages >= 0 && num_pages <= 0x7fffffff,
               "bad sizes");
   MOE_REQUIRE(head_dim > 0 && head_dim % 16 == 0 && head_dim / 2 <= moe::kPkvMaxHalf,
               "head dim must be a multiple of 16 up to %d (got %d)", 2 * moe::kPkvMaxHalf, head_dim);

@@ -1100,7 +1100,7 @@ extern "C" int moe_sample_tokens(const void *logits, int32_t logits_f32, int64_t
                                  const void *top_k_i32, int32_t top_k, const void *top_p_f32, float top_p,
                                  const void *min_p_f32, float min_p, void *token_i64, void *stream) {
   MOE_REQUIRE(logits_f32 == 0 || logits_f32 == 1, "logits are bf16 (0) or fp32 (1)");
-  MOE_REQUIRE(B >= 0 && B <= 0x7fffffff, "bad sizes");
+  MOE_REQUIRE(B >= 0 && moe::launch_fits(B, moe::kSmThreads), "bad sizes");
   MOE_REQUIRE(V >= 1 && V <= moe::kSmMaxVocab, "a row has 1 to %lld logits (got %lld)", (long long)moe::kSmMaxVocab,
               (long long)V);
   MOE_REQUIRE(stride >= V || B <= 1, "rows of logits must be apart");

@@ -51,6 +51,7 @@ REFUSED = [
     (_append, dict(stride=772), "qkv rows"),
     (_append, dict(T=-1), "bad sizes"),
     (_append, dict(T=1 << 31), "bad sizes"),
+    (_append, dict(T=1 << 24), "bad sizes"),
     (_append, dict(nq=0), "bad sizes"),
     (_append, dict(pages=-1), "bad sizes"),
     (_append, dict(pages=1 << 31), "bad sizes"),
@@ -73,6 +74,7 @@ REFUSED = [
     (_paged, dict(page_stride=1024), "page stride"),
     (_paged, dict(B=-1), "bad sizes"),
     (_paged, dict(pages=1 << 31), "bad sizes"),
+    (_paged, dict(B=1 << 20, nq=64, nkv=64, stride=4096, page_stride=64 * 16 * 64), "bad sizes"),
     (_paged, dict(width=1 << 28), "too long"),
     (_paged, dict(width=1 << 20, B=1 << 20), "too long"),
     (_paged, dict(stride=504), "q rows"),
@@ -89,6 +91,8 @@ REFUSED = [
     (_packed, dict(T=-1), "bad sizes"),
     (_packed, dict(T=1 << 30), "bad sizes"),
     (_packed, dict(B=-1), "bad sizes"),
+    (_packed, dict(T=1 << 23, B=1 << 20, nq=1 << 12, nkv=1 << 12, q_stride=1 << 18, k_stride=1 << 18, v_stride=1 << 18,
+                   q=1 << 56, k=2 << 56, v=3 << 56, out=4 << 56), "bad sizes"),
     (_packed, dict(q_stride=504), "apart"),
     (_packed, dict(k_stride=132), "aligned"),
     (_packed, dict(v_stride=64), "apart"),
@@ -99,6 +103,7 @@ REFUSED = [
     (_packed, dict(out=C - 1024), "overlap"),
     (_sample, dict(f32=2), "bf16"),
     (_sample, dict(B=-1), "bad sizes"),
+    (_sample, dict(B=1 << 22), "bad sizes"),
     (_sample, dict(V=0), "logits"),
     (_sample, dict(V=(1 << 20) + 1, stride=1 << 21), "logits"),
     (_sample, dict(stride=999), "apart"),
