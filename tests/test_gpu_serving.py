@@ -148,6 +148,32 @@ def test_paged_attention_batches(cuda_device, lens):
     _paged(cuda_device, lens, 8, 2, 128, 16, seed=len(lens))
 
 
+@pytest.mark.parametrize("nq,nkv,hd,lens", [
+    (8, 2, 64, [1 + 37 * i % 90 for i in range(1100)] + [6000, 0, 2500]),   # more sequences than workgroups at once
+    (8, 8, 64, [(i * 7) % 50 for i in range(2100)] + [700]),                # ... than arrival counters: a sequence each
+    (32, 8, 128, [0] * 130), (4, 1, 128, [0] * 90 + [9000] + [0] * 200 + [1])])
+def test_paged_attention_large_batches(cuda_device, nq, nkv, hd, lens):
+    print(f"paged attention of {len(lens)} sequences, {nq}/{nkv} heads of {hd}", flush=True)
+    _paged(cuda_device, lens, nq, nkv, hd, 16, seed=7)
+
+
+def test_paged_attention_shared_pages(cuda_device):
+    """Sequences that begin with the same pages (a common prompt), one of them listed twice."""
+    from moeinfra_amd import ops
+
+    dev, nq, nkv, hd, page = cuda_device, 8, 2, 128, 32
+    pool = Pool([100, 100], nkv, hd, page, dev, seed=15, fill=math.nan)
+    k, v = [_bf((100, nkv, hd), s) for s in (150, 151)], [_bf((100, nkv, hd), s) for s in (152, 153)]
+    for i in range(2):
+        pool.put(i, k[i], v[i])
+    table = pool.dev_table[[0, 1, 0, 0]].contiguous()
+    table[1, :2] = table[0, :2]     # keys 0 .. 63 are the first one's
+    k1, v1 = torch.cat((k[0][:64], k[1][64:])), torch.cat((v[0][:64], v[1][64:]))
+    q = _bf((4, nq, hd), 154, 1.5)
+    out = ops.paged_attention(q.to(dev), pool.k, pool.v, table, torch.tensor([100, 100, 70, 100], dtype=torch.int32, device=dev))
+    _check_paged(out, q, [k[0], k1, k[0][:70], k[0]], [v[0], v1, v[0][:70], v[0]], nkv, hd ** -0.5)
+
+
 def test_paged_attention_without_workspace_and_reuse(cuda_device):
     from moeinfra_amd import ops
 
@@ -413,6 +439,25 @@ def test_sample_tokens_odd_sizes_and_strides(cuda_device, vocab):
             got = ops.sample_tokens(wide.to(cuda_device)[:, lead:lead + vocab], u.to(cuda_device), temperature=1.3,
                                     top_p=0.8)
             assert got.cpu().tolist() == [sample(r, float(v), temperature=1.3, top_p=0.8) for r, v in zip(x, u)]
+
+
+@pytest.mark.parametrize("vocab,dtype,lead", [
+    (32768, torch.float32, 0), (32768, torch.float32, 1), (32769, torch.float32, 0), (40000, torch.float32, 3),
+    (262147, torch.float32, 0), (32768, torch.bfloat16, 0), (32768, torch.bfloat16, 5), (300001, torch.bfloat16, 1),
+    (1 << 20, torch.bfloat16, 0)])
+def test_sample_tokens_long_rows(cuda_device, vocab, dtype, lead):
+    """Rows that just fit a workgroup's registers, that just do not, and of the largest vocabulary."""
+    from moeinfra_amd import ops
+
+    x, u = _logits(3, vocab, vocab + lead, dtype)
+    wide = torch.full((3, vocab + 2 * lead), math.nan, dtype=dtype)
+    wide[:, lead:lead + vocab] = x
+    d = wide.to(cuda_device)[:, lead:lead + vocab]
+    for settings in (dict(), dict(temperature=0.0), dict(top_k=50, top_p=0.9), dict(top_p=0.7, min_p=0.001),
+                     dict(temperature=1.4, top_k=20000)):
+        print(f"sample {vocab} {dtype} {settings}", flush=True)
+        got = ops.sample_tokens(d, u.to(cuda_device), **settings).cpu().tolist()
+        assert got == [sample(r, float(v), **settings) for r, v in zip(x, u)], settings
 
 
 def test_sample_tokens_settings_per_row(cuda_device):
