@@ -341,21 +341,28 @@ def _rows(t: torch.Tensor, name: str, dev: torch.device, ndim: int) -> int:
     return strides[0] if shape[0] > 1 else (row + 7) // 8 * 8
 
 
-def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: torch.device) -> int:
-    """The page stride of a paged cache (k and v [pages, kv heads, page size, head dim], whole pages
-    at one stride)."""
+def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: torch.device):
+    """(page stride, shape) of a paged cache (k and v [pages, kv heads, page size, head dim], whole
+    pages at one stride)."""
+    if isinstance(k_cache, torch.Tensor) and isinstance(v_cache, torch.Tensor):
+        shape, strides = k_cache.shape, k_cache.stride()
+        if (len(shape) == 4 and shape[0] > 1 and strides[1:] == (shape[2] * shape[3], shape[3], 1)
+                and k_cache.dtype is _BF16 and k_cache.device == dev and v_cache.stride() == strides
+                and v_cache.shape == shape and v_cache.dtype is _BF16 and v_cache.device == dev):
+            return strides[0], shape
     stride = _rows(k_cache, "k_cache", dev, 4)
     if _rows(v_cache, "v_cache", dev, 4) != stride or k_cache.shape != v_cache.shape:
         raise ValueError(f"k_cache {tuple(k_cache.shape)} of page stride {stride} and v_cache {tuple(v_cache.shape)} of "
                          f"page stride {v_cache.stride(0)} differ")
-    return stride
+    return stride, k_cache.shape
 
 
-def _out(out: Optional[torch.Tensor], name: str, dtype: torch.dtype, dev: torch.device, shape) -> torch.Tensor:
-    """A caller's output, checked for its number of elements, or a new one."""
+def _out(out: Optional[torch.Tensor], name: str, like: torch.Tensor, *shape) -> torch.Tensor:
+    """A caller's output, checked for its number of elements, or a new one (new_empty with sizes of
+    its own takes 1.2 us, torch.empty 1.6)."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    _plain(out, name, dtype, dev)
+        return like.new_empty(*shape)
+    _plain(out, name, like.dtype, like.device)
     n = 1
     for s in shape:
         n *= s
@@ -381,8 +388,7 @@ def rope_paged_kv(qkv: torch.Tensor, positions: torch.Tensor, page_table: torch.
     _require_cuda(qkv, "qkv")
     dev = qkv.device
     stride = _rows(qkv, "qkv", dev, 2)
-    page_stride = _pages(k_cache, v_cache, dev)
-    pages, nkv, size, hd = k_cache.shape
+    page_stride, (pages, nkv, size, hd) = _pages(k_cache, v_cache, dev)
     T, row = qkv.shape
     nq = int(n_q_heads)
     if row != (nq + 2 * nkv) * hd:
@@ -394,8 +400,8 @@ def rope_paged_kv(qkv: torch.Tensor, positions: torch.Tensor, page_table: torch.
     pos = _plain(positions, "positions", _I32, dev, (T,))
     freq = _plain(inv_freq, "inv_freq", _F32, dev, (hd // 2,))
     seqs = None if seq_ids is None else _plain(seq_ids, "seq_ids", _I32, dev, (T,))
-    q_out = _out(q_out, "q_out", _BF16, dev, (T, nq * hd))
-    k_out = torch.empty((T, nkv, hd), dtype=_BF16, device=dev) if want_k else None
+    q_out = _out(q_out, "q_out", qkv, T, nq * hd)
+    k_out = qkv.new_empty(T, nkv, hd) if want_k else None
     _launch(lib().moe_rope_paged_kv_bf16, "rope_paged_kv", dev, qkv.data_ptr(), stride, T, nq, nkv, hd, freq, pos, seqs,
             table, n_seqs, width, pages, size, page_stride, q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(),
             v_cache.data_ptr())
@@ -421,8 +427,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _require_cuda(q, "q")
     dev = q.device
     stride = _rows(q, "q", dev, 3)
-    page_stride = _pages(k_cache, v_cache, dev)
-    pages, nkv, size, hd = k_cache.shape
+    page_stride, (pages, nkv, size, hd) = _pages(k_cache, v_cache, dev)
     B, nq, q_dim = q.shape
     if q_dim != hd:
         raise ValueError(f"q has head dim {q_dim}, the cache {hd}")
@@ -430,7 +435,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if page_table.ndim != 2 or page_table.shape[0] != B:
         raise ValueError(f"page_table must have {B} rows of pages (got {tuple(page_table.shape)})")
     n = _plain(lens, "lens", _I32, dev, (B,))
-    out = _out(out, "out", _BF16, dev, (B, nq, hd))
+    out = _out(out, "out", q, B, nq, hd)
     if workspace is None:
         workspace = paged_attention_workspace(B, nq, nkv, hd, dev)
     _launch(lib().moe_paged_attention_bf16, "paged_attention", dev, q.data_ptr(), stride, k_cache.data_ptr(),
@@ -456,7 +461,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu = _plain(cu_seqlens, "cu_seqlens", _I32, dev)
     if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1:
         raise ValueError(f"cu_seqlens must be [sequences + 1] (got {tuple(cu_seqlens.shape)})")
-    out = _out(out, "out", _BF16, dev, (T, nq, hd))
+    out = _out(out, "out", q, T, nq, hd)
     _launch(lib().moe_packed_attention_bf16, "packed_attention", dev, q.data_ptr(), q_stride, k.data_ptr(), k_stride,
             v.data_ptr(), v_stride, T, cu, cu_seqlens.numel() - 1, nq, k.shape[1], hd,
             hd ** -0.5 if scaling is None else scaling, out.data_ptr())
@@ -484,7 +489,12 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     B, V = logits.shape
     shape = (B,)
     numbers = _plain(u, "u", _F32, dev, shape)
-    out = _out(out, "out", torch.int64, dev, shape)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int64, device=dev)
+    else:
+        _plain(out, "out", torch.int64, dev)
+        if out.numel() != B:
+            raise ValueError("out has the wrong number of elements")
     tensor = torch.Tensor
     t = k = p = m = None
     if isinstance(temperature, tensor):
