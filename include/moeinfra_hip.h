@@ -354,7 +354,9 @@ int moe_rope_paged_kv_bf16(const void *qkv, int64_t qkv_stride, int64_t T, int32
  * dim 64, 128 or 256.  With a workspace (moe_paged_attention_workspace_bytes, enough for any
  * smaller batch too; 16-byte aligned, its first 65536 bytes zero before the first call, every call
  * leaves them zero; calls that share it must be ordered) several workgroups share a sequence's
- * keys, their results added up in a fixed order; null: one workgroup each. */
+ * keys, their results added up in a fixed order; null: one workgroup each.  q and the caches are
+ * 16-byte aligned, out 4-byte.  (Here and below the sums of weights times v are divided at the end:
+ * they leave the range of fp32 where |v| times the number of keys, or 256 times that, does.) */
 int64_t moe_paged_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
                                             int32_t head_dim);
 int moe_paged_attention_bf16(const void *q, int64_t q_stride, const void *k_cache,
@@ -370,7 +372,7 @@ int moe_paged_attention_bf16(const void *q, int64_t q_stride, const void *k_cach
  * [T, n_q, head_dim], k and v [T, n_kv, head_dim], their rows q_stride / k_stride / v_stride values
  * apart (slices of a projection's output); out [T, n_q * head_dim].  fp32 scores q.k * scaling and
  * softmax, the weights rounded to bf16 before their sum (fp32) with v.  Rows of no sequence are left
- * as they were.  head dim 64, 128 or 256. */
+ * as they were.  head dim 64, 128 or 256; q, k, v and out 16-byte aligned. */
 int moe_packed_attention_bf16(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                               const void *v, int64_t v_stride, int64_t T,
                               const void *cu_seqlens_i32, int64_t B, int32_t n_q_heads,

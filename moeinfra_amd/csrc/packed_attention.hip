@@ -165,9 +165,10 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
 //
 // Bound: a tile of 64 keys costs a wave 1024 cycles of products and about as many of vector
 // instructions (512 of them the exponentials), and LDS as many of operand reads for the 8 waves of a
-// CU; they overlap between its waves.  16384 tokens in 3 sequences, 32 / 8 heads of 128: 1640-1840 us,
-// 900-1010 TFLOP/s; many short sequences are bound by their queries and outputs (64 of 256: 335 MB in
-// 120 us).
+// CU; they overlap between its waves.  16384 tokens in 3 sequences, 32 / 8 heads of 128: 1590-1750 us,
+// 950-1040 TFLOP/s (a product of 8192^3 runs at 1190); 3333 tokens in 9 sequences 36 us, 570 TFLOP/s, their
+// few tiles a row tile; many short sequences are bound by their queries and outputs (64 of 256: 335 MB
+// in 120 us).
 //
 // A weight is 2^(s c - m) by one fused multiply-add, c = scaling * log2(e), m a rounded max s c: what
 // the rounding of m leaves cancels against the sum, as long as 2 to its power is in range.  Rows with
