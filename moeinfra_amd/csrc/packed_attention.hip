@@ -174,6 +174,11 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
 // the rounding of m leaves cancels against the sum, as long as 2 to its power is in range.  Rows with
 // references past kPkHuge (and products that overflow) are done again without.
 //
+// Long row tiles of many heads (RW = 8) and large ones (HD = 256, a wave on a SIMD) multiply the next step's
+// scores between this one's weights (8192 tokens of 16 / 16 heads of 128 292 -> 268 us, of 8 / 4 of 256
+// 388 -> 356); elsewhere a SIMD's two waves overlap as well without, and the shorter start counts (1500
+// tokens of 32 / 8 heads 36 us, 38.5 with).
+//
 // KG key groups of RW waves: with two, the second takes every other tile of the same rows, which halves
 // the chain of a row tile's keys; the groups' sums meet in LDS.
 template <int HD, int RW, int KG>
@@ -187,6 +192,7 @@ packed_attention_kernel(const PkArgs a) {
   constexpr int kStage = KG * 2 * kPlane;            // bytes of the tiles of a step
   constexpr int kDT = HD / 32;                       // 32-dim output tiles
   constexpr int kRowB = HD * 2;
+  constexpr bool kAhead = RW == 8 || HD == 256;
   static_assert(kChunks >= 1, "a wave loads a KB at least");
   __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][kStage];
   const int lane = threadIdx.x & (kWave - 1);
@@ -207,7 +213,9 @@ packed_attention_kernel(const PkArgs a) {
   // Rows past the sequence's last key repeat it (masked below).
   const uint16_t *const kb = a.k + it.tok0 * a.k_stride + (int64_t)kvh * HD;
   const uint16_t *const vb = a.v + it.tok0 * a.v_stride + (int64_t)kvh * HD;
-  auto load = [&](int at_step, uint8_t *stage) __attribute__((always_inline)) {
+  // (v_c: V, or K.)
+  auto load = [&](int at_step, auto v_c) __attribute__((always_inline)) {
+    constexpr bool kV = decltype(v_c)::value;
 #pragma unroll
     for (int n = 0; n < KG; ++n)
 #pragma unroll
@@ -215,12 +223,19 @@ packed_attention_kernel(const PkArgs a) {
         const int chunk = (loader + i * NW) * 1024, at = chunk + 16 * lane;
         const uint32_t row = at / kRowB, piece = at % kRowB / 16;
         const int64_t key = min((at_step * KG + n) * kKeys + (int)row, nkeys - 1);
-        uint8_t *const plane = stage + n * 2 * kPlane + chunk;
-        pk_load_lds(kb + key * a.k_stride + 8 * (piece ^ pk_kx<HD>(row)), plane);
-        pk_load_lds(vb + key * a.v_stride + 8 * (piece ^ pk_vx<HD>(row)), plane + kPlane);
+        uint8_t *const plane = s_kv[at_step & 1] + n * 2 * kPlane + chunk;
+        if constexpr (kV)
+          pk_load_lds(vb + key * a.v_stride + 8 * (piece ^ pk_vx<HD>(row)), plane + kPlane);
+        else
+          pk_load_lds(kb + key * a.k_stride + 8 * (piece ^ pk_kx<HD>(row)), plane);
       }
   };
-  load(0, s_kv[0]);
+  const std::false_type K_c{};
+  const std::true_type V_c{};
+  const int steps = (ntile + KG - 1) / KG;
+  load(0, K_c);
+  load(0, V_c);
+  if (kAhead && steps > 1) load(1, K_c);
 
   const int row0 = it.tile * kRows + wave * kPkRows;
   const int r = min(row0 + li, rows - 1);
@@ -258,32 +273,42 @@ packed_attention_kernel(const PkArgs a) {
   const uint32_t vkey = 4 * hh + ((lane & 15) >> 2);
   const uint32_t vrd = kPlane + vkey * kRowB + 8 * (lane & 1);
   const uint32_t vx = 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ pk_vx<HD>(vkey));
-  const int steps = (ntile + KG - 1) / KG;
-  // One step; EDGE: some row of the workgroup stops inside it.
-  auto step = [&](int n, auto edge_c) __attribute__((always_inline)) {
+  f32x16 sa[kST], sb[kST];
+  // Slice i of the products S^T of step n, 16 dims of all keys.
+  auto scores = [&](int n, int i, uint32_t ka, f32x16 (&sc)[kST]) __attribute__((always_inline)) {
+    const uint8_t *buf = s_kv[n & 1] + kgrp * 2 * kPlane;
+    if (i == 0) {
+#pragma unroll
+      for (int st = 0; st < kST; ++st)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sc[st][v] = 0.0f;
+    }
+#pragma unroll
+    for (int st = 0; st < kST; ++st) {
+      const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + krd + (ka ^ (32 * i)) + 32 * st * kRowB);
+      sc[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, qf[i]),
+                                                       sc[st], 0, 0, 0);
+    }
+  };
+  // One step: weights and sums of the scores in sc (kAhead: which are there, while the next one's are
+  // multiplied into nx).  EDGE: some row of the workgroup stops inside it (or there may be no next).
+  auto step = [&](int n, f32x16 (&sc)[kST], f32x16 (&nx)[kST], auto edge_c) __attribute__((always_inline)) {
     constexpr bool kEdge = decltype(edge_c)::value;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // step n is in its plane, and the other plane is no longer read
-    if (n + 1 < steps) load(n + 1, s_kv[(n + 1) & 1]);
+    // V of this step is in its plane, and K of this step or the next; the planes to load are no longer read.
+    __syncthreads();
+    if (n + 1 + kAhead < steps) load(n + 1 + kAhead, K_c);
+    if (n + 1 < steps) load(n + 1, V_c);
     const int k0 = (n * KG + kgrp) * kKeys;
     if (kEdge && k0 >= last) return;  // none of this wave's rows sees it
     const uint8_t *buf = s_kv[n & 1] + kgrp * 2 * kPlane;
     // (Addresses are a XOR with a constant away from these: computed, not held in registers.)
     uint32_t ka = kx, va = vx;
     asm volatile("" : "+v"(ka), "+v"(va));
-    f32x16 sc[kST];
+    if constexpr (!kAhead) {
 #pragma unroll
-    for (int st = 0; st < kST; ++st)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) sc[st][v] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < HD / 16; ++s)
-#pragma unroll
-      for (int st = 0; st < kST; ++st) {
-        const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + krd + (ka ^ (32 * s)) + 32 * st * kRowB);
-        sc[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
-                                                         __builtin_bit_cast(bf16x8, qf[s]), sc[st], 0, 0, 0);
-      }
+      for (int i = 0; i < HD / 16; ++i) scores(n, i, ka, sc);
+    }
     float mx = -INFINITY;
 #pragma unroll
     for (int st = 0; st < kST; ++st)
@@ -306,33 +331,58 @@ packed_attention_kernel(const PkArgs a) {
         for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
     }
     const float mref = m == -INFINITY ? 0.0f : m;  // before a row's first key above -inf
-    u32x4 pf[2 * kST];
+    if (kAhead && kEdge && n + 1 < steps && k0 + KG * kKeys < last) {
 #pragma unroll
-    for (int s = 0; s < 2 * kST; ++s)
+      for (int i = 0; i < HD / 16; ++i) scores(n + 1, i, ka, nx);
+    }
+    constexpr int kSlices = HD / 16 / (2 * kST);  // of the next products, per 16 keys of this step's
+#pragma unroll
+    for (int s = 0; s < 2 * kST; ++s) {
+      if constexpr (kAhead && !kEdge) {
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i) scores(n + 1, s * kSlices + i, ka, nx);
+      }
+      u32x4 pf;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int v = 8 * (s & 1) + 2 * j;
         const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v], c, -mref));
         const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v + 1], c, -mref));
         l += e0 + e1;
-        pf[s][j] = pack_bf16x2(e0, e1);
+        pf[j] = pack_bf16x2(e0, e1);
       }
-#pragma unroll
-    for (int s = 0; s < 2 * kST; ++s)
 #pragma unroll
       for (int dt = 0; dt < kDT; ++dt) {
         const uint8_t *p = buf + vrd + (va ^ (64 * dt)) + 16 * s * kRowB;
         const uint2 x0 = pk_read_tr(p), x1 = pk_read_tr(p + 8 * kRowB);
         const u32x4 x = {x0.x, x0.y, x1.x, x1.y};
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
-                                                          __builtin_bit_cast(bf16x8, pf[s]), acc[dt], 0, 0, 0);
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, pf),
+                                                          acc[dt], 0, 0, 0);
       }
+    }
   };
   // Steps that every row sees whole, then those where rows stop: apart, so that the long loop has no
   // masks and keeps its sums where they are.
   const int full = (it.tile * kRows / a.grp + 1) / (KG * kKeys);
-  for (int n = 0; n < full; ++n) step(n, std::false_type{});
-  for (int n = full; n < steps; ++n) step(n, std::true_type{});
+  int n = 0;
+  if constexpr (kAhead) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) scores(0, i, kx, sa);
+    for (; n + 3 <= full; n += 2) {  // (step n + 2, whose scores these end with, is whole)
+      step(n, sa, sb, std::false_type{});
+      step(n + 1, sb, sa, std::false_type{});
+    }
+    for (; n < steps; ++n) {
+      step(n, sa, sb, std::true_type{});
+#pragma unroll
+      for (int st = 0; st < kST; ++st) sa[st] = sb[st];
+    }
+  } else {
+    for (; n < full; ++n) step(n, sa, sa, std::false_type{});
+    for (; n < steps; ++n) step(n, sa, sa, std::true_type{});
+  }
   __syncthreads();  // (the planes are free)
   // A row wave's part of them: the second key group's sums, then the rows on their way out.
   constexpr int kJoin = KG == 1 ? kPkRows * kRowB : (16 * kDT + 4) * kWave * 4;
