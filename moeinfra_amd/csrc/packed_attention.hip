@@ -164,11 +164,11 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
 //   O^T += V^T P^T     P of a lane is the B operand as it stands; V is read transposed
 //
 // Bound: a tile of 64 keys costs a wave 1024 cycles of products and about as many of vector
-// instructions (512 of them the exponentials), and LDS as many of operand reads for the 8 waves of a
-// CU; they overlap between its waves.  16384 tokens in 3 sequences, 32 / 8 heads of 128: 1590-1750 us,
-// 950-1040 TFLOP/s (a product of 8192^3 runs at 1190); 3333 tokens in 9 sequences 36 us, 570 TFLOP/s, their
-// few tiles a row tile; many short sequences are bound by their queries and outputs (64 of 256: 335 MB
-// in 120 us).
+// instructions (512 of them the exponentials); waves of a SIMD overlap them.  Where that lasts, the
+// clock falls (16384 tokens in 3 sequences, 32 / 8 heads of 128: 1560 us, 1065 TFLOP/s, products busy 55 %
+// of the cycles at 1.8 GHz; a library product of 8192^3 runs at 1190).  3333 tokens in 9 sequences 39 us,
+// 525 TFLOP/s: few tiles a row tile.  Many short sequences: their queries and outputs (64 of 256: 335 MB in
+// 118 us).
 //
 // A weight is 2^(s c - m) by one fused multiply-add, c = scaling * log2(e), m a rounded max s c: what
 // the rounding of m leaves cancels against the sum, as long as 2 to its power is in range.  Rows with
@@ -495,11 +495,12 @@ extern "C" int moe_packed_attention_bf16(const void *q, int64_t q_stride, const 
   auto tiles = [&](int rows) { return (T * grp / rows + (B < T ? B : T)) * n_kv_heads; };
   const int64_t cus = moe::device_cu_count();
   // 128 rows a workgroup, two of them on a CU.  Few, of sequences of some length: in two key groups
-  // (1500 tokens 36 us instead of 42; 9 sequences of 3333 56 instead of 39).  Many, of more KV heads
-  // than there are XCDs, whose L2s then hold parts of several: 256 rows, which read K and V half as
-  // often (8192 tokens of 16 / 16 heads of 128 281 us instead of 304; of 32 / 8 heads the same).
+  // (1500 tokens 36 us instead of 42; 9 sequences of 3333 56 instead of 39).  Many, of long sequences:
+  // 256 rows, which read K and V half as often, but leave more rows masked at a sequence's end
+  // (32 / 8 heads of 128: 4 sequences of 4096 tokens 594 us instead of 630, 8 of 2048 338 / 345, 10 of 1500
+  // 249 / 233; 16 / 16: 8 of 1024 54 / 55.5, 40 of 256 49 / 41).
   const bool paired = head_dim != 256 && tiles(128) <= 2 * cus && T >= 256 * B;
-  const bool wide = head_dim == 128 && n_kv_heads > 8 && tiles(256) >= 2 * cus && !paired;
+  const bool wide = head_dim == 128 && T >= (grp > 1 ? 2048 : 1024) * B && tiles(256) >= 2 * cus && !paired;
   const int64_t g = tiles(wide ? 256 : 128);
   const int threads = (paired || wide ? 8 : 4) * moe::kWave;
   MOE_REQUIRE(moe::launch_fits(g, threads), "bad sizes");

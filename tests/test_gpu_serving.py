@@ -335,9 +335,36 @@ def test_packed_attention_wide_workgroups(cuda_device):
 @pytest.mark.parametrize("lens,nq,nkv,hd", [([1900, 2300], 16, 16, 128), ([300, 280], 4, 1, 64), ([900], 6, 2, 256),
                                             ([600, 599, 3], 8, 1, 128)])
 def test_packed_attention_kernels(cuda_device, lens, nq, nkv, hd):
-    # 256 rows a workgroup (many rows of 16 KV heads), two key groups (few), the large head dim.
+    # Many rows of 16 KV heads, two key groups (few rows), the large head dim.
     print(f"packed attention {lens} {nq}/{nkv} heads of {hd}", flush=True)
     _check_packed(*_packed(cuda_device, lens, nq, nkv, hd, seed=hd))
+
+
+@pytest.mark.parametrize("lens,nq,nkv", [([1030], 128, 128), ([1500, 0, 1900], 64, 64), ([2100], 64, 32), ([2051], 72, 8)])
+def test_packed_attention_256_rows(cuda_device, lens, nq, nkv):
+    """Long sequences of enough heads that workgroups take 256 rows: of a token, a token's two heads, nine."""
+    print(f"packed attention {lens} {nq}/{nkv} heads, 256 rows", flush=True)
+    _check_packed(*_packed(cuda_device, lens, nq, nkv, 128, seed=nq + nkv, gap=2))
+
+
+def test_packed_attention_256_rows_infinities(cuda_device):
+    """... with an infinity and a NaN that some of a workgroup's rows see."""
+    n, nq = 1030, 128
+
+    def spoil(q, k, v, cuts):
+        v[cuts[0] + 700, 3, 9] = math.inf
+        v[cuts[0] + 1000, 3, 10] = math.nan
+
+    out, q, k, v, cuts, s = _packed(cuda_device, [n], nq, nq, 128, seed=16, gap=1, change=spoil)
+    o = out[1:1 + n, 3].float().cpu()
+    assert torch.isinf(o[700:, 9]).all() and torch.isnan(o[1000:, 10]).all()
+    v[1 + 700, 3, 9] = v[1 + 1000, 3, 10] = 0
+    want, tol = attention(q[1:1 + n, 3], k[1:1 + n, 3], v[1:1 + n, 3], s, torch.ones((n, n), dtype=torch.bool).tril())
+    keep = torch.ones((n, 128), dtype=torch.bool)
+    keep[700:, 9] = False
+    keep[1000:, 10] = False
+    assert torch.isfinite(o[keep]).all()
+    assert_within(torch.where(keep, o, 0.0), torch.where(keep, want, 0.0), tol)
 
 
 def test_packed_attention_scalings(cuda_device):
