@@ -344,12 +344,13 @@ def _rows(t: torch.Tensor, name: str, dev: torch.device, ndim: int) -> int:
 def _pages(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: torch.device):
     """(page stride, shape) of a paged cache (k and v [pages, kv heads, page size, head dim], whole
     pages at one stride)."""
-    if isinstance(k_cache, torch.Tensor) and isinstance(v_cache, torch.Tensor):
-        shape, strides = k_cache.shape, k_cache.stride()
-        if (len(shape) == 4 and shape[0] > 1 and strides[1:] == (shape[2] * shape[3], shape[3], 1)
-                and k_cache.dtype is _BF16 and k_cache.device == dev and v_cache.stride() == strides
-                and v_cache.shape == shape and v_cache.dtype is _BF16 and v_cache.device == dev):
-            return strides[0], shape
+    if (isinstance(k_cache, torch.Tensor) and isinstance(v_cache, torch.Tensor) and k_cache.dtype is _BF16
+            and v_cache.dtype is _BF16 and k_cache.device == dev and v_cache.device == dev
+            and k_cache.is_contiguous() and v_cache.is_contiguous()):
+        shape = k_cache.shape
+        if len(shape) == 4 and shape[0] > 1 and v_cache.shape == shape:
+            _, heads, size, hd = shape
+            return heads * size * hd, shape
     stride = _rows(k_cache, "k_cache", dev, 4)
     if _rows(v_cache, "v_cache", dev, 4) != stride or k_cache.shape != v_cache.shape:
         raise ValueError(f"k_cache {tuple(k_cache.shape)} of page stride {stride} and v_cache {tuple(v_cache.shape)} of "
@@ -394,9 +395,10 @@ def rope_paged_kv(qkv: torch.Tensor, positions: torch.Tensor, page_table: torch.
     if row != (nq + 2 * nkv) * hd:
         raise ValueError(f"qkv rows have {row} values, {nq} query and {nkv} KV heads of {hd} need {(nq + 2 * nkv) * hd}")
     table = _plain(page_table, "page_table", _I32, dev)
-    if page_table.ndim != 2:
+    table_shape = page_table.shape
+    if len(table_shape) != 2:
         raise ValueError("page_table must be [sequences, pages]")
-    n_seqs, width = page_table.shape
+    n_seqs, width = table_shape
     pos = _plain(positions, "positions", _I32, dev, (T,))
     freq = _plain(inv_freq, "inv_freq", _F32, dev, (hd // 2,))
     seqs = None if seq_ids is None else _plain(seq_ids, "seq_ids", _I32, dev, (T,))
@@ -432,14 +434,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if q_dim != hd:
         raise ValueError(f"q has head dim {q_dim}, the cache {hd}")
     table = _plain(page_table, "page_table", _I32, dev)
-    if page_table.ndim != 2 or page_table.shape[0] != B:
-        raise ValueError(f"page_table must have {B} rows of pages (got {tuple(page_table.shape)})")
+    table_shape = page_table.shape
+    if len(table_shape) != 2 or table_shape[0] != B:
+        raise ValueError(f"page_table must have {B} rows of pages (got {tuple(table_shape)})")
     n = _plain(lens, "lens", _I32, dev, (B,))
     out = _out(out, "out", q, B, nq, hd)
     if workspace is None:
         workspace = paged_attention_workspace(B, nq, nkv, hd, dev)
     _launch(lib().moe_paged_attention_bf16, "paged_attention", dev, q.data_ptr(), stride, k_cache.data_ptr(),
-            v_cache.data_ptr(), pages, size, page_stride, table, page_table.shape[1], n, B, nq, nkv, hd,
+            v_cache.data_ptr(), pages, size, page_stride, table, table_shape[1], n, B, nq, nkv, hd,
             hd ** -0.5 if scaling is None else scaling, out.data_ptr(),
             _plain(workspace, "workspace", torch.uint8, dev), workspace.numel())
     return out
