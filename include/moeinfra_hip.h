@@ -372,7 +372,8 @@ int moe_paged_attention_bf16(const void *q, int64_t q_stride, const void *k_cach
  * [T, n_q, head_dim], k and v [T, n_kv, head_dim], their rows q_stride / k_stride / v_stride values
  * apart (slices of a projection's output); out [T, n_q * head_dim].  fp32 scores q.k * scaling and
  * softmax, the weights rounded to bf16 before their sum (fp32) with v.  Rows of no sequence are left
- * as they were.  head dim 64, 128 or 256; q, k, v and out 16-byte aligned. */
+ * as they were.  head dim 64, 128 or 256; q, k, v and out 16-byte aligned, k_stride and v_stride
+ * below 2^31. */
 int moe_packed_attention_bf16(const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                               const void *v, int64_t v_stride, int64_t T,
                               const void *cu_seqlens_i32, int64_t B, int32_t n_q_heads,

@@ -25,6 +25,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 struct PkArgs {
   const uint16_t *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;
+  uint32_t k_bytes, v_bytes;  // from row to row
   const int32_t *cu;
   int T, B, nq, nkv, grp;
   float scaling;
@@ -166,8 +167,8 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
 // Bound: a tile of 64 keys costs a wave 1024 cycles of products and about as many of vector
 // instructions (512 of them the exponentials); waves of a SIMD overlap them.  Where that lasts, the
 // clock falls (16384 tokens in 3 sequences, 32 / 8 heads of 128: 1560 us, 1065 TFLOP/s, products busy 55 %
-// of the cycles at 1.8 GHz; a library product of 8192^3 runs at 1190).  3333 tokens in 9 sequences 39 us,
-// 525 TFLOP/s: few tiles a row tile.  Many short sequences: their queries and outputs (64 of 256: 335 MB in
+// of the cycles at 1.8 GHz; a library product of 8192^3 runs at 1190).  3333 tokens in 9 sequences 38 us,
+// 535 TFLOP/s: few tiles a row tile.  Many short sequences: their queries and outputs (64 of 256: 335 MB in
 // 118 us).
 //
 // A weight is 2^(s c - m) by one fused multiply-add, c = scaling * log2(e), m a rounded max s c: what
@@ -222,12 +223,16 @@ packed_attention_kernel(const PkArgs a) {
       for (int i = 0; i < kChunks; ++i) {
         const int chunk = (loader + i * NW) * 1024, at = chunk + 16 * lane;
         const uint32_t row = at / kRowB, piece = at % kRowB / 16;
-        const int64_t key = min((at_step * KG + n) * kKeys + (int)row, nkeys - 1);
-        uint8_t *const plane = s_kv[at_step & 1] + n * 2 * kPlane + chunk;
-        if constexpr (kV)
-          pk_load_lds(vb + key * a.v_stride + 8 * (piece ^ pk_vx<HD>(row)), plane + kPlane);
+        const int key = min((at_step * KG + n) * kKeys + (int)row, nkeys - 1);
+        const uint32_t swz = piece ^ (kV ? pk_vx<HD>(row) : pk_kx<HD>(row));
+        uint8_t *const plane = s_kv[at_step & 1] + n * 2 * kPlane + (kV ? kPlane : 0) + chunk;
+        const uint16_t *const base = kV ? vb : kb;
+        // One multiply-add of 32-bit factors.  (Of 256 dims its bases leave no registers: 357 us for 8192
+        // tokens of 8 / 4 heads with the long product, 395 with this one.)
+        if constexpr (HD == 256)
+          pk_load_lds(base + key * (kV ? a.v_stride : a.k_stride) + 8 * swz, plane);
         else
-          pk_load_lds(kb + key * a.k_stride + 8 * (piece ^ pk_kx<HD>(row)), plane);
+          pk_load_lds((const uint8_t *)base + 16 * swz + (uint64_t)(uint32_t)key * (kV ? a.v_bytes : a.k_bytes), plane);
       }
   };
   const std::false_type K_c{};
@@ -452,13 +457,20 @@ packed_attention_kernel(const PkArgs a) {
           make_uint2(pack_bf16x2(acc[dt][v] * inv, acc[dt][v + 1] * inv),
                      pack_bf16x2(acc[dt][v + 2] * inv, acc[dt][v + 3] * inv));
   constexpr int kPieces = kRowB / 16, kStep = kWave / kPieces;  // lanes per row, rows per store
+  constexpr int kStores = kPkRows / kStep;
+  u32x4 v[kStores];
+  uint32_t lo[kStores], hi[kStores];
 #pragma unroll
-  for (int i = 0; i < kPkRows / kStep; ++i) {
+  for (int i = 0; i < kStores; ++i) {  // (all of them before the first store, as each may be skipped)
     const int row = i * kStep + lane / kPieces, piece = lane % kPieces;
-    const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + row * kRowB + 16 * (piece ^ (row & kSwz)));
-    const uint32_t lo = __shfl((uint32_t)place, row, kWave), hi = __shfl((uint32_t)(place >> 32), row, kWave);
-    if (row0 + row < rows)
-      *reinterpret_cast<u32x4 *>(a.out + (int64_t)(lo | (uint64_t)hi << 32) + 8 * piece) = v;
+    v[i] = *reinterpret_cast<const u32x4 *>(mine + row * kRowB + 16 * (piece ^ (row & kSwz)));
+    lo[i] = __shfl((uint32_t)place, row, kWave);
+    hi[i] = __shfl((uint32_t)(place >> 32), row, kWave);
+  }
+#pragma unroll
+  for (int i = 0; i < kStores; ++i) {
+    const int row = i * kStep + lane / kPieces, piece = lane % kPieces;
+    if (row0 + row < rows) *reinterpret_cast<u32x4 *>(a.out + (int64_t)(lo[i] | (uint64_t)hi[i] << 32) + 8 * piece) = v[i];
   }
 }
 
@@ -478,6 +490,7 @@ extern "C" int moe_packed_attention_bf16(const void *q, int64_t q_stride, const 
                   T * grp <= 0x7fffffff - 1024 && T <= 0x7fffffff,
               "bad sizes");
   const int64_t qrow = (int64_t)n_q_heads * head_dim, krow = (int64_t)n_kv_heads * head_dim;
+  MOE_REQUIRE(T <= 1 || (k_stride <= 0x7fffffff && v_stride <= 0x7fffffff), "rows of k and v must be less than 2^31 values apart");
   MOE_REQUIRE((q_stride | k_stride | v_stride) % 8 == 0 &&
                   (T <= 1 || (q_stride >= qrow && k_stride >= krow && v_stride >= krow)),
               "rows of q, k and v must be 16-byte aligned and apart");
@@ -491,11 +504,11 @@ extern "C" int moe_packed_attention_bf16(const void *q, int64_t q_stride, const 
                   !moe::ranges_overlap(out, ob, v, 2 * (v_stride * (T - 1) + krow)),
               "out must not overlap q, k or v");
   moe::PkArgs a{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, q_stride, k_stride, v_stride,
-                (const int32_t *)cu_seqlens_i32, (int)T, (int)B, n_q_heads, n_kv_heads, grp, scaling, (uint16_t *)out};
+                (uint32_t)(2 * k_stride), (uint32_t)(2 * v_stride), (const int32_t *)cu_seqlens_i32, (int)T, (int)B, n_q_heads, n_kv_heads, grp, scaling, (uint16_t *)out};
   auto tiles = [&](int rows) { return (T * grp / rows + (B < T ? B : T)) * n_kv_heads; };
   const int64_t cus = moe::device_cu_count();
   // 128 rows a workgroup, two of them on a CU.  Few, of sequences of some length: in two key groups
-  // (1500 tokens 36 us instead of 42; 9 sequences of 3333 56 instead of 39).  Many, of long sequences:
+  // (1500 tokens 36 us instead of 42; 3333 in 9 sequences 56 instead of 38).  Many, of long sequences:
   // 256 rows, which read K and V half as often, but leave more rows masked at a sequence's end
   // (32 / 8 heads of 128: 4 sequences of 4096 tokens 594 us instead of 630, 8 of 2048 338 / 345, 10 of 1500
   // 249 / 233; 16 / 16: 8 of 1024 54 / 55.5, 40 of 256 49 / 41).

@@ -96,6 +96,8 @@ REFUSED = [
     (_packed, dict(q_stride=504), "apart"),
     (_packed, dict(k_stride=132), "aligned"),
     (_packed, dict(v_stride=64), "apart"),
+    (_packed, dict(k_stride=1 << 31), "values apart"),
+    (_packed, dict(v_stride=1 << 40), "values apart"),
     (_packed, dict(cu=None), "null"),
     (_packed, dict(v=C + 8), "aligned"),
     (_packed, dict(out=E + 4), "aligned"),
