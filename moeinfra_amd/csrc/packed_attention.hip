@@ -191,10 +191,10 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
 //
 // Bound: a tile of 64 keys costs a wave 1024 cycles of products and about as many of vector
 // instructions (512 of them the exponentials); waves of a SIMD overlap them.  Where that lasts, the
-// clock falls (16384 tokens in 3 sequences, 32 / 8 heads of 128: 1560 us, 1065 TFLOP/s, products busy 55 %
-// of the cycles at 1.8 GHz; a library product of 8192^3 runs at 1190).  3333 tokens in 9 sequences 38 us,
-// 535 TFLOP/s: few tiles a row tile.  Many short sequences: their queries and outputs (64 of 256: 335 MB in
-// 118 us).
+// clock falls (16384 tokens in 3 sequences, 32 / 8 heads of 128: 1520-1580 us, 1050-1100 TFLOP/s, products
+// busy 55 % of the cycles at 1.8 GHz; a library product of 8192^3 runs at 1190).  3333 tokens in 9 sequences
+// 36 us, 565 TFLOP/s: a start of 3 us, mostly memory's answer, for few tiles.  Many short sequences: their
+// queries and outputs (64 of 256: 335 MB in 109 us).
 //
 // A weight is 2^(s c - m) by one fused multiply-add, c = scaling * log2(e), m a rounded max s c: what
 // the rounding of m leaves cancels against the sum, as long as 2 to its power is in range.  Rows with

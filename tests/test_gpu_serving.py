@@ -325,6 +325,15 @@ def test_packed_attention_batches(cuda_device, lens):
     _check_packed(*_packed(cuda_device, lens, 4, 2, 128, seed=len(lens)))
 
 
+@pytest.mark.parametrize("count", [31, 32, 33, 63, 64, 65, 130])
+def test_packed_attention_many_sequences(cuda_device, count):
+    """Batches around the numbers of sequences where the search for a workgroup's tile changes, with
+    equal, empty and long ones among them."""
+    print(f"packed attention of {count} sequences", flush=True)
+    lens = [(0, 1, 40, 40, 7, 170)[(i * i + i // 5) % 6] for i in range(count)]
+    _check_packed(*_packed(cuda_device, lens, 4, 2, 64, seed=count, gap=1))
+
+
 def test_packed_attention_wide_workgroups(cuda_device):
     # Enough rows for the 8-wave workgroups: 32 heads, 64 and 128 dims.
     for hd in (64, 128):
