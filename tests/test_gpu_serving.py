@@ -243,6 +243,27 @@ def test_paged_attention_extremes(cuda_device):
             assert_within(out[0], want, tol)
 
 
+@pytest.mark.parametrize("n", [9, 700, 3000])
+def test_paged_attention_infinite_values(cuda_device, n):
+    """An infinity in a value comes through as one, also from the last of a sequence's parts."""
+    from moeinfra_amd import ops
+
+    dev, nq, nkv, hd, page = cuda_device, 4, 2, 128, 16
+    pool = Pool([n], nkv, hd, page, dev, seed=18, fill=math.nan)
+    k, v, q = _bf((n, nkv, hd), 180), _bf((n, nkv, hd), 181), _bf((1, nq, hd), 182)
+    v[n - 1, 0, 5] = math.inf
+    v[0, 1, 6] = -math.inf
+    pool.put(0, k, v)
+    out = ops.paged_attention(q.to(dev), pool.k, pool.v, pool.dev_table, torch.tensor([n], dtype=torch.int32, device=dev),
+                              workspace=ops.paged_attention_workspace(1, nq, nkv, hd, dev)).cpu()
+    assert (out[0, :2, 5] == math.inf).all() and (out[0, 2:, 6] == -math.inf).all()
+    out[0, :2, 5] = out[0, 2:, 6] = v[n - 1, 0, 5] = v[0, 1, 6] = 0.0
+    want = [attention(q[0, 2 * h:2 * h + 2], k[:, h], v[:, h], hd ** -0.5) for h in range(2)]
+    for h, at in ((0, 5), (1, 6)):
+        want[h][0][:, at] = 0.0
+        assert_within(out[0, 2 * h:2 * h + 2], *want[h])
+
+
 def test_paged_attention_offsets_past_32_bits(cuda_device):
     """A pool whose far pages lie more than 2^32 bytes (and 2^31 values) into the tensors."""
     from moeinfra_amd import ops
