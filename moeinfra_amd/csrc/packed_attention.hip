@@ -450,7 +450,9 @@ packed_attention_kernel(const PkArgs a) {
   l = op_xor32<false>(l);
   // A row that stops inside a tile meets V rows that it does not see with weights of zero: an
   // infinity or NaN there would come through.  Where a result is not finite, look at those rows,
-  // and if one of them holds such a value, take this wave's rows one by one.
+  // and if one of them holds such a value, take this wave's rows one by one.  Where the wave's last
+  // tile goes past the workgroup's keys, row nkeys - 1 is one of them (it stands there again), also
+  // for rows that see it.
   float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN where a value is not finite (64 compares take 0.7 us)
 #pragma unroll
   for (int dt = 0; dt < kDT; ++dt)
@@ -459,8 +461,8 @@ packed_attention_kernel(const PkArgs a) {
   const bool bad = !((none[0] + none[1]) + (none[2] + none[3]) == 0.0f);
   if (__any(bad | huge)) {
     bool again = huge;
-    const int end = min((last + kKeys - 1) / kKeys * kKeys, nkeys);
-    for (int j = first; j < end; ++j)
+    const int whole = (last + kKeys - 1) / kKeys * kKeys, end = min(whole, nkeys);
+    for (int j = whole > nkeys ? min(first, nkeys - 1) : first; j < end; ++j)
       for (int d = lane; d < HD; d += kWave) again |= (vb[j * a.v_stride + d] & 0x7f80u) == 0x7f80u;
     if (__any(again)) {
       pk_rows_scalar<HD>(a.q + it.tok0 * a.q_stride + (int64_t)kvh * a.grp * HD, a.q_stride, kb, a.k_stride, vb,

@@ -449,6 +449,46 @@ def test_packed_attention_infinities_stay_with_the_rows_that_see_them(cuda_devic
         _check_packed(out, q, k, v, cuts[:2], s)
 
 
+@pytest.mark.parametrize("lens,nq,nkv,hd", [
+    ([1, 9, 17, 0, 33, 65, 129, 8, 64], 8, 2, 128),     # 4 heads a group: 8 n + 1
+    ([1, 9, 17, 65], 4, 1, 64), ([1, 9, 33, 41], 4, 1, 256),
+    ([1, 33, 65, 97, 32], 2, 2, 128), ([1, 33, 65], 3, 3, 256),      # 1: 32 n + 1
+    ([1, 5, 9, 61, 64, 65], 8, 1, 64), ([2, 1, 40, 70], 40, 1, 128),  # 8: 4 n + 1; 40: a token's rows in two waves
+    ([257], 4, 1, 64), ([257, 289], 4, 4, 128), ([273, 277], 16, 2, 128),  # two key groups
+    ([1025], 128, 128, 128), ([2057], 64, 16, 128)])     # 256 rows
+def test_packed_attention_infinities_of_last_tokens(cuda_device, lens, nq, nkv, hd):
+    """An infinity in the last token's values is that token's result and no other's, whatever the
+    number of rows that the sequence leaves for its last workgroup and wave."""
+    print(f"infinities of last tokens, {lens} {nq}/{nkv} heads of {hd}", flush=True)
+
+    def spoil(q, k, v, cuts):
+        for a, b in zip(cuts, cuts[1:]):
+            if b > a:
+                v[b - 1, 0, 5] = math.inf
+                v[b - 1, nkv - 1, hd - 1] = -math.inf
+
+    out, q, k, v, cuts, s = _packed(cuda_device, lens, nq, nkv, hd, seed=nq + hd, gap=1, change=spoil)
+    o, grp = out.float().cpu(), nq // nkv
+    for a, b in zip(cuts, cuts[1:]):
+        if b == a:
+            continue
+        for kh, d, x in ((0, 5, math.inf), (nkv - 1, hd - 1, -math.inf)):
+            rows = o[b - 1, kh * grp:(kh + 1) * grp, d]
+            assert bool((rows == x).all()), f"tokens {a} .. {b - 1}: {rows}"
+            o[b - 1, kh * grp:(kh + 1) * grp, d] = 0
+            v[b - 1, kh, d] = 0
+    # The others', against the same values with zeros in those places (which are left out).
+    for a, b in zip(cuts, cuts[1:]):
+        n = b - a
+        seen = torch.ones((n, n), dtype=torch.bool).tril()
+        for h in sorted({0, nq // 2, nq - 1}) if n > 0 else ():
+            want, tol = attention(q[a:b, h], k[a:b, h // grp], v[a:b, h // grp], s, seen)
+            for kh, d in ((0, 5), (nkv - 1, hd - 1)):
+                if h // grp == kh:
+                    want[n - 1, d] = 0
+            assert_within(o[a:b, h], want, tol, f"tokens {a} .. {b - 1}, head {h}")
+
+
 # ------------------------------------------------------------------ choice of tokens
 SETTINGS = [dict(), dict(temperature=0.0), dict(top_k=1), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.05),
             dict(temperature=0.7, top_k=50, top_p=0.9), dict(temperature=1.5, top_p=0.5, min_p=0.02),
