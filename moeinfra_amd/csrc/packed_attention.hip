@@ -19,7 +19,7 @@ constexpr float kPkLog2e = 1.44269504088896341f;
 // rescaled: weights up to 2^8, which fp32 sums and bf16 weights carry without loss.
 constexpr float kPkLag = 8.0f;
 constexpr float kPkHuge = 268435456.0f;  // 2^28: half a step of m is 2^3
-constexpr int kPkFew = 32;
+constexpr int kPkFew = 32;               // sequences, to which the search goes by keys (pk_item)
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -63,14 +63,19 @@ __device__ __forceinline__ void pk_load_lds(const void *src, const uint8_t *dst)
 }
 
 // A workgroup's rows: tile `tile` (of `rows` rows of token x query head of the group) of the
-// sequence of tokens tok0 .. tok0 + len - 1.  Item w of a KV head is the w-th of all tiles in
-// falling order of their tile number, i.e. of their keys, so that the longest start first
-// whatever order the sequences have.  Each wave finds it alone.  With N(L) the tiles numbered L and
-// above, item w is of the level L with N(L + 1) <= w < N(L):
-//   - up to kPkFew sequences: lane i has N(t) for its own number of tiles t; the smallest t with N(t) <= w is
-//     above L, and from there down N grows by the c sequences of that many tiles or more (a wave's 0.3
-//     us before its first load instead of 0.9);
-//   - more: N by a sum over the batch, L by bisection (64 of 256 tokens: 109 us, 117 by the other).
+// sequence of tokens tok0 .. tok0 + len - 1.  Each wave finds it alone, in a time that does not grow
+// with the batch beyond its logarithm:
+//   - up to kPkFew sequences: item w of a KV head is the w-th of all tiles in falling order of their tile
+//     number, i.e. of their keys, so that the longest start first whatever order the sequences have.
+//     With N(L) the tiles numbered L and above, item w is of the level L with N(L + 1) <= w < N(L).  Lane i
+//     has N(t) for its own number of tiles t; the smallest t with N(t) <= w is above L, and from there down N
+//     grows by the c sequences of that many tiles or more;
+//   - more: sequence i has the places from base(i) = floor(tokens before it * group / rows) + min(i, tokens
+//     before it) on, which are at least its tiles (the few left over have no rows), its last tile first.  The
+//     sequence of place w is the last one with base <= w: two rounds of loads for 4096 sequences, four
+//     for 2^20.  (32 / 8 heads of 128: 100 sequences of 256 tokens 141 us, 512 of 256 692, 512 of 20 55;
+//     in falling order of their keys, each by sums over the batch, 180, 1377 and 103.  Where the batch
+//     just fills the device once, the empty places cost: 64 of 20 11.7 instead of 9.8.)
 struct PkItem {
   int tok0, len, tile;
 };
@@ -78,10 +83,9 @@ struct PkItem {
 __device__ __forceinline__ bool pk_item(const PkArgs &a, int rows, int w, int lane, PkItem &it) {
   auto cut = [&](int i) { return min(max(a.cu[i], 0), a.T); };
   auto tiles_of = [&](int c0, int c1) { return (int)(((int64_t)max(c1 - c0, 0) * a.grp + rows - 1) / rows); };
-  auto tiles = [&](int i) { return i < a.B ? tiles_of(cut(i), cut(i + 1)) : 0; };
-  const int c0 = cut(min(lane, a.B)), c1 = cut(min(lane + 1, a.B));
-  const int t0 = tiles_of(c0, c1);  // of the first 64 sequences
   if (a.B <= kPkFew) {
+    const int c0 = cut(min(lane, a.B)), c1 = cut(min(lane + 1, a.B));
+    const int t0 = tiles_of(c0, c1);
     int n = 0;
     for (int j0 = 0; j0 < a.B; j0 += 8)
 #pragma unroll
@@ -102,46 +106,24 @@ __device__ __forceinline__ bool pk_item(const PkArgs &a, int rows, int w, int la
     it.tile = level;
     return true;
   }
-  // (Counts are exact in fp32: a batch has fewer than 2^24 tiles.)
-  auto above = [&](int level) {
-    float n[1] = {(float)max(t0 - level, 0)};
-    lane_groups_reduce<false>(n, kWave);
-    float sum = n[0];
-    for (int i0 = kWave; i0 < a.B; i0 += kWave) {
-      float more[1] = {(float)max(tiles(i0 + lane) - level, 0)};
-      lane_groups_reduce<false>(more, kWave);
-      sum += more[0];
-    }
-    return __builtin_amdgcn_readfirstlane((int)sum);
+  // Lane l looks at one sequence in 64ths of those left.
+  auto base = [&](int i) {
+    const int c = cut(i);
+    return (int)((uint32_t)c * (uint32_t)a.grp / (uint32_t)rows) + min(i, c);
   };
-  if (w >= above(0)) return false;
-  float most[1] = {(float)t0};
-  for (int i0 = kWave; i0 < a.B; i0 += kWave) most[0] = fmaxf(most[0], (float)tiles(i0 + lane));
-  lane_groups_reduce<true>(most, kWave);
-  int lo = 0, hi = __builtin_amdgcn_readfirstlane((int)most[0]);  // N(lo) > w, N(hi) <= w
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (above(mid) > w)
-      lo = mid;
-    else
-      hi = mid;
+  int lo = 0, n = a.B;
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave, at = (lane + 1) * step;
+    const int i = __builtin_ctzll(__ballot(at >= n || base(lo + min(at, n - 1)) > w));  // (lane 63's is past them)
+    lo += i * step;
+    n = min(n - i * step, step);
   }
-  int i = w - above(lo + 1);  // of the sequences that have a tile lo
-  for (int i0 = 0; i0 < a.B; i0 += kWave) {
-    const int t = i0 == 0 ? t0 : tiles(i0 + lane);
-    uint64_t has = __ballot(t > lo);
-    const int n = __popcll(has);
-    if (i < n) {
-      for (; i > 0; --i) has &= has - 1;
-      const int s = i0 + __builtin_ctzll(has);
-      it.tok0 = cut(s);
-      it.len = cut(s + 1) - it.tok0;
-      it.tile = lo;
-      return true;
-    }
-    i -= n;
-  }
-  return false;
+  // (Scalars, as above: 8192 tokens of 8 / 4 heads of 256 dims 334 us, 342 without.)
+  it.tok0 = __builtin_amdgcn_readfirstlane(cut(lo));
+  it.len = __builtin_amdgcn_readfirstlane(max(cut(lo + 1) - it.tok0, 0));
+  const int place = w - base(lo), t = tiles_of(it.tok0, it.tok0 + it.len);
+  it.tile = t - 1 - place;
+  return place >= 0 && place < t;
 }
 
 // Rows r0 .. r1 - 1 (at most 32) of a sequence without matrix products, a row at a time, a key per
@@ -194,7 +176,7 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
 // clock falls (16384 tokens in 3 sequences, 32 / 8 heads of 128: 1520-1580 us, 1050-1100 TFLOP/s, products
 // busy 55 % of the cycles at 1.8 GHz; a library product of 8192^3 runs at 1190).  3333 tokens in 9 sequences
 // 36 us, 565 TFLOP/s: a start of 3 us, mostly memory's answer, for few tiles.  Many short sequences: their
-// queries and outputs (64 of 256: 335 MB in 109 us).
+// queries and outputs (64 of 256: 335 MB in 90 us).
 //
 // A weight is 2^(s c - m) by one fused multiply-add, c = scaling * log2(e), m a rounded max s c: what
 // the rounding of m leaves cancels against the sum, as long as 2 to its power is in range.  Rows with

@@ -355,6 +355,33 @@ def test_packed_attention_many_sequences(cuda_device, count):
     _check_packed(*_packed(cuda_device, lens, 4, 2, 64, seed=count, gap=1))
 
 
+@pytest.mark.parametrize("count,nq,nkv,hd", [(4097, 4, 4, 64), (70000, 4, 1, 128), (1 << 20, 1, 1, 64)])
+def test_packed_attention_large_batches(cuda_device, count, nq, nkv, hd):
+    """Batches of up to the largest number of sequences: most of one token, whose result is its own
+    values, some empty, a few of several tokens (the first and the last among them)."""
+    from moeinfra_amd import ops
+
+    print(f"packed attention of {count} sequences", flush=True)
+    lens = torch.ones(count, dtype=torch.int64)
+    lens[5::17] = 0
+    longer = [0, 1, 64, 65, 4095, 4096, count // 2, count - 1]
+    lens[longer] = torch.tensor([150, 3, 33, 129, 2, 200, 65, 40])
+    cuts = torch.cat((torch.tensor([2]), 2 + lens.cumsum(0)))
+    T = int(cuts[-1]) + 3
+    q, k, v = (torch.randn((T, n, hd), generator=torch.Generator().manual_seed(9 + n + i)).to(torch.bfloat16)
+               for i, n in enumerate((nq, nkv, nkv)))
+    out = torch.full((T, nq, hd), 5.0, dtype=torch.bfloat16, device=cuda_device)
+    ops.packed_attention(*(t.to(cuda_device) for t in (q, k, v)), cuts.to(torch.int32).to(cuda_device), out=out)
+    out = out.cpu()
+    want = v.repeat_interleave(nq // nkv, dim=1)
+    want[:2] = want[T - 3:] = 5.0
+    for i in longer:
+        a, b = int(cuts[i]), int(cuts[i + 1])
+        _check_packed(out, q, k, v, [a, b], hd ** -0.5)
+        want[a:b] = out[a:b]
+    assert _same(out, want)
+
+
 def test_packed_attention_wide_workgroups(cuda_device):
     # Enough rows for the 8-wave workgroups: 32 heads, 64 and 128 dims.
     for hd in (64, 128):
