@@ -430,6 +430,7 @@ packed_attention_kernel(const PkArgs a) {
   }
   if (row0 >= rows) return;
   l = op_xor32<false>(l);
+  huge |= l == 0.0f;  // (all scores of the row below -2^128 / log2(e): s c overflows)
   // A row that stops inside a tile meets V rows that it does not see with weights of zero: an
   // infinity or NaN there would come through.  Where a result is not finite, look at those rows,
   // and if one of them holds such a value, take this wave's rows one by one.  Where the wave's last

@@ -516,6 +516,32 @@ def test_packed_attention_infinities_of_last_tokens(cuda_device, lens, nq, nkv, 
             assert_within(o[a:b, h], want, tol, f"tokens {a} .. {b - 1}, head {h}")
 
 
+@pytest.mark.parametrize("n,nq,nkv,hd", [(300, 2, 1, 64), (500, 4, 4, 128), (200, 2, 1, 256)])
+def test_packed_attention_large_scores_of_long_rows(cuda_device, n, nq, nkv, hd):
+    """Scores up to 3e38 in rows of two key groups, and of 256 dims, and an infinity in the last
+    token's values."""
+    print(f"large scores, {n} tokens, {nq}/{nkv} heads of {hd}", flush=True)
+
+    def big(q, k, v, cuts):
+        q[:], k[:] = 0, 0
+        q[:, :, 0] = 1.5e18
+        k[:, :, 0] = torch.linspace(-2e20, 2e20, n).to(torch.bfloat16)[:, None]
+        v[n - 1, 0, 3] = math.inf
+
+    out, q, k, v, cuts, s = _packed(cuda_device, [n], nq, nkv, hd, seed=4, scaling=1.0, change=big)
+    assert bool((out[n - 1, :nq // nkv, 3] == math.inf).all())
+    out[n - 1, :nq // nkv, 3] = v[n - 1, 0, 3] = 0
+    for t in range(n):
+        # The newest key (of equal ones, all) has the weight: those are 2^60 and more apart.
+        same = (k[:t + 1, 0, 0] == k[t, 0, 0]).nonzero()[:, 0]
+        for h in range(nq):
+            want = v[same, h // (nq // nkv)].double().mean(0)
+            tol = 2.0 ** -7 * v[same, h // (nq // nkv)].double().abs().mean(0) + 1e-6
+            if t == n - 1 and h < nq // nkv:
+                want[3] = 0  # (checked above)
+            assert_within(out[t, h], want, tol, f"token {t}, head {h}")
+
+
 # ------------------------------------------------------------------ choice of tokens
 SETTINGS = [dict(), dict(temperature=0.0), dict(top_k=1), dict(top_k=40), dict(top_p=0.9), dict(min_p=0.05),
             dict(temperature=0.7, top_k=50, top_p=0.9), dict(temperature=1.5, top_p=0.5, min_p=0.02),
