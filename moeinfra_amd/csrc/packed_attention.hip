@@ -127,7 +127,10 @@ __device__ __forceinline__ bool pk_item(const PkArgs &a, int rows, int w, int la
 }
 
 // Rows r0 .. r1 - 1 (at most 32) of a sequence without matrix products, a row at a time, a key per
-// lane: each row reads the V rows that it sees and no others.
+// lane: each row reads the V rows that it sees and no others.  This is slow (32 / 8 heads of 128: 9.5 ms for
+// the rows that an infinity meets at the end of 2048 tokens, 11 for all of them).  Rows whose own values
+// are all NaN need none of it, they are NaN whatever their weights are: a model that has come apart has
+// nothing else in its values (2048 tokens 76 us instead of 11 ms).
 template <int HD>
 __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride, const uint16_t *k, int64_t k_stride,
                                             const uint16_t *v, int64_t v_stride, int r0, int r1, int grp, int nq,
@@ -135,6 +138,13 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
   for (int r = r0; r < r1; ++r) {
     const int t = r / grp, g = r - t * grp;
     const uint16_t *qr = q + t * q_stride + (int64_t)g * HD;
+    uint16_t *dst = out + ((int64_t)t * nq + g) * HD;
+    bool all_nan = true;
+    for (int e = 0; e < HD / kWave; ++e) all_nan &= (v[t * v_stride + e * kWave + lane] & 0x7fffu) > 0x7f80u;
+    if (__all(all_nan)) {
+      for (int e = 0; e < HD / kWave; ++e) dst[e * kWave + lane] = 0x7fc0u;
+      continue;
+    }
     float m = -INFINITY, l = 0.0f, o[HD / kWave];
     for (int e = 0; e < HD / kWave; ++e) o[e] = 0.0f;
     for (int k0 = 0; k0 <= t; k0 += kWave) {
@@ -158,7 +168,6 @@ __device__ __noinline__ void pk_rows_scalar(const uint16_t *q, int64_t q_stride,
         for (int e = 0; e < HD / kWave; ++e) o[e] = fmaf(pi, bf16_to_f32(vr[e * kWave + lane]), o[e]);
       }
     }
-    uint16_t *dst = out + ((int64_t)t * nq + g) * HD;
     for (int e = 0; e < HD / kWave; ++e) dst[e * kWave + lane] = f32_to_bf16(l == 0.0f ? 0.0f : o[e] / l);
   }
 }

@@ -516,6 +516,29 @@ def test_packed_attention_infinities_of_last_tokens(cuda_device, lens, nq, nkv, 
             assert_within(o[a:b, h], want, tol, f"tokens {a} .. {b - 1}, head {h}")
 
 
+@pytest.mark.parametrize("lens,nq,nkv,hd", [([300], 4, 2, 64), ([300, 310], 4, 2, 128), ([130, 300, 70], 4, 2, 256),
+                                            ([130, 300, 70], 8, 2, 128)])
+def test_packed_attention_nan_values_from_a_token_on(cuda_device, lens, nq, nkv, hd):
+    """Values that are NaN from a token on, all of one head's (a model that has come apart): what sees
+    them is NaN, the tokens before and the other head are right."""
+    print(f"NaN from a token on, {lens} {nq}/{nkv} heads of {hd}", flush=True)
+    at = [min(100 + 7 * i, n - 1) for i, n in enumerate(lens)]
+
+    def spoil(q, k, v, cuts):
+        for a, b, i in zip(cuts, cuts[1:], at):
+            v[a + i:b, 1] = math.nan
+
+    out, q, k, v, cuts, s = _packed(cuda_device, lens, nq, nkv, hd, seed=hd, change=spoil)
+    o, grp = out.float().cpu(), nq // nkv
+    for a, b, i in zip(cuts, cuts[1:], at):
+        assert torch.isnan(o[a + i:b, grp:]).all()
+        for h in range(nq):
+            n = b - a if h < grp else i
+            want, tol = attention(q[a:a + n, h], k[a:a + n, h // grp], v[a:a + n, h // grp], s,
+                                  torch.ones((n, n), dtype=torch.bool).tril())
+            assert_within(o[a:a + n, h], want, tol, f"tokens {a} .. {a + n - 1}, head {h}")
+
+
 @pytest.mark.parametrize("n,nq,nkv,hd", [(300, 2, 1, 64), (500, 4, 4, 128), (200, 2, 1, 256)])
 def test_packed_attention_large_scores_of_long_rows(cuda_device, n, nq, nkv, hd):
     """Scores up to 3e38 in rows of two key groups, and of 256 dims, and an infinity in the last
