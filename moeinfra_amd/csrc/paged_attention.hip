@@ -105,7 +105,7 @@ __device__ __forceinline__ int pa_max(int v) {
 struct PaItem {
   int seq, n;          // sequence, its keys
   int tile0, tile1;    // this workgroup's tiles of it
-  int head, split, nact;  // workgroups head .. head + nact - 1 share it, this one is head + split
+  int head, nact;      // workgroups head .. head + nact - 1 share it
   bool inside;         // it starts inside workgroup head's tiles, not with them
 };
 
@@ -424,14 +424,12 @@ paged_attention_kernel(const PaArgs a) {
       w.tile0 = 0;
       w.tile1 = nt;
       w.nact = 1;
-      w.split = 0;
       w.head = 0;
       if (plan.per > 0 && nt > 0) {
         w.tile0 = max(begin - s0, 0);
         w.tile1 = min(end - s0, nt);
         w.head = s0 / plan.per;
         w.nact = (s0 + nt - 1) / plan.per - w.head + 1;
-        w.split = wg - w.head;
       }
       w.inside = plan.per > 0 && s0 - w.head * plan.per > 0;
       sequence(w, s0 > begin);
