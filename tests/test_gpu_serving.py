@@ -188,6 +188,26 @@ def test_paged_attention_without_workspace_and_reuse(cuda_device):
     assert not bool(ws[:65536].any())
 
 
+@pytest.mark.parametrize("nq,nkv,hd,lens", [
+    (32, 8, 128, [9000, 3, 0, 700, 5000]), (40, 2, 128, [6000, 900]), (33, 1, 128, [20000]), (8, 4, 256, [3000] * 5),
+    (8, 2, 64, [1 + 37 * i % 900 for i in range(200)] + [9000])])
+def test_paged_attention_stays_inside_its_workspace(cuda_device, nq, nkv, hd, lens):
+    """Sequences shared by workgroups write inside the workspace of the stated size only, and leave its
+    counters zero; the same call gives the same bits."""
+    from moeinfra_amd import ops
+
+    print(f"workspace of {nq}/{nkv} heads of {hd}, {len(lens)} sequences", flush=True)
+    n = ops.paged_attention_workspace(len(lens), nq, nkv, hd, cuda_device).numel()
+    guarded = torch.full((n + 8192,), 0x5a, dtype=torch.uint8, device=cuda_device)
+    ws = guarded[4096:4096 + n]
+    ws.zero_()
+    a, _ = _paged(cuda_device, lens, nq, nkv, hd, 16, seed=nq, workspace=ws)
+    assert bool((guarded[:4096] == 0x5a).all()) and bool((guarded[4096 + n:] == 0x5a).all())
+    assert not bool(ws[:65536].any())
+    b, _ = _paged(cuda_device, lens, nq, nkv, hd, 16, seed=nq, workspace=ws)
+    assert _same(a, b)
+
+
 def test_paged_attention_missing_pages_and_lengths(cuda_device):
     """Pages that the cache does not have weigh nothing; lengths clamp to the table."""
     from moeinfra_amd import ops
@@ -402,6 +422,23 @@ def test_packed_attention_256_rows(cuda_device, lens, nq, nkv):
     """Long sequences of enough heads that workgroups take 256 rows: of a token, a token's two heads, nine."""
     print(f"packed attention {lens} {nq}/{nkv} heads, 256 rows", flush=True)
     _check_packed(*_packed(cuda_device, lens, nq, nkv, 128, seed=nq + nkv, gap=2))
+
+
+@pytest.mark.parametrize("lens,nq,nkv", [([2100], 64, 16), ([4100], 32, 8)])
+def test_packed_attention_256_rows_of_groups_of_four(cuda_device, lens, nq, nkv):
+    """... and of four heads of 64 tokens; the same call gives the same bits."""
+    from moeinfra_amd import ops
+
+    print(f"packed attention {lens} {nq}/{nkv} heads, 256 rows", flush=True)
+    out, q, k, v, cuts, s = _packed(cuda_device, lens, nq, nkv, 128, seed=nq)
+    again = ops.packed_attention(*(t.to(cuda_device) for t in (q, k, v)),
+                                 torch.tensor(cuts, dtype=torch.int32, device=cuda_device))
+    assert _same(out, again)
+    n = lens[0]
+    seen = torch.ones((n, n), dtype=torch.bool).tril()
+    for h in (0, nq // 2 + 1, nq - 1):
+        want, tol = attention(q[:, h], k[:, h // 4], v[:, h // 4], s, seen)
+        assert_within(out[:, h], want, tol, f"head {h}")
 
 
 def test_packed_attention_256_rows_infinities(cuda_device):
@@ -835,6 +872,54 @@ def test_prompts_and_steps_together(cuda_device):
                 assert_within(sv.attn[i, h:h + 1], want, tol + slack * vs[i].double().abs().amax(), f"step {s}")
         assert sv.tok.cpu().tolist() == [sample(logits[i].float().cpu(), float(u[i]), temperature=0.9, top_k=100, top_p=0.95)
                                          for i in range(3)]
+
+
+def test_prompts_and_steps_by_what_passes_between_them(cuda_device):
+    """Prompts and steps as above, each operator's result against the 64-bit form of what it was given:
+    the rotated queries and keys that the call before it returned, and the cache's own rows."""
+    from moeinfra_amd import ops
+
+    dev, lens, steps = cuda_device, [37, 1, 130, 300], 3
+    sv = _Server(dev, lens, steps)
+    nq, nkv, hd, page = sv.nq, sv.nkv, sv.hd, sv.pool.page
+    qkv = _bf((sum(lens), (nq + 2 * nkv) * hd), 66).to(dev)
+    seq = torch.tensor([i for i, n in enumerate(lens) for _ in range(n)], dtype=torch.int32, device=dev)
+    pos = torch.tensor([p for n in lens for p in range(n)], dtype=torch.int32, device=dev)
+    cuts = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    q, k = ops.rope_paged_kv(qkv, pos, sv.pool.dev_table, sv.pool.k, sv.pool.v, nq, sv.inv, seq_ids=seq, want_k=True)
+    heads = qkv.cpu().view(-1, nq + 2 * nkv, hd)
+    y, tol = rope(heads[:, :nq + nkv], pos.cpu(), _inv(hd))
+    q = q.view(-1, nq, hd)
+    assert_within(q, y[:, :nq], tol[:, :nq], "q")
+    assert_within(k, y[:, nq:], tol[:, nq:], "k")
+    out = ops.packed_attention(q, k, qkv[:, (nq + nkv) * hd:].view(-1, nkv, hd),
+                               torch.tensor(cuts, dtype=torch.int32, device=dev))
+    _check_packed(out, q.cpu(), k.cpu(), heads[:, nq + nkv:], cuts, hd ** -0.5)
+
+    def cached(i, n):  # the first n rows of sequence i, from the cache
+        at = torch.arange(n)
+        p = sv.pool.table[i, at // page].long()
+        return sv.pool.k.cpu()[p, :, at % page], sv.pool.v.cpu()[p, :, at % page]
+
+    for i, n in enumerate(lens):
+        kc, vc = cached(i, n)
+        assert _same(kc, k[cuts[i]:cuts[i + 1]].cpu()) and _same(vc, heads[cuts[i]:cuts[i + 1], nq + nkv:])
+    g = torch.Generator().manual_seed(67)
+    for s in range(steps):
+        x = (torch.randn((len(lens), (nq + 2 * nkv) * hd), generator=g)).to(torch.bfloat16)
+        at = torch.tensor([n + s for n in lens], dtype=torch.int32)
+        q, _ = ops.rope_paged_kv(x.to(dev), at.to(dev), sv.pool.dev_table, sv.pool.k, sv.pool.v, nq, sv.inv)
+        q = q.view(-1, nq, hd)
+        y, tol = rope(x.view(len(lens), -1, hd)[:, :nq + nkv], at, _inv(hd))
+        assert_within(q, y[:, :nq], tol[:, :nq], f"step {s}, q")
+        both = [cached(i, n + s + 1) for i, n in enumerate(lens)]
+        for i, (kc, vc) in enumerate(both):
+            assert_within(kc[-1], y[i, nq:], tol[i, nq:], f"step {s}, k")
+            assert _same(vc[-1], x[i].view(-1, hd)[nq + nkv:])
+        out = ops.paged_attention(q, sv.pool.k, sv.pool.v, sv.pool.dev_table, (at + 1).to(dev), workspace=sv.ws)
+        _check_paged(out, q.cpu(), [kc for kc, _ in both], [vc for _, vc in both], nkv, hd ** -0.5)
+        logits, u = (out.view(len(lens), -1) @ sv.head).float(), torch.rand((len(lens),), generator=g)
+        _sampled(dev, logits.cpu(), u, temperature=0.9, top_k=100, top_p=0.95)
 
 
 def test_steps_replayed_from_a_graph(cuda_device):

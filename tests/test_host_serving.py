@@ -144,6 +144,21 @@ def test_paged_attention_workspace_grows_with_the_batch():
     assert f(-1, 32, 8, 128) == -1 and f(1, 32, 8, 96) == -1 and f(1, 9, 2, 128) == -1
 
 
+@pytest.mark.parametrize("nq,nkv,hd", [(32, 8, 128), (8, 2, 64), (40, 2, 128), (33, 1, 128), (8, 4, 256), (4, 4, 128),
+                                       (1 << 16, 1, 256)])
+def test_paged_attention_workspace_is_one_size_for_all_batches(nq, nkv, hd):
+    """One size for every batch (a workspace made for one serves any other of the same heads): the
+    counters, and two places of a partial result for each workgroup that runs at once."""
+    f = _lib.lib().moe_paged_attention_workspace_bytes
+    sizes = {f(b, nq, nkv, hd) for b in (0, 1, 7, 64, 256, 5000, 1 << 20)}
+    assert len(sizes) == 1
+    grp = nq // nkv
+    place = min(grp, 16) * (hd + 2) * 4
+    units = nkv * -(-grp // 16)
+    places, rest = divmod(sizes.pop() - 65536, place)
+    assert rest == 0 and places % (2 * units) == 0 and places >= 2 * units
+
+
 def test_wrappers_take_gpu_tensors_only():
     bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
     i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
