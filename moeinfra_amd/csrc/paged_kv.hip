@@ -29,9 +29,10 @@ __device__ __forceinline__ void rope_angle(int pos, float f, float &c, float &s)
 // and stores.  A negative position is padding: nothing of the token is written.  A token whose
 // sequence, page index or page is out of range is rotated but not cached.
 //
-// Bound: HBM (8192 tokens of 32 / 8 heads of 128, k also in token order: 218 MB in 33.5 us, 6.5 TB/s;
-// a copy of 2 GiB moves 4.9), a launch for few tokens (8: 4.2 us, 256: 4.4).  A workgroup per token
-// as its angles (64-bit products, 64 of them) serve all of its heads.
+// Bound: HBM (8192 tokens of 32 / 8 heads of 128, k also in token order: 218 MB in 43 us where the tensors
+// are others in each call, 5.1 TB/s, the rate of a copy; 34 us on the same ones again, which the device's
+// last cache holds in part), a launch for few tokens (8: 4.3 us, 256: 4.4).  A workgroup per token as its
+// angles (64-bit products, 64 of them) serve all of its heads.
 __global__ void __launch_bounds__(kPkvThreads)
 rope_paged_kv_kernel(const uint16_t *__restrict__ qkv, int64_t qkv_stride, int nq, int nkv, int hd,
                      const float *__restrict__ inv_freq, const int32_t *__restrict__ positions,
