@@ -402,6 +402,15 @@ def test_packed_attention_large_batches(cuda_device, count, nq, nkv, hd):
     assert _same(out, want)
 
 
+@pytest.mark.parametrize("count", [40, 3000])
+def test_packed_attention_mostly_empty_batches(cuda_device, count):
+    """More sequences than tokens."""
+    print(f"packed attention of {count} sequences, most of them empty", flush=True)
+    lens = [0] * count
+    lens[0], lens[count // 2], lens[count - 3] = 1, 5, 20
+    _check_packed(*_packed(cuda_device, lens, 8, 2, 128, seed=count, gap=1))
+
+
 def test_packed_attention_wide_workgroups(cuda_device):
     # Enough rows for the 8-wave workgroups: 32 heads, 64 and 128 dims.
     for hd in (64, 128):
