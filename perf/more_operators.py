@@ -439,7 +439,7 @@ def _plain_fork(st):
     held = refs + count(new) - count(table)
     # Places that the next token is written to, row by row.
     first = (new_lens // P)[:, None]
-    writes = (entry >= first) & (entry < keep_to)
+    writes = real[:, None] & (entry >= first) & (entry < keep_to)
     rows, cols = torch.nonzero(writes, as_tuple=True)
     page = new[rows, cols]
     order = torch.arange(rows.numel(), device=DEV)
@@ -608,7 +608,7 @@ def _exact_fork(st):
             for p in row:
                 if p >= 0:
                     refs[p] += by
-    wants = [(i, n // P) for i, n in enumerate(new_lens) if n // P < width]
+    wants = [(i, n // P) for i, n in enumerate(new_lens) if 0 <= parents[i] < len(old) and n // P < width]
     by_page = {}
     for w in wants:
         by_page.setdefault(new[w[0]][w[1]], []).append(w)
