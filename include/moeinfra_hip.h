@@ -401,6 +401,113 @@ int moe_sample_tokens(const void *logits, int32_t logits_f32, int64_t stride, in
                       const void *top_k_i32, int32_t top_k, const void *top_p_f32, float top_p,
                       const void *min_p_f32, float min_p, void *token_i64, void *stream);
 
+/* ---------------------------------------------------------------- decoding that branches
+ * Several continuations of a sequence at once over the paged cache: trees of drafted tokens that one
+ * pass of the model checks, and beams.
+ *
+ * A tree: sequence b's drafted tokens are nodes 0 .. n - 1, rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1
+ * of the batch (int32 [B + 1], not decreasing, inside [0, T]), at most 64, parents before their
+ * children; node 0 is the root (the last token that is certain).  masks (int64 [T], bit patterns):
+ * bit j of a node's mask says that it sees node j: itself and the nodes that it descends from.  Null:
+ * a chain, each node sees all up to itself.  Their keys and values lie behind the lens[b] keys of the
+ * sequence, node i at place lens[b] + i.
+ *
+ * moe_rope_paged_kv_slots_bf16: moe_rope_paged_kv_bf16 where token t's place in its sequence is
+ * slots[t] (int32) while its angle is positions[t]'s: a node's place is lens + i, its position
+ * lens + its depth.  A negative slot: rotated, not cached. */
+int moe_rope_paged_kv_slots_bf16(const void *qkv, int64_t qkv_stride, int64_t T, int32_t n_q_heads,
+                                 int32_t n_kv_heads, int32_t head_dim, const void *inv_freq_f32,
+                                 const void *positions_i32, const void *slots_i32,
+                                 const void *seq_ids_i32, const void *page_table_i32, int64_t n_seqs,
+                                 int64_t table_width, int64_t num_pages, int32_t page_size,
+                                 int64_t page_stride, void *q_out, void *k_out, void *k_cache,
+                                 void *v_cache, void *stream);
+
+/* moe_paged_tree_attention_bf16: q [T, n_q, head_dim] (rows q_stride values apart) of the nodes of B
+ * trees against the keys before them and those of their tree that their masks name; bits past a tree's
+ * nodes mean nothing.  Otherwise as moe_paged_attention_bf16: fp32 scores and softmax, the weights
+ * rounded to bf16 before their sum (fp32) with v; keys of pages that the cache does not have weigh
+ * nothing; what a node does not see (an infinity or NaN too) does not change its row; a row that sees
+ * no key is zeros.  Rows of no sequence, and of nodes past the 64th, are left as they were.  out
+ * [T, n_q * head_dim], 8-byte aligned.  The workspace (moe_paged_tree_attention_workspace_bytes) is one
+ * of its own, with the same rules as moe_paged_attention_bf16's. */
+int64_t moe_paged_tree_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
+                                                 int32_t head_dim);
+int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, int64_t T, const void *k_cache,
+                                  const void *v_cache, int64_t num_pages, int32_t page_size,
+                                  int64_t page_stride, const void *page_table_i32,
+                                  int64_t table_width, const void *lens_i32,
+                                  const void *cu_seqlens_i32, const void *masks_i64, int64_t B,
+                                  int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                  float scaling, void *out, void *workspace,
+                                  int64_t workspace_bytes, void *stream);
+
+/* moe_accept_drafts: which nodes the model itself would have chosen.  targets[t] (int64) is its choice
+ * after node t, drafts[t] the node's token.  A node's parent is the last node before it in its mask.
+ * The root is accepted; a node is if its parent is and its token is the choice after the parent (one
+ * without a parent is not).  Of the accepted nodes that most others lie above, the first ends the path:
+ * paths[b] (int64) has the bits of its nodes, counts[b] (int32) their number, tokens[b] (int64) is the
+ * choice after the last.  A sequence without nodes: 0, 0, -1. */
+int moe_accept_drafts(const void *targets_i64, const void *drafts_i64, const void *masks_i64,
+                      const void *cu_seqlens_i32, int64_t T, int64_t B, void *paths_i64,
+                      void *counts_i32, void *tokens_i64, void *stream);
+
+/* moe_compact_paged_kv_bf16: what the paths keep, one behind the other: of the set bits s_0 < s_1 < ..
+ * of paths[b], the keys and values at place lens[b] + s_j of sequence b go to place lens[b] + j, in all
+ * layers, as if all were read before any is written.  The caches are [layers][num_pages] pages with
+ * layer_stride values from layer to layer (a multiple of 8; the layers of a page may also lie next to
+ * each other), n_kv * page_size * head_dim values a page, head_dim a multiple of 8 up to 512.  A place
+ * whose page the table or the cache does not have is neither read nor written.  Places written to are
+ * those of one sequence only. */
+int moe_compact_paged_kv_bf16(void *k_cache, void *v_cache, int64_t layers, int64_t layer_stride,
+                              int64_t num_pages, int32_t page_size, int64_t page_stride,
+                              int32_t n_kv_heads, int32_t head_dim, const void *page_table_i32,
+                              int64_t n_seqs, int64_t table_width, const void *lens_i32,
+                              const void *paths_i64, void *stream);
+
+/* moe_beam_select: the k best continuations of each of S searches of W beams: of all beams w and tokens
+ * v those of the largest score[w] + log softmax(x[w])[v], x [S * W, V] (bf16, or fp32 with logits_f32 =
+ * 1; rows `stride` values apart, V up to 2^20), scores fp32 [S, W].  Sums over the vocabulary are of
+ * 64 bits.  Inside a beam the larger logit goes first, of equal ones the lower token; between beams the
+ * larger total, of equal ones the lower beam.  best (fp32 [S, k]) are the totals, rows (int32 [S, k])
+ * the rows s * W + w of x, tokens (int64 [S, k]) the tokens.  Logits of -inf and NaN are never chosen, a
+ * score of -inf (or NaN, or +inf) means no beam, and a beam whose logits hold +inf has no
+ * probabilities: it is none either.  What there is too little for is -inf, -1, -1.  S up to
+ * 16384, W up to 256, k up to 64.  The workspace (moe_beam_select_workspace_bytes, enough for any
+ * smaller call too; 16-byte aligned) has the same rules as moe_paged_attention_bf16's, but there must be
+ * one. */
+int64_t moe_beam_select_workspace_bytes(int64_t S, int64_t W, int32_t k);
+int moe_beam_select(const void *logits, int32_t logits_f32, int64_t stride, int64_t S, int64_t W,
+                    int64_t V, const void *scores_f32, int32_t k, void *best_f32, void *rows_i32,
+                    void *tokens_i64, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* moe_fork_pages: the rows of a page table as the next step finds them.  New row i (of n_new) goes on
+ * from row parents[i] (int32): it has that row's length, and its pages as far as the length and the
+ * `ahead` positions behind it reach (-1 behind them); a parent outside [0, n_seqs) makes it an empty row
+ * without pages.  refs (int32 [num_pages], in place) counts the rows that hold a page (and other
+ * holders, such as a kept prompt): old rows let go of theirs, new ones take theirs.  The places of the
+ * `ahead` positions are a row's alone: a page there that only such places hold stays with the first of
+ * them, row by row; every other place gets the lowest page whose count is not above zero, in the same
+ * order, and where it held one that the length reaches into, copies[i] (int32 [n_new, 3]) says {that
+ * page, the new one, positions to copy}, else {-1, -1, 0}.  A place for which no page is left is -1, and
+ * missing[0] (int32) counts them.  Places past the table's width are none.  Up to 8192 rows and 8192
+ * places.  The workspace (moe_fork_pages_workspace_bytes) is zero before the first call, every call
+ * leaves it zero; calls that share it must be ordered. */
+int64_t moe_fork_pages_workspace_bytes(int64_t num_pages);
+int moe_fork_pages(const void *page_table_i32, const void *lens_i32, int64_t n_seqs,
+                   int64_t table_width, const void *parents_i32, int64_t n_new, void *refs_i32,
+                   int64_t num_pages, int32_t page_size, int32_t ahead, void *new_table_i32,
+                   void *new_lens_i32, void *copies_i32, void *missing_i32, void *workspace,
+                   int64_t workspace_bytes, void *stream);
+
+/* moe_copy_pages_bf16: the first copies[i][2] rows of page copies[i][0] to page copies[i][1] (int32
+ * [n_copies, 3]), keys and values, all heads and layers (as moe_compact_paged_kv_bf16's).  A pair with
+ * a page that the cache does not have is none.  No page that is written to may be another pair's. */
+int moe_copy_pages_bf16(void *k_cache, void *v_cache, int64_t layers, int64_t layer_stride,
+                        int64_t num_pages, int32_t page_size, int64_t page_stride,
+                        int32_t n_kv_heads, int32_t head_dim, const void *copies_i32,
+                        int64_t n_copies, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

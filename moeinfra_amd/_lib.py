@@ -93,6 +93,20 @@ SIGNATURES = {
                                    ctypes.c_float, _vp, _vp], ctypes.c_int),
     "moe_sample_tokens": ([_vp, _i32, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _vp, _i32, _vp, ctypes.c_float,
                            _vp, ctypes.c_float, _vp, _vp], ctypes.c_int),
+    "moe_rope_paged_kv_slots_bf16": ([_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                                      _i32, _i64, _vp, _vp, _vp, _vp, _vp], ctypes.c_int),
+    "moe_paged_tree_attention_workspace_bytes": ([_i64, _i32, _i32, _i32], _i64),
+    "moe_paged_tree_attention_bf16": ([_vp, _i64, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _i64,
+                                       _i32, _i32, _i32, ctypes.c_float, _vp, _vp, _i64, _vp], ctypes.c_int),
+    "moe_accept_drafts": ([_vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp], ctypes.c_int),
+    "moe_compact_paged_kv_bf16": ([_vp, _vp, _i64, _i64, _i64, _i32, _i64, _i32, _i32, _vp, _i64, _i64, _vp, _vp,
+                                   _vp], ctypes.c_int),
+    "moe_beam_select_workspace_bytes": ([_i64, _i64, _i32], _i64),
+    "moe_beam_select": ([_vp, _i32, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _vp], ctypes.c_int),
+    "moe_fork_pages_workspace_bytes": ([_i64], _i64),
+    "moe_fork_pages": ([_vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+                       ctypes.c_int),
+    "moe_copy_pages_bf16": ([_vp, _vp, _i64, _i64, _i64, _i32, _i64, _i32, _i32, _vp, _i64, _vp], ctypes.c_int),
 }
 
 _lock = threading.Lock()

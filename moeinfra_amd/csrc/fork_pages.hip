@@ -1,0 +1,199 @@
+// Page table rows of a paged cache taken over by the sequences that continue: beams reordered, forked
+// and dropped.  A page is held by as many as its count says; a row that goes on holds its parent's pages,
+// and the places that it writes to next get pages that no other holds.
+#include "common.h"
+
+namespace moe {
+namespace {
+
+constexpr int kFpThreads = 1024;
+constexpr int kFpWaves = kFpThreads / kWave;
+constexpr int kFpRows = 8192;    // rows, and places that are written to next, of a call
+
+struct FpArgs {
+  const int32_t *table, *lens, *parents;
+  int32_t *refs, *new_table, *new_lens, *copies, *missing;
+  int64_t width, pages;
+  int old_rows, rows, page_shift, ahead, places;  // places: of a row at most
+  int32_t *writers, *lowest;                       // per page, zero between calls
+};
+
+// Sum over the threads before this one, and over all of them.
+__device__ __forceinline__ int fp_scan(int v, int *s_sum, int &all) {
+  const int lane = threadIdx.x & (kWave - 1), wave = (int)threadIdx.x >> 6;
+  int incl = v;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int x = __shfl_up(incl, d, kWave);
+    incl += lane >= d ? x : 0;
+  }
+  if (lane == kWave - 1) s_sum[wave] = incl;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kFpWaves; ++w) {
+    before += w < wave ? s_sum[w] : 0;
+    all += s_sum[w];
+  }
+  __syncthreads();
+  return before + incl - v;
+}
+
+// Counts change by atomics and are read past the first cache.
+__device__ __forceinline__ int fp_read(const int32_t *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void fp_add(int32_t *p, int v) {
+  __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// One workgroup, as each step needs all of the one before.
+__global__ void __launch_bounds__(kFpThreads)
+fork_pages_kernel(const FpArgs a) {
+  __shared__ int s_children[kFpRows], s_free[kFpRows], s_rank[kFpRows], s_sum[kFpWaves];
+  const int tid = threadIdx.x;
+  const int P = 1 << a.page_shift;
+  auto len_of = [&](int row) { return max(a.lens[row], 0); };
+  // Entries of a row of n positions from now on.
+  auto kept = [&](int n) { return min(((int64_t)n + a.ahead + P - 1) >> a.page_shift, a.width); };
+  auto parent_of = [&](int i) {
+    const int p = a.parents[i];
+    return p >= 0 && p < a.old_rows ? p : -1;
+  };
+  auto good = [&](int page) { return page >= 0 && page < a.pages; };
+  for (int i = tid; i < a.old_rows; i += kFpThreads) s_children[i] = 0;
+  __syncthreads();
+  for (int i = tid; i < a.rows; i += kFpThreads) {
+    const int p = parent_of(i);
+    if (p >= 0) atomicAdd(&s_children[p], 1);
+    a.new_lens[i] = p >= 0 ? len_of(p) : 0;
+    a.copies[3 * i] = a.copies[3 * i + 1] = -1;
+    a.copies[3 * i + 2] = 0;
+  }
+  __syncthreads();
+  // Each old row lets its pages go, each new one takes those that it keeps.
+  for (int64_t x = tid; x < a.old_rows * a.width; x += kFpThreads) {
+    const int row = (int)(x / a.width), e = (int)(x - row * a.width), page = a.table[x];
+    const int by = (e < kept(len_of(row)) ? s_children[row] : 0) - 1;
+    if (good(page) && by != 0) fp_add(a.refs + page, by);
+  }
+  for (int64_t x = tid; x < a.rows * a.width; x += kFpThreads) {
+    const int row = (int)(x / a.width), e = (int)(x - row * a.width), p = parent_of(row);
+    a.new_table[x] = p >= 0 && e < kept(len_of(p)) ? a.table[p * a.width + e] : -1;
+  }
+  __syncthreads();
+  // Place i: entry len / P + i % places of row i / places, written to next.
+  const int n = a.rows * a.places;
+  auto place = [&](int i, int &row, int &e, int &page) {
+    row = i / a.places;
+    const int p = parent_of(row);
+    if (p < 0) return false;
+    const int len = len_of(p);
+    e = (len >> a.page_shift) + i - row * a.places;
+    if (e >= kept(len)) return false;
+    page = a.table[p * a.width + e];
+    return true;
+  };
+  int row, e, page;
+  for (int i = tid; i < n; i += kFpThreads)
+    if (place(i, row, e, page) && good(page)) {
+      fp_add(a.writers + page, 1);
+      __hip_atomic_fetch_max(a.lowest + page, n - i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  __syncthreads();
+  // A page that only writers hold stays with the first of them; the others want one.
+  int wanted = 0;
+  for (int i0 = 0; i0 < n; i0 += kFpThreads) {
+    const int i = i0 + tid;
+    bool wants = false;
+    if (i < n && place(i, row, e, page))
+      wants = !(good(page) && fp_read(a.refs + page) == fp_read(a.writers + page) && fp_read(a.lowest + page) == n - i);
+    int all;
+    const int rank = wanted + fp_scan(wants, s_sum, all);
+    if (i < n) s_rank[i] = wants ? rank : -1;
+    wanted += all;
+  }
+  int found = 0;
+  for (int64_t p0 = 0; p0 < a.pages && found < wanted; p0 += kFpThreads) {
+    const bool is = p0 + tid < a.pages && fp_read(a.refs + p0 + tid) <= 0;
+    int all;
+    const int rank = found + fp_scan(is, s_sum, all);
+    if (is && rank < wanted) s_free[rank] = (int)(p0 + tid);
+    found += all;
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kFpThreads)
+    if (place(i, row, e, page) && good(page)) {
+      a.writers[page] = 0;
+      a.lowest[page] = 0;
+      if (s_rank[i] >= 0) fp_add(a.refs + page, -1);
+    }
+  __syncthreads();
+  for (int i = tid; i < n; i += kFpThreads) {
+    const int rank = s_rank[i];
+    if (rank < 0 || !place(i, row, e, page)) continue;
+    const int fresh = rank < found ? s_free[rank] : -1;
+    a.new_table[row * a.width + e] = fresh;
+    if (fresh < 0) continue;
+    __hip_atomic_store(a.refs + fresh, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int used = len_of(parent_of(row)) & (P - 1);
+    if (good(page) && used > 0 && i == row * a.places) {
+      a.copies[3 * row] = page;
+      a.copies[3 * row + 1] = fresh;
+      a.copies[3 * row + 2] = used;
+    }
+  }
+  if (tid == 0) *a.missing = max(wanted - found, 0);
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int64_t moe_fork_pages_workspace_bytes(int64_t num_pages) {
+  return num_pages < 0 || num_pages > 0x7fffffff ? -1 : 8 * (num_pages > 0 ? num_pages : 1);
+}
+
+extern "C" int moe_fork_pages(const void *page_table_i32, const void *lens_i32, int64_t n_seqs, int64_t table_width,
+                              const void *parents_i32, int64_t n_new, void *refs_i32, int64_t num_pages,
+                              int32_t page_size, int32_t ahead, void *new_table_i32, void *new_lens_i32,
+                              void *copies_i32, void *missing_i32, void *workspace, int64_t workspace_bytes,
+                              void *stream) {
+  MOE_REQUIRE(page_size >= 8 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
+              "page size must be a power of two of 8 to 4096 (got %d)", page_size);
+  MOE_REQUIRE(n_seqs >= 0 && n_seqs <= moe::kFpRows && n_new >= 0 && n_new <= moe::kFpRows,
+              "at most %d rows (got %lld, %lld)", moe::kFpRows, (long long)n_seqs, (long long)n_new);
+  MOE_REQUIRE(table_width >= 0 && table_width <= 0x7fffffff / page_size && num_pages >= 0 && num_pages <= 0x7fffffff,
+              "bad sizes");
+  MOE_REQUIRE(ahead >= 1 && ahead <= (1 << 20), "the next tokens of a row must be 1 to 2^20 (got %d)", ahead);
+  const int places = (page_size - 1 + ahead + page_size - 1) / page_size;
+  MOE_REQUIRE(n_new * places <= moe::kFpRows, "at most %d pages to be written to (got %lld rows of %d)", moe::kFpRows,
+              (long long)n_new, places);
+  MOE_REQUIRE(missing_i32 && (n_new == 0 || (parents_i32 && new_lens_i32 && copies_i32)) && (n_seqs == 0 || lens_i32) &&
+                  (table_width == 0 || ((n_seqs == 0 || page_table_i32) && (n_new == 0 || new_table_i32))) &&
+                  (num_pages == 0 || refs_i32),
+              "null pointer");
+  const int64_t need = moe_fork_pages_workspace_bytes(num_pages);
+  MOE_REQUIRE(workspace != nullptr && workspace_bytes >= need, "workspace too small: need %lld bytes, got %lld",
+              (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  MOE_REQUIRE(((uintptr_t)page_table_i32 | (uintptr_t)lens_i32 | (uintptr_t)parents_i32 | (uintptr_t)refs_i32 |
+               (uintptr_t)new_table_i32 | (uintptr_t)new_lens_i32 | (uintptr_t)copies_i32 | (uintptr_t)missing_i32 |
+               (uintptr_t)workspace) % 4 == 0,
+              "tensors must be aligned");
+  const void *p[9] = {new_table_i32, new_lens_i32, copies_i32, missing_i32, refs_i32, workspace, page_table_i32, lens_i32,
+                      parents_i32};
+  const int64_t size[9] = {4 * n_new * table_width, 4 * n_new, 12 * n_new, 4, 4 * num_pages, need,
+                           4 * n_seqs * table_width, 4 * n_seqs, 4 * n_new};
+  for (int i = 0; i < 6; ++i)
+    for (int j = i + 1; j < 9; ++j)
+      MOE_REQUIRE(!moe::ranges_overlap(p[i], size[i], p[j], size[j]),
+                  "what is written must not overlap what is read or written elsewhere");
+  moe::FpArgs a{(const int32_t *)page_table_i32, (const int32_t *)lens_i32, (const int32_t *)parents_i32,
+                (int32_t *)refs_i32, (int32_t *)new_table_i32, (int32_t *)new_lens_i32, (int32_t *)copies_i32,
+                (int32_t *)missing_i32, table_width, num_pages, (int)n_seqs, (int)n_new,
+                __builtin_ctz((unsigned)page_size), ahead, places, (int32_t *)workspace,
+                (int32_t *)workspace + num_pages};
+  hipLaunchKernelGGL(moe::fork_pages_kernel, dim3(1), dim3(moe::kFpThreads), 0, (hipStream_t)stream, a);
+  MOE_LAUNCH_CHECK();
+  return MOE_STATUS_OK;
+}

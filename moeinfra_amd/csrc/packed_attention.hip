@@ -8,7 +8,7 @@
 // product (half a step, 2^-8 of a weight), their sum is not.
 #include <type_traits>
 
-#include "common.h"
+#include "attention_tile.h"
 
 namespace moe {
 namespace {
@@ -20,8 +20,6 @@ constexpr float kPkLog2e = 1.44269504088896341f;
 constexpr float kPkLag = 8.0f;
 constexpr float kPkHuge = 268435456.0f;  // 2^28: half a step of m is 2^3
 constexpr int kPkFew = 32;               // sequences, to which the search goes by keys (pk_item)
-typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 struct PkArgs {
   const uint16_t *q, *k, *v;
@@ -32,25 +30,6 @@ struct PkArgs {
   float scaling;
   uint16_t *out;
 };
-
-// Swizzles: 16-byte piece p of K row r lies at p ^ pk_kx(r), so that the 32 rows that a read of one
-// piece touches spread over all banks; piece p of V row r at p ^ pk_vx(r), so that four keys' 64
-// bytes (a transposing read) do.
-template <int HD>
-__device__ __forceinline__ uint32_t pk_kx(uint32_t r) {
-  return HD == 64 ? (r >> 1) & 7 : r & 15;
-}
-template <int HD>
-__device__ __forceinline__ uint32_t pk_vx(uint32_t r) {
-  return HD == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2;
-}
-
-// Four bf16 values of one column from four rows: lane i of 16 reads 8 bytes of row i / 4 and gets
-// column i of the four rows' 16 columns.
-__device__ __forceinline__ uint2 pk_read_tr(const uint8_t *p) {
-  const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
-  return __builtin_bit_cast(uint2, v);
-}
 
 // 64 lanes' 16 bytes each from memory into LDS at dst + 16 * lane, without registers.  (In asm, as
 // the compiler would wait for all of them before the next transposing read of the other plane; the

@@ -7,7 +7,7 @@
 // bf16 as an operand of the second product (half a step, 2^-8 of a weight), their sum is not.
 #include <type_traits>
 
-#include "common.h"
+#include "attention_tile.h"
 
 namespace moe {
 namespace {
@@ -26,33 +26,6 @@ constexpr int kPaStart = 4;           // tiles' time that beginning a sequence t
 constexpr int64_t kPaCounterBytes = 65536;  // arrival counters at the start of the workspace
 constexpr float kPaLog2e = 1.44269504088896341f;
 
-// Partial results pass between workgroups (of other XCDs) through device-scope accesses, two
-// floats at a time.
-__device__ __forceinline__ void pa_put(float *p, float x, float y) {
-  __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint32_t, x) | (uint64_t)__builtin_bit_cast(uint32_t, y) << 32,
-                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 pa_get(const float *p) {
-  const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32)));
-}
-
-// Whether this workgroup is the last of n to arrive at *count, which it then leaves zero.  What
-// the others wrote with pa_put is there for its pa_get (their stores have completed before they
-// count themselves in).  Nothing here waits for another workgroup.
-__device__ __forceinline__ bool pa_last_of(uint32_t *count, int n) {
-  __shared__ uint32_t s_seen;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const uint32_t seen = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-    if (seen == (uint32_t)n) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_seen = seen;
-  }
-  __syncthreads();
-  return s_seen == (uint32_t)n;
-}
-
 struct PaArgs {
   const uint16_t *q;
   int64_t q_stride;
@@ -69,29 +42,6 @@ struct PaArgs {
   float *part;
   int share;  // workgroups per head group that a batch is shared by (0: a sequence each)
 };
-
-// Inclusive sum and maximum (of values of 0 and above) over the wave: row_shr 1, 2, 4, 8 within 16
-// lanes, then lane 15 and lane 31 broadcast to what follows.  The last lane's are the wave's.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int pa_dpp(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int pa_incl(int v) {
-  v += pa_dpp<0x111, 0xf>(v);
-  v += pa_dpp<0x112, 0xf>(v);
-  v += pa_dpp<0x114, 0xf>(v);
-  v += pa_dpp<0x118, 0xf>(v);
-  v += pa_dpp<0x142, 0xa>(v);
-  return v + pa_dpp<0x143, 0xc>(v);
-}
-__device__ __forceinline__ int pa_max(int v) {
-  v = max(v, pa_dpp<0x111, 0xf>(v));
-  v = max(v, pa_dpp<0x112, 0xf>(v));
-  v = max(v, pa_dpp<0x114, 0xf>(v));
-  v = max(v, pa_dpp<0x118, 0xf>(v));
-  v = max(v, pa_dpp<0x142, 0xa>(v));
-  return max(v, pa_dpp<0x143, 0xc>(v));
-}
 
 // What the workgroups of a head group share, by the lengths, which are known on the device only (each
 // wave adds them up for itself):

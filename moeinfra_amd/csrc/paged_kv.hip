@@ -4,7 +4,9 @@
 //
 //   y_i = x_i cos(p f_i) - x_{i+hd/2} sin(p f_i),  y_{i+hd/2} = x_{i+hd/2} cos(p f_i) + x_i sin(p f_i)
 //
-// for position p and frequency f_i, rounded to bf16 once.
+// for position p and frequency f_i, rounded to bf16 once.  A token's place in its sequence is its
+// position, or a slot of its own (the tokens of a drafted tree lie one behind the other, several of
+// them at one position).
 #include <initializer_list>
 
 #include "common.h"
@@ -27,7 +29,7 @@ __device__ __forceinline__ void rope_angle(int pos, float f, float &c, float &s)
 // One workgroup per token.  Its angles are evaluated once, into LDS; then a thread takes 8
 // values of the first half of a q or k head with the matching 8 of the second, 16-byte loads
 // and stores.  A negative position is padding: nothing of the token is written.  A token whose
-// sequence, page index or page is out of range is rotated but not cached.
+// slot, sequence, page index or page is out of range is rotated but not cached.
 //
 // Bound: HBM (8192 tokens of 32 / 8 heads of 128, k also in token order: 218 MB in 43 us where the tensors
 // are others in each call, 5.1 TB/s, the rate of a copy; 34 us on the same ones again, which the device's
@@ -36,24 +38,26 @@ __device__ __forceinline__ void rope_angle(int pos, float f, float &c, float &s)
 __global__ void __launch_bounds__(kPkvThreads)
 rope_paged_kv_kernel(const uint16_t *__restrict__ qkv, int64_t qkv_stride, int nq, int nkv, int hd,
                      const float *__restrict__ inv_freq, const int32_t *__restrict__ positions,
-                     const int32_t *__restrict__ seq_ids, const int32_t *__restrict__ table,
-                     int64_t n_seqs, int64_t width, int64_t num_pages, int page_shift,
-                     int64_t page_stride, uint16_t *__restrict__ q_out, uint16_t *__restrict__ k_out,
+                     const int32_t *__restrict__ slots, const int32_t *__restrict__ seq_ids,
+                     const int32_t *__restrict__ table, int64_t n_seqs, int64_t width, int64_t num_pages,
+                     int page_shift, int64_t page_stride, uint16_t *__restrict__ q_out, uint16_t *__restrict__ k_out,
                      uint16_t *__restrict__ kc, uint16_t *__restrict__ vc) {
   __shared__ float s_cos[kPkvMaxHalf], s_sin[kPkvMaxHalf];
   const int64_t t = blockIdx.x;
   const int pos = positions[t];
   if (pos < 0) return;
+  const int slot = slots != nullptr ? slots[t] : pos;
   const int64_t seq = seq_ids != nullptr ? seq_ids[t] : t;
   int64_t page = -1;
-  if (seq >= 0 && seq < n_seqs && (pos >> page_shift) < width) page = table[seq * width + (pos >> page_shift)];
+  if (slot >= 0 && seq >= 0 && seq < n_seqs && (slot >> page_shift) < width)
+    page = table[seq * width + (slot >> page_shift)];
   const bool cached = page >= 0 && page < num_pages;
   const int half = hd >> 1;
   for (int i = threadIdx.x; i < half; i += kPkvThreads) rope_angle(pos, inv_freq[i], s_cos[i], s_sin[i]);
   __syncthreads();
   const uint16_t *src = qkv + t * qkv_stride;
   // Row of head 0 in the page; a head's rows are 2^page_shift rows further on.
-  const int64_t at = cached ? page * page_stride + (int64_t)(pos & ((1 << page_shift) - 1)) * hd : 0;
+  const int64_t at = cached ? page * page_stride + (int64_t)(slot & ((1 << page_shift) - 1)) * hd : 0;
   const int64_t head_stride = (int64_t)hd << page_shift;
   const int cph = half >> 3;  // 8-value pieces per half head
   for (int idx = threadIdx.x; idx < (nq + nkv) * cph; idx += kPkvThreads) {
@@ -99,16 +103,11 @@ rope_paged_kv_kernel(const uint16_t *__restrict__ qkv, int64_t qkv_stride, int n
   }
 }
 
-}  // namespace
-}  // namespace moe
-
-extern "C" int moe_rope_paged_kv_bf16(const void *qkv, int64_t qkv_stride, int64_t T, int32_t n_q_heads,
-                                      int32_t n_kv_heads, int32_t head_dim, const void *inv_freq_f32,
-                                      const void *positions_i32, const void *seq_ids_i32,
-                                      const void *page_table_i32, int64_t n_seqs, int64_t table_width,
-                                      int64_t num_pages, int32_t page_size, int64_t page_stride,
-                                      void *q_out, void *k_out, void *k_cache, void *v_cache,
-                                      void *stream) {
+int rope_paged_kv(const void *qkv, int64_t qkv_stride, int64_t T, int32_t n_q_heads, int32_t n_kv_heads,
+                  int32_t head_dim, const void *inv_freq_f32, const void *positions_i32, const void *slots_i32,
+                  const void *seq_ids_i32, const void *page_table_i32, int64_t n_seqs, int64_t table_width,
+                  int64_t num_pages, int32_t page_size, int64_t page_stride, void *q_out, void *k_out, void *k_cache,
+                  void *v_cache, void *stream) {
   MOE_REQUIRE(T >= 0 && moe::launch_fits(T, moe::kPkvThreads) && n_q_heads > 0 && n_kv_heads > 0 &&
                   n_seqs >= 0 && table_width >= 0 && num_pages >= 0 && num_pages <= 0x7fffffff,
               "bad sizes");
@@ -143,10 +142,38 @@ extern "C" int moe_rope_paged_kv_bf16(const void *qkv, int64_t qkv_stride, int64
   MOE_REQUIRE(num_pages == 0 || k_cache != v_cache, "keys and values need caches of their own");
   hipLaunchKernelGGL(moe::rope_paged_kv_kernel, dim3((unsigned)T), dim3(moe::kPkvThreads), 0, (hipStream_t)stream,
                      (const uint16_t *)qkv, qkv_stride, n_q_heads, n_kv_heads, head_dim,
-                     (const float *)inv_freq_f32, (const int32_t *)positions_i32, (const int32_t *)seq_ids_i32,
-                     (const int32_t *)page_table_i32, n_seqs, table_width, num_pages,
+                     (const float *)inv_freq_f32, (const int32_t *)positions_i32, (const int32_t *)slots_i32,
+                     (const int32_t *)seq_ids_i32, (const int32_t *)page_table_i32, n_seqs, table_width, num_pages,
                      __builtin_ctz((unsigned)page_size), page_stride, (uint16_t *)q_out, (uint16_t *)k_out,
                      (uint16_t *)k_cache, (uint16_t *)v_cache);
   MOE_LAUNCH_CHECK();
   return MOE_STATUS_OK;
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_rope_paged_kv_bf16(const void *qkv, int64_t qkv_stride, int64_t T, int32_t n_q_heads,
+                                      int32_t n_kv_heads, int32_t head_dim, const void *inv_freq_f32,
+                                      const void *positions_i32, const void *seq_ids_i32,
+                                      const void *page_table_i32, int64_t n_seqs, int64_t table_width,
+                                      int64_t num_pages, int32_t page_size, int64_t page_stride,
+                                      void *q_out, void *k_out, void *k_cache, void *v_cache,
+                                      void *stream) {
+  return moe::rope_paged_kv(qkv, qkv_stride, T, n_q_heads, n_kv_heads, head_dim, inv_freq_f32, positions_i32, nullptr,
+                            seq_ids_i32, page_table_i32, n_seqs, table_width, num_pages, page_size, page_stride, q_out,
+                            k_out, k_cache, v_cache, stream);
+}
+
+extern "C" int moe_rope_paged_kv_slots_bf16(const void *qkv, int64_t qkv_stride, int64_t T, int32_t n_q_heads,
+                                            int32_t n_kv_heads, int32_t head_dim, const void *inv_freq_f32,
+                                            const void *positions_i32, const void *slots_i32,
+                                            const void *seq_ids_i32, const void *page_table_i32, int64_t n_seqs,
+                                            int64_t table_width, int64_t num_pages, int32_t page_size,
+                                            int64_t page_stride, void *q_out, void *k_out, void *k_cache,
+                                            void *v_cache, void *stream) {
+  MOE_REQUIRE(slots_i32 || T <= 0, "null pointer");
+  return moe::rope_paged_kv(qkv, qkv_stride, T, n_q_heads, n_kv_heads, head_dim, inv_freq_f32, positions_i32, slots_i32,
+                            seq_ids_i32, page_table_i32, n_seqs, table_width, num_pages, page_size, page_stride, q_out,
+                            k_out, k_cache, v_cache, stream);
 }

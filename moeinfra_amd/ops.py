@@ -375,13 +375,15 @@ def _out(out: Optional[torch.Tensor], name: str, like: torch.Tensor, *shape) -> 
 def rope_paged_kv(qkv: torch.Tensor, positions: torch.Tensor, page_table: torch.Tensor, k_cache: torch.Tensor,
                   v_cache: torch.Tensor, n_q_heads: int, inv_freq: torch.Tensor,
                   seq_ids: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
-                  want_k: bool = False):
+                  want_k: bool = False, slots: Optional[torch.Tensor] = None):
     """Rotary embedding of new tokens of many sequences, their keys and values written to the
     sequences' pages (``k_cache`` / ``v_cache`` [pages, kv heads, page size, head dim], bf16;
     ``page_table`` int32 [sequences, pages per sequence]).
 
     ``qkv`` bf16 [T, (q heads + 2 kv heads) * head dim]; token t stands at ``positions[t]`` (int32)
-    of sequence ``seq_ids[t]`` (int32; None: sequence t).  ``inv_freq`` fp32 [head dim / 2].
+    of sequence ``seq_ids[t]`` (int32; None: sequence t), its key and value at place ``slots[t]``
+    (int32; None: its position; the tokens of a drafted tree lie one behind the other, several of
+    them at one position).  ``inv_freq`` fp32 [head dim / 2].
     Returns (rotated q bf16 [T, q heads * head dim], rotated k bf16 [T, kv heads, head dim] | None).
     Tokens at negative positions are padding: their rows, here and in the cache, are left as they
     were.  A token whose page the table (or the cache) does not have is rotated, not cached.  No
@@ -404,6 +406,11 @@ def rope_paged_kv(qkv: torch.Tensor, positions: torch.Tensor, page_table: torch.
     seqs = None if seq_ids is None else _plain(seq_ids, "seq_ids", _I32, dev, (T,))
     q_out = _out(q_out, "q_out", qkv, T, nq * hd)
     k_out = qkv.new_empty(T, nkv, hd) if want_k else None
+    if slots is not None:
+        _launch(lib().moe_rope_paged_kv_slots_bf16, "rope_paged_kv", dev, qkv.data_ptr(), stride, T, nq, nkv, hd, freq,
+                pos, _plain(slots, "slots", _I32, dev, (T,)), seqs, table, n_seqs, width, pages, size, page_stride,
+                q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(), v_cache.data_ptr())
+        return q_out, k_out
     _launch(lib().moe_rope_paged_kv_bf16, "rope_paged_kv", dev, qkv.data_ptr(), stride, T, nq, nkv, hd, freq, pos, seqs,
             table, n_seqs, width, pages, size, page_stride, q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(),
             v_cache.data_ptr())
@@ -511,3 +518,218 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     _launch(lib().moe_sample_tokens, "sample_tokens", dev, logits.data_ptr(), int(f32), logits.stride(0) if B > 1 else V,
             B, V, numbers, t, temperature, k, top_k, p, top_p, m, min_p, out.data_ptr())
     return out
+
+
+# ----------------------------------------------------------------------------- decoding that branches
+_I64 = torch.int64
+
+
+def _layers(k_cache: torch.Tensor, v_cache: torch.Tensor):
+    """(layers, layer stride, page stride, shape of a layer) of paged caches: of one layer as in
+    ``_pages``, or of several ([layers, pages, kv heads, page size, head dim])."""
+    _require_cuda(k_cache, "k_cache")
+    dev, ndim = k_cache.device, k_cache.ndim
+    if ndim == 4:
+        stride, shape = _pages(k_cache, v_cache, dev)
+        return 1, 0, stride, shape
+    if ndim != 5:
+        raise ValueError(f"k_cache must have 4 or 5 dimensions (got {tuple(k_cache.shape)})")
+    _require_cuda(v_cache, "v_cache")
+    if v_cache.dtype is not _BF16 or v_cache.device != dev:
+        raise ValueError(f"v_cache must be {_BF16} on {dev} (got {v_cache.dtype} on {v_cache.device})")
+    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise ValueError(f"k_cache {tuple(k_cache.shape)} of strides {k_cache.stride()} and v_cache "
+                         f"{tuple(v_cache.shape)} of strides {v_cache.stride()} differ")
+    shape = k_cache.shape[1:]
+    if k_cache.shape[0] == 0:
+        return 0, 0, shape[1] * shape[2] * shape[3], shape
+    return k_cache.shape[0], k_cache.stride(0), _rows(k_cache[0], "k_cache", dev, 4), shape
+
+
+def paged_tree_attention_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Workspace of ``paged_tree_attention`` for batches of any size: made once, then shared by calls
+    that run one after the other (one stream)."""
+    n = lib().moe_paged_tree_attention_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim)
+    if n < 0:
+        raise ValueError(f"invalid attention sizes batch={batch} heads={n_q_heads}/{n_kv_heads} head_dim={head_dim}")
+    ws = torch.empty((n,), dtype=torch.uint8, device=device)
+    ws[:65536].zero_()
+    return ws
+
+
+def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                         lens: torch.Tensor, cu_seqlens: torch.Tensor, masks: Optional[torch.Tensor] = None,
+                         scaling: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted tokens, ``q`` bf16 [T, q heads, head dim], against the paged keys of their
+    sequences; bf16 [T, q heads, head dim].  Sequence b's (up to 64) are rows ``cu_seqlens[b] ..
+    cu_seqlens[b + 1] - 1`` (int32 [B + 1]); each sees the sequence's first ``lens[b]`` (int32) keys, and
+    the key at place ``lens[b] + j`` if bit j of its mask is set (``masks`` int64 [T]; None: a chain,
+    each sees the drafted ones up to itself).  ``scaling`` defaults to head_dim ** -0.5.  Rows without
+    keys are zeros, rows of no sequence are left as they were in ``out`` (without one they hold
+    anything).  ``workspace`` (``paged_tree_attention_workspace``) saves the call making one."""
+    _require_cuda(q, "q")
+    dev = q.device
+    stride = _rows(q, "q", dev, 3)
+    page_stride, (pages, nkv, size, hd) = _pages(k_cache, v_cache, dev)
+    T, nq, q_dim = q.shape
+    if q_dim != hd:
+        raise ValueError(f"q has head dim {q_dim}, the cache {hd}")
+    cu = _plain(cu_seqlens, "cu_seqlens", _I32, dev)
+    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1:
+        raise ValueError(f"cu_seqlens must be [sequences + 1] (got {tuple(cu_seqlens.shape)})")
+    B = cu_seqlens.numel() - 1
+    table = _plain(page_table, "page_table", _I32, dev)
+    table_shape = page_table.shape
+    if len(table_shape) != 2 or table_shape[0] != B:
+        raise ValueError(f"page_table must have {B} rows of pages (got {tuple(table_shape)})")
+    n = _plain(lens, "lens", _I32, dev, (B,))
+    seen = None if masks is None else _plain(masks, "masks", _I64, dev, (T,))
+    out = _out(out, "out", q, T, nq, hd)
+    if workspace is None:
+        workspace = paged_tree_attention_workspace(B, nq, nkv, hd, dev)
+    _launch(lib().moe_paged_tree_attention_bf16, "paged_tree_attention", dev, q.data_ptr(), stride, T,
+            k_cache.data_ptr(), v_cache.data_ptr(), pages, size, page_stride, table, table_shape[1], n, cu, seen, B, nq,
+            nkv, hd, hd ** -0.5 if scaling is None else scaling, out.data_ptr(),
+            _plain(workspace, "workspace", torch.uint8, dev), workspace.numel())
+    return out
+
+
+def accept_drafts(targets: torch.Tensor, drafts: torch.Tensor, cu_seqlens: torch.Tensor,
+                  masks: Optional[torch.Tensor] = None):
+    """Which drafted tokens the model itself would have chosen: ``targets`` (int64 [T]) are its choices
+    after each, ``drafts`` (int64 [T]) the tokens, ``cu_seqlens`` and ``masks`` as in
+    ``paged_tree_attention``; a token's parent is the last one before it in its mask.  The first of a
+    sequence is accepted, another one if its parent is and its token is the choice after the parent.
+    Returns, for the first of the longest accepted paths, (its tokens as bits int64 [B], their number
+    int32 [B], the choice after the last of them int64 [B]); 0, 0, -1 for sequences without tokens."""
+    _require_cuda(targets, "targets")
+    dev = targets.device
+    if targets.ndim != 1:
+        raise ValueError(f"targets must be [tokens] (got {tuple(targets.shape)})")
+    t = _plain(targets, "targets", _I64, dev)
+    shape = targets.shape
+    d = _plain(drafts, "drafts", _I64, dev, shape)
+    m = None if masks is None else _plain(masks, "masks", _I64, dev, shape)
+    cu = _plain(cu_seqlens, "cu_seqlens", _I32, dev)
+    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1:
+        raise ValueError(f"cu_seqlens must be [sequences + 1] (got {tuple(cu_seqlens.shape)})")
+    B = cu_seqlens.numel() - 1
+    paths, counts, tokens = targets.new_empty(B), cu_seqlens.new_empty(B), targets.new_empty(B)
+    _launch(lib().moe_accept_drafts, "accept_drafts", dev, t, d, m, cu, shape[0], B, paths.data_ptr(),
+            counts.data_ptr(), tokens.data_ptr())
+    return paths, counts, tokens
+
+
+def compact_paged_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor,
+                     paths: torch.Tensor) -> None:
+    """Keys and values of accepted tokens moved to where they belong, in place: of the set bits s_0 < s_1
+    < .. of ``paths[b]`` (int64 [B], from ``accept_drafts``), place ``lens[b] + s_j`` (int32 [B]) of
+    sequence b goes to place ``lens[b] + j``.  The caches are of one layer, or of all ([layers, pages,
+    kv heads, page size, head dim], pages and layers at strides of their own)."""
+    layers, layer_stride, page_stride, (pages, nkv, size, hd) = _layers(k_cache, v_cache)
+    dev = k_cache.device
+    table = _plain(page_table, "page_table", _I32, dev)
+    table_shape = page_table.shape
+    if len(table_shape) != 2:
+        raise ValueError("page_table must be [sequences, pages]")
+    B = table_shape[0]
+    _launch(lib().moe_compact_paged_kv_bf16, "compact_paged_kv", dev, k_cache.data_ptr(), v_cache.data_ptr(), layers,
+            layer_stride, pages, size, page_stride, nkv, hd, table, B, table_shape[1],
+            _plain(lens, "lens", _I32, dev, (B,)), _plain(paths, "paths", _I64, dev, (B,)))
+
+
+def beam_select_workspace(searches: int, beams: int, k: int, device) -> torch.Tensor:
+    """Workspace of ``beam_select`` for so many searches: made once, then shared by calls that run one
+    after the other (one stream)."""
+    n = lib().moe_beam_select_workspace_bytes(searches, beams, k)
+    if n < 0:
+        raise ValueError(f"invalid sizes searches={searches} beams={beams} k={k}")
+    ws = torch.empty((n,), dtype=torch.uint8, device=device)
+    ws[:65536].zero_()
+    return ws
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, workspace: Optional[torch.Tensor] = None):
+    """The ``k`` best continuations of each search: of all its beams and all tokens those of the largest
+    ``scores[s, w] + log_softmax(logits[s * W + w])``; ``logits`` bf16 or fp32 [S * W, V] (rows may lie
+    apart), ``scores`` fp32 [S, W], sums over the vocabulary in 64 bits.  Returns (totals fp32 [S, k],
+    falling; the rows of ``logits`` that go on, int32 [S, k]; tokens int64 [S, k]).  Equal ones go by beam,
+    then token.  -inf and NaN are never chosen; a score of -inf is no beam (a search's first step has
+    one), nor is a beam whose logits hold +inf; what there is too little for is -inf, -1, -1."""
+    _require_cuda(logits, "logits")
+    dev, f32 = logits.device, logits.dtype is _F32
+    if not f32 and logits.dtype is not _BF16:
+        raise ValueError(f"logits must be {_BF16} or {_F32} (got {logits.dtype})")
+    if logits.ndim != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"logits must be [rows, vocabulary] with contiguous rows (got {tuple(logits.shape)}, "
+                         f"strides {logits.stride()})")
+    base = _plain(scores, "scores", _F32, dev)
+    if scores.ndim != 2 or scores.numel() != logits.shape[0]:
+        raise ValueError(f"scores must be [searches, beams] of {logits.shape[0]} rows (got {tuple(scores.shape)})")
+    (S, W), (rows, V) = scores.shape, logits.shape
+    k = int(k)
+    if workspace is None:
+        workspace = beam_select_workspace(S, W, k, dev)
+    best = scores.new_empty(S, max(k, 0))
+    beam = torch.empty((S, max(k, 0)), dtype=_I32, device=dev)
+    token = torch.empty((S, max(k, 0)), dtype=_I64, device=dev)
+    _launch(lib().moe_beam_select, "beam_select", dev, logits.data_ptr(), int(f32), logits.stride(0) if rows > 1 else V,
+            S, W, V, base, k, best.data_ptr(), beam.data_ptr(), token.data_ptr(),
+            _plain(workspace, "workspace", torch.uint8, dev), workspace.numel())
+    return best, beam, token
+
+
+def fork_pages_workspace(pages: int, device) -> torch.Tensor:
+    """Workspace of ``fork_pages`` for a cache of so many pages: made once, then shared by calls that run
+    one after the other (one stream)."""
+    n = lib().moe_fork_pages_workspace_bytes(pages)
+    if n < 0:
+        raise ValueError(f"invalid number of pages {pages}")
+    return torch.zeros((n,), dtype=torch.uint8, device=device)
+
+
+def fork_pages(page_table: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor,
+               page_size: int, ahead: int = 1, out=None, workspace: Optional[torch.Tensor] = None):
+    """Page table rows taken over by the sequences that continue (beams reordered, forked, dropped):
+    new row i goes on from row ``parents[i]`` (int32 [N]) of ``page_table`` (int32 [B, width]) and ``lens``
+    (int32 [B]); any other number than a row's makes an empty one.  ``refs`` (int32 [pages], in place)
+    counts the holders of each page; pages of no holder are free.  The places of the next ``ahead``
+    positions become each row's alone: what others hold too is replaced by the lowest free page.
+
+    Returns (table int32 [N, width], lens int32 [N], copies int32 [N, 3], missing int32 [1]); ``out`` is
+    such a tuple to write to.  ``copies`` are for ``copy_pages``: (page, new page, positions in use), or
+    (-1, -1, 0).  ``missing`` counts places for which no page was free: -1 in the table."""
+    _require_cuda(page_table, "page_table")
+    dev = page_table.device
+    table = _plain(page_table, "page_table", _I32, dev)
+    if page_table.ndim != 2 or parents.ndim != 1 or refs.ndim != 1:
+        raise ValueError(f"page_table must be [sequences, pages], parents [rows], refs [pages] (got "
+                         f"{tuple(page_table.shape)}, {tuple(parents.shape)}, {tuple(refs.shape)})")
+    B, width = page_table.shape
+    N, pages = parents.shape[0], refs.shape[0]
+    n = _plain(lens, "lens", _I32, dev, (B,))
+    if out is None:
+        out = (page_table.new_empty(N, width), page_table.new_empty(N), page_table.new_empty(N, 3),
+               page_table.new_empty(1))
+    if workspace is None:
+        workspace = fork_pages_workspace(pages, dev)
+    _launch(lib().moe_fork_pages, "fork_pages", dev, table, n, B, width, _plain(parents, "parents", _I32, dev), N,
+            _plain(refs, "refs", _I32, dev), pages, page_size, ahead, _plain(out[0], "table", _I32, dev, (N, width)),
+            _plain(out[1], "lens", _I32, dev, (N,)), _plain(out[2], "copies", _I32, dev, (N, 3)),
+            _plain(out[3], "missing", _I32, dev, (1,)), _plain(workspace, "workspace", torch.uint8, dev),
+            workspace.numel())
+    return out
+
+
+def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, copies: torch.Tensor) -> None:
+    """The first ``copies[i, 2]`` positions of page ``copies[i, 0]`` copied to page ``copies[i, 1]`` (int32
+    [N, 3], from ``fork_pages``; pairs of pages that are not there are none), keys and values, in all
+    layers (caches as in ``compact_paged_kv``)."""
+    layers, layer_stride, page_stride, (pages, nkv, size, hd) = _layers(k_cache, v_cache)
+    dev = k_cache.device
+    pairs = _plain(copies, "copies", _I32, dev)
+    if copies.ndim != 2 or copies.shape[1] != 3:
+        raise ValueError(f"copies must be [copies, 3] (got {tuple(copies.shape)})")
+    _launch(lib().moe_copy_pages_bf16, "copy_pages", dev, k_cache.data_ptr(), v_cache.data_ptr(), layers, layer_stride,
+            pages, size, page_stride, nkv, hd, pairs, copies.shape[0])
