@@ -18,12 +18,14 @@ constexpr int kTaRows = 128;   // rows (token, query head of the group) of a wor
 constexpr int kTaWaves = kTaRows / 32;
 constexpr int kTaThreads = kTaWaves * kWave;
 constexpr float kTaLog2e = 1.44269504088896341f;
-// The running reference may lag the maximum by this much before the sums are rescaled: weights up to
-// e^5.5 = 245, which fp32 sums and bf16 weights carry without loss.
-constexpr float kTaLag = 5.5f;
+// The running reference may lag the maximum by this much (in powers of two) before the sums are
+// rescaled: weights up to 2^8, which fp32 sums and bf16 weights carry without loss.
+constexpr float kTaLag = 8.0f;
 constexpr int kTaStart = 2;    // tiles' time that beginning a row tile takes
 constexpr int kTaMinTiles = 2;
 constexpr int kTaJoin = 8;     // partial results that a thread has under way at a time
+constexpr int kTaMaxParts = 64;  // workgroups that share a row tile
+constexpr float kTaFine = 4096.0f;
 constexpr int64_t kTaCounterBytes = 65536;  // arrival counters at the start of the workspace
 constexpr int kTaMaxPage = 4096;
 
@@ -49,16 +51,16 @@ struct TaArgs {
   int place;   // floats of a partial result
 };
 
-// What is read in the place of keys that are not there.
-__device__ u32x4 ta_zeros[1];
+// What is read in the place of keys that are not there: as long as a chunk.
+__device__ u32x4 ta_zeros[1024 / 16];
 
-// 64 lanes' 16 bytes each from memory into LDS at dst + 16 * lane, without registers.  (In asm, as
-// the compiler would wait for all of them before the next transposing read of the other plane; the
-// caller waits for vmcnt(0) and a barrier before it reads dst.)
-__device__ __forceinline__ void ta_load_lds(const void *src, const uint8_t *dst) {
+// 64 lanes' 16 bytes each, at `lane` bytes from src, into LDS at dst + 16 * lane number, without
+// registers.  (In asm, as the compiler would wait for all of them before the next transposing read of the
+// other plane; the caller waits for vmcnt(0) and a barrier before it reads dst.)
+__device__ __forceinline__ void ta_load_lds(const void *src, uint32_t lane, const uint8_t *dst) {
   const uint32_t at = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)dst);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane), "s"(src)
                : "memory", "m0");
 }
 
@@ -115,6 +117,19 @@ paged_tree_attention_kernel(const TaArgs a) {
   const int64_t head_at = ((int64_t)kvh * HD) << a.page_shift;
   const int pmask = (1 << a.page_shift) - 1;
 
+  // Bytes of a chunk of K and V at which this lane finds its 16 bytes (pieces swizzled by the row).
+  const int lrow = lane / (kRowB / 16), lpiece = lane % (kRowB / 16);
+  const uint32_t klane = lrow * kRowB + 16 * (lpiece ^ pk_kx<HD>(wave * kChunkKeys + lrow));
+  const uint32_t vlane = lrow * kRowB + 16 * (lpiece ^ pk_vx<HD>(wave * kChunkKeys + lrow));
+  // Operand reads: K row 32 st + li, piece 2 s + hh.  V: lane group's dims 32 dt + 16 (l / 16 % 2) ..
+  // + 15 of keys 16 s + 8 n + 4 hh .. + 3; this lane's 8 bytes are in key l % 16 / 4 of the four.
+  const uint32_t krd = li * kRowB, kx = 16 * (hh ^ pk_kx<HD>(li));
+  const uint32_t vkey = 4 * hh + ((lane & 15) >> 2);
+  const uint32_t vrd = kPlane + vkey * kRowB + 8 * (lane & 1);
+  const uint32_t vx = 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ pk_vx<HD>(vkey));
+  const uint32_t flip = a.scaling < 0.0f ? 0x80008000u : 0u, keep = a.scaling == 0.0f ? 0u : ~0u;
+  const float c = (a.scaling == 0.0f ? 1.0f : fabsf(a.scaling)) * kTaLog2e;
+
   // Tiles tile0 .. tile1 - 1 of row tile rt of sequence b, shared by the nact workgroups from `head` on.
   auto item = [&](int b, const TaSeq &w, int rt, int tile0, int tile1, int head, int nact, bool later,
                   bool inside) __attribute__((always_inline)) {
@@ -126,12 +141,16 @@ paged_tree_attention_kernel(const TaArgs a) {
     const int t = r / a.grp;
     const int qhead = kvh * a.grp + (r - t * a.grp);
     const int64_t qrow = w.tok0 + t;
-    // Q as the B operand: column li, dims 16 s + 8 hh .. + 7.
+    // Q as the B operand: column li, dims 16 s + 8 hh .. + 7.  A negative scaling goes into its signs, one of
+    // zero into its values (masked scores, -inf, are multiplied too).
     u32x4 qf[HD / 16];
     {
       const uint16_t *qr = a.q + qrow * a.q_stride + (int64_t)qhead * HD + 8 * hh;
 #pragma unroll
-      for (int s = 0; s < HD / 16; ++s) qf[s] = *reinterpret_cast<const u32x4 *>(qr + 16 * s);
+      for (int s = 0; s < HD / 16; ++s) {
+        qf[s] = *reinterpret_cast<const u32x4 *>(qr + 16 * s);
+        qf[s] = (qf[s] ^ flip) & keep;
+      }
     }
     const uint64_t mask = (a.masks != nullptr ? (uint64_t)a.masks[qrow] : ~0ull >> (63 - t)) & (~0ull >> (64 - w.n));
     const int32_t *trow = a.table + b * a.width;
@@ -142,18 +161,18 @@ paged_tree_attention_kernel(const TaArgs a) {
     };
     // Tile `tile` into plane p; the 8-key groups whose pages exist.
     auto load = [&](int tile, int p, int ent) __attribute__((always_inline)) {
-      const uint32_t there = (uint32_t)__ballot((uint32_t)ent < (uint64_t)a.num_pages && lane < kGroups);
+      const uint32_t there = (uint32_t)__ballot((uint32_t)ent < (uint64_t)a.num_pages);
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) {
         const int chunk = wave + i * kTaWaves, first = chunk * kChunkKeys;  // (of the tile's keys)
         const int64_t page = __builtin_amdgcn_readlane(ent, first >> 3);
-        const int row = first + 16 * lane / kRowB, piece = 16 * lane % kRowB / 16;
-        const int key = tile * kKeys + row;
+        const int key = tile * kKeys + first;
         const bool has = (there >> (first >> 3) & 1) != 0 && key < w.keys;
         const int64_t at = page * a.page_stride + head_at + (int64_t)(key & pmask) * HD;
-        ta_load_lds(has ? (const void *)(a.kc + at + 8 * (piece ^ pk_kx<HD>(row))) : ta_zeros, s_kv[p] + chunk * 1024);
-        ta_load_lds(has ? (const void *)(a.vc + at + 8 * (piece ^ pk_vx<HD>(row))) : ta_zeros,
-                    s_kv[p] + kPlane + chunk * 1024);
+        // (The rows of K are swizzled by their number in the tile, of which i changes one bit of 256 dims.)
+        ta_load_lds(has ? (const void *)(a.kc + at) : ta_zeros, klane ^ (HD == 256 ? (i & 1) * 128 : 0),
+                    s_kv[p] + chunk * 1024);
+        ta_load_lds(has ? (const void *)(a.vc + at) : ta_zeros, vlane, s_kv[p] + kPlane + chunk * 1024);
       }
       return there;
     };
@@ -162,19 +181,15 @@ paged_tree_attention_kernel(const TaArgs a) {
     for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[dt][v] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    // Operand reads: K row 32 st + li, piece 2 s + hh.  V: lane group's dims 32 dt + 16 (l / 16 % 2) ..
-    // + 15 of keys 16 s + 8 n + 4 hh .. + 3; this lane's 8 bytes are in key l % 16 / 4 of the four.
-    const uint32_t krd = li * kRowB, kx = 16 * (hh ^ pk_kx<HD>(li));
-    const uint32_t vkey = 4 * hh + ((lane & 15) >> 2);
-    const uint32_t vrd = kPlane + vkey * kRowB + 8 * (lane & 1);
-    const uint32_t vx = 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ pk_vx<HD>(vkey));
-    // The products of ST 32-key parts of a tile, from part st0 on.
-    auto compute = [&](int tile, int p, uint32_t there, int st0, auto st_c) __attribute__((always_inline)) {
+    float m = -INFINITY, l = 0.0f;  // (m in units of q.k)
+    // The products of ST 32-key parts of a tile, from part st0 on.  EDGE: a row may not see all of it.
+    auto compute = [&](int tile, int p, uint32_t there, int st0, auto st_c, auto edge_c) __attribute__((always_inline)) {
       constexpr int ST = decltype(st_c)::value;
+      constexpr bool kEdge = decltype(edge_c)::value;
       const uint8_t *buf = s_kv[p] + 32 * st0 * kRowB;
-      const int k0 = tile * kKeys + 32 * st0;
-      there >>= 4 * st0;
+      // (Addresses are a XOR with a constant away from these: computed, not held in registers.)
+      uint32_t ka = kx, va = vx;
+      asm volatile("" : "+v"(ka), "+v"(va));
       f32x16 sc[ST];
 #pragma unroll
       for (int st = 0; st < ST; ++st)
@@ -184,24 +199,18 @@ paged_tree_attention_kernel(const TaArgs a) {
       for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
         for (int st = 0; st < ST; ++st) {
-          const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + krd + (kx ^ (32 * i)) + 32 * st * kRowB);
+          const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + krd + (ka ^ (32 * i)) + 32 * st * kRowB);
           sc[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
                                                            __builtin_bit_cast(bf16x8, qf[i]), sc[st], 0, 0, 0);
         }
-#pragma unroll
-      for (int st = 0; st < ST; ++st)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) sc[st][v] *= a.scaling;
-      constexpr uint32_t kAll = (1u << (4 * ST)) - 1;
-      const bool edge = k0 + 32 * ST > w.len || (there & kAll) != kAll;
       uint64_t seen = ~0ull;
-      if (edge) {
+      if constexpr (kEdge) {
         // Keys of the part that the row sees, bit by bit.
-        const int d = k0 - w.len;
+        const int d = tile * kKeys + 32 * st0 - w.len;
         seen = d >= kTaNodes ? 0 : d >= 0 ? mask >> d : -d >= 64 ? ~0ull : mask << -d | ((1ull << -d) - 1);
         uint64_t pages = 0;
 #pragma unroll
-        for (int i = 0; i < 4 * ST; ++i) pages |= (there >> i & 1) != 0 ? 0xffull << (8 * i) : 0;
+        for (int i = 0; i < 4 * ST; ++i) pages |= (there >> (4 * st0 + i) & 1) != 0 ? 0xffull << (8 * i) : 0;
         seen &= pages;
 #pragma unroll
         for (int st = 0; st < ST; ++st)
@@ -217,9 +226,9 @@ paged_tree_attention_kernel(const TaArgs a) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[st][v]);
       mx = op_xor32<true>(mx);
-      if (__any(mx > m + kTaLag)) {
+      if (__any((mx - m) * c > kTaLag)) {
         const float mn = fmaxf(m, mx);
-        const float alpha = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * kTaLog2e);
+        const float alpha = __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * c);
         m = mn;
         l *= alpha;
 #pragma unroll
@@ -228,24 +237,36 @@ paged_tree_attention_kernel(const TaArgs a) {
           for (int v = 0; v < 16; ++v) acc[dt][v] *= alpha;
       }
       const float mref = m == -INFINITY ? 0.0f : m;  // before a row's first key above -inf
+      // One multiply-add where the rounding of m c is as good as nothing (2^-12 of a weight), else the
+      // difference first.
+      const float mc = mref * c;
+      if (__all(fabsf(mc) <= kTaFine)) {
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sc[st][v] = __builtin_amdgcn_exp2f(fmaf(sc[st][v], c, -mc));
+      } else {
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sc[st][v] = __builtin_amdgcn_exp2f((sc[st][v] - mref) * c);
+      }
 #pragma unroll
       for (int st = 0; st < ST; ++st)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          // (The difference first: mref * log2(e) alone could overflow.)
-          sc[st][v] = __builtin_amdgcn_exp2f((sc[st][v] - mref) * kTaLog2e);
-          l += sc[st][v];
-        }
-      if (edge) {
+        for (int v = 0; v < 16; ++v) l += sc[st][v];
+      if constexpr (kEdge) {
         // A key that a row does not see has a weight of zero, but zero times an infinity or NaN in its
         // values would come through: where there are such, key by key instead.
         bool odd = false;
+#pragma unroll 1
         for (int at = 16 * lane; at < 32 * ST * kRowB; at += 16 * kWave) {
           const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + kPlane + at);
 #pragma unroll
           for (int e = 0; e < 4; ++e) odd |= (x[e] & 0x7f800000u) == 0x7f800000u || (x[e] & 0x7f80u) == 0x7f80u;
         }
         if (__any(odd)) {
+#pragma unroll 1
           for (int j = 0; j < 32 * ST; ++j) {
             const int mine = (j >> 5) * 16 + ((j >> 3) & 3) * 4 + (j & 3);
             float pj = 0.0f;
@@ -278,7 +299,7 @@ paged_tree_attention_kernel(const TaArgs a) {
         for (int j = 0; j < 4; ++j) pf[j] = pack_bf16x2(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
 #pragma unroll
         for (int dt = 0; dt < kDT; ++dt) {
-          const uint8_t *v = buf + vrd + (vx ^ (64 * dt)) + 16 * s * kRowB;
+          const uint8_t *v = buf + vrd + (va ^ (64 * dt)) + 16 * s * kRowB;
           const uint2 x0 = pk_read_tr(v), x1 = pk_read_tr(v + 8 * kRowB);
           const u32x4 x = {x0.x, x0.y, x1.x, x1.y};
           acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
@@ -286,29 +307,44 @@ paged_tree_attention_kernel(const TaArgs a) {
         }
       }
     };
-    {
-      uint32_t there = load(tile0, 0, entry(tile0));
-      int ent = entry(tile0 + 1);
-      for (int tile = tile0, p = 0; tile < tile1; ++tile, p ^= 1) {
+    constexpr uint32_t kAll = (1u << kGroups) - 1;
+    // All tiles by ST parts a wave, from part st0 on: those that every row sees whole, then (from the first
+    // on that has no page) the others.
+    auto walk = [&](int st0, auto st_c) __attribute__((always_inline)) {
+      uint32_t there = load(tile0, 0, entry(tile0)), next = 0;
+      int ent = entry(tile0 + 1), p = 0, tile = tile0;
+      auto arrive = [&]() __attribute__((always_inline)) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // (the tile is there, and the other plane no longer read)
-        uint32_t next = 0;
         if (tile + 1 < tile1) {
           next = load(tile + 1, p ^ 1, ent);
           ent = entry(tile + 2);
         }
-        if (busy) {
-          if constexpr (kHalves) {
-            if (half)
-              compute(tile, p, there, wave >> 1, std::integral_constant<int, 1>{});
-            else
-              compute(tile, p, there, 0, std::integral_constant<int, 2>{});
-          } else {
-            compute(tile, p, there, 0, std::integral_constant<int, 1>{});
-          }
-        }
-        there = next;
+      };
+      for (const int whole = min(w.len / kKeys, tile1); tile < whole && there == kAll; ++tile, p ^= 1, there = next) {
+        arrive();
+        if (busy) compute(tile, p, there, st0, st_c, std::false_type{});
       }
+      for (; tile < tile1; ++tile, p ^= 1, there = next) {
+        arrive();
+        // What lies behind the last key in its chunk has been loaded too: zeros in its place.
+        const int end = w.keys - tile * kKeys, more = -end & (kChunkKeys - 1);
+        if (end < kKeys && more != 0) {
+          const int tid = threadIdx.x;
+          if (tid < more * (kRowB / 16))
+            *reinterpret_cast<u32x4 *>(s_kv[p] + kPlane + end * kRowB + 16 * tid) = (u32x4){0, 0, 0, 0};
+          __syncthreads();
+        }
+        if (busy) compute(tile, p, there, st0, st_c, std::true_type{});
+      }
+    };
+    if constexpr (kHalves) {
+      if (half)
+        walk(wave >> 1, std::integral_constant<int, 1>{});
+      else
+        walk(0, std::integral_constant<int, 2>{});
+    } else {
+      walk(0, std::integral_constant<int, 1>{});
     }
     __syncthreads();  // (the planes are free)
     l = op_xor32<false>(l);
@@ -327,8 +363,8 @@ paged_tree_attention_kernel(const TaArgs a) {
       if (wave < 2 && busy) {
         const float4 ml = o[4 * kDT * kWave];
         const float mn = fmaxf(m, ml.x), mref = mn == -INFINITY ? 0.0f : mn;
-        const float a0 = __builtin_amdgcn_exp2f((m - mref) * kTaLog2e);
-        const float a1 = __builtin_amdgcn_exp2f((ml.x - mref) * kTaLog2e);
+        const float a0 = __builtin_amdgcn_exp2f((m - mref) * c);
+        const float a1 = __builtin_amdgcn_exp2f((ml.x - mref) * c);
         m = mn;
         l = l * a0 + ml.y * a1;
 #pragma unroll
@@ -345,66 +381,84 @@ paged_tree_attention_kernel(const TaArgs a) {
     }
     // This wave's rows as results.
     const bool writes = busy && !(half && wave >= 2);
-    auto put = [&](float inv) __attribute__((always_inline)) {
-      if (row0 + li >= rows) return;
-      uint16_t *const o = a.out + (qrow * a.nq + qhead) * HD + 4 * hh;
-#pragma unroll
-      for (int dt = 0; dt < kDT; ++dt)
-#pragma unroll
-        for (int v = 0; v < 16; v += 4)
-          *reinterpret_cast<uint2 *>(o + 32 * dt + 2 * v) =
-              make_uint2(pack_bf16x2(acc[dt][v] * inv, acc[dt][v + 1] * inv),
-                         pack_bf16x2(acc[dt][v + 2] * inv, acc[dt][v + 3] * inv));
-    };
     if (nact == 1) {
-      if (writes) put(l == 0.0f ? 0.0f : 1.0f / l);  // (no key at all: zeros)
-      __syncthreads();                                // (before the planes are used again)
+      if (writes && row0 + li < rows) {  // (no key at all: zeros)
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint16_t *const o = a.out + (qrow * a.nq + qhead) * HD + 4 * hh;
+#pragma unroll
+        for (int dt = 0; dt < kDT; ++dt)
+#pragma unroll
+          for (int v = 0; v < 16; v += 4)
+            *reinterpret_cast<uint2 *>(o + 32 * dt + 2 * v) =
+                make_uint2(pack_bf16x2(acc[dt][v] * inv, acc[dt][v + 1] * inv),
+                           pack_bf16x2(acc[dt][v + 2] * inv, acc[dt][v + 3] * inv));
+      }
+      __syncthreads();  // (before the planes are used again)
       return;
     }
     // A partial result: two values of each lane next to each other, then the rows' m and l.
-    const int at = row0 - base;  // of the wave's rows in the tile
-    float *const own = a.part + ((int64_t)(2 * wg + (later ? 1 : 0)) * a.nkv + kvh) * a.place;
     const int limit = min(rows - base, kTaRows);  // rows of the tile
     const int sums = (limit + 31) / 32 * 32 * HD;
+    float *const own = a.part + ((int64_t)(2 * wg + (later ? 1 : 0)) * a.nkv + kvh) * a.place;
     if (writes) {
 #pragma unroll
       for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
         for (int v = 0; v < 16; v += 2)
-          pa_put(own + at * HD + ((8 * dt + v / 2) * kWave + lane) * 2, acc[dt][v], acc[dt][v + 1]);
-      if (hh == 0) pa_put(own + sums + 2 * (at + li), m, l);
+          pa_put(own + (row0 - base) * HD + ((8 * dt + v / 2) * kWave + lane) * 2, acc[dt][v], acc[dt][v + 1]);
+      if (hh == 0) pa_put(own + sums + 2 * (row0 - base + li), m, l);
     }
     if (!pa_last_of(a.count + ((int64_t)b * a.rtiles + rt) * a.nkv + kvh, nact)) return;
     // The last of the row tile's workgroups adds their results up, in the order of the keys.  Result y
     // is workgroup head + y's: in its first place, but in its last if the row tile starts inside its part
     // (y = 0).
-    auto result = [&](int y) {
-      return a.part + ((int64_t)(2 * (head + y) + (y == 0 && inside ? 1 : 0)) * a.nkv + kvh) * a.place;
-    };
-    if (writes) {
-      float mm = -INFINITY;
-      for (int y = 0; y < nact; ++y) mm = fmaxf(mm, pa_get(result(y) + sums + 2 * (at + li)).x);
-      const float mref = mm == -INFINITY ? 0.0f : mm;
-      float ll = 0.0f;
+    const uint32_t step = 2 * (uint32_t)a.nkv * (uint32_t)a.place;
+    const float *const all = a.part + (int64_t)head * step + (int64_t)kvh * a.place;
+    const uint32_t first = inside ? (uint32_t)a.nkv * (uint32_t)a.place : 0;
+    auto result = [&](int y, int at) { return pa_get(all + ((uint32_t)y * step + (y == 0 ? first : 0) + (uint32_t)at)); };
+    // Their weights in LDS: a lane per result.
+    float *const s_w = reinterpret_cast<float *>(&s_kv[0][0]);
+    for (int i0 = wave * 8; i0 < limit; i0 += 8 * kTaWaves) {
+      float2 ml[8];
 #pragma unroll
-      for (int dt = 0; dt < kDT; ++dt)
+      for (int i = 0; i < 8; ++i) ml[i] = result(min(lane, nact - 1), sums + 2 * min(i0 + i, limit - 1));
+      float mx[8], ll[8];
 #pragma unroll
-        for (int v = 0; v < 16; ++v) acc[dt][v] = 0.0f;
-      for (int y = 0; y < nact; ++y) {
-        const float *const p = result(y);
-        const float2 ml = pa_get(p + sums + 2 * (at + li));
-        const float f = __builtin_amdgcn_exp2f((ml.x - mref) * kTaLog2e);
-        ll = fmaf(f, ml.y, ll);
+      for (int i = 0; i < 8; ++i) mx[i] = ml[i].x;
+      lane_groups_reduce<true>(mx, kWave);
 #pragma unroll
-        for (int dt = 0; dt < kDT; ++dt)
-#pragma unroll
-          for (int v = 0; v < 16; v += 2) {
-            const float2 x = pa_get(p + at * HD + ((8 * dt + v / 2) * kWave + lane) * 2);
-            acc[dt][v] = fmaf(f, x.x, acc[dt][v]);
-            acc[dt][v + 1] = fmaf(f, x.y, acc[dt][v + 1]);
-          }
+      for (int i = 0; i < 8; ++i) {
+        mx[i] = __builtin_amdgcn_exp2f((ml[i].x - (mx[i] == -INFINITY ? 0.0f : mx[i])) * c);
+        ll[i] = lane < nact ? mx[i] * ml[i].y : 0.0f;
       }
-      put(ll == 0.0f ? 0.0f : 1.0f / ll);
+      lane_groups_reduce<false>(ll, kWave);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < limit) s_w[(i0 + i) * kTaMaxParts + lane] = lane < nact ? (ll[i] == 0.0f ? 0.0f : mx[i] / ll[i]) : 0.0f;
+    }
+    __syncthreads();
+    // A thread takes two neighbouring values, kTaJoin results under way at a time.
+    for (int i = threadIdx.x; i < sums / 2; i += kTaThreads) {
+      const int at = i & (kWave - 1), word = i >> 6;               // lane, and two of its values
+      const int rr = word / (8 * kDT) * 32 + (at & 31), pair = word % (8 * kDT);
+      const float *const f = s_w + min(rr, limit - 1) * kTaMaxParts;
+      float o0 = 0.0f, o1 = 0.0f;
+      for (int y0 = 0; y0 < nact; y0 += kTaJoin) {
+        float2 x[kTaJoin];
+#pragma unroll
+        for (int y = 0; y < kTaJoin; ++y) x[y] = result(min(y0 + y, nact - 1), 2 * i);
+#pragma unroll
+        for (int y = 0; y < kTaJoin; ++y) {  // (loads past the last result repeat it: zeros in their place)
+          o0 = fmaf(f[y0 + y], y0 + y < nact ? x[y].x : 0.0f, o0);
+          o1 = fmaf(f[y0 + y], y0 + y < nact ? x[y].y : 0.0f, o1);
+        }
+      }
+      if (rr < limit) {
+        const int rg = base + rr, tok = rg / a.grp;
+        const int dim = 32 * (pair >> 3) + 8 * ((pair & 7) >> 1) + 4 * (at >> 5) + 2 * (pair & 1);
+        *reinterpret_cast<uint32_t *>(a.out + ((int64_t)(w.tok0 + tok) * a.nq + kvh * a.grp + rg - tok * a.grp) * HD + dim) =
+            pack_bf16x2(o0, o1);
+      }
     }
     __syncthreads();  // (as above)
   };
@@ -415,13 +469,17 @@ paged_tree_attention_kernel(const TaArgs a) {
     if (rt < w.rtiles) item(b, w, rt, 0, w.tiles, 0, 1, false, false);
     return;
   }
-  int total = 0;
+  int total = 0, most = 0;
   for (int i0 = 0; i0 < a.B; i0 += kWave) {
     const TaSeq s = ta_seq(a, i0 + lane, kKeys);
     total += s.rtiles * (s.tiles + kTaStart);
+    most = max(most, s.tiles);
   }
+  most = __builtin_amdgcn_readlane(pa_max(most), kWave - 1);
   total = __builtin_amdgcn_readlane(pa_incl(total), kWave - 1);
-  const int per = max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), kTaStart + kTaMinTiles);
+  // (A row tile meets at most kTaMaxParts workgroups, also where it starts inside the part of one.)
+  const int per = max(max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), kTaStart + kTaMinTiles),
+                      (most + kTaMaxParts - 3) / (kTaMaxParts - 2));
   const int begin = min(wg, a.share) * per, end = begin + per;
   if (begin >= total) return;
   int before = 0;  // of the sequences before these 64
