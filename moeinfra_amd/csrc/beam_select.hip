@@ -15,10 +15,12 @@ namespace {
 constexpr int kBsThreads = 256;
 constexpr int kBsWaves = kBsThreads / kWave;
 constexpr int kBsMost = 64;      // continuations of a search at most
-constexpr int kBsPieces = 4;     // 16-byte pieces that a thread holds
+constexpr int kBsPieces = 8;     // 16-byte pieces that a thread holds
 constexpr int kBsMaxVocab = 1 << 20;
 constexpr int kBsMaxBeams = 256;
 constexpr int kBsMaxChunks = 64; // workgroups of a row at most
+constexpr int kBsFew = 4;        // continuations that a thread holds
+constexpr int kBsFinal = 1024;   // continuations of a search that are ranked at once
 constexpr int kBsGroups = 2048;  // workgroups that rows are divided up to
 constexpr int64_t kBsCounterBytes = 65536;  // arrival counters at the start of the workspace
 
@@ -52,23 +54,27 @@ __device__ __forceinline__ float bs_value(uint32_t o) {
 // A logit and its place: the larger logit first, of equal ones the lower index.
 __device__ __forceinline__ uint64_t bs_key(uint32_t o, uint32_t i) { return o == 0 ? 0 : (uint64_t)o << 32 | ~i; }
 
-// e^d for d <= 0 to 2^-42 of its value: e^r 2^n with |r| <= ln 2 / 2, e^r by its series up to r^10 / 10!.
-__device__ __forceinline__ double bs_exp(double d) {
-  d = fmax(d, -700.0);
-  const double n = rint(d * 1.4426950408889634074);
-  const double r = fma(n, -0.69314718055994530942, d);
-  double p = 1.0 / 3628800;
-  p = fma(p, r, 1.0 / 362880);
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)n);
+// e^d for -700 <= d <= 0 to 2^-39 of its value: 2^(n / 32) e^r, n a whole number and |r| <= ln 2 / 64; 2^(j / 32)
+// of a table, e^r by its series up to r^4 / 4!.  (A table of a bank each: lanes of one entry share it.)
+constexpr int kBsTable = 32;
+__device__ __forceinline__ void bs_table(double *s_tab) {
+  if (threadIdx.x < kBsTable) s_tab[threadIdx.x] = exp2((double)threadIdx.x / kBsTable);
+}
+// The factors of e^d: {e^r, 2^(n / 32)}.
+__device__ __forceinline__ double2 bs_exp(double d, const double *s_tab) {
+  constexpr double kUnit = 0.69314718055994530942 / kBsTable, kWhole = 6755399441055744.0;  // 1.5 * 2^52
+  const double t = d * (1.0 / kUnit);
+  const double s = t + kWhole;      // n in its last bits
+  const double f = t - (s - kWhole);
+  const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, s);
+  double p = kUnit * kUnit * kUnit * kUnit / 24;
+  p = fma(p, f, kUnit * kUnit * kUnit / 6);
+  p = fma(p, f, kUnit * kUnit / 2);
+  p = fma(p, f, kUnit);
+  p = fma(p, f, 1.0);
+  const uint64_t b = __builtin_bit_cast(uint64_t, s_tab[n & (kBsTable - 1)]);
+  const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)(n >> 5) << 20);
+  return make_double2(p, __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b));
 }
 
 template <class T>
@@ -97,6 +103,9 @@ __device__ __forceinline__ bool bs_before(uint64_t t0, uint32_t a0, uint64_t t1,
 
 // Workgroup c of a row finds the k largest of its part, their maximum and sum; the last workgroup of a
 // search to arrive puts them together.
+//
+// The k largest: the threads' maxima fall into 64 groups; of the k-th largest of those (its upper 16 bits)
+// and above there are k values at least, and few more, which go to a list and are ranked.
 template <bool F32>
 __global__ void __launch_bounds__(kBsThreads)
 beam_select_kernel(const BsArgs a) {
@@ -104,151 +113,257 @@ beam_select_kernel(const BsArgs a) {
   constexpr int kPer = 16 / sizeof(E);              // values of a piece
   constexpr int kHeld = kBsPieces * kPer;           // of a thread
   constexpr int kList = kBsMost * kHeld + kBsMost;  // those of k threads, and the best so far
-  __shared__ uint64_t s_key[kBsThreads], s_list[kList], s_best[kBsMost];
-  __shared__ uint32_t s_at[kList];
-  __shared__ double s_sum[kBsWaves], s_lse[kBsMaxBeams];
-  __shared__ float s_max[kBsWaves], s_top[kBsMaxBeams];
+  constexpr uint32_t kLeast = 0x80;                 // upper 16 bits of the lowest finite value's order
+  __shared__ uint64_t s_list[kList], s_key[kBsThreads], s_best[kBsMost];
+  __shared__ uint32_t s_at[kBsFinal];
+  __shared__ double s_tab[kBsTable], s_sum[kBsWaves], s_lse[kBsMaxBeams];
+  __shared__ float s_max[kBsWaves][kWave], s_top[kBsMaxBeams];
   __shared__ uint64_t s_least;
-  __shared__ uint32_t s_least_at, s_n, s_seen;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
+  __shared__ uint32_t s_n, s_seen;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = (int)(blockIdx.x / (unsigned)a.chunks), c = (int)(blockIdx.x - (unsigned)row * a.chunks);
   const int search = row / a.W;
   const int v0 = c * a.chunk, v1 = min(v0 + a.chunk, a.V);
   const E *const x = (const E *)a.x + row * a.stride;
   // Pieces begin where memory's 16 bytes do.
   const int lead = (int)((uintptr_t)(x + v0) % 16 / sizeof(E));
-  for (int i = tid; i < kBsMost; i += kBsThreads) s_best[i] = 0;
-  float m = -INFINITY;   // of all so far
-  double sum = 0.0;      // this thread's
-  __syncthreads();
+  bs_table(s_tab);
+  if (tid < kBsMost) s_best[tid] = 0;
+  if (tid == 0) s_n = 0, s_least = 1;
+  float m = -INFINITY;  // of the wave's so far
+  double sum = 0.0;     // this thread's
   for (int i0 = v0 - lead; i0 < v1; i0 += kBsThreads * kHeld) {
-    float h[kHeld];
+    u32x4 h[kBsPieces];
+    auto first = [&](int p) { return i0 + (p * kBsThreads + tid) * kPer; };
+    auto some = [&](int p) { return i0 + p * kBsThreads * kPer < v1; };  // (the same for the workgroup)
+    auto value = [&](int p, int e) {
+      const uint32_t w = F32 ? h[p][e] : h[p][e >> 1];
+      return F32 ? __builtin_bit_cast(float, w) : e & 1 ? bf16hi_to_f32(w) : bf16lo_to_f32(w);
+    };
 #pragma unroll
     for (int p = 0; p < kBsPieces; ++p) {
-      const int i = i0 + (p * kBsThreads + tid) * kPer;
+      const int i = first(p);
+      h[p] = F32 ? (u32x4){0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}  // -inf
+                 : (u32x4){0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+      if (!some(p)) continue;
       if (i >= v0 && i + kPer <= v1) {
-        const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(x + i));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t word = w[e];  // (a bit cast of w[e] itself is one of w[0])
-          if constexpr (F32) {
-            h[p * kPer + e] = __builtin_bit_cast(float, word);
-          } else {
-            h[p * kPer + 2 * e] = bf16lo_to_f32(word);
-            h[p * kPer + 2 * e + 1] = bf16hi_to_f32(word);
-          }
-        }
+        h[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(x + i));
       } else {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          h[p * kPer + e] = -INFINITY;
+        for (int e = 0; e < kPer; ++e)
           if (i + e >= v0 && i + e < v1) {
             if constexpr (F32)
-              h[p * kPer + e] = x[i + e];
+              h[p][e] = __builtin_bit_cast(uint32_t, x[i + e]);
             else
-              h[p * kPer + e] = bf16_to_f32(x[i + e]);
+              h[p][e >> 1] = e & 1 ? (h[p][e >> 1] & 0xffffu) | (uint32_t)x[i + e] << 16
+                                   : (h[p][e >> 1] & 0xffff0000u) | x[i + e];
           }
-        }
       }
     }
-    auto index = [&](int j) { return (uint32_t)(i0 + (j / kPer * kBsThreads + tid) * kPer + j % kPer); };
-    uint64_t top = 0;
     float mx = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      h[j] = h[j] > -INFINITY ? h[j] : -INFINITY;  // (NaN too)
-      mx = fmaxf(mx, h[j]);
-      const uint64_t key = bs_key(bs_order(h[j]), index(j));
-      top = key > top ? key : top;
+    for (int p = 0; p < kBsPieces; ++p)
+      if (some(p)) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const float v = value(p, e);
+          mx = v > mx ? v : mx;  // (a maximum with a signaling NaN is NaN)
+        }
+      }
+    __syncthreads();  // (the round before, the table)
+    s_max[wave][lane] = mx;
+    float wm[1] = {mx};
+    lane_groups_reduce<true>(wm, kWave);
+    if (wm[0] > m) {
+      if (m > -INFINITY) {
+        const double2 f = bs_exp(fmax((double)m - (double)wm[0], -700.0), s_tab);
+        sum = sum * f.x * f.y;
+      }
+      m = wm[0];
     }
-    s_key[tid] = top;
-    const float wm = bs_wave_max(mx);
-    if (lane == 0) s_max[wave] = wm;
-    if (tid == 0) s_n = 0, s_least = 1;
+    if (m > -INFINITY) {
+      // (-inf and NaN weigh as good as nothing.  A row of +inf has no probabilities: its sum is not looked at.)
+      const double md = (double)m;
+#pragma unroll
+      for (int p = 0; p < kBsPieces; ++p)
+        if (some(p)) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const double2 f = bs_exp(fmax((double)value(p, e) - md, -700.0), s_tab);
+            sum = fma(f.x, f.y, sum);
+          }
+        }
+    }
     __syncthreads();
-    float mn = m;
-#pragma unroll
-    for (int w = 0; w < kBsWaves; ++w) mn = fmaxf(mn, s_max[w]);
-    // (A row of +inf has no probabilities: its sum is not needed, and NaN.)
-    if (mn > -INFINITY) {
-      sum *= m == -INFINITY ? 0.0 : bs_exp((double)m - (double)mn);
-#pragma unroll
-      for (int j = 0; j < kHeld; ++j) sum += h[j] == -INFINITY ? 0.0 : bs_exp((double)h[j] - (double)mn);
-      m = mn;
-    }
-    // The k-th largest of the threads' largest: all that could be among the k best are as large.
     const uint64_t worst = s_best[a.k - 1];
-    if (__syncthreads_or(top > worst)) {
+    // The largest 16 bits that k groups reach, bit by bit.
+    float g = s_max[0][lane];
+#pragma unroll
+    for (int w = 1; w < kBsWaves; ++w) g = fmaxf(g, s_max[w][lane]);
+    const uint32_t og = bs_order(g) >> 16;
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint32_t to = t | 1u << bit;
+      if (__popcll(__ballot(og >= to)) >= a.k) t = to;
+    }
+    t = max(t, kLeast);
+    t = max(t, (uint32_t)(worst >> 48));
+    const float least = bs_value(t << 16);
+    if (__ballot(g >= least) == 0) continue;  // (the same for the workgroup: none is better than all so far)
+    auto index = [&](int p, int e) { return (uint32_t)(first(p) + e); };
+    auto add = [&](uint64_t key) {
+      const uint32_t at = atomicAdd(&s_n, 1u);
+      if (at < (uint32_t)kList) s_list[at] = key;
+    };
+    if (mx >= least) {
+#pragma unroll
+      for (int p = 0; p < kBsPieces; ++p)
+        if (some(p)) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const float v = value(p, e);
+            if (v >= least) {
+              const uint64_t key = bs_key(bs_order(v), index(p, e));
+              if (key > worst) add(key);
+            }
+          }
+        }
+    }
+    if (tid < a.k && s_best[tid] != 0) add(s_best[tid]);
+    __syncthreads();
+    if (s_n > (uint32_t)kList) {
+      // Too many alike for the list: by value and index, the k-th largest of the threads' largest.
+      uint64_t top = 0;
+#pragma unroll
+      for (int p = 0; p < kBsPieces; ++p)
+        if (some(p)) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const uint64_t key = bs_key(bs_order(value(p, e)), index(p, e));
+            top = key > top ? key : top;
+          }
+        }
+      s_key[tid] = top;
+      __syncthreads();
+      if (tid == 0) s_n = 0;
       int ahead = 0;
       for (int j = 0; j < kBsThreads; ++j) ahead += s_key[j] > top;
       if (ahead == a.k - 1 && top != 0) s_least = top;
       __syncthreads();
-      const uint64_t least = s_least > worst ? s_least : worst + 1;
+      const uint64_t from = s_least > worst ? s_least : worst + 1;
 #pragma unroll
-      for (int j = 0; j < kHeld; ++j) {
-        const uint64_t key = bs_key(bs_order(h[j]), index(j));
-        if (key >= least) s_list[atomicAdd(&s_n, 1u)] = key;
-      }
-      if (tid < a.k && s_best[tid] != 0) s_list[atomicAdd(&s_n, 1u)] = s_best[tid];
+      for (int p = 0; p < kBsPieces; ++p)
+        if (some(p)) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const uint64_t key = bs_key(bs_order(value(p, e)), index(p, e));
+            if (key >= from) add(key);
+          }
+        }
+      if (tid < a.k && s_best[tid] != 0) add(s_best[tid]);
       __syncthreads();
-      const int n = (int)s_n;
-      for (int i = tid; i < n; i += kBsThreads) {
-        const uint64_t key = s_list[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += s_list[j] > key;
-        if (rank < a.k) s_best[rank] = key;
-      }
+    }
+    const int n = (int)s_n;
+    for (int i = tid; i < n; i += kBsThreads) {
+      const uint64_t key = s_list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += s_list[j] > key;
+      if (rank < a.k) s_best[rank] = key;
     }
     __syncthreads();
+    if (tid == 0) s_n = 0, s_least = 1;
   }
+  // The waves' sums, to the largest of their maxima.
   sum = bs_wave_sum(sum);
-  if (lane == 0) s_sum[wave] = sum;
+  __syncthreads();
+  if (lane == 0) {
+    s_sum[wave] = sum;
+    s_max[wave][0] = m;
+  }
   __syncthreads();
   const int words = a.k + 2;
   {
     uint64_t *const p = a.part + (int64_t)blockIdx.x * words;
     if (tid == 0) {
+      float top = s_max[0][0];
+#pragma unroll
+      for (int w = 1; w < kBsWaves; ++w) top = fmaxf(top, s_max[w][0]);
       double all = 0.0;
 #pragma unroll
-      for (int w = 0; w < kBsWaves; ++w) all += s_sum[w];
-      bs_put(p, __builtin_bit_cast(uint32_t, m));
+      for (int w = 0; w < kBsWaves; ++w)
+        if (s_max[w][0] > -INFINITY) {
+          const double2 f = bs_exp(fmax((double)s_max[w][0] - (double)top, -700.0), s_tab);
+          all = fma(s_sum[w] * f.x, f.y, all);
+        }
+      bs_put(p, __builtin_bit_cast(uint32_t, top));
       bs_put(p + 1, __builtin_bit_cast(uint64_t, all));
     }
-    for (int i = tid; i < a.k; i += kBsThreads) bs_put(p + 2 + i, s_best[i]);
+    if (tid >= kWave && tid < kWave + a.k) bs_put(p + 2 + tid - kWave, s_best[tid - kWave]);
   }
   // The last of the search's workgroups to arrive goes on (nothing waits).
+  const int groups = a.W * a.chunks;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
     const uint32_t seen = __hip_atomic_fetch_add(a.count + search, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-    if (seen == (uint32_t)(a.W * a.chunks))
+    if (seen == (uint32_t)groups)
       __hip_atomic_store(a.count + search, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     s_seen = seen;
     s_n = 0;
-    s_least = 1;
-    s_least_at = 0xffffffffu;
   }
   __syncthreads();
-  if (s_seen != (uint32_t)(a.W * a.chunks)) return;
-  const uint64_t *const all = a.part + (int64_t)search * a.W * a.chunks * words;
+  if (s_seen != (uint32_t)groups) return;
+  const uint64_t *const all = a.part + (int64_t)search * groups * words;
+  const int n_all = groups * a.k;
+  auto key_of = [&](int i) {
+    const int g = i / a.k;
+    return bs_get(all + (int64_t)g * words + 2 + (i - g * a.k));
+  };
+  uint64_t keys[kBsFew];
+#pragma unroll
+  for (int j = 0; j < kBsFew; ++j) keys[j] = key_of(min(tid + j * kBsThreads, n_all - 1));
+  // Each part's maximum and sum; then each row's.
+  static_assert(kList >= kBsGroups, "the parts' maxima and sums fit the list");
+  double *const s_part = reinterpret_cast<double *>(s_list);
+  float *const s_pm = &s_max[0][0];
+  constexpr int kFew = kBsWaves * kWave;  // parts whose maxima fit s_max; of more they are read again
+  auto part_max = [&](int g) { return __builtin_bit_cast(float, (uint32_t)bs_get(all + (int64_t)g * words)); };
+  auto part_sum = [&](int g) { return __builtin_bit_cast(double, bs_get(all + (int64_t)g * words + 1)); };
+  for (int g = tid; g < groups; g += kBsThreads) {
+    const float pm = part_max(g);
+    s_part[g] = part_sum(g);
+    if (g < kFew) s_pm[g] = pm;
+  }
+  __syncthreads();
   for (int w = tid; w < a.W; w += kBsThreads) {
     float top = -INFINITY;
-    for (int i = 0; i < a.chunks; ++i)
-      top = fmaxf(top, __builtin_bit_cast(float, (uint32_t)bs_get(all + (int64_t)(w * a.chunks + i) * words)));
-    double total = 0.0;
-    if (top > -INFINITY && top < INFINITY)
-      for (int i = 0; i < a.chunks; ++i) {
-        const uint64_t *const p = all + (int64_t)(w * a.chunks + i) * words;
-        const float mi = __builtin_bit_cast(float, (uint32_t)bs_get(p));
-        if (mi > -INFINITY) total += __builtin_bit_cast(double, bs_get(p + 1)) * bs_exp((double)mi - (double)top);
-      }
+    for (int i = 0; i < a.chunks; ++i) {
+      const int g = w * a.chunks + i;
+      top = fmaxf(top, g < kFew ? s_pm[g] : part_max(g));
+    }
     s_top[w] = top;
+  }
+  __syncthreads();
+  for (int g = tid; g < groups; g += kBsThreads) {
+    const float pm = g < kFew ? s_pm[g] : part_max(g), top = s_top[g / a.chunks];
+    double part = 0.0;
+    if (pm > -INFINITY && top < INFINITY) {
+      const double2 f = bs_exp(fmax((double)pm - (double)top, -700.0), s_tab);
+      part = s_part[g] * f.x * f.y;
+    }
+    s_part[g] = part;
+  }
+  __syncthreads();
+  for (int w = tid; w < a.W; w += kBsThreads) {
+    double total = 0.0;
+    for (int i = 0; i < a.chunks; ++i) total += s_part[w * a.chunks + i];
     s_lse[w] = log(total);
   }
   __syncthreads();
-  auto cand = [&](int i) {  // (of W * chunks * k)
-    const int g = i / a.k, w = g / a.chunks;
-    const uint64_t key = bs_get(all + (int64_t)g * words + 2 + (i - g * a.k));
+  auto cand = [&](int i, uint64_t key) {  // (of W * chunks * k)
+    const int w = i / a.k / a.chunks;
     const float score = a.scores[search * a.W + w];
     BsCand r{0, 0xffffffffu};
     if (key == 0 || !(score > -INFINITY && score < INFINITY) || !(s_top[w] < INFINITY)) return r;
@@ -258,33 +373,37 @@ beam_select_kernel(const BsArgs a) {
     r.total = b >> 63 ? ~b : b | 1ull << 63;
     return r;
   };
-  const int n_all = a.W * a.chunks * a.k;
-  BsCand top{0, 0xffffffffu};
-  for (int i = tid; i < n_all; i += kBsThreads) {
-    const BsCand x = cand(i);
-    if (bs_before(x.total, x.at, top.total, top.at)) top = x;
+  // Again the k-th largest of 64 groups' largest, by the totals' upper 32 bits.
+  uint32_t most = 0;
+  BsCand few[kBsFew];
+#pragma unroll
+  for (int j = 0; j < kBsFew; ++j) {
+    few[j] = cand(min(tid + j * kBsThreads, n_all - 1), tid + j * kBsThreads < n_all ? keys[j] : 0);
+    most = max(most, (uint32_t)(few[j].total >> 32));
   }
-  s_key[tid] = top.total;
-  s_at[tid] = top.at;
+  for (int i = tid + kBsFew * kBsThreads; i < n_all; i += kBsThreads) most = max(most, (uint32_t)(cand(i, key_of(i)).total >> 32));
+  s_at[tid] = most;
   __syncthreads();
-  int ahead = 0;
-  for (int j = 0; j < kBsThreads; ++j) ahead += bs_before(s_key[j], s_at[j], top.total, top.at);
-  if (ahead == a.k - 1 && top.total != 0) {
-    s_least = top.total;
-    s_least_at = top.at;
+#pragma unroll
+  for (int w = 0; w < kBsWaves; ++w) most = max(most, s_at[w * kWave + lane]);
+  uint32_t least = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t to = least | 1u << bit;
+    if (__popcll(__ballot(most >= to)) >= a.k) least = to;
   }
-  __syncthreads();
-  const uint64_t least = s_least;
-  const uint32_t least_at = s_least_at;
-  for (int i = tid; i < n_all; i += kBsThreads) {
-    const BsCand x = cand(i);
-    if (x.total == 0 || bs_before(least, least_at, x.total, x.at)) continue;
+  __syncthreads();  // (s_at is used again)
+  auto add = [&](const BsCand &x) {
+    if (x.total == 0 || (uint32_t)(x.total >> 32) < least) return;
     const uint32_t at = atomicAdd(&s_n, 1u);
-    if (at < (uint32_t)kList) {
+    if (at < (uint32_t)kBsFinal) {
       s_list[at] = x.total;
       s_at[at] = x.at;
     }
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < kBsFew; ++j) add(few[j]);
+  for (int i = tid + kBsFew * kBsThreads; i < n_all; i += kBsThreads) add(cand(i, key_of(i)));
   __syncthreads();
   auto put = [&](int rank, uint64_t total, uint32_t at) {
     const int64_t o = (int64_t)search * a.k + rank;
@@ -293,8 +412,8 @@ beam_select_kernel(const BsArgs a) {
     a.rows[o] = total == 0 ? -1 : search * a.W + (int)w;
     a.tokens[o] = total == 0 ? -1 : (int64_t)(at - w * (uint32_t)a.V);
   };
-  const int n = (int)min(s_n, (uint32_t)kList);
-  if (s_n <= (uint32_t)kList) {
+  const int n = (int)min(s_n, (uint32_t)kBsFinal);
+  if (s_n <= (uint32_t)kBsFinal) {
     for (int i = tid; i < n; i += kBsThreads) {
       const uint64_t total = s_list[i];
       const uint32_t at = s_at[i];
@@ -310,7 +429,7 @@ beam_select_kernel(const BsArgs a) {
   for (int rank = 0; rank < a.k; ++rank) {
     BsCand next{0, 0xffffffffu};
     for (int i = tid; i < n_all; i += kBsThreads) {
-      const BsCand x = cand(i);
+      const BsCand x = cand(i, key_of(i));
       if (bs_before(last.total, last.at, x.total, x.at) && bs_before(x.total, x.at, next.total, next.at)) next = x;
     }
     __syncthreads();

@@ -447,6 +447,21 @@ def test_beam_select_masked_rows(cuda_device, dtype):
     _check_beams(ops.beam_select(x, scores, k), x, scores, k)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_beam_select_signaling_nans(cuda_device, dtype):
+    """NaNs of every kind stand for nothing, also where they share a thread with the best."""
+    from moeinfra_amd import ops
+
+    V, k = 9001, 20
+    x = _logits(6, V, 8, dtype)
+    bits = x.view(torch.int16 if dtype is torch.bfloat16 else torch.int32)
+    nans = [0x7f81, 0xff81 - 65536, 0x7fc0] if dtype is torch.bfloat16 else [0x7f800001, 0xff80ff80 - (1 << 32), 0x7fc00000]
+    for i, n in enumerate(nans):
+        bits[:, 5 + i::7] = n
+    x, scores = x.to(cuda_device), torch.zeros((3, 2), device=cuda_device)
+    _check_beams(ops.beam_select(x, scores, k), x, scores, k)
+
+
 def test_beam_select_workspaces(cuda_device):
     from moeinfra_amd import ops
 
