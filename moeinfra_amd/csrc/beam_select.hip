@@ -15,13 +15,13 @@ namespace {
 constexpr int kBsThreads = 256;
 constexpr int kBsWaves = kBsThreads / kWave;
 constexpr int kBsMost = 64;      // continuations of a search at most
-constexpr int kBsPieces = 8;     // 16-byte pieces that a thread holds
+constexpr int kBsPieces = 4;     // 16-byte pieces that a thread holds
 constexpr int kBsMaxVocab = 1 << 20;
 constexpr int kBsMaxBeams = 256;
 constexpr int kBsMaxChunks = 64; // workgroups of a row at most
 constexpr int kBsFew = 4;        // continuations that a thread holds
-constexpr int kBsFinal = 1024;   // continuations of a search that are ranked at once
-constexpr int kBsGroups = 2048;  // workgroups that rows are divided up to
+constexpr int kBsList = 1024;    // candidates that are ranked at once
+constexpr int kBsGroups = 1024;  // workgroups that rows are divided up to
 constexpr int64_t kBsCounterBytes = 65536;  // arrival counters at the start of the workspace
 
 struct BsArgs {
@@ -54,27 +54,57 @@ __device__ __forceinline__ float bs_value(uint32_t o) {
 // A logit and its place: the larger logit first, of equal ones the lower index.
 __device__ __forceinline__ uint64_t bs_key(uint32_t o, uint32_t i) { return o == 0 ? 0 : (uint64_t)o << 32 | ~i; }
 
-// e^d for -700 <= d <= 0 to 2^-39 of its value: 2^(n / 32) e^r, n a whole number and |r| <= ln 2 / 64; 2^(j / 32)
-// of a table, e^r by its series up to r^4 / 4!.  (A table of a bank each: lanes of one entry share it.)
-constexpr int kBsTable = 32;
-__device__ __forceinline__ void bs_table(double *s_tab) {
-  if (threadIdx.x < kBsTable) s_tab[threadIdx.x] = exp2((double)threadIdx.x / kBsTable);
+// e^d for -700 <= d <= 0 to 2^-38 of its value, from t = 128 d / ln 2: 2^(n / 128) e^r, n a whole number and
+// |r| <= ln 2 / 256; 2^(j / 128) of a table, e^r by its series up to r^3 / 3!.  An entry's upper word lacks
+// j 2^13, so that adding n 2^13 to it leaves n / 128's whole part in its exponent.
+constexpr int kBsTable = 128;
+constexpr double kBsUnit = 0.69314718055994530942 / kBsTable;
+constexpr double kBsLow = -700.0;
+__device__ __forceinline__ void bs_table(uint2 *s_tab) {
+  if (threadIdx.x < kBsTable) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, exp2((double)threadIdx.x / kBsTable));
+    s_tab[threadIdx.x] = make_uint2((uint32_t)b, (uint32_t)(b >> 32) - (threadIdx.x << 13));
+  }
 }
-// The factors of e^d: {e^r, 2^(n / 32)}.
-__device__ __forceinline__ double2 bs_exp(double d, const double *s_tab) {
-  constexpr double kUnit = 0.69314718055994530942 / kBsTable, kWhole = 6755399441055744.0;  // 1.5 * 2^52
-  const double t = d * (1.0 / kUnit);
-  const double s = t + kWhole;      // n in its last bits
-  const double f = t - (s - kWhole);
-  const int n = (int)(uint32_t)__builtin_bit_cast(uint64_t, s);
-  double p = kUnit * kUnit * kUnit * kUnit / 24;
-  p = fma(p, f, kUnit * kUnit * kUnit / 6);
-  p = fma(p, f, kUnit * kUnit / 2);
-  p = fma(p, f, kUnit);
-  p = fma(p, f, 1.0);
-  const uint64_t b = __builtin_bit_cast(uint64_t, s_tab[n & (kBsTable - 1)]);
-  const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)(n >> 5) << 20);
-  return make_double2(p, __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)b));
+// Added to a sum: those of N, the table's entries of all of them under way at once.
+template <int N>
+__device__ __forceinline__ void bs_add_exp(double &sum, double (&t)[N], const uint2 *s_tab) {
+  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
+  uint32_t n[N];
+  uint2 b[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double s = t[i] + kWhole;              // n in its last bits
+    t[i] -= s - kWhole;
+    n[i] = (uint32_t)__builtin_bit_cast(uint64_t, s);
+    b[i] = s_tab[n[i] & (kBsTable - 1)];
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  double part[2] = {0.0, 0.0};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    double p = kBsUnit * kBsUnit * kBsUnit / 6;
+    p = fma(p, t[i], kBsUnit * kBsUnit / 2);
+    p = fma(p, t[i], kBsUnit);
+    p = fma(p, t[i], 1.0);
+    part[i & 1] = fma(p, __builtin_bit_cast(double, (uint64_t)(b[i].y + (n[i] << 13)) << 32 | b[i].x), part[i & 1]);
+  }
+  sum += part[0] + part[1];
+}
+__device__ __forceinline__ double bs_exp(double d, const uint2 *s_tab) {
+  double t[1] = {fmax(d, kBsLow) * (1.0 / kBsUnit)}, sum = 0.0;
+  bs_add_exp<1>(sum, t, s_tab);
+  return sum;
+}
+
+// The larger of two patterns as signed integers: of a word, or of each half.
+template <bool F32>
+__device__ __forceinline__ int32_t bs_most(uint32_t x, uint32_t y) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (F32)
+    return max((int32_t)x, (int32_t)y);
+  else
+    return __builtin_bit_cast(int32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2, x), __builtin_bit_cast(s16x2, y)));
 }
 
 template <class T>
@@ -107,18 +137,17 @@ __device__ __forceinline__ bool bs_before(uint64_t t0, uint32_t a0, uint64_t t1,
 // The k largest: the threads' maxima fall into 64 groups; of the k-th largest of those (its upper 16 bits)
 // and above there are k values at least, and few more, which go to a list and are ranked.
 template <bool F32>
-__global__ void __launch_bounds__(kBsThreads)
+__global__ void __launch_bounds__(kBsThreads, 4)
 beam_select_kernel(const BsArgs a) {
   using E = typename std::conditional<F32, float, uint16_t>::type;
   constexpr int kPer = 16 / sizeof(E);              // values of a piece
   constexpr int kHeld = kBsPieces * kPer;           // of a thread
-  constexpr int kList = kBsMost * kHeld + kBsMost;  // those of k threads, and the best so far
   constexpr uint32_t kLeast = 0x80;                 // upper 16 bits of the lowest finite value's order
-  __shared__ uint64_t s_list[kList], s_key[kBsThreads], s_best[kBsMost];
-  __shared__ uint32_t s_at[kBsFinal];
-  __shared__ double s_tab[kBsTable], s_sum[kBsWaves], s_lse[kBsMaxBeams];
+  __shared__ uint64_t s_list[kBsList], s_key[kBsThreads], s_best[kBsMost];
+  __shared__ uint32_t s_at[kBsList];
+  __shared__ double s_sum[kBsWaves], s_lse[kBsMaxBeams];
+  __shared__ uint2 s_tab[kBsTable];
   __shared__ float s_max[kBsWaves][kWave], s_top[kBsMaxBeams];
-  __shared__ uint64_t s_least;
   __shared__ uint32_t s_n, s_seen;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -130,141 +159,131 @@ beam_select_kernel(const BsArgs a) {
   const int lead = (int)((uintptr_t)(x + v0) % 16 / sizeof(E));
   bs_table(s_tab);
   if (tid < kBsMost) s_best[tid] = 0;
-  if (tid == 0) s_n = 0, s_least = 1;
-  float m = -INFINITY;  // of the wave's so far
-  double sum = 0.0;     // this thread's
-  for (int i0 = v0 - lead; i0 < v1; i0 += kBsThreads * kHeld) {
-    u32x4 h[kBsPieces];
-    auto first = [&](int p) { return i0 + (p * kBsThreads + tid) * kPer; };
-    auto some = [&](int p) { return i0 + p * kBsThreads * kPer < v1; };  // (the same for the workgroup)
-    auto value = [&](int p, int e) {
-      const uint32_t w = F32 ? h[p][e] : h[p][e >> 1];
-      return F32 ? __builtin_bit_cast(float, w) : e & 1 ? bf16hi_to_f32(w) : bf16lo_to_f32(w);
-    };
+  if (tid == 0) s_n = 0;
+  __syncthreads();
+  auto value_of = [](u32x4 w, int e) __attribute__((always_inline)) {
+    const uint32_t x = w[F32 ? e : e >> 1];
+    return F32 ? __builtin_bit_cast(float, x) : e & 1 ? bf16hi_to_f32(x) : bf16lo_to_f32(x);
+  };
+  auto add = [&](uint64_t key) {
+    const uint32_t at = atomicAdd(&s_n, 1u);
+    if (at < (uint32_t)kBsList) s_list[at] = key;
+  };
+  float m = -INFINITY;       // of the wave's so far
+  double sum = 0.0;          // this thread's
+  float least = -INFINITY;   // what goes to the list, once it is known
+  u32x4 h[kBsPieces], ahead[kBsPieces];
+  auto some = [&](int i0, int p) { return i0 + p * kBsThreads * kPer < v1; };  // (the same for the workgroup)
+  auto load = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
     for (int p = 0; p < kBsPieces; ++p) {
-      const int i = first(p);
-      h[p] = F32 ? (u32x4){0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}  // -inf
-                 : (u32x4){0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
-      if (!some(p)) continue;
+      const int i = i0 + (p * kBsThreads + tid) * kPer;
+      ahead[p] = F32 ? (u32x4){0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}  // -inf
+                     : (u32x4){0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+      if (!some(i0, p)) continue;
       if (i >= v0 && i + kPer <= v1) {
-        h[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(x + i));
+        ahead[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(x + i));
       } else {
 #pragma unroll
         for (int e = 0; e < kPer; ++e)
           if (i + e >= v0 && i + e < v1) {
             if constexpr (F32)
-              h[p][e] = __builtin_bit_cast(uint32_t, x[i + e]);
+              ahead[p][e] = __builtin_bit_cast(uint32_t, x[i + e]);
             else
-              h[p][e >> 1] = e & 1 ? (h[p][e >> 1] & 0xffffu) | (uint32_t)x[i + e] << 16
-                                   : (h[p][e >> 1] & 0xffff0000u) | x[i + e];
+              ahead[p][e >> 1] = e & 1 ? (ahead[p][e >> 1] & 0xffffu) | (uint32_t)x[i + e] << 16
+                                       : (ahead[p][e >> 1] & 0xffff0000u) | x[i + e];
           }
       }
     }
-    float mx = -INFINITY;
+  };
+  constexpr int kRound = kBsThreads * kHeld;
+  if (v0 < v1) load(v0 - lead);
+  for (int i0 = v0 - lead; i0 < v1; i0 += kRound) {
 #pragma unroll
-    for (int p = 0; p < kBsPieces; ++p)
-      if (some(p)) {
+    for (int p = 0; p < kBsPieces; ++p) h[p] = ahead[p];
+    if (i0 + kRound < v1) load(i0 + kRound);
+    // The largest, as integers of the patterns: right if one is not negative and none is NaN.
+    int32_t pm[kBsPieces], im = INT32_MIN;  // (of bf16 two halves)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const float v = value(p, e);
-          mx = v > mx ? v : mx;  // (a maximum with a signaling NaN is NaN)
+    for (int p = 0; p < kBsPieces; ++p) {
+      pm[p] = bs_most<F32>(bs_most<F32>(h[p][0], h[p][1]), bs_most<F32>(h[p][2], h[p][3]));
+      im = p == 0 ? pm[0] : bs_most<F32>(im, pm[p]);
+    }
+    if (!F32) im = max(im >> 16, (int32_t)(int16_t)im) << 16;
+    float mx = __builtin_bit_cast(float, im);
+    if (im < 0 || im > 0x7f800000) {
+      mx = -INFINITY;
+#pragma unroll
+      for (int p = 0; p < kBsPieces; ++p)
+        if (some(i0, p)) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const float v = value_of(h[p], e);
+            mx = v > mx ? v : mx;  // (a maximum with a signaling NaN would be NaN)
+          }
         }
-      }
-    __syncthreads();  // (the round before, the table)
-    s_max[wave][lane] = mx;
+    }
     float wm[1] = {mx};
     lane_groups_reduce<true>(wm, kWave);
+    wm[0] = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, wm[0])));
     if (wm[0] > m) {
-      if (m > -INFINITY) {
-        const double2 f = bs_exp(fmax((double)m - (double)wm[0], -700.0), s_tab);
-        sum = sum * f.x * f.y;
-      }
+      if (m > -INFINITY) sum *= bs_exp((double)m - (double)wm[0], s_tab);
       m = wm[0];
     }
     if (m > -INFINITY) {
       // (-inf and NaN weigh as good as nothing.  A row of +inf has no probabilities: its sum is not looked at.)
-      const double md = (double)m;
+      const double md = (double)m, mt = -md * (1.0 / kBsUnit);
+      const bool near = fabsf(m) <= 4096.0f;  // (one multiply-add: m 128 / ln 2 rounds by 2^-34, 2^-41 of a weight)
 #pragma unroll
       for (int p = 0; p < kBsPieces; ++p)
-        if (some(p)) {
+        if (some(i0, p)) {
+          double t[kPer];
+          if (near) {
 #pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            const double2 f = bs_exp(fmax((double)value(p, e) - md, -700.0), s_tab);
-            sum = fma(f.x, f.y, sum);
+            for (int e = 0; e < kPer; ++e) t[e] = fmax(fma((double)value_of(h[p], e), 1.0 / kBsUnit, mt), kBsLow / kBsUnit);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) t[e] = fmax((double)value_of(h[p], e) - md, kBsLow) * (1.0 / kBsUnit);
           }
+          bs_add_exp<kPer>(sum, t, s_tab);
         }
     }
-    __syncthreads();
-    const uint64_t worst = s_best[a.k - 1];
-    // The largest 16 bits that k groups reach, bit by bit.
-    float g = s_max[0][lane];
-#pragma unroll
-    for (int w = 1; w < kBsWaves; ++w) g = fmaxf(g, s_max[w][lane]);
-    const uint32_t og = bs_order(g) >> 16;
-    uint32_t t = 0;
-#pragma unroll
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t to = t | 1u << bit;
-      if (__popcll(__ballot(og >= to)) >= a.k) t = to;
-    }
-    t = max(t, kLeast);
-    t = max(t, (uint32_t)(worst >> 48));
-    const float least = bs_value(t << 16);
-    if (__ballot(g >= least) == 0) continue;  // (the same for the workgroup: none is better than all so far)
-    auto index = [&](int p, int e) { return (uint32_t)(first(p) + e); };
-    auto add = [&](uint64_t key) {
-      const uint32_t at = atomicAdd(&s_n, 1u);
-      if (at < (uint32_t)kList) s_list[at] = key;
-    };
-    if (mx >= least) {
-#pragma unroll
-      for (int p = 0; p < kBsPieces; ++p)
-        if (some(p)) {
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            const float v = value(p, e);
-            if (v >= least) {
-              const uint64_t key = bs_key(bs_order(v), index(p, e));
-              if (key > worst) add(key);
-            }
-          }
-        }
-    }
-    if (tid < a.k && s_best[tid] != 0) add(s_best[tid]);
-    __syncthreads();
-    if (s_n > (uint32_t)kList) {
-      // Too many alike for the list: by value and index, the k-th largest of the threads' largest.
-      uint64_t top = 0;
-#pragma unroll
-      for (int p = 0; p < kBsPieces; ++p)
-        if (some(p)) {
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            const uint64_t key = bs_key(bs_order(value(p, e)), index(p, e));
-            top = key > top ? key : top;
-          }
-        }
-      s_key[tid] = top;
+    float from = least;
+    if (least == -INFINITY) {
+      // The largest 16 bits that k groups reach, bit by bit: what is as large goes to the list, from now on
+      // too (until then all that there is).
+      s_max[wave][lane] = mx;
       __syncthreads();
-      if (tid == 0) s_n = 0;
-      int ahead = 0;
-      for (int j = 0; j < kBsThreads; ++j) ahead += s_key[j] > top;
-      if (ahead == a.k - 1 && top != 0) s_least = top;
-      __syncthreads();
-      const uint64_t from = s_least > worst ? s_least : worst + 1;
+      float g = s_max[0][lane];
+#pragma unroll
+      for (int w = 1; w < kBsWaves; ++w) g = fmaxf(g, s_max[w][lane]);
+      const uint32_t og = bs_order(g) >> 16;
+      uint32_t t = 0;
+#pragma unroll
+      for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t to = t | 1u << bit;
+        if (__popcll(__ballot(og >= to)) >= a.k) t = to;
+      }
+      from = bs_value(max(t, kLeast) << 16);
+      if (t >= kLeast) least = from;
+      __syncthreads();  // (before the maxima are written again)
+    }
+    if (mx >= from) {
+      // (A piece's largest pattern is enough to tell that none is above a positive value.)
+      const int32_t low = from > 0.0f ? __builtin_bit_cast(int32_t, from) : INT32_MIN;
 #pragma unroll
       for (int p = 0; p < kBsPieces; ++p)
-        if (some(p)) {
+        if ((F32 ? pm[p] : max(pm[p] & (int32_t)0xffff0000, (int32_t)((uint32_t)pm[p] << 16))) >= low) {
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
-            const uint64_t key = bs_key(bs_order(value(p, e)), index(p, e));
-            if (key >= from) add(key);
+            const float v = value_of(h[p], e);
+            if (v >= from) add(bs_key(bs_order(v), (uint32_t)(i0 + (p * kBsThreads + tid) * kPer + e)));
           }
         }
-      if (tid < a.k && s_best[tid] != 0) add(s_best[tid]);
-      __syncthreads();
     }
+  }
+  __syncthreads();
+  if (s_n <= (uint32_t)kBsList) {
     const int n = (int)s_n;
     for (int i = tid; i < n; i += kBsThreads) {
       const uint64_t key = s_list[i];
@@ -272,8 +291,29 @@ beam_select_kernel(const BsArgs a) {
       for (int j = 0; j < n; ++j) rank += s_list[j] > key;
       if (rank < a.k) s_best[rank] = key;
     }
-    __syncthreads();
-    if (tid == 0) s_n = 0, s_least = 1;
+  } else {
+    // More than the list holds (many alike, or rising): one by one, from memory.
+    uint64_t last = ~0ull;
+    for (int rank = 0; rank < a.k; ++rank) {
+      uint64_t top = 0;
+      for (int i = v0 + tid; i < v1; i += kBsThreads) {
+        float v;
+        if constexpr (F32)
+          v = x[i];
+        else
+          v = bf16_to_f32(x[i]);
+        const uint64_t key = bs_key(bs_order(v), (uint32_t)i);
+        top = key < last && key > top ? key : top;
+      }
+      top = bs_wave_max(top);
+      __syncthreads();
+      if (lane == 0) s_key[wave] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kBsWaves; ++w) top = s_key[w] > top ? s_key[w] : top;
+      last = top;
+      if (tid == 0) s_best[rank] = top;
+    }
   }
   // The waves' sums, to the largest of their maxima.
   sum = bs_wave_sum(sum);
@@ -294,8 +334,7 @@ beam_select_kernel(const BsArgs a) {
 #pragma unroll
       for (int w = 0; w < kBsWaves; ++w)
         if (s_max[w][0] > -INFINITY) {
-          const double2 f = bs_exp(fmax((double)s_max[w][0] - (double)top, -700.0), s_tab);
-          all = fma(s_sum[w] * f.x, f.y, all);
+          all = fma(s_sum[w], bs_exp((double)s_max[w][0] - (double)top, s_tab), all);
         }
       bs_put(p, __builtin_bit_cast(uint32_t, top));
       bs_put(p + 1, __builtin_bit_cast(uint64_t, all));
@@ -325,7 +364,7 @@ beam_select_kernel(const BsArgs a) {
 #pragma unroll
   for (int j = 0; j < kBsFew; ++j) keys[j] = key_of(min(tid + j * kBsThreads, n_all - 1));
   // Each part's maximum and sum; then each row's.
-  static_assert(kList >= kBsGroups, "the parts' maxima and sums fit the list");
+  static_assert(kBsList >= kBsGroups && kBsList >= kBsMaxBeams, "the parts' maxima and sums fit the list");
   double *const s_part = reinterpret_cast<double *>(s_list);
   float *const s_pm = &s_max[0][0];
   constexpr int kFew = kBsWaves * kWave;  // parts whose maxima fit s_max; of more they are read again
@@ -350,8 +389,7 @@ beam_select_kernel(const BsArgs a) {
     const float pm = g < kFew ? s_pm[g] : part_max(g), top = s_top[g / a.chunks];
     double part = 0.0;
     if (pm > -INFINITY && top < INFINITY) {
-      const double2 f = bs_exp(fmax((double)pm - (double)top, -700.0), s_tab);
-      part = s_part[g] * f.x * f.y;
+      part = s_part[g] * bs_exp((double)pm - (double)top, s_tab);
     }
     s_part[g] = part;
   }
@@ -386,24 +424,24 @@ beam_select_kernel(const BsArgs a) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kBsWaves; ++w) most = max(most, s_at[w * kWave + lane]);
-  uint32_t least = 0;
+  uint32_t lowest = 0;
 #pragma unroll
   for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t to = least | 1u << bit;
-    if (__popcll(__ballot(most >= to)) >= a.k) least = to;
+    const uint32_t to = lowest | 1u << bit;
+    if (__popcll(__ballot(most >= to)) >= a.k) lowest = to;
   }
   __syncthreads();  // (s_at is used again)
-  auto add = [&](const BsCand &x) {
-    if (x.total == 0 || (uint32_t)(x.total >> 32) < least) return;
+  auto rank_too = [&](const BsCand &x) {
+    if (x.total == 0 || (uint32_t)(x.total >> 32) < lowest) return;
     const uint32_t at = atomicAdd(&s_n, 1u);
-    if (at < (uint32_t)kBsFinal) {
+    if (at < (uint32_t)kBsList) {
       s_list[at] = x.total;
       s_at[at] = x.at;
     }
   };
 #pragma unroll
-  for (int j = 0; j < kBsFew; ++j) add(few[j]);
-  for (int i = tid + kBsFew * kBsThreads; i < n_all; i += kBsThreads) add(cand(i, key_of(i)));
+  for (int j = 0; j < kBsFew; ++j) rank_too(few[j]);
+  for (int i = tid + kBsFew * kBsThreads; i < n_all; i += kBsThreads) rank_too(cand(i, key_of(i)));
   __syncthreads();
   auto put = [&](int rank, uint64_t total, uint32_t at) {
     const int64_t o = (int64_t)search * a.k + rank;
@@ -412,8 +450,8 @@ beam_select_kernel(const BsArgs a) {
     a.rows[o] = total == 0 ? -1 : search * a.W + (int)w;
     a.tokens[o] = total == 0 ? -1 : (int64_t)(at - w * (uint32_t)a.V);
   };
-  const int n = (int)min(s_n, (uint32_t)kBsFinal);
-  if (s_n <= (uint32_t)kBsFinal) {
+  const int n = (int)min(s_n, (uint32_t)kBsList);
+  if (s_n <= (uint32_t)kBsList) {
     for (int i = tid; i < n; i += kBsThreads) {
       const uint64_t total = s_list[i];
       const uint32_t at = s_at[i];
@@ -443,12 +481,13 @@ beam_select_kernel(const BsArgs a) {
   }
 }
 
-// Workgroups of a row: as many as the device takes at once have work, each a piece per thread at least.
-int bs_chunks(int64_t rows, int64_t V) {
+// Workgroups of a row: as many as the device takes at once have work, each a piece per thread at lowest.
+int bs_chunks(int64_t rows, int64_t W, int64_t V) {
   int64_t c = rows > 0 ? kBsGroups / rows : 1;
   const int64_t most = (V + kBsThreads * 8 - 1) / (kBsThreads * 8);
   c = c < most ? c : most;
   c = c < kBsMaxChunks ? c : kBsMaxChunks;
+  c = c < kBsList / W ? c : kBsList / W;
   return c < 1 ? 1 : (int)c;
 }
 bool bs_sizes_ok(int64_t S, int64_t W, int64_t k) {
@@ -495,7 +534,7 @@ extern "C" int moe_beam_select(const void *logits, int32_t logits_f32, int64_t s
   a.W = (int)W;
   a.V = (int)V;
   a.k = k;
-  a.chunks = moe::bs_chunks(rows, V);
+  a.chunks = moe::bs_chunks(rows, W, V);
   // (Whole 16-byte pieces.)
   a.chunk = (int)(((V + a.chunks - 1) / a.chunks + 7) / 8 * 8);
   a.scores = (const float *)scores_f32;
