@@ -54,29 +54,30 @@ __device__ __forceinline__ float bs_value(uint32_t o) {
 // A logit and its place: the larger logit first, of equal ones the lower index.
 __device__ __forceinline__ uint64_t bs_key(uint32_t o, uint32_t i) { return o == 0 ? 0 : (uint64_t)o << 32 | ~i; }
 
-// e^d for -700 <= d <= 0 to 2^-38 of its value, from t = 128 d / ln 2: 2^(n / 128) e^r, n a whole number and
-// |r| <= ln 2 / 256; 2^(j / 128) of a table, e^r by its series up to r^3 / 3!.  An entry's upper word lacks
-// j 2^13, so that adding n 2^13 to it leaves n / 128's whole part in its exponent.
-constexpr int kBsTable = 128;
+// e^d for -700 <= d <= 0 to 2^-42 of its value, from t = 256 d / ln 2 + kBsBias: 2^(n / 256) e^r, n the whole
+// part of t (without the bias) and r of its fraction, 0 <= r < ln 2 / 256; 2^(j / 256) of a table, e^r by its
+// series up to r^3 / 3!.  An entry's upper word lacks the bias and j, 2^12 times, so that adding t's whole part
+// times 2^12 to it leaves that of n / 256 in its exponent.
+constexpr int kBsTable = 256;
 constexpr double kBsUnit = 0.69314718055994530942 / kBsTable;
 constexpr double kBsLow = -700.0;
+constexpr int kBsBias = 1 << 18;
+static_assert(kBsBias % kBsTable == 0 && kBsBias > -kBsLow / kBsUnit + 1, "t is never negative");
 __device__ __forceinline__ void bs_table(uint2 *s_tab) {
   if (threadIdx.x < kBsTable) {
     const uint64_t b = __builtin_bit_cast(uint64_t, exp2((double)threadIdx.x / kBsTable));
-    s_tab[threadIdx.x] = make_uint2((uint32_t)b, (uint32_t)(b >> 32) - (threadIdx.x << 13));
+    s_tab[threadIdx.x] = make_uint2((uint32_t)b, (uint32_t)(b >> 32) - ((threadIdx.x + kBsBias) << 12));
   }
 }
 // Added to a sum: those of N, the table's entries of all of them under way at once.
 template <int N>
 __device__ __forceinline__ void bs_add_exp(double &sum, double (&t)[N], const uint2 *s_tab) {
-  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
   uint32_t n[N];
   uint2 b[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const double s = t[i] + kWhole;              // n in its last bits
-    t[i] -= s - kWhole;
-    n[i] = (uint32_t)__builtin_bit_cast(uint64_t, s);
+    n[i] = (uint32_t)t[i];
+    t[i] = __builtin_amdgcn_fract(t[i]);
     b[i] = s_tab[n[i] & (kBsTable - 1)];
   }
   __builtin_amdgcn_sched_barrier(0);
@@ -87,12 +88,12 @@ __device__ __forceinline__ void bs_add_exp(double &sum, double (&t)[N], const ui
     p = fma(p, t[i], kBsUnit * kBsUnit / 2);
     p = fma(p, t[i], kBsUnit);
     p = fma(p, t[i], 1.0);
-    part[i & 1] = fma(p, __builtin_bit_cast(double, (uint64_t)(b[i].y + (n[i] << 13)) << 32 | b[i].x), part[i & 1]);
+    part[i & 1] = fma(p, __builtin_bit_cast(double, (uint64_t)(b[i].y + (n[i] << 12)) << 32 | b[i].x), part[i & 1]);
   }
   sum += part[0] + part[1];
 }
 __device__ __forceinline__ double bs_exp(double d, const uint2 *s_tab) {
-  double t[1] = {fmax(d, kBsLow) * (1.0 / kBsUnit)}, sum = 0.0;
+  double t[1] = {fmax(d, kBsLow) * (1.0 / kBsUnit) + kBsBias}, sum = 0.0;
   bs_add_exp<1>(sum, t, s_tab);
   return sum;
 }
@@ -105,6 +106,16 @@ __device__ __forceinline__ int32_t bs_most(uint32_t x, uint32_t y) {
     return max((int32_t)x, (int32_t)y);
   else
     return __builtin_bit_cast(int32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2, x), __builtin_bit_cast(s16x2, y)));
+}
+
+// Values below -500 as -500.
+template <bool F32>
+__device__ __forceinline__ uint32_t bs_floor(uint32_t x) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  if constexpr (F32)
+    return min(x, 0xc3fa0000u);
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, x), (u16x2){0xc3fa, 0xc3fa}));
 }
 
 template <class T>
@@ -232,18 +243,24 @@ beam_select_kernel(const BsArgs a) {
     }
     if (m > -INFINITY) {
       // (-inf and NaN weigh as good as nothing.  A row of +inf has no probabilities: its sum is not looked at.)
-      const double md = (double)m, mt = -md * (1.0 / kBsUnit);
-      const bool near = fabsf(m) <= 4096.0f;  // (one multiply-add: m 128 / ln 2 rounds by 2^-34, 2^-41 of a weight)
+      // Where a low value as good as nothing is one of -500 too, by a minimum of the patterns (unsigned, they
+      // rise as values fall below zero; positive NaN stay), and one multiply-add: m 256 / ln 2 rounds by 2^-35, 2^-43 of a weight.
+      const double md = (double)m, mt = kBsBias - md * (1.0 / kBsUnit);
+      const bool near = m >= -400.0f && m <= 200.0f && !__any(im > 0x7f800000);
 #pragma unroll
       for (int p = 0; p < kBsPieces; ++p)
         if (some(i0, p)) {
           double t[kPer];
           if (near) {
+            u32x4 w;
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) t[e] = fmax(fma((double)value_of(h[p], e), 1.0 / kBsUnit, mt), kBsLow / kBsUnit);
+            for (int e = 0; e < 4; ++e) w[e] = bs_floor<F32>(h[p][e]);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) t[e] = fma((double)value_of(w, e), 1.0 / kBsUnit, mt);
           } else {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) t[e] = fmax((double)value_of(h[p], e) - md, kBsLow) * (1.0 / kBsUnit);
+            for (int e = 0; e < kPer; ++e)
+              t[e] = fmax((double)value_of(h[p], e) - md, kBsLow) * (1.0 / kBsUnit) + kBsBias;
           }
           bs_add_exp<kPer>(sum, t, s_tab);
         }
