@@ -14,23 +14,25 @@ namespace moe {
 namespace {
 
 constexpr int kTaNodes = 64;   // drafted tokens of a sequence at most (bits of a mask)
-constexpr int kTaRows = 128;   // rows (token, query head of the group) of a workgroup
-constexpr int kTaWaves = kTaRows / 32;
-constexpr int kTaThreads = kTaWaves * kWave;
+constexpr int kTaTile = 64;    // keys that a batch is divided by
+constexpr int kTaUnit = 32;    // keys of a unit: what one wave multiplies, what the ring holds
 constexpr float kTaLog2e = 1.44269504088896341f;
 // The running reference may lag the maximum by this much (in powers of two) before the sums are
 // rescaled: weights up to 2^8, which fp32 sums and bf16 weights carry without loss.
 constexpr float kTaLag = 8.0f;
+constexpr float kTaFine = 4096.0f;
 constexpr int kTaStart = 2;    // tiles' time that beginning a row tile takes
 constexpr int kTaMinTiles = 2;
-constexpr int kTaJoin = 8;     // partial results that a thread has under way at a time
 constexpr int kTaMaxParts = 64;  // workgroups that share a row tile
-constexpr float kTaFine = 4096.0f;
+constexpr int kTaPages = 1024;   // page entries at hand
 constexpr int64_t kTaCounterBytes = 65536;  // arrival counters at the start of the workspace
 constexpr int kTaMaxPage = 4096;
 
-constexpr int ta_resident(int hd) { return hd == 256 ? 1 : 2; }  // workgroups of a CU
-constexpr int ta_keys(int hd) { return hd == 256 ? 32 : 64; }    // of a tile
+// Waves of a workgroup, one on a CU (of 256 dims a wave takes the registers of a SIMD); its rows (token,
+// query head of the group), 32 a wave; units in the ring.
+constexpr int ta_waves(int hd) { return hd == 256 ? 4 : 8; }
+constexpr int ta_rows(int hd) { return 32 * ta_waves(hd); }
+constexpr int ta_ring(int hd) { return 1024 / hd; }
 
 struct TaArgs {
   const uint16_t *q;
@@ -57,11 +59,18 @@ __device__ u32x4 ta_zeros[1024 / 16];
 // 64 lanes' 16 bytes each, at `lane` bytes from src, into LDS at dst + 16 * lane number, without
 // registers.  (In asm, as the compiler would wait for all of them before the next transposing read of the
 // other plane; the caller waits for vmcnt(0) and a barrier before it reads dst.)
-__device__ __forceinline__ void ta_load_lds(const void *src, uint32_t lane, const uint8_t *dst) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)dst);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane), "s"(src)
+__device__ __forceinline__ void ta_load_lds(const void *src, uint32_t lane, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(lane), "s"(src)
                : "memory", "m0");
+}
+
+// Four floats that pass between workgroups (of other XCDs): a device-scope store (whose completion
+// pa_last_of waits for), and loads that go past this XCD's caches.
+__device__ __forceinline__ void ta_put(float *p, f32x4 v) {
+  asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(v) : "memory");
+}
+__device__ __forceinline__ f32x4 ta_get(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 16));  // (16: sc1)
 }
 
 // A sequence: its first token's row, tokens, keys before them, keys with them, row and key tiles.
@@ -69,7 +78,7 @@ struct TaSeq {
   int tok0, n, len, keys, rtiles, tiles;
 };
 
-__device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_keys) {
+__device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_rows) {
   TaSeq s{0, 0, 0, 0, 0, 0};
   if (b >= a.B) return s;
   s.tok0 = min(max(a.cu[b], 0), a.T);
@@ -79,8 +88,8 @@ __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_keys) {
   const int cap = (int)(all < 0x7ffffc00 ? all : 0x7ffffc00);
   s.len = min(max(a.lens[b], 0), cap);
   s.keys = min(s.len + s.n, cap);
-  s.rtiles = (s.n * a.grp + kTaRows - 1) / kTaRows;
-  s.tiles = s.n > 0 ? max(1, (s.keys + tile_keys - 1) / tile_keys) : 0;
+  s.rtiles = (s.n * a.grp + tile_rows - 1) / tile_rows;
+  s.tiles = s.n > 0 ? max(1, (s.keys + kTaTile - 1) / kTaTile) : 0;
   return s;
 }
 
@@ -88,41 +97,49 @@ __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_keys) {
 // group's heads share the K and V tiles.  All row tiles of a KV head's batch lie one behind the other,
 // key tile by key tile, each behind kTaStart of nothing (what it costs to begin one); each of the KV
 // head's workgroups takes as much of that, and the last of those that share a row tile to arrive adds
-// their results up.  A workgroup takes 128 rows against its tiles, which come from memory straight into
-// one of two LDS planes while the other is multiplied:
+// their results up.  A workgroup's keys come from memory straight into a ring of units in LDS, some steps
+// ahead of the one that is multiplied:
 //
-//   S^T = K Q^T        lane (row of queries l % 32) holds 16 keys of its row per 32-key half
+//   S^T = K Q^T        lane (row of queries l % 32) holds 16 keys of its row per unit
 //   O^T += V^T P^T     P of a lane is the B operand as it stands; V is read transposed
 //
-// Up to 64 rows the waves are two for the rows and two for the halves of a tile.
+// With rows for more than half of the waves, each wave takes 32 rows against all units; else the waves are
+// two groups, for every other unit.
 template <int HD>
-__global__ void __launch_bounds__(kTaThreads, ta_resident(HD))
+__global__ void __launch_bounds__(ta_waves(HD) *kWave)
 paged_tree_attention_kernel(const TaArgs a) {
-  constexpr int kKeys = ta_keys(HD);
-  constexpr int kST = kKeys / 32;
+  constexpr int NW = ta_waves(HD), kThreads = NW * kWave, kRows = ta_rows(HD);
   constexpr int kRowB = HD * 2;
-  constexpr int kPlane = kKeys * kRowB;                 // bytes of a K or V tile
-  constexpr int kChunks = kPlane / 1024 / kTaWaves;      // 1 KB loads per wave and tile of K (and of V)
+  constexpr int kPlane = kTaUnit * kRowB;                // bytes of a unit's keys, and of its values
+  constexpr int kUnitB = 2 * kPlane;
+  constexpr int NU = ta_ring(HD);
   constexpr int kChunkKeys = 1024 / kRowB;
+  constexpr int kPer = HD == 256 ? 4 : 1;                // 1 KB chunks of K, and of V, of a unit per wave
+  constexpr int kLoads = HD == 64 ? 1 : 2 * kPer;        // (of 64 dims a wave loads either)
   constexpr int kDT = HD / 32;                           // 32-dim output tiles
-  constexpr int kGroups = kKeys / 8;                     // of 8 keys: a page is never less
-  constexpr bool kHalves = kST == 2;
-  __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2 * kPlane];
-  static_assert(kChunks * kTaWaves * 1024 == kPlane && kChunkKeys <= 8, "whole chunks, each of one page");
-  static_assert(!kHalves || 2 * (16 * kDT + 4) * kWave * 4 <= 4 * kPlane, "two waves' sums fit the planes");
+  __shared__ __attribute__((aligned(1024))) uint8_t s_kv[NU * kUnitB];
+  __shared__ int32_t s_page[kTaPages];
+  static_assert(kLoads * NW * 1024 == kUnitB && kChunkKeys <= 8, "whole chunks, each of one page");
+  static_assert(NW / 2 * (16 * kDT + 4) * kWave * 4 <= NU * kUnitB && kRows * kTaMaxParts * 4 <= NU * kUnitB,
+                "half of the waves' sums, and the parts' weights, fit the ring");
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int li = lane & 31, hh = lane >> 5;
   const int wg = (int)(blockIdx.x / (unsigned)a.nkv), kvh = (int)(blockIdx.x - (unsigned)wg * a.nkv);
   const int64_t head_at = ((int64_t)kvh * HD) << a.page_shift;
   const int pmask = (1 << a.page_shift) - 1;
-
-  // Bytes of a chunk of K and V at which this lane finds its 16 bytes (pieces swizzled by the row).
+  const uint32_t ring = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)s_kv);
+  const void *zeros = ta_zeros;
+  asm volatile("" : "+s"(zeros));  // (not loaded again and again)
+  // Bytes of a chunk at which this lane finds its 16 bytes (pieces swizzled by the row).
   const int lrow = lane / (kRowB / 16), lpiece = lane % (kRowB / 16);
-  const uint32_t klane = lrow * kRowB + 16 * (lpiece ^ pk_kx<HD>(wave * kChunkKeys + lrow));
-  const uint32_t vlane = lrow * kRowB + 16 * (lpiece ^ pk_vx<HD>(wave * kChunkKeys + lrow));
-  // Operand reads: K row 32 st + li, piece 2 s + hh.  V: lane group's dims 32 dt + 16 (l / 16 % 2) ..
-  // + 15 of keys 16 s + 8 n + 4 hh .. + 3; this lane's 8 bytes are in key l % 16 / 4 of the four.
+  const int mychunk = HD == 64 ? wave & 3 : wave, myrow = mychunk * kChunkKeys + lrow;
+  const bool mine_v = HD == 64 && wave >= 4;
+  const uint32_t klane = lrow * kRowB + 16 * (lpiece ^ (mine_v ? pk_vx<HD>(myrow) : pk_kx<HD>(myrow)));
+  const uint32_t vlane = lrow * kRowB + 16 * (lpiece ^ pk_vx<HD>(myrow));
+  // Operand reads: K row li, piece 2 s + hh.  V: lane group's dims 32 dt + 16 (l / 16 % 2) .. + 15 of
+  // keys 16 s + 8 n + 4 hh .. + 3; this lane's 8 bytes are in key l % 16 / 4 of the four.
   const uint32_t krd = li * kRowB, kx = 16 * (hh ^ pk_kx<HD>(li));
   const uint32_t vkey = 4 * hh + ((lane & 15) >> 2);
   const uint32_t vrd = kPlane + vkey * kRowB + 8 * (lane & 1);
@@ -133,9 +150,11 @@ paged_tree_attention_kernel(const TaArgs a) {
   // Tiles tile0 .. tile1 - 1 of row tile rt of sequence b, shared by the nact workgroups from `head` on.
   auto item = [&](int b, const TaSeq &w, int rt, int tile0, int tile1, int head, int nact, bool later,
                   bool inside) __attribute__((always_inline)) {
-    const int rows = w.n * a.grp, base = rt * kTaRows;
-    const bool half = kHalves && rows - base <= kTaRows / 2;
-    const int row0 = base + (half ? wave & 1 : wave) * 32;
+    const int rows = w.n * a.grp, base = rt * kRows;
+    const int limit = min(rows - base, kRows);               // rows of the tile
+    const bool two = limit <= kRows / 2;                      // groups of waves
+    const int wrow = two ? wave % (NW / 2) : wave, group = two ? wave / (NW / 2) : 0, ngroup = two ? 2 : 1;
+    const int row0 = base + wrow * 32;
     const bool busy = row0 < rows;
     const int r = min(row0 + li, rows - 1);
     const int t = r / a.grp;
@@ -147,84 +166,86 @@ paged_tree_attention_kernel(const TaArgs a) {
     {
       const uint16_t *qr = a.q + qrow * a.q_stride + (int64_t)qhead * HD + 8 * hh;
 #pragma unroll
-      for (int s = 0; s < HD / 16; ++s) {
-        qf[s] = *reinterpret_cast<const u32x4 *>(qr + 16 * s);
-        qf[s] = (qf[s] ^ flip) & keep;
-      }
+      for (int s = 0; s < HD / 16; ++s) qf[s] = *reinterpret_cast<const u32x4 *>(qr + 16 * s);
     }
-    const uint64_t mask = (a.masks != nullptr ? (uint64_t)a.masks[qrow] : ~0ull >> (63 - t)) & (~0ull >> (64 - w.n));
+    uint64_t mask = a.masks != nullptr ? (uint64_t)a.masks[qrow] : ~0ull >> (63 - t);
     const int32_t *trow = a.table + b * a.width;
-    // Page entry of lane l's 8 keys of a tile (-1: none of them is there).
-    auto entry = [&](int tile) {
-      const int64_t key = (int64_t)tile * kKeys + 8 * lane;
-      return lane < kGroups && key < w.keys ? trow[key >> a.page_shift] : -1;
-    };
-    // Tile `tile` into plane p; the 8-key groups whose pages exist.
-    auto load = [&](int tile, int p, int ent) __attribute__((always_inline)) {
-      const uint32_t there = (uint32_t)__ballot((uint32_t)ent < (uint64_t)a.num_pages);
+    const int u1 = min(2 * tile1, (w.keys + kTaUnit - 1) / kTaUnit);  // the last unit's end
+    // (A thread's first page entry on its way with the queries; these have to be there before the first
+    // load that is not waited for.)
+    const int32_t entry0 =
+        w.keys > 0 ? trow[min((2 * tile0 * kTaUnit >> a.page_shift) + (int)threadIdx.x, (w.keys - 1) >> a.page_shift)] : -1;
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int chunk = wave + i * kTaWaves, first = chunk * kChunkKeys;  // (of the tile's keys)
-        const int64_t page = __builtin_amdgcn_readlane(ent, first >> 3);
-        const int key = tile * kKeys + first;
-        const bool has = (there >> (first >> 3) & 1) != 0 && key < w.keys;
-        const int64_t at = page * a.page_stride + head_at + (int64_t)(key & pmask) * HD;
-        // (The rows of K are swizzled by their number in the tile, of which i changes one bit of 256 dims.)
-        ta_load_lds(has ? (const void *)(a.kc + at) : ta_zeros, klane ^ (HD == 256 ? (i & 1) * 128 : 0),
-                    s_kv[p] + chunk * 1024);
-        ta_load_lds(has ? (const void *)(a.vc + at) : ta_zeros, vlane, s_kv[p] + kPlane + chunk * 1024);
-      }
-      return there;
-    };
+    for (int s = 0; s < HD / 16; ++s) {
+      qf[s] = (qf[s] ^ flip) & keep;
+      asm volatile("" : "+v"(qf[s]));
+    }
+    mask &= ~0ull >> (64 - w.n);
+    asm volatile("" : "+v"(mask));
+
     f32x16 acc[kDT];
 #pragma unroll
     for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[dt][v] = 0.0f;
     float m = -INFINITY, l = 0.0f;  // (m in units of q.k)
-    // The products of ST 32-key parts of a tile, from part st0 on.  EDGE: a row may not see all of it.
-    auto compute = [&](int tile, int p, uint32_t there, int st0, auto st_c, auto edge_c) __attribute__((always_inline)) {
-      constexpr int ST = decltype(st_c)::value;
+    int pbase = 0;                  // page entries at hand: from this one on
+    bool odd_pages = false;         // some of them do not exist
+    // The products of unit u, which lies at buf.  EDGE: a row may not see all of it.
+    auto compute = [&](int u, const uint8_t *buf, auto edge_c) __attribute__((always_inline)) {
       constexpr bool kEdge = decltype(edge_c)::value;
-      const uint8_t *buf = s_kv[p] + 32 * st0 * kRowB;
       // (Addresses are a XOR with a constant away from these: computed, not held in registers.)
       uint32_t ka = kx, va = vx;
       asm volatile("" : "+v"(ka), "+v"(va));
-      f32x16 sc[ST];
+      f32x16 sc;
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
+      for (int v = 0; v < 16; ++v) sc[v] = 0.0f;
+      constexpr int kK = HD == 256 ? 4 : HD / 16;  // operands at a time (of 256 dims all would spill)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) sc[st][v] = 0.0f;
+      for (int i0 = 0; i0 < HD / 16; i0 += kK) {
+        u32x4 x[kK];
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i)
+        for (int i = 0; i < kK; ++i) x[i] = *reinterpret_cast<const u32x4 *>(buf + krd + (ka ^ (32 * (i0 + i))));
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int st = 0; st < ST; ++st) {
-          const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + krd + (ka ^ (32 * i)) + 32 * st * kRowB);
-          sc[st] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
-                                                           __builtin_bit_cast(bf16x8, qf[i]), sc[st], 0, 0, 0);
-        }
-      uint64_t seen = ~0ull;
+        for (int i = 0; i < kK; ++i)
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x[i]),
+                                                       __builtin_bit_cast(bf16x8, qf[i0 + i]), sc, 0, 0, 0);
+      }
+      // V of the second product on its way meanwhile (of 256 dims it would spill).
+      constexpr int kV = HD == 256 ? 1 : kDT;
+      uint2 vt[2][kV][2];
+      auto fetch = [&](int s, int dt, uint2 (&x)[2]) __attribute__((always_inline)) {
+        const uint8_t *v = buf + vrd + (va ^ (64 * dt)) + 16 * s * kRowB;
+        x[0] = pk_read_tr(v);
+        x[1] = pk_read_tr(v + 8 * kRowB);
+      };
+      if constexpr (HD != 256 && !kEdge) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int dt = 0; dt < kDT; ++dt) fetch(s, dt, vt[s][dt]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      uint32_t seen = ~0u;
       if constexpr (kEdge) {
-        // Keys of the part that the row sees, bit by bit.
-        const int d = tile * kKeys + 32 * st0 - w.len;
-        seen = d >= kTaNodes ? 0 : d >= 0 ? mask >> d : -d >= 64 ? ~0ull : mask << -d | ((1ull << -d) - 1);
-        uint64_t pages = 0;
+        // Keys of the unit that the row sees, bit by bit.
+        const int d = u * kTaUnit - w.len;
+        seen = d >= kTaNodes ? 0 : d >= 0 ? (uint32_t)(mask >> d) : -d >= 32 ? ~0u : (uint32_t)mask << -d | ((1u << -d) - 1);
+        if (w.keys - u * kTaUnit < 32) seen &= (1u << (w.keys - u * kTaUnit)) - 1;  // (the table may end before the tree)
+        if (odd_pages) {
+          const int key = min(u * kTaUnit + 8 * (lane & 3), w.keys - 1);
+          const uint64_t there = __ballot((uint32_t)s_page[(key >> a.page_shift) - pbase] < (uint64_t)a.num_pages);
 #pragma unroll
-        for (int i = 0; i < 4 * ST; ++i) pages |= (there >> (4 * st0 + i) & 1) != 0 ? 0xffull << (8 * i) : 0;
-        seen &= pages;
+          for (int i = 0; i < 4; ++i) seen &= (there >> i & 1) != 0 ? ~0u : ~(0xffu << (8 * i));
+        }
 #pragma unroll
-        for (int st = 0; st < ST; ++st)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int j = 32 * st + 8 * (v >> 2) + (v & 3);
-            sc[st][v] = (seen >> (4 * hh) >> j & 1) != 0 ? sc[st][v] : -INFINITY;
-          }
+        for (int v = 0; v < 16; ++v)
+          sc[v] = (seen >> (4 * hh) >> (8 * (v >> 2) + (v & 3)) & 1) != 0 ? sc[v] : -INFINITY;
       }
       float mx = -INFINITY;
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[st][v]);
+      for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[v]);
       mx = op_xor32<true>(mx);
       if (__any((mx - m) * c > kTaLag)) {
         const float mn = fmaxf(m, mx);
@@ -242,38 +263,32 @@ paged_tree_attention_kernel(const TaArgs a) {
       const float mc = mref * c;
       if (__all(fabsf(mc) <= kTaFine)) {
 #pragma unroll
-        for (int st = 0; st < ST; ++st)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) sc[st][v] = __builtin_amdgcn_exp2f(fmaf(sc[st][v], c, -mc));
+        for (int v = 0; v < 16; ++v) sc[v] = __builtin_amdgcn_exp2f(fmaf(sc[v], c, -mc));
       } else {
 #pragma unroll
-        for (int st = 0; st < ST; ++st)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) sc[st][v] = __builtin_amdgcn_exp2f((sc[st][v] - mref) * c);
+        for (int v = 0; v < 16; ++v) sc[v] = __builtin_amdgcn_exp2f((sc[v] - mref) * c);
       }
+      float part[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) l += sc[st][v];
+      for (int v = 4; v < 16; ++v) part[v & 3] += sc[v];
+      l += (part[0] + part[1]) + (part[2] + part[3]);
       if constexpr (kEdge) {
         // A key that a row does not see has a weight of zero, but zero times an infinity or NaN in its
         // values would come through: where there are such, key by key instead.
         bool odd = false;
 #pragma unroll 1
-        for (int at = 16 * lane; at < 32 * ST * kRowB; at += 16 * kWave) {
+        for (int at = 16 * lane; at < kPlane; at += 16 * kWave) {
           const u32x4 x = *reinterpret_cast<const u32x4 *>(buf + kPlane + at);
 #pragma unroll
           for (int e = 0; e < 4; ++e) odd |= (x[e] & 0x7f800000u) == 0x7f800000u || (x[e] & 0x7f80u) == 0x7f80u;
         }
         if (__any(odd)) {
 #pragma unroll 1
-          for (int j = 0; j < 32 * ST; ++j) {
-            const int mine = (j >> 5) * 16 + ((j >> 3) & 3) * 4 + (j & 3);
+          for (int j = 0; j < kTaUnit; ++j) {
+            const int mine = ((j >> 3) & 3) * 4 + (j & 3);
             float pj = 0.0f;
 #pragma unroll
-            for (int st = 0; st < ST; ++st)
-#pragma unroll
-              for (int v = 0; v < 16; ++v) pj = mine == 16 * st + v ? sc[st][v] : pj;
+            for (int v = 0; v < 16; ++v) pj = mine == v ? sc[v] : pj;
             pj = bf16r(__shfl(pj, li + 32 * ((j >> 2) & 1), kWave));
             if ((seen >> j & 1) == 0) continue;
 #pragma unroll
@@ -293,65 +308,108 @@ paged_tree_attention_kernel(const TaArgs a) {
         }
       }
 #pragma unroll
-      for (int s = 0; s < 2 * ST; ++s) {
+      for (int s = 0; s < 2; ++s) {
         u32x4 pf;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pf[j] = pack_bf16x2(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
+        for (int j = 0; j < 4; ++j) pf[j] = pack_bf16x2(sc[8 * s + 2 * j], sc[8 * s + 2 * j + 1]);
 #pragma unroll
         for (int dt = 0; dt < kDT; ++dt) {
-          const uint8_t *v = buf + vrd + (va ^ (64 * dt)) + 16 * s * kRowB;
-          const uint2 x0 = pk_read_tr(v), x1 = pk_read_tr(v + 8 * kRowB);
-          const u32x4 x = {x0.x, x0.y, x1.x, x1.y};
+          uint2 own[2];
+          if constexpr (HD == 256 || kEdge) fetch(s, dt, own);
+          const uint2 *const y = HD == 256 || kEdge ? own : vt[s][dt % kV];
+          const u32x4 x = {y[0].x, y[0].y, y[1].x, y[1].y};
           acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x),
                                                             __builtin_bit_cast(bf16x8, pf), acc[dt], 0, 0, 0);
         }
       }
     };
-    constexpr uint32_t kAll = (1u << kGroups) - 1;
-    // All tiles by ST parts a wave, from part st0 on: those that every row sees whole, then (from the first
-    // on that has no page) the others.
-    auto walk = [&](int st0, auto st_c) __attribute__((always_inline)) {
-      uint32_t there = load(tile0, 0, entry(tile0)), next = 0;
-      int ent = entry(tile0 + 1), p = 0, tile = tile0;
-      auto arrive = [&]() __attribute__((always_inline)) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // (the tile is there, and the other plane no longer read)
-        if (tile + 1 < tile1) {
-          next = load(tile + 1, p ^ 1, ent);
-          ent = entry(tile + 2);
+    // Units u .. u + UPS - 1 to their places in the ring.  (What lies behind the last key in its chunk is
+    // loaded too; chunks behind it, and of pages that do not exist, are zeros.)
+    auto load = [&](int u) __attribute__((always_inline)) {
+      constexpr int UPS = 2;
+      auto first = [&](int i) { return u * kTaUnit + (i / kPer) * kTaUnit + (mychunk + i % kPer * NW) * kChunkKeys; };
+      const int key = first(lane & (UPS * kPer - 1));
+      const int32_t page = s_page[min(key < w.keys ? (key >> a.page_shift) - pbase : 0, kTaPages - 1)];
+#pragma unroll
+      for (int i = 0; i < UPS * kPer; ++i) {
+        const int k = first(i);
+        const int64_t p = __builtin_amdgcn_readlane(page, i);
+        const bool has = k < w.keys && (uint64_t)p < (uint64_t)a.num_pages;
+        const int64_t at = p * a.page_stride + head_at + (int64_t)(k & pmask) * HD;
+        const int chunk = mychunk + i % kPer * NW;
+        const uint32_t dst = ring + ((uint32_t)(u + i / kPer) & (NU - 1)) * kUnitB + chunk * 1024;
+        if constexpr (HD == 64) {
+          ta_load_lds(has ? (const void *)((mine_v ? a.vc : a.kc) + at) : zeros, klane, dst + (mine_v ? kPlane : 0));
+        } else {
+          // (The rows of K are swizzled by their number in the unit, of which i changes one bit of 256 dims.)
+          ta_load_lds(has ? (const void *)(a.kc + at) : zeros, klane ^ (HD == 256 ? (i & 1) * 128 : 0), dst);
+          ta_load_lds(has ? (const void *)(a.vc + at) : zeros, vlane, dst + kPlane);
         }
-      };
-      for (const int whole = min(w.len / kKeys, tile1); tile < whole && there == kAll; ++tile, p ^= 1, there = next) {
-        arrive();
-        if (busy) compute(tile, p, there, st0, st_c, std::false_type{});
-      }
-      for (; tile < tile1; ++tile, p ^= 1, there = next) {
-        arrive();
-        // What lies behind the last key in its chunk has been loaded too: zeros in its place.
-        const int end = w.keys - tile * kKeys, more = -end & (kChunkKeys - 1);
-        if (end < kKeys && more != 0) {
-          const int tid = threadIdx.x;
-          if (tid < more * (kRowB / 16))
-            *reinterpret_cast<u32x4 *>(s_kv[p] + kPlane + end * kRowB + 16 * tid) = (u32x4){0, 0, 0, 0};
-          __syncthreads();
-        }
-        if (busy) compute(tile, p, there, st0, st_c, std::true_type{});
       }
     };
-    if constexpr (kHalves) {
-      if (half)
-        walk(wave >> 1, std::integral_constant<int, 1>{});
-      else
-        walk(0, std::integral_constant<int, 2>{});
-    } else {
-      walk(0, std::integral_constant<int, 1>{});
+    // Units ub .. ue - 1, two a step, of which a wave takes both, or with two groups one.
+    auto walk = [&](int ub, int ue) __attribute__((always_inline)) {
+      constexpr int UPS = 2;
+      constexpr int kAhead = NU / UPS - 1;  // steps
+      constexpr int kWait = (kAhead - 1) * UPS * kLoads;
+      static_assert(kAhead >= 1 && kWait < 64, "loads that may be under way");
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (ub + i * UPS < ue) load(ub + i * UPS);
+      int u = ub;
+      // Step u is there, and that before it no longer read; the next one to load takes its place.
+      auto arrive = [&]() __attribute__((always_inline)) {
+        if (u + kAhead * UPS < ue + UPS)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWait) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (u + kAhead * UPS < ue) load(u + kAhead * UPS);
+      };
+      // Those that every row sees whole, then the others.
+      const int whole = odd_pages ? ub : min(w.len / kTaUnit, ue);
+      for (; u + UPS <= whole; u += UPS) {
+        arrive();
+#pragma unroll 1
+        for (int i = busy ? group : UPS; i < UPS; i += ngroup) compute(u + i, s_kv + ((uint32_t)(u + i) & (NU - 1)) * kUnitB, std::false_type{});
+      }
+      for (; u < ue; u += UPS) {
+        arrive();
+        const int end = w.keys - u * kTaUnit, more = -end & (kChunkKeys - 1);
+        if (end < UPS * kTaUnit && more != 0) {  // (zeros behind the last key in its chunk of V)
+          const int tid = threadIdx.x;
+          if (tid < more * (kRowB / 16))
+            *reinterpret_cast<u32x4 *>(s_kv + ((uint32_t)(u + end / kTaUnit) & (NU - 1)) * kUnitB + kPlane + end % kTaUnit * kRowB + 16 * tid) =
+                (u32x4){0, 0, 0, 0};
+          __syncthreads();
+        }
+#pragma unroll 1
+        for (int i = busy ? group : UPS; i < UPS && u + i < ue; i += ngroup)
+          compute(u + i, s_kv + ((uint32_t)(u + i) & (NU - 1)) * kUnitB, std::true_type{});
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();  // (the ring is free)
+    };
+    // As many units at a time as there is room for page entries.
+    const int span = min((kTaPages - 2) << a.page_shift, 1 << 24) / kTaTile * (kTaTile / kTaUnit);
+    for (int ub = 2 * tile0; ub < u1; ub += span) {
+      const int ue = min(ub + span, u1);
+      pbase = ub * kTaUnit >> a.page_shift;
+      const int last = (min(ue * kTaUnit, w.keys) - 1) >> a.page_shift;
+      bool bad = false;
+      for (int i = threadIdx.x; i <= last - pbase; i += kThreads) {
+        const int32_t page = ub == 2 * tile0 && i == (int)threadIdx.x ? entry0 : trow[pbase + i];
+        s_page[i] = page;
+        bad |= (uint32_t)page >= (uint64_t)a.num_pages;
+      }
+      odd_pages = __syncthreads_or(bad) != 0;
+      walk(ub, ue);
     }
-    __syncthreads();  // (the planes are free)
     l = op_xor32<false>(l);
-    if (half) {
-      // The second half's sums through LDS.
-      float4 *const o = reinterpret_cast<float4 *>(&s_kv[0][0] + (wave & 1) * (16 * kDT + 4) * kWave * 4) + lane;
-      if (wave >= 2 && busy) {
+    if (two) {
+      // The second group's sums through LDS.
+      float4 *const o = reinterpret_cast<float4 *>(s_kv + wrow * (16 * kDT + 4) * kWave * 4) + lane;
+      if (group == 1 && busy) {
 #pragma unroll
         for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
@@ -360,7 +418,7 @@ paged_tree_attention_kernel(const TaArgs a) {
         o[4 * kDT * kWave] = make_float4(m, l, 0.0f, 0.0f);
       }
       __syncthreads();
-      if (wave < 2 && busy) {
+      if (group == 0 && busy) {
         const float4 ml = o[4 * kDT * kWave];
         const float mn = fmaxf(m, ml.x), mref = mn == -INFINITY ? 0.0f : mn;
         const float a0 = __builtin_amdgcn_exp2f((m - mref) * c);
@@ -380,7 +438,7 @@ paged_tree_attention_kernel(const TaArgs a) {
       }
     }
     // This wave's rows as results.
-    const bool writes = busy && !(half && wave >= 2);
+    const bool writes = busy && group == 0;
     if (nact == 1) {
       if (writes && row0 + li < rows) {  // (no key at all: zeros)
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -393,20 +451,20 @@ paged_tree_attention_kernel(const TaArgs a) {
                 make_uint2(pack_bf16x2(acc[dt][v] * inv, acc[dt][v + 1] * inv),
                            pack_bf16x2(acc[dt][v + 2] * inv, acc[dt][v + 3] * inv));
       }
-      __syncthreads();  // (before the planes are used again)
+      __syncthreads();  // (before the ring is used again)
       return;
     }
-    // A partial result: two values of each lane next to each other, then the rows' m and l.
-    const int limit = min(rows - base, kTaRows);  // rows of the tile
+    // A partial result: four values of each lane next to each other, then the rows' m and l.
     const int sums = (limit + 31) / 32 * 32 * HD;
     float *const own = a.part + ((int64_t)(2 * wg + (later ? 1 : 0)) * a.nkv + kvh) * a.place;
     if (writes) {
 #pragma unroll
       for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
-        for (int v = 0; v < 16; v += 2)
-          pa_put(own + (row0 - base) * HD + ((8 * dt + v / 2) * kWave + lane) * 2, acc[dt][v], acc[dt][v + 1]);
-      if (hh == 0) pa_put(own + sums + 2 * (row0 - base + li), m, l);
+        for (int v = 0; v < 16; v += 4)
+          ta_put(own + wrow * 32 * HD + ((4 * dt + v / 4) * kWave + lane) * 4,
+                 (f32x4){acc[dt][v], acc[dt][v + 1], acc[dt][v + 2], acc[dt][v + 3]});
+      if (hh == 0) pa_put(own + sums + 2 * (wrow * 32 + li), m, l);
     }
     if (!pa_last_of(a.count + ((int64_t)b * a.rtiles + rt) * a.nkv + kvh, nact)) return;
     // The last of the row tile's workgroups adds their results up, in the order of the keys.  Result y
@@ -414,14 +472,29 @@ paged_tree_attention_kernel(const TaArgs a) {
     // (y = 0).
     const uint32_t step = 2 * (uint32_t)a.nkv * (uint32_t)a.place;
     const float *const all = a.part + (int64_t)head * step + (int64_t)kvh * a.place;
-    const uint32_t first = inside ? (uint32_t)a.nkv * (uint32_t)a.place : 0;
-    auto result = [&](int y, int at) { return pa_get(all + ((uint32_t)y * step + (y == 0 ? first : 0) + (uint32_t)at)); };
+    const uint32_t place0 = inside ? (uint32_t)a.nkv * (uint32_t)a.place : 0;
+    auto at_part = [&](int y) { return (uint32_t)y * step + (y == 0 ? place0 : 0); };
+    // (Bytes from `all` on: the workspace has less than 2^31.)
+    const __amdgpu_buffer_rsrc_t parts = __builtin_amdgcn_make_buffer_rsrc((void *)all, 0, 0x7fffffff, 0x00020000);
+    // A thread takes four neighbouring values at a time: kItems of them and kTogether results under way, the
+    // first while the weights are found.
+    constexpr int kItems = 4, kTogether = 4;
+    const int quads = sums / 4;
+    f32x4 x[kItems][kTogether];
+    auto fetch = [&](int i0, int y0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < kItems; ++k)
+#pragma unroll
+        for (int y = 0; y < kTogether; ++y)  // (past the last the last again)
+          x[k][y] = ta_get(parts, 4 * at_part(min(y0 + y, nact - 1)) + 16 * min(i0 + k * kThreads, quads - 1));
+    };
+    fetch(threadIdx.x, 0);
     // Their weights in LDS: a lane per result.
-    float *const s_w = reinterpret_cast<float *>(&s_kv[0][0]);
-    for (int i0 = wave * 8; i0 < limit; i0 += 8 * kTaWaves) {
+    float *const s_w = reinterpret_cast<float *>(s_kv);
+    for (int i0 = wave * 8; i0 < limit; i0 += 8 * NW) {
       float2 ml[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ml[i] = result(min(lane, nact - 1), sums + 2 * min(i0 + i, limit - 1));
+      for (int i = 0; i < 8; ++i) ml[i] = pa_get(all + at_part(min(lane, nact - 1)) + sums + 2 * min(i0 + i, limit - 1));
       float mx[8], ll[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx[i] = ml[i].x;
@@ -437,57 +510,62 @@ paged_tree_attention_kernel(const TaArgs a) {
         if (i0 + i < limit) s_w[(i0 + i) * kTaMaxParts + lane] = lane < nact ? (ll[i] == 0.0f ? 0.0f : mx[i] / ll[i]) : 0.0f;
     }
     __syncthreads();
-    // A thread takes two neighbouring values, kTaJoin results under way at a time.
-    for (int i = threadIdx.x; i < sums / 2; i += kTaThreads) {
-      const int at = i & (kWave - 1), word = i >> 6;               // lane, and two of its values
-      const int rr = word / (8 * kDT) * 32 + (at & 31), pair = word % (8 * kDT);
-      const float *const f = s_w + min(rr, limit - 1) * kTaMaxParts;
-      float o0 = 0.0f, o1 = 0.0f;
-      for (int y0 = 0; y0 < nact; y0 += kTaJoin) {
-        float2 x[kTaJoin];
+    for (int i0 = threadIdx.x; i0 < quads; i0 += kItems * kThreads) {
+      f32x4 o[kItems];
 #pragma unroll
-        for (int y = 0; y < kTaJoin; ++y) x[y] = result(min(y0 + y, nact - 1), 2 * i);
+      for (int k = 0; k < kItems; ++k) o[k] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      auto row_of = [&](int i) { return (i >> 6) / (4 * kDT) * 32 + (i & 31); };
+      for (int y0 = 0; y0 < nact; y0 += kTogether) {
+        if (y0 > 0 || i0 >= kItems * kThreads) fetch(i0, y0);
 #pragma unroll
-        for (int y = 0; y < kTaJoin; ++y) {  // (loads past the last result repeat it: zeros in their place)
-          o0 = fmaf(f[y0 + y], y0 + y < nact ? x[y].x : 0.0f, o0);
-          o1 = fmaf(f[y0 + y], y0 + y < nact ? x[y].y : 0.0f, o1);
+        for (int k = 0; k < kItems; ++k) {
+          const float *const f = s_w + min(row_of(min(i0 + k * kThreads, quads - 1)), limit - 1) * kTaMaxParts + y0;
+#pragma unroll
+          for (int y = 0; y < kTogether; ++y)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[k][e] = fmaf(f[y], y0 + y < nact ? x[k][y][e] : 0.0f, o[k][e]);
         }
       }
-      if (rr < limit) {
-        const int rg = base + rr, tok = rg / a.grp;
-        const int dim = 32 * (pair >> 3) + 8 * ((pair & 7) >> 1) + 4 * (at >> 5) + 2 * (pair & 1);
-        *reinterpret_cast<uint32_t *>(a.out + ((int64_t)(w.tok0 + tok) * a.nq + kvh * a.grp + rg - tok * a.grp) * HD + dim) =
-            pack_bf16x2(o0, o1);
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) {
+        const int i = i0 + k * kThreads, rr = row_of(i);
+        if (i >= quads || rr >= limit) continue;
+        const int rg = base + rr, tok = rg / a.grp, dim = 8 * ((i >> 6) % (4 * kDT)) + 4 * ((i & 63) >> 5);
+        *reinterpret_cast<uint2 *>(a.out + ((int64_t)(w.tok0 + tok) * a.nq + kvh * a.grp + rg - tok * a.grp) * HD + dim) =
+            make_uint2(pack_bf16x2(o[k][0], o[k][1]), pack_bf16x2(o[k][2], o[k][3]));
       }
     }
     __syncthreads();  // (as above)
   };
 
-  if (a.share == 0) {
-    const int b = wg / a.rtiles, rt = wg - b * a.rtiles;
-    const TaSeq w = ta_seq(a, b, kKeys);
-    if (rt < w.rtiles) item(b, w, rt, 0, w.tiles, 0, 1, false, false);
-    return;
+  // This workgroup's part of it all: places begin .. end - 1, or (share = 0) row tile wg % rtiles of a
+  // sequence.
+  const bool whole = a.share == 0;
+  const int seq = whole ? wg / a.rtiles : 0;
+  int per = 1, begin = 0, end = 0;
+  if (!whole) {
+    int total = 0, most = 0;
+    for (int i0 = 0; i0 < a.B; i0 += kWave) {
+      const TaSeq s = ta_seq(a, i0 + lane, kRows);
+      total += s.rtiles * (s.tiles + kTaStart);
+      most = max(most, s.tiles);
+    }
+    most = __builtin_amdgcn_readlane(pa_max(most), kWave - 1);
+    total = __builtin_amdgcn_readlane(pa_incl(total), kWave - 1);
+    // (A row tile meets at most kTaMaxParts workgroups, also where it starts inside the part of one.)
+    per = max(max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), kTaStart + kTaMinTiles),
+              (most + kTaMaxParts - 3) / (kTaMaxParts - 2));
+    begin = min(wg, a.share) * per;
+    end = begin + per;
+    if (begin >= total) return;
   }
-  int total = 0, most = 0;
-  for (int i0 = 0; i0 < a.B; i0 += kWave) {
-    const TaSeq s = ta_seq(a, i0 + lane, kKeys);
-    total += s.rtiles * (s.tiles + kTaStart);
-    most = max(most, s.tiles);
-  }
-  most = __builtin_amdgcn_readlane(pa_max(most), kWave - 1);
-  total = __builtin_amdgcn_readlane(pa_incl(total), kWave - 1);
-  // (A row tile meets at most kTaMaxParts workgroups, also where it starts inside the part of one.)
-  const int per = max(max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), kTaStart + kTaMinTiles),
-                      (most + kTaMaxParts - 3) / (kTaMaxParts - 2));
-  const int begin = min(wg, a.share) * per, end = begin + per;
-  if (begin >= total) return;
   int before = 0;  // of the sequences before these 64
-  for (int i0 = 0; i0 < a.B; i0 += kWave) {
-    const TaSeq s = ta_seq(a, i0 + lane, kKeys);
+  for (int i0 = seq & ~(kWave - 1); i0 < a.B; i0 += kWave) {
+    const TaSeq s = ta_seq(a, i0 + lane, kRows);
     const int cost = s.rtiles * (s.tiles + kTaStart), incl = pa_incl(cost), start = before + incl - cost;
     before += __builtin_amdgcn_readlane(incl, kWave - 1);
-    for (uint64_t mine = __ballot(cost > 0 && start < end && start + cost > begin); mine != 0; mine &= mine - 1) {
+    uint64_t mine = whole ? 1ull << (seq & (kWave - 1)) : __ballot(cost > 0 && start < end && start + cost > begin);
+    for (; mine != 0; mine &= mine - 1) {
       const int from = __builtin_ctzll(mine);
       TaSeq w;
       w.tok0 = __builtin_amdgcn_readlane(s.tok0, from);
@@ -496,25 +574,25 @@ paged_tree_attention_kernel(const TaArgs a) {
       w.keys = __builtin_amdgcn_readlane(s.keys, from);
       w.rtiles = __builtin_amdgcn_readlane(s.rtiles, from);
       w.tiles = __builtin_amdgcn_readlane(s.tiles, from);
-      for (int rt = 0; rt < w.rtiles; ++rt) {
-        // The row tile's first place.
-        const int s0 = __builtin_amdgcn_readlane(start, from) + rt * (w.tiles + kTaStart) + kTaStart;
-        const int tile0 = max(begin - s0, 0), tile1 = min(end - s0, w.tiles);
+      const int at = __builtin_amdgcn_readlane(start, from) + kTaStart, only = wg - seq * a.rtiles;
+      for (int rt = whole ? only : 0; rt < (whole ? min(only + 1, w.rtiles) : w.rtiles); ++rt) {
+        const int s0 = at + rt * (w.tiles + kTaStart);  // the row tile's first place
+        const int tile0 = whole ? 0 : max(begin - s0, 0), tile1 = whole ? w.tiles : min(end - s0, w.tiles);
         if (tile0 >= tile1) continue;
-        const int head = s0 / per, nact = (s0 + w.tiles - 1) / per - head + 1;
+        const int head = s0 / per, nact = whole ? 1 : (s0 + w.tiles - 1) / per - head + 1;
         item(i0 + from, w, rt, tile0, tile1, head, nact, s0 > begin, s0 > head * per);
       }
     }
-    if (before >= end) break;
+    if (whole || before >= end) break;
   }
 }
 
-int64_t ta_share(int32_t nkv, int hd) {
-  const int64_t s = ta_resident(hd) * (int64_t)device_cu_count() / nkv;
+int64_t ta_share(int32_t nkv) {
+  const int64_t s = (int64_t)device_cu_count() / nkv;
   return s < 1 ? 1 : s;
 }
 int64_t ta_place(int32_t grp, int hd) {
-  const int64_t rows = (int64_t)kTaNodes * grp < kTaRows ? kTaNodes * grp : kTaRows;
+  const int64_t rows = (int64_t)kTaNodes * grp < ta_rows(hd) ? kTaNodes * grp : ta_rows(hd);
   return rows * (hd + 2);
 }
 
@@ -529,7 +607,7 @@ bool ta_sizes_ok(int64_t B, int32_t nq, int32_t nkv, int32_t hd) {
 extern "C" int64_t moe_paged_tree_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
                                                             int32_t head_dim) {
   if (!moe::ta_sizes_ok(B, n_q_heads, n_kv_heads, head_dim)) return -1;
-  return moe::kTaCounterBytes + 2 * moe::ta_share(n_kv_heads, head_dim) * n_kv_heads *
+  return moe::kTaCounterBytes + 2 * moe::ta_share(n_kv_heads) * n_kv_heads *
                                     moe::ta_place(n_q_heads / n_kv_heads, head_dim) * 4;
 }
 
@@ -550,7 +628,7 @@ extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, in
   MOE_REQUIRE(page_size >= 8 && page_size <= moe::kTaMaxPage && (page_size & (page_size - 1)) == 0,
               "page size must be a power of two of 8 to %d (got %d)", moe::kTaMaxPage, page_size);
   const int32_t grp = n_q_heads / n_kv_heads;
-  const int64_t rtiles = ((int64_t)moe::kTaNodes * grp + moe::kTaRows - 1) / moe::kTaRows;
+  const int64_t rtiles = ((int64_t)moe::kTaNodes * grp + moe::ta_rows(head_dim) - 1) / moe::ta_rows(head_dim);
   // The tiles of a call are counted in 32 bits: of 32 keys, for each row tile.
   MOE_REQUIRE(table_width <= 0x7fffffff / page_size &&
                   (B == 0 || table_width * page_size <= ((int64_t)1 << 35) / (B * rtiles) - 128),
@@ -604,13 +682,13 @@ extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, in
   a.part = workspace ? (float *)((char *)workspace + moe::kTaCounterBytes) : nullptr;
   a.place = (int)moe::ta_place(grp, head_dim);
   const bool split = workspace != nullptr && B * rtiles * n_kv_heads <= moe::kTaCounterBytes / 4;
-  a.share = split ? (int)moe::ta_share(n_kv_heads, head_dim) : 0;
+  a.share = split ? (int)moe::ta_share(n_kv_heads) : 0;
   const int64_t groups = (split ? a.share : B * rtiles) * n_kv_heads;
-  MOE_REQUIRE(moe::launch_fits(groups, moe::kTaThreads), "bad sizes");
+  MOE_REQUIRE(moe::launch_fits(groups, moe::ta_waves(head_dim) * moe::kWave), "bad sizes");
   auto kern = head_dim == 64    ? moe::paged_tree_attention_kernel<64>
               : head_dim == 128 ? moe::paged_tree_attention_kernel<128>
                                 : moe::paged_tree_attention_kernel<256>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(moe::kTaThreads), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(moe::ta_waves(head_dim) * moe::kWave), 0, (hipStream_t)stream, a);
   MOE_LAUNCH_CHECK();
   return MOE_STATUS_OK;
 }
