@@ -21,6 +21,7 @@ constexpr float kTaLog2e = 1.44269504088896341f;
 // rescaled: weights up to 2^8, which fp32 sums and bf16 weights carry without loss.
 constexpr float kTaLag = 8.0f;
 constexpr float kTaFine = 4096.0f;
+constexpr int kTaAll = 2;
 constexpr int kTaStart = 2;    // tiles' time that beginning a row tile takes
 constexpr int kTaMinTiles = 2;
 constexpr int kTaMaxParts = 64;  // workgroups that share a row tile
@@ -60,7 +61,7 @@ __device__ u32x4 ta_zeros[1024 / 16];
 // registers.  (In asm, as the compiler would wait for all of them before the next transposing read of the
 // other plane; the caller waits for vmcnt(0) and a barrier before it reads dst.)
 __device__ __forceinline__ void ta_load_lds(const void *src, uint32_t lane, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(lane), "s"(src)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(dst), "v"(lane), "s"(src)
                : "memory", "m0");
 }
 
@@ -73,13 +74,14 @@ __device__ __forceinline__ f32x4 ta_get(__amdgpu_buffer_rsrc_t r, uint32_t at) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 16));  // (16: sc1)
 }
 
-// A sequence: its first token's row, tokens, keys before them, keys with them, row and key tiles.
+// A sequence: its first token's row, tokens, keys before them, keys with them, row and key tiles, what
+// one of these costs (in one group of waves twice what it costs two).
 struct TaSeq {
-  int tok0, n, len, keys, rtiles, tiles;
+  int tok0, n, len, keys, rtiles, tiles, each;
 };
 
 __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_rows) {
-  TaSeq s{0, 0, 0, 0, 0, 0};
+  TaSeq s{0, 0, 0, 0, 0, 0, 1};
   if (b >= a.B) return s;
   s.tok0 = min(max(a.cu[b], 0), a.T);
   s.n = min(min(max(a.cu[b + 1], s.tok0), a.T) - s.tok0, kTaNodes);
@@ -89,6 +91,7 @@ __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_rows) {
   s.len = min(max(a.lens[b], 0), cap);
   s.keys = min(s.len + s.n, cap);
   s.rtiles = (s.n * a.grp + tile_rows - 1) / tile_rows;
+  s.each = s.n * a.grp > tile_rows / 2 ? kTaAll : 1;
   s.tiles = s.n > 0 ? max(1, (s.keys + kTaTile - 1) / kTaTile) : 0;
   return s;
 }
@@ -118,7 +121,7 @@ paged_tree_attention_kernel(const TaArgs a) {
   constexpr int kLoads = HD == 64 ? 1 : 2 * kPer;        // (of 64 dims a wave loads either)
   constexpr int kDT = HD / 32;                           // 32-dim output tiles
   __shared__ __attribute__((aligned(1024))) uint8_t s_kv[NU * kUnitB];
-  __shared__ int32_t s_page[kTaPages];
+  __shared__ int64_t s_page[kTaPages];  // bytes from a cache's start to this head's rows of the page, -1: none
   static_assert(kLoads * NW * 1024 == kUnitB && kChunkKeys <= 8, "whole chunks, each of one page");
   static_assert(NW / 2 * (16 * kDT + 4) * kWave * 4 <= NU * kUnitB && kRows * kTaMaxParts * 4 <= NU * kUnitB,
                 "half of the waves' sums, and the parts' weights, fit the ring");
@@ -153,9 +156,11 @@ paged_tree_attention_kernel(const TaArgs a) {
     const int rows = w.n * a.grp, base = rt * kRows;
     const int limit = min(rows - base, kRows);               // rows of the tile
     const bool two = limit <= kRows / 2;                      // groups of waves
-    const int wrow = two ? wave % (NW / 2) : wave, group = two ? wave / (NW / 2) : 0, ngroup = two ? 2 : 1;
+    // (Neighbouring waves lie on different SIMDs: those of few rows first.)
+    const int side = !two ? NW : limit > kRows / 4 ? NW / 2 : limit > kRows / 8 ? NW / 4 : NW > 4 ? NW / 8 : 1;
+    const int wrow = wave & (side - 1), group = wave / side, ngroup = two ? 2 : 1;
     const int row0 = base + wrow * 32;
-    const bool busy = row0 < rows;
+    const bool busy = group < ngroup && row0 < rows;
     const int r = min(row0 + li, rows - 1);
     const int t = r / a.grp;
     const int qhead = kvh * a.grp + (r - t * a.grp);
@@ -191,13 +196,12 @@ paged_tree_attention_kernel(const TaArgs a) {
     float m = -INFINITY, l = 0.0f;  // (m in units of q.k)
     int pbase = 0;                  // page entries at hand: from this one on
     bool odd_pages = false;         // some of them do not exist
-    // The products of unit u, which lies at buf.  EDGE: a row may not see all of it.
-    auto compute = [&](int u, const uint8_t *buf, auto edge_c) __attribute__((always_inline)) {
-      constexpr bool kEdge = decltype(edge_c)::value;
-      // (Addresses are a XOR with a constant away from these: computed, not held in registers.)
-      uint32_t ka = kx, va = vx;
-      asm volatile("" : "+v"(ka), "+v"(va));
-      f32x16 sc;
+    auto at_unit = [&](int u) { return s_kv + ((uint32_t)u & (NU - 1)) * kUnitB; };
+    // S of the unit at buf.
+    auto scores = [&](const uint8_t *buf, f32x16 &sc) __attribute__((always_inline)) {
+      // (Addresses are a XOR with a constant away from this: computed, not held in registers.)
+      uint32_t ka = kx;
+      asm volatile("" : "+v"(ka));
 #pragma unroll
       for (int v = 0; v < 16; ++v) sc[v] = 0.0f;
       constexpr int kK = HD == 256 ? 4 : HD / 16;  // operands at a time (of 256 dims all would spill)
@@ -212,6 +216,15 @@ paged_tree_attention_kernel(const TaArgs a) {
           sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x[i]),
                                                        __builtin_bit_cast(bf16x8, qf[i0 + i]), sc, 0, 0, 0);
       }
+    };
+    // The products of unit u.  EDGE: a row may not see all of it.
+    auto compute = [&](int u, auto edge_c) __attribute__((always_inline)) {
+      constexpr bool kEdge = decltype(edge_c)::value;
+      const uint8_t *const buf = at_unit(u);
+      uint32_t va = vx;
+      asm volatile("" : "+v"(va));
+      f32x16 sc;
+      scores(buf, sc);
       // V of the second product on its way meanwhile (of 256 dims it would spill).
       constexpr int kV = HD == 256 ? 1 : kDT;
       uint2 vt[2][kV][2];
@@ -235,7 +248,7 @@ paged_tree_attention_kernel(const TaArgs a) {
         if (w.keys - u * kTaUnit < 32) seen &= (1u << (w.keys - u * kTaUnit)) - 1;  // (the table may end before the tree)
         if (odd_pages) {
           const int key = min(u * kTaUnit + 8 * (lane & 3), w.keys - 1);
-          const uint64_t there = __ballot((uint32_t)s_page[(key >> a.page_shift) - pbase] < (uint64_t)a.num_pages);
+          const uint64_t there = __ballot(s_page[(key >> a.page_shift) - pbase] >= 0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) seen &= (there >> i & 1) != 0 ? ~0u : ~(0xffu << (8 * i));
         }
@@ -323,69 +336,83 @@ paged_tree_attention_kernel(const TaArgs a) {
         }
       }
     };
-    // Units u .. u + UPS - 1 to their places in the ring.  (What lies behind the last key in its chunk is
-    // loaded too; chunks behind it, and of pages that do not exist, are zeros.)
-    auto load = [&](int u) __attribute__((always_inline)) {
-      constexpr int UPS = 2;
-      auto first = [&](int i) { return u * kTaUnit + (i / kPer) * kTaUnit + (mychunk + i % kPer * NW) * kChunkKeys; };
-      const int key = first(lane & (UPS * kPer - 1));
-      const int32_t page = s_page[min(key < w.keys ? (key >> a.page_shift) - pbase : 0, kTaPages - 1)];
+    // Where lane i finds chunk i's page (chunk i % kPer of this wave of unit u + i / kPer).
+    auto first = [&](int u, int i) { return (u + i / kPer) * kTaUnit + (mychunk + i % kPer * NW) * kChunkKeys; };
+    auto entry = [&](int u) {
+      const int key = min(first(u, lane & (2 * kPer - 1)), w.keys - 1);
+      return s_page[min((key >> a.page_shift) - pbase, kTaPages - 1)];
+    };
+    // Unit u + j, whose pages are in `ent`, to its place in the ring.  (What lies behind the last key in its
+    // chunk is loaded too; chunks behind it, and of pages that do not exist, are zeros.)
+    auto load = [&](int u, int j, int64_t ent) __attribute__((always_inline)) {
+      const uint32_t dst = ring + ((uint32_t)(u + j) & (NU - 1)) * kUnitB;
+      const bool some = odd_pages || (u + j + 1) * kTaUnit > w.keys;
 #pragma unroll
-      for (int i = 0; i < UPS * kPer; ++i) {
-        const int k = first(i);
-        const int64_t p = __builtin_amdgcn_readlane(page, i);
-        const bool has = k < w.keys && (uint64_t)p < (uint64_t)a.num_pages;
-        const int64_t at = p * a.page_stride + head_at + (int64_t)(k & pmask) * HD;
-        const int chunk = mychunk + i % kPer * NW;
-        const uint32_t dst = ring + ((uint32_t)(u + i / kPer) & (NU - 1)) * kUnitB + chunk * 1024;
+      for (int i = 0; i < kPer; ++i) {
+        const int k = first(u, j * kPer + i);
+        const uint32_t lo = __builtin_amdgcn_readlane((int)ent, j * kPer + i);
+        const int32_t hi = __builtin_amdgcn_readlane((int)(ent >> 32), j * kPer + i);
+        const int64_t at = ((int64_t)hi << 32 | lo) + (int64_t)(uint32_t)((k & pmask) * kRowB);
+        const uint8_t *ks = (const uint8_t *)(mine_v ? a.vc : a.kc) + at, *vs = (const uint8_t *)a.vc + at;
+        if (some) {
+          ks = k < w.keys && hi >= 0 ? ks : (const uint8_t *)zeros;
+          vs = k < w.keys && hi >= 0 ? vs : (const uint8_t *)zeros;
+        }
+        const int chunk = mychunk + i * NW;
         if constexpr (HD == 64) {
-          ta_load_lds(has ? (const void *)((mine_v ? a.vc : a.kc) + at) : zeros, klane, dst + (mine_v ? kPlane : 0));
+          ta_load_lds(ks, klane, dst + (mine_v ? kPlane : 0) + chunk * 1024);
         } else {
           // (The rows of K are swizzled by their number in the unit, of which i changes one bit of 256 dims.)
-          ta_load_lds(has ? (const void *)(a.kc + at) : zeros, klane ^ (HD == 256 ? (i & 1) * 128 : 0), dst);
-          ta_load_lds(has ? (const void *)(a.vc + at) : zeros, vlane, dst + kPlane);
+          ta_load_lds(ks, klane ^ (HD == 256 ? (i & 1) * 128 : 0), dst + chunk * 1024);
+          ta_load_lds(vs, vlane, dst + kPlane + chunk * 1024);
         }
       }
     };
-    // Units ub .. ue - 1, two a step, of which a wave takes both, or with two groups one.
+    // Units ub .. ue - 1, one a step for all waves, or with two groups one for each.
     auto walk = [&](int ub, int ue) __attribute__((always_inline)) {
-      constexpr int UPS = 2;
-      constexpr int kAhead = NU / UPS - 1;  // steps
-      constexpr int kWait = (kAhead - 1) * UPS * kLoads;
-      static_assert(kAhead >= 1 && kWait < 64, "loads that may be under way");
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (ub + i * UPS < ue) load(ub + i * UPS);
+      constexpr int kWait1 = (NU - 2) * kLoads, kWait2 = (NU - 4) * kLoads;  // loads that may be under way
+      static_assert(NU >= 4 && kWait1 < 64, "as many as can be waited for");
+      const int ahead = NU - ngroup;
+      for (int u = ub; u < ub + ahead; u += ngroup) {
+        if (u >= ue) break;
+        const int64_t ent = entry(u);
+        load(u, 0, ent);
+        if (two) load(u, 1, ent);
+      }
       int u = ub;
+      int64_t ent = entry(u + ahead);
       // Step u is there, and that before it no longer read; the next one to load takes its place.
       auto arrive = [&]() __attribute__((always_inline)) {
-        if (u + kAhead * UPS < ue + UPS)
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWait) : "memory");
-        else
+        if (u + ahead - ngroup >= ue)
           asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else if (two)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWait2) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWait1) : "memory");
         __syncthreads();
-        if (u + kAhead * UPS < ue) load(u + kAhead * UPS);
+        if (u + ahead < ue) {
+          load(u + ahead, 0, ent);
+          if (two) load(u + ahead, 1, ent);
+          ent = entry(u + ahead + ngroup);
+        }
       };
       // Those that every row sees whole, then the others.
       const int whole = odd_pages ? ub : min(w.len / kTaUnit, ue);
-      for (; u + UPS <= whole; u += UPS) {
+      for (; u + ngroup <= whole; u += ngroup) {
         arrive();
-#pragma unroll 1
-        for (int i = busy ? group : UPS; i < UPS; i += ngroup) compute(u + i, s_kv + ((uint32_t)(u + i) & (NU - 1)) * kUnitB, std::false_type{});
+        if (busy) compute(u + group, std::false_type{});
       }
-      for (; u < ue; u += UPS) {
+      for (; u < ue; u += ngroup) {
         arrive();
         const int end = w.keys - u * kTaUnit, more = -end & (kChunkKeys - 1);
-        if (end < UPS * kTaUnit && more != 0) {  // (zeros behind the last key in its chunk of V)
+        if (end < ngroup * kTaUnit && more != 0) {  // (zeros behind the last key in its chunk of V)
           const int tid = threadIdx.x;
           if (tid < more * (kRowB / 16))
-            *reinterpret_cast<u32x4 *>(s_kv + ((uint32_t)(u + end / kTaUnit) & (NU - 1)) * kUnitB + kPlane + end % kTaUnit * kRowB + 16 * tid) =
-                (u32x4){0, 0, 0, 0};
+            *reinterpret_cast<u32x4 *>(s_kv + ((uint32_t)(u + end / kTaUnit) & (NU - 1)) * kUnitB + kPlane +
+                                       end % kTaUnit * kRowB + 16 * tid) = (u32x4){0, 0, 0, 0};
           __syncthreads();
         }
-#pragma unroll 1
-        for (int i = busy ? group : UPS; i < UPS && u + i < ue; i += ngroup)
-          compute(u + i, s_kv + ((uint32_t)(u + i) & (NU - 1)) * kUnitB, std::true_type{});
+        if (busy && u + group < ue) compute(u + group, std::true_type{});
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();  // (the ring is free)
@@ -399,8 +426,9 @@ paged_tree_attention_kernel(const TaArgs a) {
       bool bad = false;
       for (int i = threadIdx.x; i <= last - pbase; i += kThreads) {
         const int32_t page = ub == 2 * tile0 && i == (int)threadIdx.x ? entry0 : trow[pbase + i];
-        s_page[i] = page;
-        bad |= (uint32_t)page >= (uint64_t)a.num_pages;
+        const bool is = (uint32_t)page < (uint64_t)a.num_pages;
+        s_page[i] = is ? 2 * (page * a.page_stride + head_at) : -1;
+        bad |= !is;
       }
       odd_pages = __syncthreads_or(bad) != 0;
       walk(ub, ue);
@@ -547,8 +575,8 @@ paged_tree_attention_kernel(const TaArgs a) {
     int total = 0, most = 0;
     for (int i0 = 0; i0 < a.B; i0 += kWave) {
       const TaSeq s = ta_seq(a, i0 + lane, kRows);
-      total += s.rtiles * (s.tiles + kTaStart);
-      most = max(most, s.tiles);
+      total += s.rtiles * (s.tiles * s.each + kTaStart);
+      most = max(most, s.tiles * s.each);
     }
     most = __builtin_amdgcn_readlane(pa_max(most), kWave - 1);
     total = __builtin_amdgcn_readlane(pa_incl(total), kWave - 1);
@@ -562,7 +590,7 @@ paged_tree_attention_kernel(const TaArgs a) {
   int before = 0;  // of the sequences before these 64
   for (int i0 = seq & ~(kWave - 1); i0 < a.B; i0 += kWave) {
     const TaSeq s = ta_seq(a, i0 + lane, kRows);
-    const int cost = s.rtiles * (s.tiles + kTaStart), incl = pa_incl(cost), start = before + incl - cost;
+    const int cost = s.rtiles * (s.tiles * s.each + kTaStart), incl = pa_incl(cost), start = before + incl - cost;
     before += __builtin_amdgcn_readlane(incl, kWave - 1);
     uint64_t mine = whole ? 1ull << (seq & (kWave - 1)) : __ballot(cost > 0 && start < end && start + cost > begin);
     for (; mine != 0; mine &= mine - 1) {
@@ -574,12 +602,15 @@ paged_tree_attention_kernel(const TaArgs a) {
       w.keys = __builtin_amdgcn_readlane(s.keys, from);
       w.rtiles = __builtin_amdgcn_readlane(s.rtiles, from);
       w.tiles = __builtin_amdgcn_readlane(s.tiles, from);
+      w.each = __builtin_amdgcn_readlane(s.each, from);
       const int at = __builtin_amdgcn_readlane(start, from) + kTaStart, only = wg - seq * a.rtiles;
       for (int rt = whole ? only : 0; rt < (whole ? min(only + 1, w.rtiles) : w.rtiles); ++rt) {
-        const int s0 = at + rt * (w.tiles + kTaStart);  // the row tile's first place
-        const int tile0 = whole ? 0 : max(begin - s0, 0), tile1 = whole ? w.tiles : min(end - s0, w.tiles);
+        // (The row tile's first place; its tile t is at s0 + t * each.)
+        const int s0 = at + rt * (w.tiles * w.each + kTaStart);
+        const int tile0 = whole || begin <= s0 ? 0 : (begin - s0 + w.each - 1) / w.each;
+        const int tile1 = whole ? w.tiles : end <= s0 ? 0 : min((end - s0 + w.each - 1) / w.each, w.tiles);
         if (tile0 >= tile1) continue;
-        const int head = s0 / per, nact = whole ? 1 : (s0 + w.tiles - 1) / per - head + 1;
+        const int head = s0 / per, nact = whole ? 1 : (s0 + (w.tiles - 1) * w.each) / per - head + 1;
         item(i0 + from, w, rt, tile0, tile1, head, nact, s0 > begin, s0 > head * per);
       }
     }
@@ -607,8 +638,8 @@ bool ta_sizes_ok(int64_t B, int32_t nq, int32_t nkv, int32_t hd) {
 extern "C" int64_t moe_paged_tree_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
                                                             int32_t head_dim) {
   if (!moe::ta_sizes_ok(B, n_q_heads, n_kv_heads, head_dim)) return -1;
-  return moe::kTaCounterBytes + 2 * moe::ta_share(n_kv_heads) * n_kv_heads *
-                                    moe::ta_place(n_q_heads / n_kv_heads, head_dim) * 4;
+  const int64_t share = moe::ta_share(n_kv_heads);  // (one workgroup has no parts)
+  return moe::kTaCounterBytes + (share > 1 ? 2 * share * n_kv_heads * moe::ta_place(n_q_heads / n_kv_heads, head_dim) * 4 : 0);
 }
 
 extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, int64_t T, const void *k_cache,
