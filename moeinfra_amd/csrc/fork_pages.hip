@@ -48,6 +48,144 @@ __device__ __forceinline__ void fp_add(int32_t *p, int v) {
   __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// The same for up to kFpFew rows and places, whose lengths, parents, pages and counts of writers lie in LDS
+// (a hash of pages), so that memory answers five times only, one after the other: the lengths, the table,
+// the counts' changes, the writers' counts, the free pages'.
+constexpr int kFpFew = 2048;
+constexpr int kFpSlots = 2 * kFpFew;
+constexpr int kFpTogether = 4;  // entries, and counts, that a thread has under way
+
+__global__ void __launch_bounds__(kFpThreads)
+fork_few_pages_kernel(const FpArgs a) {
+  __shared__ int s_len[kFpFew], s_parent[kFpFew], s_children[kFpFew], s_page[kFpFew], s_rank[kFpFew];
+  __shared__ int s_key[kFpSlots], s_writers[kFpSlots], s_sum[kFpWaves];
+  int *const s_free = s_children;  // (once these are counted)
+  const int tid = threadIdx.x;
+  const int P = 1 << a.page_shift;
+  auto kept = [&](int n) { return (int)min(((int64_t)n + a.ahead + P - 1) >> a.page_shift, a.width); };
+  auto good = [&](int page) { return page >= 0 && page < a.pages; };
+  const int n = a.rows * a.places;
+  for (int i = tid; i < a.old_rows; i += kFpThreads) {
+    s_len[i] = max(a.lens[i], 0);
+    s_children[i] = 0;
+  }
+  for (int i = tid; i < a.rows; i += kFpThreads) {
+    const int p = a.parents[i];
+    s_parent[i] = p >= 0 && p < a.old_rows ? p : -1;
+  }
+  for (int i = tid; i < n; i += kFpThreads) s_page[i] = -2;  // (no place)
+  for (int i = tid; i < kFpSlots; i += kFpThreads) {
+    s_key[i] = -1;
+    s_writers[i] = 0;
+  }
+  __syncthreads();
+  for (int i = tid; i < a.rows; i += kFpThreads) {
+    const int p = s_parent[i];
+    if (p >= 0) atomicAdd(&s_children[p], 1);
+    a.new_lens[i] = p >= 0 ? s_len[p] : 0;
+    a.copies[3 * i] = a.copies[3 * i + 1] = -1;
+    a.copies[3 * i + 2] = 0;
+  }
+  __syncthreads();
+  // Each old row lets its pages go, each new one takes those that it keeps.
+  const int width = (int)a.width, old_all = a.old_rows * width, new_all = a.rows * width;
+  for (int x0 = tid; x0 < old_all; x0 += kFpTogether * kFpThreads) {
+    int page[kFpTogether];
+#pragma unroll
+    for (int k = 0; k < kFpTogether; ++k) page[k] = a.table[min(x0 + k * kFpThreads, old_all - 1)];
+#pragma unroll
+    for (int k = 0; k < kFpTogether; ++k) {
+      const int x = x0 + k * kFpThreads;
+      if (x >= old_all || !good(page[k])) continue;
+      const int row = x / width, by = (x - row * width < kept(s_len[row]) ? s_children[row] : 0) - 1;
+      if (by != 0) fp_add(a.refs + page[k], by);
+    }
+  }
+  for (int x0 = tid; x0 < new_all; x0 += kFpTogether * kFpThreads) {
+    int page[kFpTogether];
+#pragma unroll
+    for (int k = 0; k < kFpTogether; ++k) {
+      const int x = min(x0 + k * kFpThreads, new_all - 1), row = x / width;
+      page[k] = s_parent[row] >= 0 ? a.table[(int64_t)s_parent[row] * width + (x - row * width)] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kFpTogether; ++k) {
+      const int x = x0 + k * kFpThreads;
+      if (x >= new_all) continue;
+      const int row = x / width, e = x - row * width, p = s_parent[row];
+      const bool keeps = p >= 0 && e < kept(s_len[max(p, 0)]);
+      a.new_table[x] = keeps ? page[k] : -1;
+      if (!keeps || e < s_len[p] >> a.page_shift) continue;
+      // Place i: entry len / P + i % places of row i / places, written to next.
+      const int i = row * a.places + e - (s_len[p] >> a.page_shift);
+      s_page[i] = good(page[k]) ? page[k] : -1;
+      if (!good(page[k])) continue;
+      uint32_t slot = (uint32_t)page[k] * 2654435761u >> 20;
+      static_assert(kFpSlots == 1 << 12, "the hash's upper 12 bits");
+      for (int held; (held = atomicCAS(&s_key[slot], -1, page[k])) != -1 && held != page[k];) slot = (slot + 1) & (kFpSlots - 1);
+      atomicAdd(&s_writers[slot], 1);
+      s_rank[i] = (int)slot;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < kFpSlots; i += kFpThreads) s_key[i] = n;
+  __syncthreads();
+  for (int i = tid; i < n; i += kFpThreads)
+    if (s_page[i] >= 0) atomicMin(&s_key[s_rank[i]], i);  // the first of a page's writers
+  __syncthreads();
+  // A page that only writers hold stays with the first of them; the others want one.
+  int wanted = 0;
+  for (int i0 = 0; i0 < n; i0 += kFpThreads) {
+    const int i = i0 + tid, page = i < n ? s_page[i] : -2;
+    bool wants = page == -1;
+    if (page >= 0) wants = s_key[s_rank[i]] != i || fp_read(a.refs + page) != s_writers[s_rank[i]];
+    int all;
+    const int rank = wanted + fp_scan(wants, s_sum, all);
+    if (i < n) s_rank[i] = wants ? rank : -1;
+    wanted += all;
+  }
+  int found = 0;
+  for (int64_t p0 = 0; p0 < a.pages && found < wanted; p0 += kFpTogether * kFpThreads) {
+    // (A thread's counts lie next to each other: free pages in rising order.)
+    int is[kFpTogether], mine = 0, all;
+    const int64_t at = p0 + kFpTogether * tid;
+#pragma unroll
+    for (int k = 0; k < kFpTogether; ++k) is[k] = fp_read(a.refs + min(at + k, a.pages - 1));
+#pragma unroll
+    for (int k = 0; k < kFpTogether; ++k) {
+      is[k] = at + k < a.pages && is[k] <= 0;
+      mine += is[k];
+    }
+    int rank = found + fp_scan(mine, s_sum, all);
+#pragma unroll
+    for (int k = 0; k < kFpTogether; ++k) {
+      if (is[k] && rank < wanted) s_free[rank] = (int)(at + k);
+      rank += is[k];
+    }
+    found += all;
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kFpThreads)
+    if (s_rank[i] >= 0 && s_page[i] >= 0) fp_add(a.refs + s_page[i], -1);
+  __syncthreads();
+  for (int i = tid; i < n; i += kFpThreads) {
+    const int rank = s_rank[i];
+    if (rank < 0) continue;
+    const int row = i / a.places, len = s_len[s_parent[row]], e = (len >> a.page_shift) + i - row * a.places;
+    const int fresh = rank < found ? s_free[rank] : -1;
+    a.new_table[row * width + e] = fresh;
+    if (fresh < 0) continue;
+    __hip_atomic_store(a.refs + fresh, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int used = len & (P - 1);
+    if (s_page[i] >= 0 && used > 0 && i == row * a.places) {
+      a.copies[3 * row] = s_page[i];
+      a.copies[3 * row + 1] = fresh;
+      a.copies[3 * row + 2] = used;
+    }
+  }
+  if (tid == 0) *a.missing = max(wanted - found, 0);
+}
+
 // One workgroup, as each step needs all of the one before.
 __global__ void __launch_bounds__(kFpThreads)
 fork_pages_kernel(const FpArgs a) {
@@ -193,7 +331,9 @@ extern "C" int moe_fork_pages(const void *page_table_i32, const void *lens_i32, 
                 (int32_t *)missing_i32, table_width, num_pages, (int)n_seqs, (int)n_new,
                 __builtin_ctz((unsigned)page_size), ahead, places, (int32_t *)workspace,
                 (int32_t *)workspace + num_pages};
-  hipLaunchKernelGGL(moe::fork_pages_kernel, dim3(1), dim3(moe::kFpThreads), 0, (hipStream_t)stream, a);
+  const bool few = n_seqs <= moe::kFpFew && n_new * places <= moe::kFpFew && n_seqs * table_width < (1 << 30) &&
+                   n_new * table_width < (1 << 30);
+  hipLaunchKernelGGL(few ? moe::fork_few_pages_kernel : moe::fork_pages_kernel, dim3(1), dim3(moe::kFpThreads), 0, (hipStream_t)stream, a);
   MOE_LAUNCH_CHECK();
   return MOE_STATUS_OK;
 }

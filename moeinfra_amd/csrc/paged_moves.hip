@@ -77,20 +77,22 @@ compact_paged_kv_kernel(const PmCache c, const int32_t *__restrict__ table, int6
   }
 }
 
-// A workgroup per copy, layer and kind (keys, values).
+// A workgroup per copy, layer, kind (keys, values) and group of heads, of about kPmFew pieces a thread.
 //
 // Bound: HBM where there are many copies, else the launch.
 __global__ void __launch_bounds__(kPmThreads)
-copy_pages_kernel(const PmCache c, const int32_t *__restrict__ copies) {
-  const int64_t unit = blockIdx.x >> 1, copy = unit / c.layers, layer = unit - copy * c.layers;
+copy_pages_kernel(const PmCache c, const int32_t *__restrict__ copies, int hgroups) {
+  const int64_t kind = blockIdx.x / hgroups, unit = kind >> 1, copy = unit / c.layers, layer = unit - copy * c.layers;
+  const int hg = (int)(blockIdx.x - kind * hgroups);
   const int64_t src = copies[3 * copy], dst = copies[3 * copy + 1];
   const int rows = min(copies[3 * copy + 2], 1 << c.page_shift);
   if (src < 0 || src >= c.pages || dst < 0 || dst >= c.pages || src == dst || rows <= 0) return;
-  uint16_t *const base = (blockIdx.x & 1 ? c.v : c.k) + layer * c.layer_stride;
+  const int h0 = (int)((int64_t)c.nkv * hg / hgroups), h1 = (int)((int64_t)c.nkv * (hg + 1) / hgroups);
+  const int64_t head_stride = (int64_t)c.hd << c.page_shift;
+  uint16_t *const base = (kind & 1 ? c.v : c.k) + layer * c.layer_stride + h0 * head_stride;
   const uint16_t *const from = base + src * c.page_stride;
   uint16_t *const to = base + dst * c.page_stride;
-  const int64_t head_stride = (int64_t)c.hd << c.page_shift;
-  const uint32_t per_head = (uint32_t)rows * (uint32_t)(c.hd >> 3), all = per_head * (uint32_t)c.nkv;
+  const uint32_t per_head = (uint32_t)rows * (uint32_t)(c.hd >> 3), all = per_head * (uint32_t)(h1 - h0);
   for (uint32_t i0 = threadIdx.x; i0 < all; i0 += kPmFew * kPmThreads) {
     u32x4 x[kPmFew];
     int64_t at[kPmFew];
@@ -174,13 +176,17 @@ extern "C" int moe_copy_pages_bf16(void *k_cache, void *v_cache, int64_t layers,
   if (const int rc = moe::pm_cache(k_cache, v_cache, layers, layer_stride, num_pages, page_size, page_stride, n_kv_heads,
                                    head_dim, c))
     return rc;
-  MOE_REQUIRE(n_copies >= 0 && n_copies <= 0x7fffffff && moe::launch_fits(2 * n_copies * layers, moe::kPmThreads),
+  // Heads of a workgroup: whole pages of them are some kPmFew pieces a thread.
+  const int64_t pieces = (int64_t)n_kv_heads * page_size * (head_dim / 8), each = moe::kPmFew * moe::kPmThreads;
+  int64_t hgroups = (pieces + each - 1) / each;
+  hgroups = hgroups < n_kv_heads ? hgroups : n_kv_heads;
+  MOE_REQUIRE(n_copies >= 0 && n_copies <= 0x7fffffff && moe::launch_fits(2 * n_copies * layers * hgroups, moe::kPmThreads),
               "bad sizes");
   if (n_copies == 0 || layers == 0 || num_pages == 0) return MOE_STATUS_OK;
   MOE_REQUIRE(copies_i32, "null pointer");
   MOE_REQUIRE((uintptr_t)copies_i32 % 4 == 0, "tensors must be aligned");
-  hipLaunchKernelGGL(moe::copy_pages_kernel, dim3((unsigned)(2 * n_copies * layers)), dim3(moe::kPmThreads), 0,
-                     (hipStream_t)stream, c, (const int32_t *)copies_i32);
+  hipLaunchKernelGGL(moe::copy_pages_kernel, dim3((unsigned)(2 * n_copies * layers * hgroups)), dim3(moe::kPmThreads), 0,
+                     (hipStream_t)stream, c, (const int32_t *)copies_i32, (int)hgroups);
   MOE_LAUNCH_CHECK();
   return MOE_STATUS_OK;
 }
