@@ -154,8 +154,8 @@ beam_select_kernel(const BsArgs a) {
   constexpr int kPer = 16 / sizeof(E);              // values of a piece
   constexpr int kHeld = kBsPieces * kPer;           // of a thread
   constexpr uint32_t kLeast = 0x80;                 // upper 16 bits of the lowest finite value's order
-  __shared__ uint64_t s_list[kBsList], s_key[kBsThreads], s_best[kBsMost];
-  __shared__ uint32_t s_at[kBsList];
+  __shared__ uint64_t s_list[kBsList + 8], s_key[kBsThreads], s_best[kBsMost];
+  __shared__ uint32_t s_at[kBsList + 8];
   __shared__ double s_sum[kBsWaves], s_lse[kBsMaxBeams];
   __shared__ uint2 s_tab[kBsTable];
   __shared__ float s_max[kBsWaves][kWave], s_top[kBsMaxBeams];
@@ -302,10 +302,14 @@ beam_select_kernel(const BsArgs a) {
   __syncthreads();
   if (s_n <= (uint32_t)kBsList) {
     const int n = (int)s_n;
+    if (tid < 8) s_list[n + tid] = 0;
+    __syncthreads();
     for (int i = tid; i < n; i += kBsThreads) {
       const uint64_t key = s_list[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += s_list[j] > key;
+      for (int j = 0; j < n; j += 8)  // (eight reads under way)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank += s_list[j + e] > key;
       if (rank < a.k) s_best[rank] = key;
     }
   } else {
@@ -469,11 +473,15 @@ beam_select_kernel(const BsArgs a) {
   };
   const int n = (int)min(s_n, (uint32_t)kBsList);
   if (s_n <= (uint32_t)kBsList) {
+    if (tid < 8) s_list[n + tid] = 0;
+    __syncthreads();
     for (int i = tid; i < n; i += kBsThreads) {
       const uint64_t total = s_list[i];
       const uint32_t at = s_at[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += bs_before(s_list[j], s_at[j], total, at);
+      for (int j = 0; j < n; j += 8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank += bs_before(s_list[j + e], s_at[j + e], total, at);
       if (rank < a.k) put(rank, total, at);
     }
     for (int i = n + tid; i < a.k; i += kBsThreads) put(i, 0, 0);

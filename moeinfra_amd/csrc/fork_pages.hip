@@ -53,7 +53,8 @@ __device__ __forceinline__ void fp_add(int32_t *p, int v) {
 // the counts' changes, the writers' counts, the free pages'.
 constexpr int kFpFew = 2048;
 constexpr int kFpSlots = 2 * kFpFew;
-constexpr int kFpTogether = 4;  // entries, and counts, that a thread has under way
+constexpr int kFpTogether = 4;  // counts that a thread has under way
+constexpr int kFpEntries = 8;   // entries of the table, old ones and new ones each
 
 __global__ void __launch_bounds__(kFpThreads)
 fork_few_pages_kernel(const FpArgs a) {
@@ -89,30 +90,23 @@ fork_few_pages_kernel(const FpArgs a) {
   __syncthreads();
   // Each old row lets its pages go, each new one takes those that it keeps.
   const int width = (int)a.width, old_all = a.old_rows * width, new_all = a.rows * width;
-  for (int x0 = tid; x0 < old_all; x0 += kFpTogether * kFpThreads) {
-    int page[kFpTogether];
+  for (int x0 = tid; x0 < max(old_all, new_all); x0 += kFpEntries * kFpThreads) {
+    int was[kFpEntries], page[kFpEntries];
 #pragma unroll
-    for (int k = 0; k < kFpTogether; ++k) page[k] = a.table[min(x0 + k * kFpThreads, old_all - 1)];
-#pragma unroll
-    for (int k = 0; k < kFpTogether; ++k) {
-      const int x = x0 + k * kFpThreads;
-      if (x >= old_all || !good(page[k])) continue;
-      const int row = x / width, by = (x - row * width < kept(s_len[row]) ? s_children[row] : 0) - 1;
-      if (by != 0) fp_add(a.refs + page[k], by);
-    }
-  }
-  for (int x0 = tid; x0 < new_all; x0 += kFpTogether * kFpThreads) {
-    int page[kFpTogether];
-#pragma unroll
-    for (int k = 0; k < kFpTogether; ++k) {
-      const int x = min(x0 + k * kFpThreads, new_all - 1), row = x / width;
-      page[k] = s_parent[row] >= 0 ? a.table[(int64_t)s_parent[row] * width + (x - row * width)] : -1;
+    for (int k = 0; k < kFpEntries; ++k) {
+      const int x = x0 + k * kFpThreads, row = x / width;
+      was[k] = x < old_all ? a.table[x] : -1;
+      page[k] = x < new_all && s_parent[row] >= 0 ? a.table[s_parent[row] * width + (x - row * width)] : -1;
     }
 #pragma unroll
-    for (int k = 0; k < kFpTogether; ++k) {
-      const int x = x0 + k * kFpThreads;
+    for (int k = 0; k < kFpEntries; ++k) {
+      const int x = x0 + k * kFpThreads, row = x / width, e = x - row * width;
+      if (good(was[k])) {
+        const int by = (e < kept(s_len[row]) ? s_children[row] : 0) - 1;
+        if (by != 0) fp_add(a.refs + was[k], by);
+      }
       if (x >= new_all) continue;
-      const int row = x / width, e = x - row * width, p = s_parent[row];
+      const int p = s_parent[row];
       const bool keeps = p >= 0 && e < kept(s_len[max(p, 0)]);
       a.new_table[x] = keeps ? page[k] : -1;
       if (!keeps || e < s_len[p] >> a.page_shift) continue;

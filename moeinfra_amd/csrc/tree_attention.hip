@@ -21,9 +21,9 @@ constexpr float kTaLog2e = 1.44269504088896341f;
 // rescaled: weights up to 2^8, which fp32 sums and bf16 weights carry without loss.
 constexpr float kTaLag = 8.0f;
 constexpr float kTaFine = 4096.0f;
-constexpr int kTaAll = 2;
+constexpr int kTaAll = 2;      // places of a tile that takes all waves
 constexpr int kTaStart = 2;    // tiles' time that beginning a row tile takes
-constexpr int kTaMinTiles = 2;
+constexpr int kTaLeast = 2;    // places of a workgroup at least (a tile)
 constexpr int kTaMaxParts = 64;  // workgroups that share a row tile
 constexpr int kTaPages = 1024;   // page entries at hand
 constexpr int64_t kTaCounterBytes = 65536;  // arrival counters at the start of the workspace
@@ -581,7 +581,7 @@ paged_tree_attention_kernel(const TaArgs a) {
     most = __builtin_amdgcn_readlane(pa_max(most), kWave - 1);
     total = __builtin_amdgcn_readlane(pa_incl(total), kWave - 1);
     // (A row tile meets at most kTaMaxParts workgroups, also where it starts inside the part of one.)
-    per = max(max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), kTaStart + kTaMinTiles),
+    per = max(max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), kTaLeast),
               (most + kTaMaxParts - 3) / (kTaMaxParts - 2));
     begin = min(wg, a.share) * per;
     end = begin + per;
