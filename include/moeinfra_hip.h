@@ -429,8 +429,11 @@ int moe_rope_paged_kv_slots_bf16(const void *qkv, int64_t qkv_stride, int64_t T,
  * rounded to bf16 before their sum (fp32) with v; keys of pages that the cache does not have weigh
  * nothing; what a node does not see (an infinity or NaN too) does not change its row; a row that sees
  * no key is zeros.  Rows of no sequence, and of nodes past the 64th, are left as they were.  out
- * [T, n_q * head_dim], 8-byte aligned.  The workspace (moe_paged_tree_attention_workspace_bytes) is one
- * of its own, with the same rules as moe_paged_attention_bf16's. */
+ * [T, n_q * head_dim], 8-byte aligned.  With a workspace (moe_paged_tree_attention_workspace_bytes, of one
+ * size for all batches of the same heads; 16-byte aligned; calls that share it must be ordered, what it
+ * holds before a call does not matter) several workgroups share a tree's keys, and a second launch adds
+ * their results up in a fixed order; null: a workgroup for each KV head and 256 rows (128 of 256 dims) of
+ * token and query head. */
 int64_t moe_paged_tree_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
                                                  int32_t head_dim);
 int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, int64_t T, const void *k_cache,

@@ -26,7 +26,6 @@ constexpr int kTaStart = 2;    // tiles' time that beginning a row tile takes
 constexpr int kTaLeast = 2;    // places of a workgroup at least (a tile)
 constexpr int kTaMaxParts = 64;  // workgroups that share a row tile
 constexpr int kTaPages = 1024;   // page entries at hand
-constexpr int64_t kTaCounterBytes = 65536;  // arrival counters at the start of the workspace
 constexpr int kTaMaxPage = 4096;
 
 // Waves of a workgroup, one on a CU (of 256 dims a wave takes the registers of a SIMD); its rows (token,
@@ -34,6 +33,12 @@ constexpr int kTaMaxPage = 4096;
 constexpr int ta_waves(int hd) { return hd == 256 ? 4 : 8; }
 constexpr int ta_rows(int hd) { return 32 * ta_waves(hd); }
 constexpr int ta_ring(int hd) { return 1024 / hd; }
+
+// A row tile that begins in a workgroup's part and goes on in others: its first row's token, rows, the first
+// one's number in its sequence, workgroups; whether it is the later one of the first's two results.
+struct TaJoin {
+  int tok0, rows, base, nact, later, unused[3];
+};
 
 struct TaArgs {
   const uint16_t *q;
@@ -48,7 +53,7 @@ struct TaArgs {
   int T, B, nq, nkv, grp, rtiles;
   float scaling;
   uint16_t *out;
-  uint32_t *count;
+  TaJoin *joins;  // of each workgroup
   float *part;
   int share;   // workgroups per KV head that a batch is shared by (0: a row tile each)
   int place;   // floats of a partial result
@@ -63,15 +68,6 @@ __device__ u32x4 ta_zeros[1024 / 16];
 __device__ __forceinline__ void ta_load_lds(const void *src, uint32_t lane, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(dst), "v"(lane), "s"(src)
                : "memory", "m0");
-}
-
-// Four floats that pass between workgroups (of other XCDs): a device-scope store (whose completion
-// pa_last_of waits for), and loads that go past this XCD's caches.
-__device__ __forceinline__ void ta_put(float *p, f32x4 v) {
-  asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(v) : "memory");
-}
-__device__ __forceinline__ f32x4 ta_get(__amdgpu_buffer_rsrc_t r, uint32_t at) {
-  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 16));  // (16: sc1)
 }
 
 // A sequence: its first token's row, tokens, keys before them, keys with them, row and key tiles, what
@@ -150,9 +146,9 @@ paged_tree_attention_kernel(const TaArgs a) {
   const uint32_t flip = a.scaling < 0.0f ? 0x80008000u : 0u, keep = a.scaling == 0.0f ? 0u : ~0u;
   const float c = (a.scaling == 0.0f ? 1.0f : fabsf(a.scaling)) * kTaLog2e;
 
-  // Tiles tile0 .. tile1 - 1 of row tile rt of sequence b, shared by the nact workgroups from `head` on.
-  auto item = [&](int b, const TaSeq &w, int rt, int tile0, int tile1, int head, int nact, bool later,
-                  bool inside) __attribute__((always_inline)) {
+  // Tiles tile0 .. tile1 - 1 of row tile rt of sequence b, shared by nact workgroups (later: it is not the first of
+  // this one's).
+  auto item = [&](int b, const TaSeq &w, int rt, int tile0, int tile1, int nact, bool later) __attribute__((always_inline)) {
     const int rows = w.n * a.grp, base = rt * kRows;
     const int limit = min(rows - base, kRows);               // rows of the tile
     const bool two = limit <= kRows / 2;                      // groups of waves
@@ -465,10 +461,9 @@ paged_tree_attention_kernel(const TaArgs a) {
           }
       }
     }
-    // This wave's rows as results.
-    const bool writes = busy && group == 0;
+    // This wave's rows, done or in part.
     if (nact == 1) {
-      if (writes && row0 + li < rows) {  // (no key at all: zeros)
+      if (busy && group == 0 && row0 + li < rows) {  // (no key at all: zeros)
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         uint16_t *const o = a.out + (qrow * a.nq + qhead) * HD + 4 * hh;
 #pragma unroll
@@ -483,85 +478,16 @@ paged_tree_attention_kernel(const TaArgs a) {
       return;
     }
     // A partial result: four values of each lane next to each other, then the rows' m and l.
-    const int sums = (limit + 31) / 32 * 32 * HD;
     float *const own = a.part + ((int64_t)(2 * wg + (later ? 1 : 0)) * a.nkv + kvh) * a.place;
-    if (writes) {
+    if (group == 0 && busy) {
 #pragma unroll
       for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
         for (int v = 0; v < 16; v += 4)
-          ta_put(own + wrow * 32 * HD + ((4 * dt + v / 4) * kWave + lane) * 4,
-                 (f32x4){acc[dt][v], acc[dt][v + 1], acc[dt][v + 2], acc[dt][v + 3]});
-      if (hh == 0) pa_put(own + sums + 2 * (wrow * 32 + li), m, l);
-    }
-    if (!pa_last_of(a.count + ((int64_t)b * a.rtiles + rt) * a.nkv + kvh, nact)) return;
-    // The last of the row tile's workgroups adds their results up, in the order of the keys.  Result y
-    // is workgroup head + y's: in its first place, but in its last if the row tile starts inside its part
-    // (y = 0).
-    const uint32_t step = 2 * (uint32_t)a.nkv * (uint32_t)a.place;
-    const float *const all = a.part + (int64_t)head * step + (int64_t)kvh * a.place;
-    const uint32_t place0 = inside ? (uint32_t)a.nkv * (uint32_t)a.place : 0;
-    auto at_part = [&](int y) { return (uint32_t)y * step + (y == 0 ? place0 : 0); };
-    // (Bytes from `all` on: the workspace has less than 2^31.)
-    const __amdgpu_buffer_rsrc_t parts = __builtin_amdgcn_make_buffer_rsrc((void *)all, 0, 0x7fffffff, 0x00020000);
-    // A thread takes four neighbouring values at a time: kItems of them and kTogether results under way, the
-    // first while the weights are found.
-    constexpr int kItems = 4, kTogether = 4;
-    const int quads = sums / 4;
-    f32x4 x[kItems][kTogether];
-    auto fetch = [&](int i0, int y0) __attribute__((always_inline)) {
-#pragma unroll
-      for (int k = 0; k < kItems; ++k)
-#pragma unroll
-        for (int y = 0; y < kTogether; ++y)  // (past the last the last again)
-          x[k][y] = ta_get(parts, 4 * at_part(min(y0 + y, nact - 1)) + 16 * min(i0 + k * kThreads, quads - 1));
-    };
-    fetch(threadIdx.x, 0);
-    // Their weights in LDS: a lane per result.
-    float *const s_w = reinterpret_cast<float *>(s_kv);
-    for (int i0 = wave * 8; i0 < limit; i0 += 8 * NW) {
-      float2 ml[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ml[i] = pa_get(all + at_part(min(lane, nact - 1)) + sums + 2 * min(i0 + i, limit - 1));
-      float mx[8], ll[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx[i] = ml[i].x;
-      lane_groups_reduce<true>(mx, kWave);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        mx[i] = __builtin_amdgcn_exp2f((ml[i].x - (mx[i] == -INFINITY ? 0.0f : mx[i])) * c);
-        ll[i] = lane < nact ? mx[i] * ml[i].y : 0.0f;
-      }
-      lane_groups_reduce<false>(ll, kWave);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i0 + i < limit) s_w[(i0 + i) * kTaMaxParts + lane] = lane < nact ? (ll[i] == 0.0f ? 0.0f : mx[i] / ll[i]) : 0.0f;
-    }
-    __syncthreads();
-    for (int i0 = threadIdx.x; i0 < quads; i0 += kItems * kThreads) {
-      f32x4 o[kItems];
-#pragma unroll
-      for (int k = 0; k < kItems; ++k) o[k] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-      auto row_of = [&](int i) { return (i >> 6) / (4 * kDT) * 32 + (i & 31); };
-      for (int y0 = 0; y0 < nact; y0 += kTogether) {
-        if (y0 > 0 || i0 >= kItems * kThreads) fetch(i0, y0);
-#pragma unroll
-        for (int k = 0; k < kItems; ++k) {
-          const float *const f = s_w + min(row_of(min(i0 + k * kThreads, quads - 1)), limit - 1) * kTaMaxParts + y0;
-#pragma unroll
-          for (int y = 0; y < kTogether; ++y)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[k][e] = fmaf(f[y], y0 + y < nact ? x[k][y][e] : 0.0f, o[k][e]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kItems; ++k) {
-        const int i = i0 + k * kThreads, rr = row_of(i);
-        if (i >= quads || rr >= limit) continue;
-        const int rg = base + rr, tok = rg / a.grp, dim = 8 * ((i >> 6) % (4 * kDT)) + 4 * ((i & 63) >> 5);
-        *reinterpret_cast<uint2 *>(a.out + ((int64_t)(w.tok0 + tok) * a.nq + kvh * a.grp + rg - tok * a.grp) * HD + dim) =
-            make_uint2(pack_bf16x2(o[k][0], o[k][1]), pack_bf16x2(o[k][2], o[k][3]));
-      }
+          *reinterpret_cast<f32x4 *>(own + wrow * 32 * HD + ((4 * dt + v / 4) * kWave + lane) * 4) =
+              (f32x4){acc[dt][v], acc[dt][v + 1], acc[dt][v + 2], acc[dt][v + 3]};
+      if (hh == 0)
+        *reinterpret_cast<float2 *>(own + (limit + 31) / 32 * 32 * HD + 2 * (wrow * 32 + li)) = make_float2(m, l);
     }
     __syncthreads();  // (as above)
   };
@@ -571,6 +497,7 @@ paged_tree_attention_kernel(const TaArgs a) {
   const bool whole = a.share == 0;
   const int seq = whole ? wg / a.rtiles : 0;
   int per = 1, begin = 0, end = 0;
+  TaJoin join{0, 0, 0, 0, 0, {0, 0, 0}};
   if (!whole) {
     int total = 0, most = 0;
     for (int i0 = 0; i0 < a.B; i0 += kWave) {
@@ -583,9 +510,8 @@ paged_tree_attention_kernel(const TaArgs a) {
     // (A row tile meets at most kTaMaxParts workgroups, also where it starts inside the part of one.)
     per = max(max((int)(((uint32_t)total + a.share - 1) / (uint32_t)a.share), kTaLeast),
               (most + kTaMaxParts - 3) / (kTaMaxParts - 2));
-    begin = min(wg, a.share) * per;
+    begin = wg * per;
     end = begin + per;
-    if (begin >= total) return;
   }
   int before = 0;  // of the sequences before these 64
   for (int i0 = seq & ~(kWave - 1); i0 < a.B; i0 += kWave) {
@@ -610,12 +536,90 @@ paged_tree_attention_kernel(const TaArgs a) {
         const int tile0 = whole || begin <= s0 ? 0 : (begin - s0 + w.each - 1) / w.each;
         const int tile1 = whole ? w.tiles : end <= s0 ? 0 : min((end - s0 + w.each - 1) / w.each, w.tiles);
         if (tile0 >= tile1) continue;
-        const int head = s0 / per, nact = whole ? 1 : (s0 + (w.tiles - 1) * w.each) / per - head + 1;
-        item(i0 + from, w, rt, tile0, tile1, head, nact, s0 > begin, s0 > head * per);
+        const int nact = whole ? 1 : (s0 + (w.tiles - 1) * w.each) / per - s0 / per + 1;
+        item(i0 + from, w, rt, tile0, tile1, nact, s0 > begin);
+        if (nact > 1 && tile0 == 0) join = {w.tok0, min(w.n * a.grp - rt * kRows, kRows), rt * kRows, nact, s0 > begin, {0, 0, 0}};
       }
     }
     if (whole || before >= end) break;
   }
+  if (!whole && threadIdx.x == 0) a.joins[wg * a.nkv + kvh] = join;
+}
+
+// The results of the workgroups that share a row tile added up, in the order of the keys: a workgroup takes 32
+// rows of what began in one workgroup's part.
+constexpr int kTjThreads = 256;
+template <int HD>
+__global__ void __launch_bounds__(kTjThreads)
+paged_tree_join_kernel(const TaArgs a) {
+  constexpr int kSlices = ta_rows(HD) / 32, kItems = 32 * HD / 4 / kTjThreads;
+  constexpr int kTogether = HD == 256 ? 4 : 8;  // results under way, kItems of each
+  __shared__ float s_w[32][kTaMaxParts + 1];
+  const int unit = (int)(blockIdx.x / kSlices), r0 = 32 * (int)(blockIdx.x % kSlices);
+  const int wg = unit / a.nkv, kvh = unit - wg * a.nkv;
+  const TaJoin j = a.joins[unit];
+  if (j.nact < 2 || r0 >= j.rows) return;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
+  const float c = (a.scaling == 0.0f ? 1.0f : fabsf(a.scaling)) * kTaLog2e;
+  // Result y is workgroup wg + y's: its first place, but (y = 0) its last if the row tile begins inside its part.
+  const int64_t step = 2 * (int64_t)a.nkv * a.place;
+  const float *const all = a.part + wg * step + (int64_t)kvh * a.place;
+  const int64_t first = j.later ? (int64_t)a.nkv * a.place : 0;
+  auto part = [&](int y) { return all + (y * step + (y == 0 ? first : 0)); };
+  const int sums = (j.rows + 31) / 32 * 32 * HD;
+  f32x4 x[kItems][kTogether];
+  auto fetch = [&](int y0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int y = 0; y < kTogether; ++y) {  // (past the last the last again)
+      const float *const p = part(min(y0 + y, j.nact - 1)) + r0 * HD + 4 * tid;
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) x[k][y] = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(p + 4 * k * kTjThreads));
+    }
+  };
+  fetch(0);
+  // Their weights: a lane per result, eight rows a wave.
+  {
+    float2 ml[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      ml[i] = *reinterpret_cast<const float2 *>(part(min(lane, j.nact - 1)) + sums + 2 * (r0 + 8 * wave + i));
+    float mx[8], ll[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx[i] = ml[i].x;
+    lane_groups_reduce<true>(mx, kWave);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      mx[i] = __builtin_amdgcn_exp2f((ml[i].x - (mx[i] == -INFINITY ? 0.0f : mx[i])) * c);
+      ll[i] = lane < j.nact ? mx[i] * ml[i].y : 0.0f;
+    }
+    lane_groups_reduce<false>(ll, kWave);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)  // (no key at all: zeros)
+      s_w[8 * wave + i][lane] = lane < j.nact && ll[i] != 0.0f ? mx[i] / ll[i] : 0.0f;
+  }
+  __syncthreads();
+  const int row = lane & 31;  // (of each of its items)
+  f32x4 o[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) o[k] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  for (int y0 = 0; y0 < j.nact; y0 += kTogether) {
+    if (y0 > 0) fetch(y0);
+#pragma unroll
+    for (int y = 0; y < kTogether; ++y) {
+      const float f = s_w[row][y0 + y];
+#pragma unroll
+      for (int k = 0; k < kItems; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[k][e] = fmaf(f, y0 + y < j.nact ? x[k][y][e] : 0.0f, o[k][e]);
+    }
+  }
+  if (r0 + row >= j.rows) return;
+  const int r = j.base + r0 + row, tok = r / a.grp;
+  uint16_t *const out = a.out + ((int64_t)(j.tok0 + tok) * a.nq + kvh * a.grp + r - tok * a.grp) * HD + 4 * (lane >> 5);
+#pragma unroll
+  for (int k = 0; k < kItems; ++k)  // (8 dims for each 64 items)
+    *reinterpret_cast<uint2 *>(out + 8 * (wave + k * (kTjThreads / kWave))) =
+        make_uint2(pack_bf16x2(o[k][0], o[k][1]), pack_bf16x2(o[k][2], o[k][3]));
 }
 
 int64_t ta_share(int32_t nkv) {
@@ -638,8 +642,8 @@ bool ta_sizes_ok(int64_t B, int32_t nq, int32_t nkv, int32_t hd) {
 extern "C" int64_t moe_paged_tree_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
                                                             int32_t head_dim) {
   if (!moe::ta_sizes_ok(B, n_q_heads, n_kv_heads, head_dim)) return -1;
-  const int64_t share = moe::ta_share(n_kv_heads);  // (one workgroup has no parts)
-  return moe::kTaCounterBytes + (share > 1 ? 2 * share * n_kv_heads * moe::ta_place(n_q_heads / n_kv_heads, head_dim) * 4 : 0);
+  const int64_t share = moe::ta_share(n_kv_heads), groups = share > 1 ? share * n_kv_heads : 0;
+  return groups * ((int64_t)sizeof(moe::TaJoin) + 2 * moe::ta_place(n_q_heads / n_kv_heads, head_dim) * 4);
 }
 
 extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, int64_t T, const void *k_cache,
@@ -709,17 +713,26 @@ extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, in
   a.rtiles = (int)rtiles;
   a.scaling = scaling;
   a.out = (uint16_t *)out;
-  a.count = (uint32_t *)workspace;
-  a.part = workspace ? (float *)((char *)workspace + moe::kTaCounterBytes) : nullptr;
+  const int64_t share = moe::ta_share(n_kv_heads);
+  a.joins = (moe::TaJoin *)workspace;
+  a.part = workspace ? (float *)(a.joins + share * n_kv_heads) : nullptr;
   a.place = (int)moe::ta_place(grp, head_dim);
-  const bool split = workspace != nullptr && B * rtiles * n_kv_heads <= moe::kTaCounterBytes / 4;
-  a.share = split ? (int)moe::ta_share(n_kv_heads) : 0;
-  const int64_t groups = (split ? a.share : B * rtiles) * n_kv_heads;
+  // (With a workgroup per KV head only, it has all there is.)
+  a.share = workspace != nullptr && share > 1 ? (int)share : 0;
+  const int64_t groups = (a.share > 0 ? a.share : B * rtiles) * n_kv_heads;
   MOE_REQUIRE(moe::launch_fits(groups, moe::ta_waves(head_dim) * moe::kWave), "bad sizes");
   auto kern = head_dim == 64    ? moe::paged_tree_attention_kernel<64>
               : head_dim == 128 ? moe::paged_tree_attention_kernel<128>
                                 : moe::paged_tree_attention_kernel<256>;
   hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(moe::ta_waves(head_dim) * moe::kWave), 0, (hipStream_t)stream, a);
   MOE_LAUNCH_CHECK();
+  if (a.share > 0) {
+    auto join = head_dim == 64    ? moe::paged_tree_join_kernel<64>
+                : head_dim == 128 ? moe::paged_tree_join_kernel<128>
+                                  : moe::paged_tree_join_kernel<256>;
+    const int64_t slices = moe::ta_rows(head_dim) / 32;
+    hipLaunchKernelGGL(join, dim3((unsigned)(groups * slices)), dim3(moe::kTjThreads), 0, (hipStream_t)stream, a);
+    MOE_LAUNCH_CHECK();
+  }
   return MOE_STATUS_OK;
 }

@@ -552,9 +552,7 @@ def paged_tree_attention_workspace(batch: int, n_q_heads: int, n_kv_heads: int, 
     n = lib().moe_paged_tree_attention_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim)
     if n < 0:
         raise ValueError(f"invalid attention sizes batch={batch} heads={n_q_heads}/{n_kv_heads} head_dim={head_dim}")
-    ws = torch.empty((n,), dtype=torch.uint8, device=device)
-    ws[:65536].zero_()
-    return ws
+    return torch.empty((n,), dtype=torch.uint8, device=device)
 
 
 def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,

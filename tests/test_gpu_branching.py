@@ -136,7 +136,7 @@ def test_paged_tree_attention_rows_of_no_sequence(cuda_device):
 
 def test_paged_tree_attention_workspaces(cuda_device):
     """The same bits without a workspace of the caller's, with one of another batch, and again; writes
-    stay inside; counters end as zeros."""
+    stay inside; what it holds before does not matter."""
     from moeinfra_amd import ops
 
     dev = cuda_device
@@ -144,14 +144,14 @@ def test_paged_tree_attention_workspaces(cuda_device):
     n = ops.paged_tree_attention_workspace(1, 32, 8, 128, dev).numel()
     guarded = torch.full((n + 8192,), 0x5a, dtype=torch.uint8, device=dev)
     ws = guarded[4096:4096 + n]
-    ws[:65536].zero_()
     a = t.run(workspace=ws)
     t.check(a)
     other = Trees(dev, [3000] * 9, [17] * 9, 32, 8, 128, 16, seed=6)
     other.check(other.run(workspace=ws))
     assert _same(a, t.run(workspace=ws)) and _same(a, t.run())
     assert bool((guarded[:4096] == 0x5a).all()) and bool((guarded[4096 + n:] == 0x5a).all())
-    assert not bool(ws[:65536].any())
+    ws.fill_(0xff)
+    assert _same(a, t.run(workspace=ws))
 
 
 def test_paged_tree_attention_missing_pages_and_lengths(cuda_device):
