@@ -527,6 +527,14 @@ _I64 = torch.int64
 def _layers(k_cache: torch.Tensor, v_cache: torch.Tensor):
     """(layers, layer stride, page stride, shape of a layer) of paged caches: of one layer as in
     ``_pages``, or of several ([layers, pages, kv heads, page size, head dim])."""
+    if (isinstance(k_cache, torch.Tensor) and isinstance(v_cache, torch.Tensor) and k_cache.ndim == 5 and k_cache.is_cuda
+            and k_cache.dtype is _BF16 and v_cache.dtype is _BF16 and k_cache.device == v_cache.device
+            and k_cache.is_contiguous() and v_cache.is_contiguous()):
+        shape = k_cache.shape
+        if v_cache.shape == shape:
+            layers, pages, heads, size, hd = shape
+            row = heads * size * hd
+            return layers, pages * row, row, (pages, heads, size, hd)
     _require_cuda(k_cache, "k_cache")
     dev, ndim = k_cache.device, k_cache.ndim
     if ndim == 4:
