@@ -121,6 +121,61 @@ def test_paged_tree_attention_more_row_tiles_than_counters(cuda_device):
     t.check(t.run())
 
 
+@pytest.mark.parametrize("nq,nkv,hd,lens,counts", [
+    (8, 2, 128, [20000, 0, 8176, 5], [40, 3, 64, 1]), (8, 1, 64, [17000, 9000], [64, 2]), (8, 4, 256, [8200, 1], [33, 9]),
+    (40, 2, 128, [300, 8150], [64, 64])])
+def test_paged_tree_attention_without_a_workspace(cuda_device, nq, nkv, hd, lens, counts):
+    """The C call without one: a workgroup for each KV head and row tile, which finds more page entries
+    than it holds at a time."""
+    from moeinfra_amd import _lib, ops
+
+    print(f"tree attention {nq}/{nkv} heads of {hd} without a workspace", flush=True)
+    t = Trees(cuda_device, lens, counts, nq, nkv, hd, 8, seed=21)
+    q, out, dev = t.q.to(cuda_device), torch.full_like(t.q, 9.0, device=cuda_device), cuda_device
+    n, cu, masks = _i32(t.lens, dev), _i32(t.cuts, dev), t.dev_masks()
+    _lib.check(_lib.lib().moe_paged_tree_attention_bf16(
+        q.data_ptr(), q.stride(0), t.T, t.pool.k.data_ptr(), t.pool.v.data_ptr(), t.pool.pages, 8, t.pool.k.stride(0),
+        t.pool.dev_table.data_ptr(), t.pool.dev_table.shape[1], n.data_ptr(), cu.data_ptr(), masks.data_ptr(), len(lens), nq,
+        nkv, hd, hd ** -0.5, out.data_ptr(), None, 0, torch.cuda.current_stream().cuda_stream), "tree attention")
+    t.check(out)
+    # With one the same within two roundings of the output and of the weights.
+    assert float((out.float() - t.run().float()).abs().max()) <= 4 * 2.0 ** -8 * float(max(v.float().abs().max() for v in t.v))
+
+
+def test_paged_tree_attention_more_kv_heads_than_workgroups_at_once(cuda_device):
+    print("tree attention of 300 KV heads", flush=True)
+    t = Trees(cuda_device, [70, 0, 33], [9, 64, 1], 300, 300, 64, 16, seed=22)
+    t.check(t.run())
+
+
+def test_far_pages(cuda_device):
+    """Pages more than 2^32 bytes apart: attention, the embedding, moves and copies."""
+    from moeinfra_amd import ops
+
+    dev, nq, nkv, hd, page, apart = cuda_device, 8, 2, 64, 16, (1 << 31) + 64 * 1024
+    both = torch.empty(3 * apart + 4 * nkv * page * hd, dtype=torch.bfloat16, device=dev)   # 13 GB
+    shape, strides = (4, nkv, page, hd), (apart, page * hd, hd, 1)
+    k, v = both.as_strided(shape, strides), both.as_strided(shape, strides, 2 * nkv * page * hd)
+    keys, vals = _bf((4 * page, nkv, hd), 31), _bf((4 * page, nkv, hd), 32)
+    table = _i32([[2, 0, 3, 1]], dev)
+    for i, p in enumerate([2, 0, 3, 1]):
+        k[p] = keys[i * page:(i + 1) * page].transpose(0, 1).to(dev)
+        v[p] = vals[i * page:(i + 1) * page].transpose(0, 1).to(dev)
+    q = _bf((10, nq, hd), 33, 1.5)
+    out = ops.paged_tree_attention(q.to(dev), k, v, table, _i32([50], dev), _i32([0, 10], dev))
+    see = ref.seen(ref.chain(10), 50).repeat_interleave(4, dim=0)
+    for h in range(nkv):
+        want, tol = attention(q[:, 4 * h:4 * h + 4].reshape(40, hd), keys[:60, h], vals[:60, h], hd ** -0.5, seen=see)
+        assert_within(out[:, 4 * h:4 * h + 4].reshape(40, hd), want, tol, f"head {h}")
+    ops.compact_paged_kv(k, v, table, _i32([15], dev), ref.words([1 << 33 | 1 << 20], dev))   # places 35, 48 to 15, 16
+    assert _same(k[2, :, 15], keys[35]) and _same(v[0, :, 0], vals[48]) and _same(k[0, :, 1], keys[17])
+    ops.copy_pages(k, v, _i32([[3, 1, 5]], dev))
+    assert _same(k[1, :, :5], keys[32:37].transpose(0, 1)) and _same(v[1, :, 5], vals[53])
+    x = _bf((1, (nq + 2 * nkv) * hd), 34)
+    _, y = ops.rope_paged_kv(x.to(dev), _i32([7], dev), table, k, v, nq, _inv(hd).to(dev), want_k=True, slots=_i32([63], dev))
+    assert _same(k[1, :, 15], y[0]) and _same(v[1, :, 15], x.view(-1, hd)[nq + nkv:])
+
+
 def test_paged_tree_attention_rows_of_no_sequence(cuda_device):
     """Rows before the first sequence, behind the last one, and of nodes past the 64th."""
     lens, counts = [20, 300, 5], [7, 64, 70]
