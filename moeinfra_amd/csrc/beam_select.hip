@@ -158,7 +158,7 @@ beam_select_kernel(const BsArgs a) {
   __shared__ uint32_t s_at[kBsList + 8];
   __shared__ double s_sum[kBsWaves], s_lse[kBsMaxBeams];
   __shared__ uint2 s_tab[kBsTable];
-  __shared__ float s_max[kBsWaves][kWave], s_top[kBsMaxBeams];
+  __shared__ float s_max[kBsWaves][kWave], s_top[kBsMaxBeams], s_score[kBsMaxBeams];
   __shared__ uint32_t s_n, s_seen;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -381,49 +381,44 @@ beam_select_kernel(const BsArgs a) {
     const int g = i / a.k;
     return bs_get(all + (int64_t)g * words + 2 + (i - g * a.k));
   };
+  // Where there are more than twice kBsFew a thread, the first few of each part tell what has to be looked at, as
+  // they are in falling order.
+  const bool many = n_all > 2 * kBsFew * kBsThreads;
+  const int depth = many ? min(a.k, kBsFew) : a.k, n_first = groups * depth;
+  auto number = [&](int i) { return i / depth * a.k + i % depth; };
   uint64_t keys[kBsFew];
+  auto load_keys = [&](int i0) {
 #pragma unroll
-  for (int j = 0; j < kBsFew; ++j) keys[j] = key_of(min(tid + j * kBsThreads, n_all - 1));
-  // Each part's maximum and sum; then each row's.
-  static_assert(kBsList >= kBsGroups && kBsList >= kBsMaxBeams, "the parts' maxima and sums fit the list");
+    for (int j = 0; j < kBsFew; ++j) keys[j] = key_of(number(min(i0 + j * kBsThreads, n_first - 1)));
+  };
+  load_keys(tid);
+  for (int w = tid; w < a.W; w += kBsThreads) s_score[w] = a.scores[search * a.W + w];
+  // Each part's maximum and sum; then each row's, a lane per part.
+  static_assert(kBsList >= kBsGroups && kBsList >= kBsMaxBeams && kBsMaxChunks <= kWave, "a row's parts fit a wave, all the list");
   double *const s_part = reinterpret_cast<double *>(s_list);
-  float *const s_pm = &s_max[0][0];
-  constexpr int kFew = kBsWaves * kWave;  // parts whose maxima fit s_max; of more they are read again
-  auto part_max = [&](int g) { return __builtin_bit_cast(float, (uint32_t)bs_get(all + (int64_t)g * words)); };
-  auto part_sum = [&](int g) { return __builtin_bit_cast(double, bs_get(all + (int64_t)g * words + 1)); };
+  float *const s_pm = reinterpret_cast<float *>(s_at);
   for (int g = tid; g < groups; g += kBsThreads) {
-    const float pm = part_max(g);
-    s_part[g] = part_sum(g);
-    if (g < kFew) s_pm[g] = pm;
+    s_pm[g] = __builtin_bit_cast(float, (uint32_t)bs_get(all + (int64_t)g * words));
+    s_part[g] = __builtin_bit_cast(double, bs_get(all + (int64_t)g * words + 1));
   }
   __syncthreads();
-  for (int w = tid; w < a.W; w += kBsThreads) {
-    float top = -INFINITY;
-    for (int i = 0; i < a.chunks; ++i) {
-      const int g = w * a.chunks + i;
-      top = fmaxf(top, g < kFew ? s_pm[g] : part_max(g));
+  for (int w = wave; w < a.W; w += kBsWaves) {
+    const bool has = lane < a.chunks;
+    const int g = w * a.chunks + min(lane, a.chunks - 1);
+    const float pm = s_pm[g];
+    float top[1] = {pm};
+    lane_groups_reduce<true>(top, kWave);
+    const bool some = has && pm > -INFINITY && top[0] < INFINITY;
+    const double total = bs_wave_sum(some ? s_part[g] * bs_exp((double)pm - (double)top[0], s_tab) : 0.0);
+    if (lane == 0) {
+      s_top[w] = top[0];
+      s_lse[w] = log(total);
     }
-    s_top[w] = top;
-  }
-  __syncthreads();
-  for (int g = tid; g < groups; g += kBsThreads) {
-    const float pm = g < kFew ? s_pm[g] : part_max(g), top = s_top[g / a.chunks];
-    double part = 0.0;
-    if (pm > -INFINITY && top < INFINITY) {
-      part = s_part[g] * bs_exp((double)pm - (double)top, s_tab);
-    }
-    s_part[g] = part;
-  }
-  __syncthreads();
-  for (int w = tid; w < a.W; w += kBsThreads) {
-    double total = 0.0;
-    for (int i = 0; i < a.chunks; ++i) total += s_part[w * a.chunks + i];
-    s_lse[w] = log(total);
   }
   __syncthreads();
   auto cand = [&](int i, uint64_t key) {  // (of W * chunks * k)
     const int w = i / a.k / a.chunks;
-    const float score = a.scores[search * a.W + w];
+    const float score = s_score[w];
     BsCand r{0, 0xffffffffu};
     if (key == 0 || !(score > -INFINITY && score < INFINITY) || !(s_top[w] < INFINITY)) return r;
     r.at = (uint32_t)w * (uint32_t)a.V + ~(uint32_t)key;
@@ -435,12 +430,15 @@ beam_select_kernel(const BsArgs a) {
   // Again the k-th largest of 64 groups' largest, by the totals' upper 32 bits.
   uint32_t most = 0;
   BsCand few[kBsFew];
+  for (int i0 = tid; i0 < n_first; i0 += kBsFew * kBsThreads) {
+    if (i0 != tid) load_keys(i0);
 #pragma unroll
-  for (int j = 0; j < kBsFew; ++j) {
-    few[j] = cand(min(tid + j * kBsThreads, n_all - 1), tid + j * kBsThreads < n_all ? keys[j] : 0);
-    most = max(most, (uint32_t)(few[j].total >> 32));
+    for (int j = 0; j < kBsFew; ++j) {
+      const int i = i0 + j * kBsThreads;
+      few[j] = cand(number(min(i, n_first - 1)), i < n_first ? keys[j] : 0);
+      most = max(most, (uint32_t)(few[j].total >> 32));
+    }
   }
-  for (int i = tid + kBsFew * kBsThreads; i < n_all; i += kBsThreads) most = max(most, (uint32_t)(cand(i, key_of(i)).total >> 32));
   s_at[tid] = most;
   __syncthreads();
 #pragma unroll
@@ -460,9 +458,32 @@ beam_select_kernel(const BsArgs a) {
       s_at[at] = x.at;
     }
   };
+  if (!many) {
+    for (int i0 = tid; i0 < n_all; i0 += kBsFew * kBsThreads) {
+      if (n_all > kBsFew * kBsThreads) load_keys(i0);
 #pragma unroll
-  for (int j = 0; j < kBsFew; ++j) rank_too(few[j]);
-  for (int i = tid + kBsFew * kBsThreads; i < n_all; i += kBsThreads) rank_too(cand(i, key_of(i)));
+      for (int j = 0; j < kBsFew; ++j) {
+        const int i = i0 + j * kBsThreads;
+        if (i < n_all) rank_too(n_all > kBsFew * kBsThreads ? cand(i, keys[j]) : few[j]);
+      }
+    }
+  } else {
+    // A part a thread, as far as its continuations are large enough.
+    for (int g = tid; g < groups; g += kBsThreads) {
+      bool on = true;
+      for (int i0 = 0; i0 < a.k && on; i0 += kBsFew) {
+#pragma unroll
+        for (int j = 0; j < kBsFew; ++j) keys[j] = key_of(g * a.k + min(i0 + j, a.k - 1));
+#pragma unroll
+        for (int j = 0; j < kBsFew; ++j)
+          if (i0 + j < a.k) {
+            const BsCand x = cand(g * a.k + i0 + j, keys[j]);
+            on &= x.total != 0 && (uint32_t)(x.total >> 32) >= lowest;
+            rank_too(x);
+          }
+      }
+    }
+  }
   __syncthreads();
   auto put = [&](int rank, uint64_t total, uint32_t at) {
     const int64_t o = (int64_t)search * a.k + rank;
