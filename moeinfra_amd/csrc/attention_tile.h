@@ -1,5 +1,5 @@
 // What the attention kernels share: K and V tiles in LDS and the way back into the matrix
-// instructions' registers, sums over a wave's lanes, partial results passed between workgroups.
+// instructions' registers, sums over a wave's lanes.
 #pragma once
 
 #include "common.h"
@@ -50,33 +50,6 @@ __device__ __forceinline__ int pa_max(int v) {
   v = max(v, pa_dpp<0x118, 0xf>(v));
   v = max(v, pa_dpp<0x142, 0xa>(v));
   return max(v, pa_dpp<0x143, 0xc>(v));
-}
-
-// Partial results pass between workgroups (of other XCDs) through device-scope accesses, two
-// floats at a time.
-__device__ __forceinline__ void pa_put(float *p, float x, float y) {
-  __hip_atomic_store((uint64_t *)p, __builtin_bit_cast(uint32_t, x) | (uint64_t)__builtin_bit_cast(uint32_t, y) << 32,
-                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 pa_get(const float *p) {
-  const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32)));
-}
-
-// Whether this workgroup is the last of n to arrive at *count, which it then leaves zero.  What
-// the others wrote with pa_put is there for its pa_get (their stores have completed before they
-// count themselves in).  Nothing here waits for another workgroup.
-__device__ __forceinline__ bool pa_last_of(uint32_t *count, int n) {
-  __shared__ uint32_t s_seen;
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const uint32_t seen = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-    if (seen == (uint32_t)n) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_seen = seen;
-  }
-  __syncthreads();
-  return s_seen == (uint32_t)n;
 }
 
 }  // namespace

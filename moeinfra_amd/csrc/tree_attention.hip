@@ -21,8 +21,10 @@ constexpr float kTaLog2e = 1.44269504088896341f;
 // rescaled: weights up to 2^8, which fp32 sums and bf16 weights carry without loss.
 constexpr float kTaLag = 8.0f;
 constexpr float kTaFine = 4096.0f;
-constexpr int kTaAll = 2;      // places of a tile that takes all waves
-constexpr int kTaStart = 2;    // tiles' time that beginning a row tile takes
+// Places of a tile that takes all waves (24 ragged trees: 101 us; as one 115, as three 106), and that beginning a
+// row tile takes.
+constexpr int kTaAll = 2;
+constexpr int kTaStart = 2;
 constexpr int kTaLeast = 2;    // places of a workgroup at least (a tile)
 constexpr int kTaMaxParts = 64;  // workgroups that share a row tile
 constexpr int kTaPages = 1024;   // page entries at hand
@@ -104,6 +106,12 @@ __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_rows) {
 //
 // With rows for more than half of the waves, each wave takes 32 rows against all units; else the waves are
 // two groups, for every other unit.
+//
+// Bound: HBM for small trees (32 / 8 heads of 128, 16 trees of 16 tokens, 32768 keys: 2.15 GB in 344 us, 6.3 TB/s,
+// with streamed loads; 394 without the hint, 413 with two workgroups of four waves a CU and two planes of 64 keys).
+// Large ones (8 of 64 tokens, 16384 keys: 182 us, 755 TFLOP/s): a wave's unit takes 2000 cycles alone and 2200
+// beside another wave of its SIMD, of which reading K and V from LDS is half; loads alone are 108 us.  Beginning
+// and ending a row tile takes 8 us.
 template <int HD>
 __global__ void __launch_bounds__(ta_waves(HD) *kWave)
 paged_tree_attention_kernel(const TaArgs a) {
@@ -119,8 +127,8 @@ paged_tree_attention_kernel(const TaArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t s_kv[NU * kUnitB];
   __shared__ int64_t s_page[kTaPages];  // bytes from a cache's start to this head's rows of the page, -1: none
   static_assert(kLoads * NW * 1024 == kUnitB && kChunkKeys <= 8, "whole chunks, each of one page");
-  static_assert(NW / 2 * (16 * kDT + 4) * kWave * 4 <= NU * kUnitB && kRows * kTaMaxParts * 4 <= NU * kUnitB,
-                "half of the waves' sums, and the parts' weights, fit the ring");
+  static_assert(NW / 2 * (16 * kDT + 4) * kWave * 4 <= NU * kUnitB,
+                "half of the waves' sums fit the ring");
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int li = lane & 31, hh = lane >> 5;
@@ -547,7 +555,9 @@ paged_tree_attention_kernel(const TaArgs a) {
 }
 
 // The results of the workgroups that share a row tile added up, in the order of the keys: a workgroup takes 32
-// rows of what began in one workgroup's part.
+// rows of what began in one workgroup's part.  (By the last workgroup to arrive, without this launch, one of 900
+// keys took 16.1 us instead of 16.9, but 4 of 16000 keys of 16 / 1 heads, up to 62 parts of 256 rows each, 108
+// instead of 52.)
 constexpr int kTjThreads = 256;
 template <int HD>
 __global__ void __launch_bounds__(kTjThreads)
