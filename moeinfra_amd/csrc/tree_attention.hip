@@ -20,6 +20,7 @@ constexpr float kTaLog2e = 1.44269504088896341f;
 // The running reference may lag the maximum by this much (in powers of two) before the sums are
 // rescaled: weights up to 2^8, which fp32 sums and bf16 weights carry without loss.
 constexpr float kTaLag = 8.0f;
+// Up to here the reference may be a factor of the exponent's multiply-add (in powers of two).
 constexpr float kTaFine = 4096.0f;
 // Places of a tile that takes all waves (24 ragged trees: 101 us; as one 115, as three 106), and that beginning a
 // row tile takes.
@@ -66,7 +67,8 @@ __device__ u32x4 ta_zeros[1024 / 16];
 
 // 64 lanes' 16 bytes each, at `lane` bytes from src, into LDS at dst + 16 * lane number, without
 // registers.  (In asm, as the compiler would wait for all of them before the next transposing read of the
-// other plane; the caller waits for vmcnt(0) and a barrier before it reads dst.)
+// other plane; the caller waits until no more loads than those of later steps are under way, and a barrier,
+// before it reads dst.  Streamed, as each key is read once.)
 __device__ __forceinline__ void ta_load_lds(const void *src, uint32_t lane, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(dst), "v"(lane), "s"(src)
                : "memory", "m0");
@@ -97,9 +99,9 @@ __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_rows) {
 // Rows of one KV head are (token, query head of its group), r = token * group + head, so that the
 // group's heads share the K and V tiles.  All row tiles of a KV head's batch lie one behind the other,
 // key tile by key tile, each behind kTaStart of nothing (what it costs to begin one); each of the KV
-// head's workgroups takes as much of that, and the last of those that share a row tile to arrive adds
-// their results up.  A workgroup's keys come from memory straight into a ring of units in LDS, some steps
-// ahead of the one that is multiplied:
+// head's workgroups takes as much of that, and a second launch adds up the results of those that share a
+// row tile.  A workgroup's keys come from memory straight into a ring of units in LDS, some steps ahead of
+// the one that is multiplied:
 //
 //   S^T = K Q^T        lane (row of queries l % 32) holds 16 keys of its row per unit
 //   O^T += V^T P^T     P of a lane is the B operand as it stands; V is read transposed

@@ -462,6 +462,23 @@ def test_beam_select_equal_and_ordered_logits(cuda_device):
                 _check_beams(ops.beam_select(x, scores, k), x, scores, k)
 
 
+@pytest.mark.parametrize("W,V,k", [(16, 40000, 32), (16, 131072, 16), (64, 9000, 64), (3, 300000, 64)])
+def test_beam_select_more_alike_than_the_lists_hold(cuda_device, W, V, k):
+    """Parts and searches with thousands of equal continuations, with few large ones among them."""
+    from moeinfra_amd import ops
+
+    print(f"{W} beams of {V} equal logits, {k} best", flush=True)
+    x = torch.zeros((W, V), dtype=torch.bfloat16)
+    scores = torch.zeros((1, W))
+    for step in range(3):
+        if step == 1:
+            x[W // 2, [5, V // 2, V - 1]] = 1.0
+        if step == 2:
+            scores = -torch.arange(W)[None].float() / 1024
+        dx, ds = x.to(cuda_device), scores.to(cuda_device)
+        _check_beams(ops.beam_select(dx, ds, k), dx, ds, k)
+
+
 def test_beam_select_near_totals(cuda_device):
     """Beams whose totals differ in the ninth digit only, by sums over the vocabulary."""
     from moeinfra_amd import ops
