@@ -60,6 +60,7 @@ struct TaArgs {
   float *part;
   int share;   // workgroups per KV head that a batch is shared by (0: a row tile each)
   int place;   // floats of a partial result
+  int slices;  // of 32 rows that a row tile may have
 };
 
 // What is read in the place of keys that are not there: as long as a chunk.
@@ -564,10 +565,10 @@ constexpr int kTjThreads = 256;
 template <int HD>
 __global__ void __launch_bounds__(kTjThreads)
 paged_tree_join_kernel(const TaArgs a) {
-  constexpr int kSlices = ta_rows(HD) / 32, kItems = 32 * HD / 4 / kTjThreads;
+  constexpr int kItems = 32 * HD / 4 / kTjThreads;
   constexpr int kTogether = HD == 256 ? 4 : 8;  // results under way, kItems of each
   __shared__ float s_w[32][kTaMaxParts + 1];
-  const int unit = (int)(blockIdx.x / kSlices), r0 = 32 * (int)(blockIdx.x % kSlices);
+  const int unit = (int)(blockIdx.x / (unsigned)a.slices), r0 = 32 * (int)(blockIdx.x - (unsigned)unit * a.slices);
   const int wg = unit / a.nkv, kvh = unit - wg * a.nkv;
   const TaJoin j = a.joins[unit];
   if (j.nact < 2 || r0 >= j.rows) return;
@@ -731,6 +732,8 @@ extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, in
   a.place = (int)moe::ta_place(grp, head_dim);
   // (With a workgroup per KV head only, it has all there is.)
   a.share = workspace != nullptr && share > 1 ? (int)share : 0;
+  const int64_t most = (T < moe::kTaNodes ? T : moe::kTaNodes) * grp;
+  a.slices = (int)((most < moe::ta_rows(head_dim) ? most + 31 : moe::ta_rows(head_dim)) / 32);
   const int64_t groups = (a.share > 0 ? a.share : B * rtiles) * n_kv_heads;
   MOE_REQUIRE(moe::launch_fits(groups, moe::ta_waves(head_dim) * moe::kWave), "bad sizes");
   auto kern = head_dim == 64    ? moe::paged_tree_attention_kernel<64>
@@ -742,8 +745,7 @@ extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, in
     auto join = head_dim == 64    ? moe::paged_tree_join_kernel<64>
                 : head_dim == 128 ? moe::paged_tree_join_kernel<128>
                                   : moe::paged_tree_join_kernel<256>;
-    const int64_t slices = moe::ta_rows(head_dim) / 32;
-    hipLaunchKernelGGL(join, dim3((unsigned)(groups * slices)), dim3(moe::kTjThreads), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(join, dim3((unsigned)(groups * a.slices)), dim3(moe::kTjThreads), 0, (hipStream_t)stream, a);
     MOE_LAUNCH_CHECK();
   }
   return MOE_STATUS_OK;
