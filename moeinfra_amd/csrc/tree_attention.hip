@@ -110,9 +110,9 @@ __device__ __forceinline__ TaSeq ta_seq(const TaArgs &a, int b, int tile_rows) {
 // With rows for more than half of the waves, each wave takes 32 rows against all units; else the waves are
 // two groups, for every other unit.
 //
-// Bound: HBM for small trees (32 / 8 heads of 128, 16 trees of 16 tokens, 32768 keys: 2.15 GB in 344 us, 6.3 TB/s,
+// Bound: HBM for small trees (32 / 8 heads of 128, 16 trees of 16 tokens, 32768 keys: 2.15 GB in 339 us, 6.35 TB/s,
 // with streamed loads; 394 without the hint, 413 with two workgroups of four waves a CU and two planes of 64 keys).
-// Large ones (8 of 64 tokens, 16384 keys: 182 us, 755 TFLOP/s): a wave's unit takes 2000 cycles alone and 2200
+// Large ones (8 of 64 tokens, 16384 keys: 182 to 188 us, 740 TFLOP/s): a wave's unit takes 2000 cycles alone and 2200
 // beside another wave of its SIMD, of which reading K and V from LDS is half; loads alone are 108 us.  Beginning
 // and ending a row tile takes 8 us.
 template <int HD>
@@ -559,14 +559,14 @@ paged_tree_attention_kernel(const TaArgs a) {
 
 // The results of the workgroups that share a row tile added up, in the order of the keys: a workgroup takes 32
 // rows of what began in one workgroup's part.  (By the last workgroup to arrive, without this launch, one of 900
-// keys took 16.1 us instead of 16.9, but 4 of 16000 keys of 16 / 1 heads, up to 62 parts of 256 rows each, 108
+// keys took 16.1 us, now 14.8, and 4 of 16000 keys of 16 / 1 heads, up to 62 parts of 256 rows each, 108
 // instead of 52.)
 constexpr int kTjThreads = 256;
 template <int HD>
 __global__ void __launch_bounds__(kTjThreads)
 paged_tree_join_kernel(const TaArgs a) {
   constexpr int kItems = 32 * HD / 4 / kTjThreads;
-  constexpr int kTogether = HD == 256 ? 4 : 8;  // results under way, kItems of each
+  constexpr int kTogether = HD == 256 ? 2 : 4;  // results under way, kItems of each (twice as many: fewer waves, 4 us more)
   __shared__ float s_w[32][kTaMaxParts + 1];
   const int unit = (int)(blockIdx.x / (unsigned)a.slices), r0 = 32 * (int)(blockIdx.x - (unsigned)unit * a.slices);
   const int wg = unit / a.nkv, kvh = unit - wg * a.nkv;
