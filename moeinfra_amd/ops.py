@@ -524,6 +524,14 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
 _I64 = torch.int64
 
 
+def _int32(v, name: str) -> int:
+    """A number that an entry point takes in 32 bits."""
+    v = int(v)
+    if not -1 << 31 <= v < 1 << 31:
+        raise ValueError(f"{name} must fit 32 bits (got {v})")
+    return v
+
+
 def _layers(k_cache: torch.Tensor, v_cache: torch.Tensor):
     """(layers, layer stride, page stride, shape of a layer) of paged caches: of one layer as in
     ``_pages``, or of several ([layers, pages, kv heads, page size, head dim])."""
@@ -557,7 +565,8 @@ def _layers(k_cache: torch.Tensor, v_cache: torch.Tensor):
 def paged_tree_attention_workspace(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
     """Workspace of ``paged_tree_attention`` for batches of any size: made once, then shared by calls
     that run one after the other (one stream)."""
-    n = lib().moe_paged_tree_attention_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim)
+    n = lib().moe_paged_tree_attention_workspace_bytes(batch, _int32(n_q_heads, "n_q_heads"),
+                                                       _int32(n_kv_heads, "n_kv_heads"), _int32(head_dim, "head_dim"))
     if n < 0:
         raise ValueError(f"invalid attention sizes batch={batch} heads={n_q_heads}/{n_kv_heads} head_dim={head_dim}")
     return torch.empty((n,), dtype=torch.uint8, device=device)
@@ -648,7 +657,7 @@ def compact_paged_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: t
 def beam_select_workspace(searches: int, beams: int, k: int, device) -> torch.Tensor:
     """Workspace of ``beam_select`` for so many searches: made once, then shared by calls that run one
     after the other (one stream)."""
-    n = lib().moe_beam_select_workspace_bytes(searches, beams, k)
+    n = lib().moe_beam_select_workspace_bytes(searches, beams, _int32(k, "k"))
     if n < 0:
         raise ValueError(f"invalid sizes searches={searches} beams={beams} k={k}")
     ws = torch.empty((n,), dtype=torch.uint8, device=device)
@@ -674,7 +683,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, workspace: O
     if scores.ndim != 2 or scores.numel() != logits.shape[0]:
         raise ValueError(f"scores must be [searches, beams] of {logits.shape[0]} rows (got {tuple(scores.shape)})")
     (S, W), (rows, V) = scores.shape, logits.shape
-    k = int(k)
+    k = _int32(k, "k")
     if workspace is None:
         workspace = beam_select_workspace(S, W, k, dev)
     best = scores.new_empty(S, max(k, 0))
@@ -715,6 +724,7 @@ def fork_pages(page_table: torch.Tensor, lens: torch.Tensor, parents: torch.Tens
     B, width = page_table.shape
     N, pages = parents.shape[0], refs.shape[0]
     n = _plain(lens, "lens", _I32, dev, (B,))
+    page_size, ahead = _int32(page_size, "page_size"), _int32(ahead, "ahead")
     if out is None:
         out = (page_table.new_empty(N, width), page_table.new_empty(N), page_table.new_empty(N, 3),
                page_table.new_empty(1))

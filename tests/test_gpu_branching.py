@@ -993,3 +993,8 @@ def test_wrappers_refuse_what_does_not_fit(cuda_device):
     t = i32(2, 3)
     with pytest.raises(ValueError, match="overlap"):
         ops.fork_pages(t, i32(2), i32(2), i32(9), 8, out=(t, i32(2), i32(2, 3), i32(1)))
+    for args, what in ((((1 << 32) + 8, 1), "page_size must fit"), ((8, (1 << 32) + 1), "ahead must fit")):
+        with pytest.raises(ValueError, match=what):
+            ops.fork_pages(i32(2, 3), i32(2), i32(2), i32(9), args[0], ahead=args[1])
+    with pytest.raises(ValueError, match="k must fit"):
+        ops.beam_select(bf(4, 9), f32(2, 2), (1 << 32) + 2)

@@ -233,3 +233,8 @@ def test_wrappers_take_gpu_tensors_only():
         ops.beam_select_workspace(4, 8, 65, "cpu")
     with pytest.raises(ValueError, match="invalid number of pages"):
         ops.fork_pages_workspace(-1, "cpu")
+    # Numbers are refused where they would lose their upper bits on the way.
+    with pytest.raises(ValueError, match="k must fit"):
+        ops.beam_select_workspace(4, 8, (1 << 32) + 4, "cpu")
+    with pytest.raises(ValueError, match="head_dim must fit"):
+        ops.paged_tree_attention_workspace(4, 8, 2, (1 << 32) + 64, "cpu")
