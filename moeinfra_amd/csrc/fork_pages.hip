@@ -1,7 +1,7 @@
 // Page table rows of a paged cache taken over by the sequences that continue: beams reordered, forked
 // and dropped.  A page is held by as many as its count says; a row that goes on holds its parent's pages,
 // and the places that it writes to next get pages that no other holds.
-#include "common.h"
+#include "attention_tile.h"
 
 namespace moe {
 namespace {
@@ -18,24 +18,15 @@ struct FpArgs {
   int32_t *writers, *lowest;                       // per page, zero between calls
 };
 
-// Sum over the threads before this one, and over all of them.
+// Sum over the threads before this one, and over all of them.  (Shuffles in place of the wave sums: 1 us a call more.)
 __device__ __forceinline__ int fp_scan(int v, int *s_sum, int &all) {
-  const int lane = threadIdx.x & (kWave - 1), wave = (int)threadIdx.x >> 6;
-  int incl = v;
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int x = __shfl_up(incl, d, kWave);
-    incl += lane >= d ? x : 0;
-  }
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int incl = pa_incl(v);
   if (lane == kWave - 1) s_sum[wave] = incl;
   __syncthreads();
-  int before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kFpWaves; ++w) {
-    before += w < wave ? s_sum[w] : 0;
-    all += s_sum[w];
-  }
+  const int sums = pa_incl(lane < kFpWaves ? s_sum[lane] : 0);
+  all = __builtin_amdgcn_readlane(sums, kFpWaves - 1);
+  const int before = wave > 0 ? __builtin_amdgcn_readlane(sums, wave - 1) : 0;
   __syncthreads();
   return before + incl - v;
 }
@@ -50,8 +41,10 @@ __device__ __forceinline__ void fp_add(int32_t *p, int v) {
 
 // The same for up to kFpFew rows and places, whose lengths, parents, pages and counts of writers lie in LDS
 // (a hash of pages), so that memory answers five times only, one after the other: the lengths, the table,
-// the counts' changes, the writers' counts, the free pages'.  That is what bounds it: 256 rows of up to 25 pages
-// 13 us (17 with four entries a thread under way, as below 17), 8 rows 6; 2048 rows of 20 pages some 45.
+// the counts' changes, the writers' counts, the free pages'.  That is what bounds it, for many rows also one CU's
+// loads and atomics (2.3 and 2 us for 256 rows of up to 25 pages): 12 us for these, 8 rows 6, 2048 rows of 20 pages
+// some 42.  (The page of each place loaded by itself, or the first counts along with the writers', changed
+// nothing; counts by loads of 16 bytes, behind a fence, 1 us more for 8 rows.)
 constexpr int kFpFew = 2048;
 constexpr int kFpSlots = 2 * kFpFew;
 constexpr int kFpTogether = 4;  // counts that a thread has under way
@@ -61,6 +54,8 @@ __global__ void __launch_bounds__(kFpThreads)
 fork_few_pages_kernel(const FpArgs a) {
   __shared__ int s_len[kFpFew], s_parent[kFpFew], s_children[kFpFew], s_page[kFpFew], s_rank[kFpFew];
   __shared__ int s_key[kFpSlots], s_writers[kFpSlots], s_sum[kFpWaves];
+  __shared__ int s_kept[kFpFew];  // entries of an old row that go on
+  __shared__ int4 s_new[kFpFew];  // of a new row: its parent's first entry, entries, of them the first written to
   int *const s_free = s_children;  // (once these are counted)
   const int tid = threadIdx.x;
   const int P = 1 << a.page_shift;
@@ -68,7 +63,9 @@ fork_few_pages_kernel(const FpArgs a) {
   auto good = [&](int page) { return page >= 0 && page < a.pages; };
   const int n = a.rows * a.places;
   for (int i = tid; i < a.old_rows; i += kFpThreads) {
-    s_len[i] = max(a.lens[i], 0);
+    const int len = max(a.lens[i], 0);
+    s_len[i] = len;
+    s_kept[i] = kept(len);
     s_children[i] = 0;
   }
   for (int i = tid; i < a.rows; i += kFpThreads) {
@@ -81,38 +78,50 @@ fork_few_pages_kernel(const FpArgs a) {
     s_writers[i] = 0;
   }
   __syncthreads();
+  const int width = (int)a.width, old_all = a.old_rows * width, new_all = a.rows * width;
   for (int i = tid; i < a.rows; i += kFpThreads) {
     const int p = s_parent[i];
     if (p >= 0) atomicAdd(&s_children[p], 1);
-    a.new_lens[i] = p >= 0 ? s_len[p] : 0;
+    const int len = p >= 0 ? s_len[p] : 0;
+    s_new[i] = make_int4(max(p, 0) * width, p >= 0 ? s_kept[p] : 0, len >> a.page_shift, 0);
+    a.new_lens[i] = len;
     a.copies[3 * i] = a.copies[3 * i + 1] = -1;
     a.copies[3 * i + 2] = 0;
   }
   __syncthreads();
   // Each old row lets its pages go, each new one takes those that it keeps.
-  const int width = (int)a.width, old_all = a.old_rows * width, new_all = a.rows * width;
+  int row = width > 0 ? tid / width : 0, e = tid - row * width;
+  const int rows_on = width > 0 ? kFpThreads / width : 0, e_on = kFpThreads - rows_on * width;
   for (int x0 = tid; x0 < max(old_all, new_all); x0 += kFpEntries * kFpThreads) {
-    int was[kFpEntries], page[kFpEntries];
+    int was[kFpEntries], page[kFpEntries], rows[kFpEntries], es[kFpEntries];
 #pragma unroll
     for (int k = 0; k < kFpEntries; ++k) {
-      const int x = x0 + k * kFpThreads, row = x / width;
+      const int x = x0 + k * kFpThreads;
+      rows[k] = row;
+      es[k] = e;
       was[k] = x < old_all ? a.table[x] : -1;
-      page[k] = x < new_all && s_parent[row] >= 0 ? a.table[s_parent[row] * width + (x - row * width)] : -1;
+      page[k] = -1;
+      if (x < new_all && e < s_new[row].y) page[k] = a.table[s_new[row].x + e];
+      row += rows_on;
+      e += e_on;
+      if (e >= width) {
+        e -= width;
+        ++row;
+      }
     }
 #pragma unroll
     for (int k = 0; k < kFpEntries; ++k) {
-      const int x = x0 + k * kFpThreads, row = x / width, e = x - row * width;
+      const int x = x0 + k * kFpThreads;
       if (good(was[k])) {
-        const int by = (e < kept(s_len[row]) ? s_children[row] : 0) - 1;
+        const int by = (es[k] < s_kept[rows[k]] ? s_children[rows[k]] : 0) - 1;
         if (by != 0) fp_add(a.refs + was[k], by);
       }
       if (x >= new_all) continue;
-      const int p = s_parent[row];
-      const bool keeps = p >= 0 && e < kept(s_len[max(p, 0)]);
-      a.new_table[x] = keeps ? page[k] : -1;
-      if (!keeps || e < s_len[p] >> a.page_shift) continue;
+      a.new_table[x] = page[k];
+      const int4 to = s_new[rows[k]];
+      if (es[k] >= to.y || es[k] < to.z) continue;
       // Place i: entry len / P + i % places of row i / places, written to next.
-      const int i = row * a.places + e - (s_len[p] >> a.page_shift);
+      const int i = rows[k] * a.places + es[k] - to.z;
       s_page[i] = good(page[k]) ? page[k] : -1;
       if (!good(page[k])) continue;
       uint32_t slot = (uint32_t)page[k] * 2654435761u >> 20;
