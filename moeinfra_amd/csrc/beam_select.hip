@@ -36,6 +36,9 @@ struct BsArgs {
   uint64_t *part;                // per workgroup: m, sum, k keys
 };
 
+// 16 bytes at any address of a value.
+typedef u32x4 bs_piece __attribute__((aligned(2)));
+
 __device__ __forceinline__ void bs_put(uint64_t *p, uint64_t v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -172,8 +175,8 @@ beam_select_kernel(const BsArgs a) {
   const int search = row / a.W;
   const int v0 = c * a.chunk, v1 = min(v0 + a.chunk, a.V);
   const E *const x = (const E *)a.x + row * a.stride;
-  // Pieces begin where memory's 16 bytes do.
-  const int lead = (int)((uintptr_t)(x + v0) % 16 / sizeof(E));
+  // Pieces begin at v0, not where memory's 16 bytes do: which thread adds up which values must not hang on where a
+  // row lies, or equal beams would have sums of different roundings and go out of order.
   bs_table(s_tab);
   if (tid < kBsMost) s_best[tid] = 0;
   if (tid == 0) s_n = 0;
@@ -198,12 +201,12 @@ beam_select_kernel(const BsArgs a) {
       ahead[p] = F32 ? (u32x4){0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u}  // -inf
                      : (u32x4){0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
       if (!some(i0, p)) continue;
-      if (i >= v0 && i + kPer <= v1) {
-        ahead[p] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(x + i));
+      if (i + kPer <= v1) {
+        ahead[p] = __builtin_nontemporal_load(reinterpret_cast<const bs_piece *>(x + i));
       } else {
 #pragma unroll
         for (int e = 0; e < kPer; ++e)
-          if (i + e >= v0 && i + e < v1) {
+          if (i + e < v1) {
             if constexpr (F32)
               ahead[p][e] = __builtin_bit_cast(uint32_t, x[i + e]);
             else
@@ -214,8 +217,8 @@ beam_select_kernel(const BsArgs a) {
     }
   };
   constexpr int kRound = kBsThreads * kHeld;
-  if (v0 < v1) load(v0 - lead);
-  for (int i0 = v0 - lead; i0 < v1; i0 += kRound) {
+  if (v0 < v1) load(v0);
+  for (int i0 = v0; i0 < v1; i0 += kRound) {
 #pragma unroll
     for (int p = 0; p < kBsPieces; ++p) h[p] = ahead[p];
     if (i0 + kRound < v1) load(i0 + kRound);

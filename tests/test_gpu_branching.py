@@ -552,6 +552,39 @@ def test_beam_select_workspaces(cuda_device):
     assert not bool(ws[:65536].any())
 
 
+def _equal_beams(W, k, x, score, dtype):
+    """What W beams of equal scores and the logits x [V] give: the larger logit first, of equal ones the lower beam,
+    then token.  (Totals of equal logits are equal, so a logit's tokens go beam by beam.)"""
+    v, at = torch.sort(x.to(dtype).double(), descending=True, stable=True)
+    want, i = [], 0
+    while len(want) < k:
+        same = int((v == v[i]).sum())
+        want += [(w, int(t)) for w in range(W) for t in at[i:i + same][:k]]
+        i += same
+    return want[:k]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [50257, 32001, 151669, 1999])
+def test_beam_select_equal_beams_at_any_alignment(cuda_device, V, dtype):
+    """Beams of the same logits and scores: in order, wherever their rows begin; the same totals from every view."""
+    from moeinfra_amd import ops
+
+    W, k = 5, 12
+    for seed in range(6):
+        x = _logits(1, V, seed, dtype)
+        want = _equal_beams(W, k, x[0], 0.0, dtype)
+        totals = []
+        for lead, pad in ((0, 0), (0, 8 - V % 8), (1, 3), (3, 4), (5, 9)):
+            base = torch.full((W, V + pad + lead), math.inf, dtype=dtype, device=cuda_device)
+            base[:, lead:lead + V] = x.to(cuda_device)
+            best, rows, tokens = ops.beam_select(base[:, lead:lead + V], torch.full((1, W), -1.5, device=cuda_device), k)
+            got = list(zip(rows[0].tolist(), tokens[0].tolist()))
+            assert got == want, f"seed {seed}, {lead} values before a row and {pad} behind it"
+            totals.append(best)
+        assert all(torch.equal(t, totals[0]) for t in totals)
+
+
 # ------------------------------------------------------------------ forked pages
 def _check_fork(dev, table, lens, parents, refs, page, ahead=1, workspace=None):
     from moeinfra_amd import ops
