@@ -471,9 +471,9 @@ int moe_compact_paged_kv_bf16(void *k_cache, void *v_cache, int64_t layers, int6
 /* moe_beam_select: the k best continuations of each of S searches of W beams: of all beams w and tokens
  * v those of the largest score[w] + log softmax(x[w])[v], x [S * W, V] (bf16, or fp32 with logits_f32 =
  * 1; rows `stride` values apart, V up to 2^20), scores fp32 [S, W].  Sums over the vocabulary are of
- * 64 bits, and the same for equal rows of a call, wherever they lie.  Inside a beam the larger logit
- * goes first, of equal ones the lower token; between beams the larger total, of equal ones the lower
- * beam.  best (fp32 [S, k]) are the totals, rows (int32 [S, k])
+ * 64 bits, of exponentials to 2^-42 of their values, and the same for equal rows of a call, wherever they
+ * lie.  Inside a beam the larger logit goes first, of equal ones the lower token; between beams the
+ * larger total, of equal ones the lower beam.  best (fp32 [S, k]) are the totals, rows (int32 [S, k])
  * the rows s * W + w of x, tokens (int64 [S, k]) the tokens.  Logits of -inf and NaN are never chosen, a
  * score of -inf (or NaN, or +inf) means no beam, and a beam whose logits hold +inf has no
  * probabilities: it is none either.  What there is too little for is -inf, -1, -1.  S up to

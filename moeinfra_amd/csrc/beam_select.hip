@@ -57,14 +57,25 @@ __device__ __forceinline__ float bs_value(uint32_t o) {
 // A logit and its place: the larger logit first, of equal ones the lower index.
 __device__ __forceinline__ uint64_t bs_key(uint32_t o, uint32_t i) { return o == 0 ? 0 : (uint64_t)o << 32 | ~i; }
 
-// e^d for -700 <= d <= 0 to 2^-42 of its value, from t = 256 d / ln 2 + kBsBias: 2^(n / 256) e^r, n the whole
-// part of t (without the bias) and r of its fraction, 0 <= r < ln 2 / 256; 2^(j / 256) of a table, e^r by its
-// series up to r^3 / 3!.  An entry's upper word lacks the bias and j, 2^12 times, so that adding t's whole part
-// times 2^12 to it leaves that of n / 256 in its exponent.
+// e^d for -700 <= d <= 0 to 2^-42 of its value, from t = 256 d / ln 2 + kBsBias: 2^(n / 256) e^(u x), u = ln 2 / 256,
+// n the whole part of t (without the bias) and x, 0 <= x < 1, its fraction; 2^(j / 256) of a table.  An entry's upper
+// word lacks the bias and j, 2^12 times, so that adding t's whole part times 2^12 to it leaves that of n / 256 in its
+// exponent.  t's roundings are 2^-42.5 of a weight at most.
+//
+// e^(u x) is its series up to x^4 less u^4 / 24 of the polynomial x^4 + g3 x^3 + g2 x^2 + g1 x that is smallest on
+// [0, 1]: a Chebyshev polynomial of degree 4, its argument (1 + z) x - z so that its first zero, -z = -cos(pi / 8),
+// lies at 0 (e^0 stays 1).  That takes x^4 away, and what is left out is 2^-45.4 at most, to both sides; the series up to x^3
+// by itself lacks 2^-38.7, always to one side, which told the better of two beams wrongly when 2^-40 lay between
+// them.
 constexpr int kBsTable = 256;
 constexpr double kBsUnit = 0.69314718055994530942 / kBsTable;
 constexpr double kBsLow = -700.0;
 constexpr int kBsBias = 1 << 18;
+constexpr double kBsZ = 0.92387953251128675613, kBsA = 1 + kBsZ;
+constexpr double kBsFourth = kBsUnit * kBsUnit * kBsUnit * kBsUnit / 24;
+constexpr double kBsC1 = kBsUnit - kBsFourth * (2 * kBsZ - 4 * kBsZ * kBsZ * kBsZ) / (kBsA * kBsA * kBsA);
+constexpr double kBsC2 = kBsUnit * kBsUnit / 2 - kBsFourth * (6 * kBsZ * kBsZ - 1) / (kBsA * kBsA);
+constexpr double kBsC3 = kBsUnit * kBsUnit * kBsUnit / 6 + kBsFourth * 4 * kBsZ / kBsA;
 static_assert(kBsBias % kBsTable == 0 && kBsBias > -kBsLow / kBsUnit + 1, "t is never negative");
 __device__ __forceinline__ void bs_table(uint2 *s_tab) {
   if (threadIdx.x < kBsTable) {
@@ -87,9 +98,8 @@ __device__ __forceinline__ void bs_add_exp(double &sum, double (&t)[N], const ui
   double part[2] = {0.0, 0.0};
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    double p = kBsUnit * kBsUnit * kBsUnit / 6;
-    p = fma(p, t[i], kBsUnit * kBsUnit / 2);
-    p = fma(p, t[i], kBsUnit);
+    double p = fma(kBsC3, t[i], kBsC2);
+    p = fma(p, t[i], kBsC1);
     p = fma(p, t[i], 1.0);
     part[i & 1] = fma(p, __builtin_bit_cast(double, (uint64_t)(b[i].y + (n[i] << 12)) << 32 | b[i].x), part[i & 1]);
   }

@@ -585,6 +585,29 @@ def test_beam_select_equal_beams_at_any_alignment(cuda_device, V, dtype):
         assert all(torch.equal(t, totals[0]) for t in totals)
 
 
+@pytest.mark.parametrize("part", [0.02, 0.25, 0.5, 0.75, 0.98])
+def test_beam_select_sums_tell_totals_of_two_to_the_minus_40_apart(cuda_device, part):
+    """Exponentials to 2^-42: of two beams whose best totals lie 2^-40 apart the better one comes first, whatever
+    places between two entries of a table of 256 powers of two the logits of one of them take."""
+    from moeinfra_amd import ops
+
+    V, unit = 2000, math.log(2) / 256
+    fp32 = lambda v: torch.tensor(v, dtype=torch.float32).tolist()
+    lse = lambda r: math.log(math.fsum(math.exp(v) for v in r))   # (2^-50 of itself)
+    other = fp32([0.0] + [-(j - 0.001) * unit for j in range(1, V)])
+    for ahead in (2.0 ** -40, -2.0 ** -40):
+        row = fp32([0.0] + [-(j + 1 - part) * unit for j in range(1, V - 1)])
+        # The score in steps of 2^-24 of itself, the rest by a logit far below.
+        score = fp32([lse(row + [-16.0]) - lse(other) - ahead])[0]
+        rest = math.exp(score + lse(other) + ahead) - math.fsum(math.exp(v) for v in row)
+        row = row + fp32([math.log(rest)])
+        gap = (0.0 - lse(other)) - (score - lse(row))
+        assert abs(gap - ahead) < 2.0 ** -46
+        x = torch.tensor([row, other], device=cuda_device)
+        got = ops.beam_select(x, torch.tensor([[score, 0.0]], device=cuda_device), 2)
+        assert got[1].tolist()[0] == ([1, 0] if ahead > 0 else [0, 1]) and got[2].tolist() == [[0, 0]]
+
+
 # ------------------------------------------------------------------ forked pages
 def _check_fork(dev, table, lens, parents, refs, page, ahead=1, workspace=None):
     from moeinfra_amd import ops
