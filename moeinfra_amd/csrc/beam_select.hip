@@ -146,12 +146,18 @@ __device__ __forceinline__ double bs_wave_sum(double v) {
   return v;
 }
 
-// A continuation of a search: its total, rising with it (0: none), and its place, beam * V + token.
+// A continuation of a search: its total, rising with it (0: none), and what goes first of equal totals: the lower
+// beam (from bit 52 on), inside it the larger logit (its order, inverted, from bit 20 on: logits may differ where
+// their totals round to the same), then the lower token.
 struct BsCand {
-  uint64_t total;
-  uint32_t at;
+  uint64_t total, at;
 };
-__device__ __forceinline__ bool bs_before(uint64_t t0, uint32_t a0, uint64_t t1, uint32_t a1) {
+constexpr int kBsTokenBits = 20, kBsBeamBit = kBsTokenBits + 32;
+static_assert(kBsMaxVocab <= 1 << kBsTokenBits && kBsMaxBeams <= 1 << (64 - kBsBeamBit), "beam, logit and token fit 64 bits");
+__device__ __forceinline__ uint64_t bs_at(int w, uint64_t key) {
+  return (uint64_t)w << kBsBeamBit | (uint64_t)~(uint32_t)(key >> 32) << kBsTokenBits | ~(uint32_t)key;
+}
+__device__ __forceinline__ bool bs_before(uint64_t t0, uint64_t a0, uint64_t t1, uint64_t a1) {
   return t0 > t1 || (t0 == t1 && a0 < a1);
 }
 
@@ -173,8 +179,7 @@ beam_select_kernel(const BsArgs a) {
   constexpr int kPer = 16 / sizeof(E);              // values of a piece
   constexpr int kHeld = kBsPieces * kPer;           // of a thread
   constexpr uint32_t kLeast = 0x80;                 // upper 16 bits of the lowest finite value's order
-  __shared__ uint64_t s_list[kBsList + 8], s_key[kBsThreads], s_best[kBsMost];
-  __shared__ uint32_t s_at[kBsList + 8];
+  __shared__ uint64_t s_list[kBsList + 8], s_at[kBsList + 8], s_key[kBsThreads], s_best[kBsMost];
   __shared__ double s_sum[kBsWaves], s_lse[kBsMaxBeams];
   __shared__ uint2 s_tab[kBsTable];
   __shared__ float s_max[kBsWaves][kWave], s_top[kBsMaxBeams], s_score[kBsMaxBeams];
@@ -438,9 +443,9 @@ beam_select_kernel(const BsArgs a) {
   auto cand = [&](int i, uint64_t key) {  // (of W * chunks * k)
     const int w = i / a.k / a.chunks;
     const float score = s_score[w];
-    BsCand r{0, 0xffffffffu};
+    BsCand r{0, ~0ull};
     if (key == 0 || !(score > -INFINITY && score < INFINITY) || !(s_top[w] < INFINITY)) return r;
-    r.at = (uint32_t)w * (uint32_t)a.V + ~(uint32_t)key;
+    r.at = bs_at(w, key);
     const double total = (double)score + (((double)bs_value((uint32_t)(key >> 32)) - (double)s_top[w]) - s_lse[w]);
     const uint64_t b = __builtin_bit_cast(uint64_t, total + 0.0);
     r.total = b >> 63 ? ~b : b | 1ull << 63;
@@ -461,7 +466,7 @@ beam_select_kernel(const BsArgs a) {
   s_at[tid] = most;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kBsWaves; ++w) most = max(most, s_at[w * kWave + lane]);
+  for (int w = 0; w < kBsWaves; ++w) most = max(most, (uint32_t)s_at[w * kWave + lane]);
   uint32_t lowest = 0;
 #pragma unroll
   for (int bit = 31; bit >= 0; --bit) {
@@ -504,12 +509,11 @@ beam_select_kernel(const BsArgs a) {
     }
   }
   __syncthreads();
-  auto put = [&](int rank, uint64_t total, uint32_t at) {
+  auto put = [&](int rank, uint64_t total, uint64_t at) {
     const int64_t o = (int64_t)search * a.k + rank;
-    const uint32_t w = at / (uint32_t)a.V;
     a.best[o] = total == 0 ? -INFINITY : (float)__builtin_bit_cast(double, total >> 63 ? total & ~(1ull << 63) : ~total);
-    a.rows[o] = total == 0 ? -1 : search * a.W + (int)w;
-    a.tokens[o] = total == 0 ? -1 : (int64_t)(at - w * (uint32_t)a.V);
+    a.rows[o] = total == 0 ? -1 : search * a.W + (int)(at >> kBsBeamBit);
+    a.tokens[o] = total == 0 ? -1 : (int64_t)(at & ((1u << kBsTokenBits) - 1));
   };
   const int n = (int)min(s_n, (uint32_t)kBsList);
   if (s_n <= (uint32_t)kBsList) {
@@ -517,7 +521,7 @@ beam_select_kernel(const BsArgs a) {
     __syncthreads();
     for (int i = tid; i < n; i += kBsThreads) {
       const uint64_t total = s_list[i];
-      const uint32_t at = s_at[i];
+      const uint64_t at = s_at[i];
       int rank = 0;
       for (int j = 0; j < n; j += 8)
 #pragma unroll
@@ -530,7 +534,7 @@ beam_select_kernel(const BsArgs a) {
   // More than the list holds (many equal lists in one thread's hands): one by one.
   BsCand last{~0ull, 0};
   for (int rank = 0; rank < a.k; ++rank) {
-    BsCand next{0, 0xffffffffu};
+    BsCand next{0, ~0ull};
     for (int i = tid; i < n_all; i += kBsThreads) {
       const BsCand x = cand(i, key_of(i));
       if (bs_before(last.total, last.at, x.total, x.at) && bs_before(x.total, x.at, next.total, next.at)) next = x;
@@ -540,7 +544,7 @@ beam_select_kernel(const BsArgs a) {
     s_list[tid] = next.at;
     __syncthreads();
     for (int j = 0; j < kBsThreads; ++j)
-      if (bs_before(s_key[j], (uint32_t)s_list[j], next.total, next.at)) next = {s_key[j], (uint32_t)s_list[j]};
+      if (bs_before(s_key[j], s_list[j], next.total, next.at)) next = {s_key[j], s_list[j]};
     last = next;
     if (tid == 0) put(rank, next.total, next.at);
   }

@@ -670,8 +670,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int, workspace: O
     ``scores[s, w] + log_softmax(logits[s * W + w])``; ``logits`` bf16 or fp32 [S * W, V] (rows may lie
     apart), ``scores`` fp32 [S, W], sums over the vocabulary in 64 bits.  Returns (totals fp32 [S, k],
     falling; the rows of ``logits`` that go on, int32 [S, k]; tokens int64 [S, k]).  Equal ones go by beam,
-    then token.  -inf and NaN are never chosen; a score of -inf is no beam (a search's first step has
-    one), nor is a beam whose logits hold +inf; what there is too little for is -inf, -1, -1."""
+    inside it by logit, then token.  -inf and NaN are never chosen; a score of -inf is no beam (a search's
+    first step has one), nor is a beam whose logits hold +inf; what there is too little for is -inf, -1, -1."""
     _require_cuda(logits, "logits")
     dev, f32 = logits.device, logits.dtype is _F32
     if not f32 and logits.dtype is not _BF16:

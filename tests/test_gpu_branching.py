@@ -608,6 +608,26 @@ def test_beam_select_sums_tell_totals_of_two_to_the_minus_40_apart(cuda_device, 
         assert got[1].tolist()[0] == ([1, 0] if ahead > 0 else [0, 1]) and got[2].tolist() == [[0, 0]]
 
 
+@pytest.mark.parametrize("W,V,score", [(1, 40, -20.0), (2, 40, -20.0), (2, 100000, -20.0), (3, 5000, -1e20), (16, 70000, -20.0)])
+def test_beam_select_logits_nearer_than_their_totals(cuda_device, W, V, score):
+    """Logits that differ by less than a step of the totals: the larger one first, the lower beam's before the
+    others', and the first k of them whatever k."""
+    from moeinfra_amd import ops
+
+    g = torch.Generator().manual_seed(V)
+    x = torch.full((W, V), -30.0)
+    at = torch.randperm(V, generator=g)[:80]
+    for w in range(W):   # (the same exponentials at the same places: the same sums)
+        x[w, at] = (torch.randperm(len(at), generator=g).float() + 1) * 1e-20
+    scores = torch.full((1, W), score)
+    x, scores = x.to(cuda_device), scores.to(cuda_device)
+    order = torch.sort(x[0].double().cpu(), descending=True, stable=True).indices.tolist()
+    for k in (1, 2, 3, 9, 30, min(64, V)):
+        best, rows, tokens = ops.beam_select(x, scores, k)
+        assert rows.tolist() == [[0] * k] and tokens.tolist() == [order[:k]], f"the best {k}"
+        assert bool((best == best[0, 0]).all())
+
+
 # ------------------------------------------------------------------ forked pages
 def _check_fork(dev, table, lens, parents, refs, page, ahead=1, workspace=None):
     from moeinfra_amd import ops
