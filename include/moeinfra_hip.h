@@ -494,8 +494,9 @@ int moe_beam_select(const void *logits, int32_t logits_f32, int64_t stride, int6
  * them, row by row; every other place gets the lowest page whose count is not above zero, in the same
  * order, and where it held one that the length reaches into, copies[i] (int32 [n_new, 3]) says {that
  * page, the new one, positions to copy}, else {-1, -1, 0}.  A place for which no page is left is -1, and
- * missing[0] (int32) counts them.  Places past the table's width are none.  Up to 8192 rows and 8192
- * places.  The workspace (moe_fork_pages_workspace_bytes) is zero before the first call, every call
+ * missing[0] (int32) counts them (such a row has let go of a page that it shared there, with its keys in
+ * it).  Places past the table's width are none.  Up to 8192 rows and 8192 places.  The workspace
+ * (moe_fork_pages_workspace_bytes) is zero before the first call, every call
  * leaves it zero; calls that share it must be ordered. */
 int64_t moe_fork_pages_workspace_bytes(int64_t num_pages);
 int moe_fork_pages(const void *page_table_i32, const void *lens_i32, int64_t n_seqs,

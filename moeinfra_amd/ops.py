@@ -714,7 +714,8 @@ def fork_pages(page_table: torch.Tensor, lens: torch.Tensor, parents: torch.Tens
 
     Returns (table int32 [N, width], lens int32 [N], copies int32 [N, 3], missing int32 [1]); ``out`` is
     such a tuple to write to.  ``copies`` are for ``copy_pages``: (page, new page, positions in use), or
-    (-1, -1, 0).  ``missing`` counts places for which no page was free: -1 in the table."""
+    (-1, -1, 0).  ``missing`` counts places for which no page was free: -1 in the table
+    (also where the row shared a partly filled page: its keys there are lost to it)."""
     _require_cuda(page_table, "page_table")
     dev = page_table.device
     table = _plain(page_table, "page_table", _I32, dev)

@@ -3,6 +3,7 @@ drafted tokens, their acceptance and compaction, beam selection, forked and copi
 from __future__ import annotations
 
 import math
+import os
 import random
 
 import pytest
@@ -12,6 +13,8 @@ import branching_ref as ref
 from serving_ref import Pool, assert_within, attention, rope
 
 pytestmark = pytest.mark.gpu
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def _bf(shape, seed, std=1.0):
@@ -888,6 +891,40 @@ def test_beams_together(cuda_device):
     # All searches end: every page is free again.
     ops.fork_pages(table, lens, _i32([-1] * S * W, dev), refs, page, workspace=fws)
     assert not bool(refs.any())
+
+
+def test_beam_step_as_documented(cuda_device):
+    """The loop body of INTEGRATION.md, step after step: each row's pages hold its history, whose length `lens` is."""
+    from moeinfra_amd import ops
+
+    with open(os.path.join(REPO, "INTEGRATION.md")) as f:
+        text = f.read()
+    lines = text[text.index("scores, rows, tokens = ops.beam_select("):].split("```")[0].splitlines()
+    at = [i for i, line in enumerate(lines) if line.startswith("q, _ =")]
+    assert len(at) == 1
+    dev, page_size, W, S, pages = cuda_device, 8, 3, 2, 64
+    toy = Toy(dev)
+    k_all, v_all = (torch.full((1, pages, toy.nkv, page_size, toy.hd), math.nan, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    refs = torch.zeros(pages, dtype=torch.int32, device=dev)
+    table = torch.full((S * W, 6), -1, dtype=torch.int32, device=dev)
+    lens = torch.zeros(S * W, dtype=torch.int32, device=dev)
+    scores = torch.zeros((S, W), device=dev)
+    env = dict(ops=ops, S=S, W=W, n_q=toy.nq, n_kv=toy.nkv, head_dim=toy.hd, page_size=page_size, inv_freq=toy.inv, table=table,
+               lens=lens, refs=refs, scores=scores, k_all=k_all, v_all=v_all, k_cache=k_all[0], v_cache=v_all[0],
+               bws=ops.beam_select_workspace(S, W, W, dev), fws=ops.fork_pages_workspace(pages, dev))
+    history = [[] for _ in range(S * W)]
+    for step in range(20):
+        env["logits"] = _logits(S * W, toy.vocab, 200 + step, torch.float32).to(dev)
+        exec("\n".join(lines[:at[0]]), env)
+        env["qkv"] = toy.emb[env["tokens"].flatten()]
+        exec("\n".join(lines[at[0]:]), env)
+        history = [history[p] + [t] for p, t in zip(env["rows"].flatten().tolist(), env["tokens"].flatten().tolist())]
+        assert env["lens"].tolist() == [step + 1] * (S * W) and int(env["missing"]) == 0
+        for i in range(S * W):
+            _check_cache(toy, k_all[0], v_all[0], env["table"][i].cpu(), page_size, history[i])
+        q = env["q"].view(S * W, toy.nq, toy.hd)
+        o = ops.paged_attention(q, k_all[0], v_all[0], env["table"], _i32([step + 1] * (S * W), dev))
+        assert _same(o, env["attn"])
 
 
 def _graph(run):
