@@ -433,7 +433,7 @@ int moe_rope_paged_kv_slots_bf16(const void *qkv, int64_t qkv_stride, int64_t T,
  * size for all batches of the same heads; 16-byte aligned; calls that share it must be ordered, what it
  * holds before a call does not matter) several workgroups share a tree's keys, and a second launch adds
  * their results up in a fixed order; null: a workgroup for each KV head and 256 rows (128 of 256 dims) of
- * token and query head. */
+ * token and query head.  out and the workspace overlap neither the inputs nor each other. */
 int64_t moe_paged_tree_attention_workspace_bytes(int64_t B, int32_t n_q_heads, int32_t n_kv_heads,
                                                  int32_t head_dim);
 int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, int64_t T, const void *k_cache,

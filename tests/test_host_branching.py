@@ -187,6 +187,14 @@ def test_refused_before_any_launch(call, change, needle):
     assert needle in _lib.lib().moe_last_error().decode()
 
 
+@pytest.mark.parametrize("kw", [dict(ws=A), dict(ws=A - 4096), dict(ws=E), dict(ws=E + 64), dict(ws=F), dict(ws=G), dict(ws=C - 64),
+                                dict(ws=B), dict(ws=D), dict(ws=I), dict(out=C - 8), dict(out=B), dict(out=D), dict(out=I)])
+def test_tree_attention_refuses_a_workspace_or_output_in_its_inputs(kw):
+    """What the workgroups write while others still read: the workspace and out, against all inputs and each other."""
+    assert _tree(**{"ws": H, "ws_bytes": 1 << 36, **kw}) == _lib.MOE_STATUS_INVALID_ARGUMENT
+    assert "overlap" in _lib.lib().moe_last_error().decode()
+
+
 def test_empty_calls_do_nothing():
     assert _slots(T=0, qkv=None, q=None, slots=None) == 0
     assert _tree(B=0, cu=None, lens=None) == 0
