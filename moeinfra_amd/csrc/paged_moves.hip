@@ -181,7 +181,9 @@ extern "C" int moe_copy_pages_bf16(void *k_cache, void *v_cache, int64_t layers,
   const int64_t pieces = (int64_t)n_kv_heads * page_size * (head_dim / 8), each = moe::kPmFew * moe::kPmThreads;
   int64_t hgroups = (pieces + each - 1) / each;
   hgroups = hgroups < n_kv_heads ? hgroups : n_kv_heads;
-  MOE_REQUIRE(n_copies >= 0 && n_copies <= 0x7fffffff && moe::launch_fits(2 * n_copies * layers * hgroups, moe::kPmThreads),
+  // (The first product first: all three may pass 64 bits.)
+  MOE_REQUIRE(n_copies >= 0 && n_copies <= 0x7fffffff && moe::launch_fits(2 * n_copies * layers, moe::kPmThreads) &&
+                  moe::launch_fits(2 * n_copies * layers * hgroups, moe::kPmThreads),
               "bad sizes");
   if (n_copies == 0 || layers == 0 || num_pages == 0) return MOE_STATUS_OK;
   MOE_REQUIRE(copies_i32, "null pointer");

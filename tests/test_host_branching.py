@@ -195,6 +195,14 @@ def test_tree_attention_refuses_a_workspace_or_output_in_its_inputs(kw):
     assert "overlap" in _lib.lib().moe_last_error().decode()
 
 
+@pytest.mark.parametrize("n", [(1 << 31) - 1, (1 << 30) + (1 << 20)])
+def test_copies_beyond_64_bits_are_refused(n):
+    """Copies times layers times groups of heads wrap around 64 bits: too many, not few."""
+    big = dict(layers=1 << 16, layer_stride=1 << 40, pages=1, page=512, nkv=65535, hd=256, page_stride=1 << 33, n=n)
+    assert _copy(**big) == _lib.MOE_STATUS_INVALID_ARGUMENT
+    assert "bad sizes" in _lib.lib().moe_last_error().decode()
+
+
 def test_empty_calls_do_nothing():
     assert _slots(T=0, qkv=None, q=None, slots=None) == 0
     assert _tree(B=0, cu=None, lens=None) == 0
