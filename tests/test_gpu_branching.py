@@ -125,6 +125,32 @@ def test_paged_tree_attention_more_row_tiles_than_counters(cuda_device):
 
 
 @pytest.mark.parametrize("nq,nkv,hd,lens,counts", [
+    (8, 8, 64, [i * 7 % 50 for i in range(2100)] + [700], [1 + i % 2 for i in range(2101)]),
+    (8, 2, 128, [i * 37 % 300 for i in range(130)], [0 if i % 5 == 2 or i in (63, 64) else 1 + i * 11 % 64 for i in range(130)]),
+    (16, 1, 128, [i % 70 for i in range(65)], [0] * 63 + [64, 40])])
+def test_paged_tree_attention_of_many_sequences_without_a_workspace(cuda_device, nq, nkv, hd, lens, counts):
+    """The C call without one: a workgroup for each sequence, KV head and row tile, also past the 64th sequence."""
+    from moeinfra_amd import _lib
+
+    print(f"tree attention of {len(lens)} sequences without a workspace", flush=True)
+    dev = cuda_device
+    t = Trees(dev, lens, counts, nq, nkv, hd, 16, seed=23, lead=2, behind=3)
+    q, out = t.q.to(dev), torch.full_like(t.q, 9.0, device=dev)
+    n, cu, masks = _i32(t.lens, dev), _i32(t.cuts, dev), t.dev_masks()
+    _lib.check(_lib.lib().moe_paged_tree_attention_bf16(
+        q.data_ptr(), q.stride(0), t.T, t.pool.k.data_ptr(), t.pool.v.data_ptr(), t.pool.pages, 16, t.pool.k.stride(0),
+        t.pool.dev_table.data_ptr(), t.pool.dev_table.shape[1], n.data_ptr(), cu.data_ptr(), masks.data_ptr(), len(lens), nq,
+        nkv, hd, hd ** -0.5, out.data_ptr(), None, 0, torch.cuda.current_stream().cuda_stream), "tree attention")
+    t.check(out)
+    assert bool((out[:2] == 9.0).all()) and bool((out[t.T - 3:] == 9.0).all())
+    shared = t.run()
+    t.check(shared)
+    # With one the same within two roundings of the output and of the weights.
+    got, want = out[2:t.T - 3].float(), shared[2:t.T - 3].float()
+    assert float((got - want).abs().max()) <= 4 * 2.0 ** -8 * float(max(v.float().abs().max() for v in t.v if len(v)))
+
+
+@pytest.mark.parametrize("nq,nkv,hd,lens,counts", [
     (8, 2, 128, [20000, 0, 8176, 5], [40, 3, 64, 1]), (8, 1, 64, [17000, 9000], [64, 2]), (8, 4, 256, [8200, 1], [33, 9]),
     (40, 2, 128, [300, 8150], [64, 64])])
 def test_paged_tree_attention_without_a_workspace(cuda_device, nq, nkv, hd, lens, counts):
@@ -698,6 +724,50 @@ def test_fork_pages_most_rows(cuda_device):
     table, refs = [[i, -1] for i in range(rows)], [1] * rows + [0] * (pages - rows)
     lens = [rng.randint(0, 8) for _ in range(rows)]
     _check_fork(cuda_device, table, lens, [rng.randrange(rows) for _ in range(rows)], refs, page)
+
+
+@pytest.mark.parametrize("rows,page,ahead,spare", [(2049, 8, 1, 900), (2048, 16, 1, 900), (2100, 8, 12, 2000), (1025, 8, 9, 1500),
+                                                   (1024, 8, 9, 1500), (4000, 16, 1, 3000), (683, 8, 17, 700)])
+def test_fork_pages_of_many_rows_step_by_step(cuda_device, rows, page, ahead, spare):
+    """Around and above what is chosen in LDS (2048 rows and places): steps of random beams over prompts that many
+    rows share and that are held from outside too, with one workspace, which every step leaves zero; pages run out."""
+    from moeinfra_amd import ops
+
+    print(f"{rows} rows, {ahead} tokens ahead, pages of {page}", flush=True)
+    rng = random.Random(rows + ahead)
+    width, prompts = 9, 40
+    table, lens, refs = [], [], [0] * 3
+    for i in range(rows):
+        if i < prompts:                # the prompts' rows, their first pages held from outside
+            n = rng.randint(1, 3 * page)
+            ids = list(range(len(refs), len(refs) + (n + page - 1) // page))
+            refs += [2] + [1] * (len(ids) - 1)
+        else:
+            j = rng.randrange(prompts)
+            n, ids = lens[j], [p for p in table[j] if p >= 0]
+            for p in ids:
+                refs[p] += 1
+        table.append(ids + [-1] * (width - len(ids)))
+        lens.append(n)
+    # Pages for some steps: each row's places, and what is spare.
+    refs += [0] * (rows * ((ahead + page - 1) // page + 1) + spare)
+    ws = ops.fork_pages_workspace(len(refs), cuda_device)
+    parents, ran_out = list(range(rows)), False
+    for step in range(6):
+        want_missing = ref.fork([list(r) for r in table], lens, parents, list(refs), page, ahead)[3]
+        ran_out |= want_missing > 0
+        table, lens, refs = _check_fork(cuda_device, table, lens, parents, refs, page, ahead, ws)
+        assert not bool(ws.any()), f"step {step}"
+        lens = [min(n + rng.randint(0, ahead), width * page) for n in lens]
+        # (Some rows end, many go on from a few, the others from themselves.)
+        few = [rng.randrange(rows) for _ in range(20)]
+        parents = [rng.choice((i, i, i, rng.choice(few), -1 if step == 2 else i)) for i in range(rows)]
+        if step == 3:
+            # No page is free but a few.
+            free = [p for p, c in enumerate(refs) if c <= 0]
+            for p in free[5:]:
+                refs[p] = 1
+    assert ran_out
 
 
 # ------------------------------------------------------------------ together
