@@ -168,10 +168,11 @@ __device__ __forceinline__ bool bs_before(uint64_t t0, uint64_t a0, uint64_t t1,
 // and above there are k values at least, and few more, which go to a list and are ranked.  Later rounds keep
 // that bound, and have no barriers.
 //
-// Bound: vector instructions (64 x 4 rows of 131072 bf16: 36 us, of it 12 the exponentials at 12 instructions
-// each, of 64 bits at 4.9 cycles where those of 32 take 4.5; 16 the loads alone, 6 the choice, 5 the join of the
-// last search), for few rows latency (1 x 4 x 32000: 11 us, three trips to memory after the values').  1024
-// workgroups, all at once: 2048 of half the length 48 us, when 42 was the time.
+// Bound: phases one behind the other, of which little overlaps (64 x 4 rows of 131072 bf16: 34 to 36 us; each by itself:
+// 16 the loads, 12 the exponentials at 12 instructions each, of 64 bits at 4.9 cycles where those of 32 take 4.5, 6 the
+// choice, 5 the join of the last search; fp32 40; 50257 bf16 24), for few rows latency (1 x 4 x 32000: 11 us, three
+// trips to memory after the values), for large W k the join (1 x 16 x 131072 of 16: 34 us).  1024 workgroups, all at
+// once: 2048 of half the length 48 us, when 42 was the time.
 template <bool F32>
 __global__ void __launch_bounds__(kBsThreads, 4)
 beam_select_kernel(const BsArgs a) {

@@ -190,7 +190,8 @@ fork_few_pages_kernel(const FpArgs a) {
   if (tid == 0) *a.missing = max(wanted - found, 0);
 }
 
-// One workgroup, as each step needs all of the one before.
+// One workgroup, as each step needs all of the one before.  Bound: one CU's loads and atomics, with counts of writers
+// in memory: 2049 rows of up to 20 pages 68 us (2048 by the above 34), 4096 133, 8192 263.
 __global__ void __launch_bounds__(kFpThreads)
 fork_pages_kernel(const FpArgs a) {
   __shared__ int s_children[kFpRows], s_free[kFpRows], s_rank[kFpRows], s_sum[kFpWaves];

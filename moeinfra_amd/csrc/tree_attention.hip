@@ -22,8 +22,8 @@ constexpr float kTaLog2e = 1.44269504088896341f;
 constexpr float kTaLag = 8.0f;
 // Up to here the reference may be a factor of the exponent's multiply-add (in powers of two).
 constexpr float kTaFine = 4096.0f;
-// Places of a tile that takes all waves (24 ragged trees: 101 us; as one 115, as three 106), and that beginning a
-// row tile takes.
+// Places of a tile that takes all waves (24 ragged trees: 87 us; as one 102, as three 94), and that beginning a row
+// tile takes.
 constexpr int kTaAll = 2;
 constexpr int kTaStart = 2;
 constexpr int kTaLeast = 2;    // places of a workgroup at least (a tile)
@@ -69,7 +69,7 @@ __device__ u32x4 ta_zeros[1024 / 16];
 // 64 lanes' 16 bytes each, at `lane` bytes from src, into LDS at dst + 16 * lane number, without
 // registers.  (In asm, as the compiler would wait for all of them before the next transposing read of the
 // other plane; the caller waits until no more loads than those of later steps are under way, and a barrier,
-// before it reads dst.  Streamed, as each key is read once.)
+// before it reads dst.  Streamed, as each key is read once for a row tile, and most trees are one.)
 __device__ __forceinline__ void ta_load_lds(const void *src, uint32_t lane, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(dst), "v"(lane), "s"(src)
                : "memory", "m0");
@@ -558,9 +558,9 @@ paged_tree_attention_kernel(const TaArgs a) {
 }
 
 // The results of the workgroups that share a row tile added up, in the order of the keys: a workgroup takes 32
-// rows of what began in one workgroup's part.  (By the last workgroup to arrive, without this launch, one of 900
-// keys took 16.1 us, now 14.8, and 4 of 16000 keys of 16 / 1 heads, up to 62 parts of 256 rows each, 108
-// instead of 52.)
+// rows of what began in one workgroup's part.  (Joined by the last workgroup to arrive instead, in the same build
+// without this launch, one chain of 900 keys took 16.1 us against 16.9, but 4 of 16000 keys of 16 / 1 heads, up to 62
+// parts of 256 rows each, 108 against 52, and 8 of 16384 keys and 64 tokens 208 against 202.)
 constexpr int kTjThreads = 256;
 template <int HD>
 __global__ void __launch_bounds__(kTjThreads)
