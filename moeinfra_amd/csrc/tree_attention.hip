@@ -697,6 +697,11 @@ extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, in
               "tensors must be aligned");
   const int64_t cb = num_pages > 0 ? 2 * ((num_pages - 1) * page_stride + page_row) : 0;
   const int64_t need = moe_paged_tree_attention_workspace_bytes(B, n_q_heads, n_kv_heads, head_dim);
+  if (workspace != nullptr) {
+    MOE_REQUIRE(workspace_bytes >= need, "workspace too small: need %lld bytes, got %lld", (long long)need,
+                (long long)workspace_bytes);
+    MOE_REQUIRE((uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
+  }
   const void *p[9] = {out, workspace, q, k_cache, v_cache, page_table_i32, lens_i32, cu_seqlens_i32, masks_i64};
   const int64_t size[9] = {2 * T * row, need, 2 * (q_stride * (T - 1) + row), cb, cb, 4 * B * table_width, 4 * B,
                            4 * (B + 1), 8 * T};
@@ -704,11 +709,6 @@ extern "C" int moe_paged_tree_attention_bf16(const void *q, int64_t q_stride, in
     for (int j = i + 1; j < 9; ++j)
       MOE_REQUIRE(!moe::ranges_overlap(p[i], size[i], p[j], size[j]),
                   "out and the workspace must not overlap the inputs or each other");
-  if (workspace != nullptr) {
-    MOE_REQUIRE(workspace_bytes >= need, "workspace too small: need %lld bytes, got %lld", (long long)need,
-                (long long)workspace_bytes);
-    MOE_REQUIRE((uintptr_t)workspace % 16 == 0, "workspace must be 16-byte aligned");
-  }
   moe::TaArgs a{};
   a.q = (const uint16_t *)q;
   a.q_stride = q_stride;
