@@ -64,9 +64,9 @@ __device__ __forceinline__ uint64_t bs_key(uint32_t o, uint32_t i) { return o ==
 //
 // e^(u x) is its series up to x^4 less u^4 / 24 of the polynomial x^4 + g3 x^3 + g2 x^2 + g1 x that is smallest on
 // [0, 1]: a Chebyshev polynomial of degree 4, its argument (1 + z) x - z so that its first zero, -z = -cos(pi / 8),
-// lies at 0 (e^0 stays 1).  That takes x^4 away, and what is left out is 2^-45.4 at most, to both sides; the series up to x^3
-// by itself lacks 2^-38.7, always to one side, which told the better of two beams wrongly when 2^-40 lay between
-// them.
+// lies at 0 (e^0 stays 1).  That takes x^4 away, and what is left out is 2^-45.4 at most, to both sides; the series up
+// to x^3 by itself lacks 2^-38.7, always to one side, which told the better of two beams wrongly when 2^-40 lay
+// between them.
 constexpr int kBsTable = 256;
 constexpr double kBsUnit = 0.69314718055994530942 / kBsTable;
 constexpr double kBsLow = -700.0;
@@ -168,8 +168,8 @@ __device__ __forceinline__ bool bs_before(uint64_t t0, uint64_t a0, uint64_t t1,
 // and above there are k values at least, and few more, which go to a list and are ranked.  Later rounds keep
 // that bound, and have no barriers.
 //
-// Bound: phases one behind the other, of which little overlaps (64 x 4 rows of 131072 bf16: 34 to 36 us; each by itself:
-// 16 the loads, 12 the exponentials at 12 instructions each, of 64 bits at 4.9 cycles where those of 32 take 4.5, 6 the
+// Bound: phases one behind the other, of which little overlaps (64 x 4 rows of 131072 bf16: 34 to 36 us; each by
+// itself: 16 the loads, 12 the exponentials at 12 instructions each, of 64 bits at 4.9 cycles where those of 32 take 4.5, 6 the
 // choice, 5 the join of the last search; fp32 40; 50257 bf16 24), for few rows latency (1 x 4 x 32000: 11 us, three
 // trips to memory after the values), for large W k the join (1 x 16 x 131072 of 16: 34 us).  1024 workgroups, all at
 // once: 2048 of half the length 48 us, when 42 was the time.

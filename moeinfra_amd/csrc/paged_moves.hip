@@ -23,7 +23,8 @@ struct PmCache {
 // stores.
 //
 // Bound: HBM where there are many rows (64 sequences, up to 9 tokens kept, 32 layers of 8 heads of 128: 59 MB in
-// 17.5 us where the caches are others in each call, 10.5 on the same ones again), else the launch and a chain of loads (path and length, page entries, rows; 3.1 us).
+// 17.5 us where the caches are others in each call, 10.5 on the same ones again), else the launch and a chain of
+// loads (path and length, page entries, rows; 3.1 us).
 __global__ void __launch_bounds__(kPmThreads)
 compact_paged_kv_kernel(const PmCache c, const int32_t *__restrict__ table, int64_t width,
                         const int32_t *__restrict__ lens, const int64_t *__restrict__ paths) {

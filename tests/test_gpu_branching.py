@@ -2,6 +2,7 @@
 drafted tokens, their acceptance and compaction, beam selection, forked and copied pages."""
 from __future__ import annotations
 
+import glob
 import math
 import os
 import random
@@ -964,12 +965,16 @@ def test_beams_together(cuda_device):
 
 
 def test_beam_step_as_documented(cuda_device):
-    """The loop body of INTEGRATION.md, step after step: each row's pages hold its history, whose length `lens` is."""
+    """The documents' loop body, step after step: each row's pages hold its history, whose length `lens` is."""
     from moeinfra_amd import ops
 
-    with open(os.path.join(REPO, "INTEGRATION.md")) as f:
-        text = f.read()
-    lines = text[text.index("scores, rows, tokens = ops.beam_select("):].split("```")[0].splitlines()
+    begin = "scores, rows, tokens = ops.beam_select("
+    found = []
+    for name in sorted(glob.glob(os.path.join(REPO, "*.md"))):
+        with open(name) as f:
+            found += f.read().split(begin)[1:]
+    assert len(found) == 1
+    lines = (begin + found[0].split("```")[0]).splitlines()
     at = [i for i, line in enumerate(lines) if line.startswith("q, _ =")]
     assert len(at) == 1
     dev, page_size, W, S, pages = cuda_device, 8, 3, 2, 64
